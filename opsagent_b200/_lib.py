@@ -28,6 +28,15 @@ class OaChatResp(C.Structure):
                 ("completion_tokens", C.c_int32), ("finish_reason", C.c_int32), ("token_ids", C.POINTER(C.c_int32))]
 
 
+class OaPageTable(C.Structure):
+    """Host arrays of a caller's paged cache: block_tables [n_rows, max_pages_per_seq], lens [n_rows], refs [num_pages]."""
+    _fields_ = [("block_tables", C.c_void_p), ("lens", C.c_void_p), ("refs", C.c_void_p), ("n_rows", C.c_int32), ("max_pages_per_seq", C.c_int32), ("num_pages", C.c_int32)]
+
+
+class OaPageMove(C.Structure):
+    _fields_ = [("src", C.c_int32), ("dst", C.c_int32), ("tokens", C.c_int32)]
+
+
 # every symbol include/opsagent_b200.h declares (tests/test_abi.py checks the library exports all of them)
 SYMBOLS = [
     "oa_engine_create", "oa_engine_destroy", "oa_chat_complete", "oa_chat_submit", "oa_chat_wait", "oa_free_resp",
@@ -35,6 +44,7 @@ SYMBOLS = [
     "oa_debug_prefill_logits", "oa_bench_decode", "oa_k_rmsnorm", "oa_k_gemm", "oa_k_init_weight", "oa_k_paged_attention",
     "oa_kernel_launches", "oa_version", "oa_host_apply_chat_template", "oa_host_decode_plan", "oa_host_decode_attention_plan", "oa_host_streamk_plan", "oa_host_bpe_encode", "oa_host_bpe_decode", "oa_host_model_info",
     "oa_k_gemm_streamk", "oa_k_hybrid_gemm", "oa_k_gemm_ext", "oa_host_gemm_kernel", "oa_host_gemm_pair_width", "oa_host_gemm_pair_swapped", "oa_host_prefill_attention_kernel", "oa_debug_kernel_times", "oa_engine_serve", "oa_host_grammar_step", "oa_host_grammar_step_ex", "oa_host_grammar_token_mask", "oa_http_start", "oa_http_port", "oa_http_stats", "oa_http_stop", "oa_http_last_error", "oa_host_json_roundtrip", "oa_chat_cancel", "oa_chat_submit_ex", "oa_chat_wait_ex", "oa_trace_step",
+    "oa_host_rotary_freqs", "oa_k_rotary", "oa_k_rotary_cache", "oa_host_cache_grow", "oa_host_cache_free", "oa_host_cache_fork", "oa_host_cache_compact", "oa_k_cache_copy", "oa_k_prefix_attention",
 ]
 
 _lib = None
@@ -80,6 +90,16 @@ def load() -> C.CDLL:
     L.oa_debug_kernel_times.argtypes = [vp, C.c_char_p, C.c_size_t, i32]; L.oa_debug_kernel_times.restype = C.c_int
     L.oa_k_init_weight.argtypes = [vp, u64, u64, C.c_int64, C.c_int64, C.c_int64, f32, f32, vp]; L.oa_k_init_weight.restype = C.c_int
     L.oa_k_paged_attention.argtypes = [vp, vp, vp, i32, vp, i32, vp, vp, i32, i32, i32, i32, i32, vp]; L.oa_k_paged_attention.restype = C.c_int
+    i64, f64, table, moves = C.c_int64, C.c_double, C.POINTER(OaPageTable), C.POINTER(OaPageMove)
+    L.oa_host_rotary_freqs.argtypes = [i32, f64, i32, f64, f64, f64, i32, vp, C.POINTER(f32)]; L.oa_host_rotary_freqs.restype = C.c_int
+    L.oa_k_rotary.argtypes = [vp, i64, vp, i64, vp, i32, i32, i32, i32, i32, vp, f32, i32, i32, vp]; L.oa_k_rotary.restype = C.c_int
+    L.oa_k_rotary_cache.argtypes = [vp, i64, vp, vp, i64, vp, i64, vp, i32, vp, vp, i32, i32, i32, i32, i32, i32, vp, f32, vp, vp]; L.oa_k_rotary_cache.restype = C.c_int
+    L.oa_host_cache_grow.argtypes = [table, i32, i32]; L.oa_host_cache_grow.restype = C.c_int
+    L.oa_host_cache_free.argtypes = [table, vp, i32]; L.oa_host_cache_free.restype = C.c_int
+    L.oa_host_cache_fork.argtypes = [table, i32, vp, i32, moves, i32, C.POINTER(i32)]; L.oa_host_cache_fork.restype = C.c_int
+    L.oa_host_cache_compact.argtypes = [table, moves, i32, C.POINTER(i32)]; L.oa_host_cache_compact.restype = C.c_int
+    L.oa_k_cache_copy.argtypes = [vp, i32, i32, i32, i32, i32, moves, i32, vp]; L.oa_k_cache_copy.restype = C.c_int
+    L.oa_k_prefix_attention.argtypes = [vp, i64, vp, i64, vp, i32, vp, i32, vp, vp, i32, vp, i32, vp, i32, i32, i32, i32, f32, vp, vp]; L.oa_k_prefix_attention.restype = C.c_int
     L.oa_host_apply_chat_template.argtypes = [C.c_char_p, C.POINTER(OaMsg), i32, vp, i32, C.POINTER(i32)]; L.oa_host_apply_chat_template.restype = C.c_int
     L.oa_host_bpe_encode.argtypes = [C.c_char_p, C.c_char_p, i32, vp, i32, C.POINTER(i32)]; L.oa_host_bpe_encode.restype = C.c_int
     L.oa_host_bpe_decode.argtypes = [C.c_char_p, vp, i32, vp, i32, C.POINTER(i32)]; L.oa_host_bpe_decode.restype = C.c_int

@@ -20,46 +20,13 @@
 #include "model.hpp"
 #include "hybrid_kernels.hpp"
 #include "pinned_pool.hpp"
+#include "call_scratch.hpp"
 #include "sk_consumers.cuh"
 #include "tokenizer.hpp"
 
 using namespace oa;
 
 namespace {
-// Scratch of one call (partials, plans, tables) comes from a stream-ordered pool of this library's own, one per device, made at the first use:
-// cudaMalloc and cudaFree stop the whole device and cost 0.1 ms to several ms a call, more than most kernels here (paged attention of 6 x 3000
-// tokens: 10 us of kernels in a call of 0.7 ms and more; from the pool 0.05 ms).  An allocation is ordered on the call's stream, so calls on
-// several streams and threads never share a block; what the pool keeps between calls is bounded, the rest goes back to the device when a call
-// synchronises.
-constexpr uint64_t SCRATCH_KEEP_BYTES = 64ull << 20;
-cudaMemPool_t scratch_pool() {
-    static std::mutex mu;
-    static cudaMemPool_t pools[64] = {};         // by device; nothing here may throw through the C boundary
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
-    std::lock_guard<std::mutex> lk(mu);
-    cudaMemPool_t& pool = pools[dev];
-    if (!pool) {
-        cudaMemPoolProps props{};
-        props.allocType = cudaMemAllocationTypePinned; props.handleTypes = cudaMemHandleTypeNone;
-        props.location.type = cudaMemLocationTypeDevice; props.location.id = dev;
-        if (cudaMemPoolCreate(&pool, &props) != cudaSuccess) { pool = nullptr; return nullptr; }
-        uint64_t keep = SCRATCH_KEEP_BYTES;
-        cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep);
-    }
-    return pool;
-}
-struct DevBuf {
-    void* p = nullptr;
-    cudaStream_t s;
-    DevBuf(size_t n, cudaStream_t stream) : s(stream) {
-        if (n == 0) return;
-        cudaMemPool_t pool = scratch_pool();
-        if (!pool || cudaMallocFromPoolAsync(&p, n, pool, s) != cudaSuccess) p = nullptr;
-    }
-    DevBuf(const DevBuf&) = delete;
-    ~DevBuf() { if (p) cudaFreeAsync(p, s); }
-};
 // Pinned host memory for the arrays of one call: a copy from pageable memory is pushed or staged by the calling thread (6 to 10 us for 8 to 16 KB, against 2
 // to 3 from pinned memory in a loop of its own; six conversations of 1750 tokens: 40.3 -> 38.3 us a call).  A buffer belongs to one call at a time and goes
 // back once the call's stream has passed its copy.  (A kernel that reads the pinned buffer instead of a copy was slower than either for such sizes: it and

@@ -30,6 +30,7 @@ namespace oa {
 
 static thread_local std::string g_last_error;
 static int fail(int code, const std::string& msg) { g_last_error = msg; return code; }
+int call_failed(int code, const char* why) { try { g_last_error = why; } catch (const std::exception&) { } return code; }
 
 // selects `dev` on the calling thread for a scope and restores what was current before (the CUDA current device is per thread)
 struct CallerDevice {
