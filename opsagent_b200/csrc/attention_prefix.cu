@@ -8,8 +8,9 @@
 //  prefix_part_kernel: all rows of a prefix against its keys is a product of matrices (128 conversations of 4 heads a group: 512 rows a key/value head), so it
 //    runs on tcgen05: 128 rows (as many tokens' heads of a group as fit) x 128 keys a unit, S = Q K^T in two TMEM buffers, P over S's own columns as the second
 //    product's operand, O in TMEM.  One row a thread, reference maximum raised (and O rescaled) only where a score passes it by 2^8.
-//  own_part_kernel: a sequence's own keys have only its few heads as rows: streamed through shared memory by TMA and multiplied on the 16-row warp path,
-//    a page's 64 tokens over four warps, like decode attention over a whole context (attention.cu).
+//  own_part_kernel: a sequence's own keys have only its few heads as rows: streamed through shared memory by TMA and multiplied on the warp path of 16 x 8 x 16
+//    products, a page's 64 tokens over four warps, with tokens and channels as the 16 rows and the heads as the 8 columns (nothing of a product is empty for 8 heads a
+//    group, and O takes D / 4 registers a lane).
 //
 // Both deal their units (128 keys of a row tile; a page of a sequence and key/value head) out contiguously, the same number to every CTA: unit u is CTA
 // floor(((u + 1) G - 1) / total)'s, so what parts an item has, and in which slot (CTA + item) each of them lies, follows from lengths alone.  The plan is made on the
@@ -21,27 +22,27 @@
 #include "kernels.hpp"
 #include "cache_ops.hpp"
 
+
 namespace oa {
 
-constexpr int PRE_THREADS = 192;        // producer, issuer, four softmax warps
-constexpr int OWN_THREADS = 160;        // four consumer warps, producer
+constexpr int PRE_SOFTMAX = 256;        // threads of a row tile: two softmax warpgroups
+constexpr int OWN_CONSUMERS = 256, OWN_THREADS = OWN_CONSUMERS + 64;        // eight consumer warps, producer, a warp that brings an item's states together
 constexpr int KEY_TILE = 128;
+constexpr int JOIN_THREADS = 256;
 
 OA_DEVINL float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }        // nothing seen: any reference will do, 2^(-inf - 0) is 0
-OA_DEVINL int own_pages(int len) { return len > CACHE_PAGE ? (len + CACHE_PAGE - 1) / CACHE_PAGE : 1; }       // an empty sequence has a page without tokens: somebody writes its row
+OA_DEVINL int pages_of(int len) { return (len + CACHE_PAGE - 1) / CACHE_PAGE; }
 // of a grid's CTAs the first min(grid, total) have units, each at least one: an item's parts are those of consecutive CTAs
 OA_DEVINL int64_t busy_ctas(int64_t grid, int64_t total) { return total < grid ? (total > 0 ? total : 1) : grid; }
-OA_DEVINL int64_t first_unit(int64_t cta, int64_t busy, int64_t total) { return cta < busy ? total * cta / busy : total; }
-OA_DEVINL int cta_of(int64_t unit, int64_t busy, int64_t total) { return (int)(((unit + 1) * busy - 1) / total); }
+OA_DEVINL int64_t quotient(int64_t a, int64_t b) { return (uint64_t)a >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b); }      // a >= 0, b > 0; a 64-bit division takes several times as long
+OA_DEVINL int64_t first_unit(int64_t cta, int64_t busy, int64_t total) { return cta < busy ? quotient(total * cta, busy) : total; }
+OA_DEVINL int cta_of(int64_t unit, int64_t busy, int64_t total) { return (int)quotient((unit + 1) * busy - 1, total); }
 OA_DEVINL void report(const PrefixAttnArgs& a) { if (a.status) *a.status = 400; }
 
-// What the prefixes' part looks like, the same in both kernels: run bounds that never fall, lengths that fit their tables
-struct Prefixes {
-    int row0[PREFIX_MAX], rows[PREFIX_MAX], len[PREFIX_MAX], tiles[PREFIX_MAX], key_tiles[PREFIX_MAX], item0[PREFIX_MAX];
-    int64_t unit0[PREFIX_MAX], units;
-};
-OA_DEVINL void read_prefixes(const PrefixAttnArgs& a, Prefixes& px, int tile_tokens, int lane) {      // one warp
-    int r0 = 0, r1 = 0, len = 0; bool wrong = false;
+// The runs of rows that share a prefix: bounds that never fall, lengths that fit their tables (0 where nobody sees it)
+OA_DEVINL void read_runs(const PrefixAttnArgs& a, int lane, int& row0, int& rows, int& len) {      // one warp, a lane a prefix
+    int r0 = 0, r1 = 0; bool wrong = false;
+    len = 0;
     if (lane < a.n_prefixes) {
         r0 = __ldcg(a.prefix_rows + lane); r1 = __ldcg(a.prefix_rows + lane + 1); len = __ldcg(a.prefix_lens + lane);
         wrong = r0 < 0 || r1 < r0 || r1 > a.n_seqs || len < 0 || len > (int64_t)a.max_prefix_pages * CACHE_PAGE;
@@ -49,121 +50,144 @@ OA_DEVINL void read_prefixes(const PrefixAttnArgs& a, Prefixes& px, int tile_tok
         len = (int)min((int64_t)max(len, 0), (int64_t)a.max_prefix_pages * CACHE_PAGE);
     }
     if (wrong) report(a);
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int below = __shfl_up_sync(0xffffffffu, r0, o); if (lane >= o) r0 = max(r0, below); }
+    for (int o = 1; o < a.n_prefixes; o <<= 1) { const int below = __shfl_up_sync(0xffffffffu, r0, o); if (lane >= o) r0 = max(r0, below); }
     r1 = max(r0, r1);
     const bool some = lane < a.n_prefixes && r1 > r0 && len > 0;
-    const int tiles = some ? (r1 - r0 + tile_tokens - 1) / tile_tokens : 0, key_tiles = some ? (len + KEY_TILE - 1) / KEY_TILE : 0;
-    int items = tiles * a.n_kv; int64_t units = (int64_t)items * key_tiles;
-    const int items_own = items; const int64_t units_own = units;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int i = __shfl_up_sync(0xffffffffu, items, o); const int64_t u = __shfl_up_sync(0xffffffffu, units, o);
-        if (lane >= o) { items += i; units += u; }
-    }
-    px.row0[lane] = r0; px.rows[lane] = some ? r1 - r0 : 0; px.len[lane] = len; px.tiles[lane] = tiles; px.key_tiles[lane] = key_tiles;
-    px.item0[lane] = items - items_own; px.unit0[lane] = units - units_own;
-    if (lane == 31) px.units = units;
+    row0 = r0; rows = some ? r1 - r0 : 0; len = some ? len : 0;
+}
+// What the prefixes' part looks like: a prefix's rows, tokens, row tiles and key tiles, and the pieces that its items (a row tile and a key/value head) are cut into along the keys
+struct PrefixPieces { int row0[PREFIX_MAX], rows[PREFIX_MAX], len[PREFIX_MAX], tiles[PREFIX_MAX], key_tiles[PREFIX_MAX], split[PREFIX_MAX], piece0[PREFIX_MAX], pieces; };
+OA_DEVINL void cut_prefixes(const PrefixAttnArgs& a, PrefixPieces& px, int lane) {      // one warp
+    int row0, rows, len;
+    read_runs(a, lane, row0, rows, len);
+    const int tile_tokens = KEY_TILE / (a.n_heads / a.n_kv), tiles = (rows + tile_tokens - 1) / tile_tokens, key_tiles = (len + KEY_TILE - 1) / KEY_TILE, items = tiles * a.n_kv;
+    // Pieces of at most `most` key tiles, as many as make the CTA with most work end first, where a piece costs what PIECE_COST tiles do besides its own; every lane weighs
+    // one number of them, up to 144 for the longest prefix.  No more pieces than CTAs and items together: the scratch has that many slots.
+    constexpr int PIECE_COST = 3;
+    const int longest = __reduce_max_sync(0xffffffffu, key_tiles), all_items = __reduce_add_sync(0xffffffffu, items);
+    const int want = lane < 16 ? lane + 1 : 16 + 8 * (lane - 15), most = (max(longest, 1) + want - 1) / want;
+    int64_t n = 0;
+    for (int p = 0; p < a.n_prefixes; ++p) n += (int64_t)__shfl_sync(0xffffffffu, items, p) * ((__shfl_sync(0xffffffffu, key_tiles, p) + most - 1) / most);
+    const int64_t cost = quotient(n + a.pre_ctas - 1, a.pre_ctas) * (most + PIECE_COST);
+    const unsigned key = n > (int64_t)a.pre_ctas + all_items ? 0xffffffffu : (unsigned)min(cost, (int64_t)0x3ffffff) << 5 | (unsigned)lane;
+    const unsigned best = __reduce_min_sync(0xffffffffu, key);
+    const int cut = __shfl_sync(0xffffffffu, most, (int)(best & 31u)), split = (key_tiles + cut - 1) / cut;
+    int pieces = items * split;
+    const int mine = pieces;
+    for (int o = 1; o < a.n_prefixes; o <<= 1) { const int below = __shfl_up_sync(0xffffffffu, pieces, o); if (lane >= o) pieces += below; }
+    px.row0[lane] = row0; px.rows[lane] = rows; px.len[lane] = len; px.tiles[lane] = tiles; px.key_tiles[lane] = key_tiles; px.split[lane] = split;
+    px.piece0[lane] = pieces - mine;
+    if (lane == a.n_prefixes - 1) px.pieces = pieces;
 }
 
 // =============================================================================================
 // the prefixes' part
 // =============================================================================================
-template <int D>
+template <int D, int SLOTS>          // SLOTS: tiles of 128 keys or values in the ring
 struct PreCfg {
     static constexpr int HALVES = D / 64;
     static constexpr int HALF_BYTES = 128 * 128;                 // 128 rows x 64 bf16 columns under the 128-byte swizzle
-    static constexpr int TILE_BYTES = HALVES * HALF_BYTES;       // Q, and K or V of 128 keys
-    static constexpr int NK = 2, NV = 1;
-    static constexpr int SMEM_BYTES = (1 + NK + NV) * TILE_BYTES + 256;
-    static constexpr uint32_t O_COL = 256;                       // TMEM: S[0] and P[0] at 0, S[1] and P[1] at 128, O at 256
+    static constexpr int TILE_BYTES = HALVES * HALF_BYTES;       // Q of a row tile, and K or V of 128 keys
+    static constexpr int THREADS = 64 + PRE_SOFTMAX;             // producer, issuer, softmax warps
+    static constexpr int XCH_BYTES = (2 * 2 + 2) * 128 * 4;      // a row's two maxima of a tile, [tile parity][warpgroup][row], and its two sums of a piece
+    static constexpr int SMEM_BYTES = (1 + SLOTS) * TILE_BYTES + 256 + XCH_BYTES;
+    static constexpr uint32_t O_COL = 256;                       // TMEM: S and P of the tiles in turn at 0 and 128, O at 256
 };
-struct PreSeg { int g, kvh, tile, k0, k1, item; };
-// the segment that begins at unit u, at most `left` units long; g0: a prefix at or before it
-OA_DEVINL PreSeg pre_segment(const Prefixes& px, int64_t u, int64_t left, int g0, int n_prefixes) {
-    PreSeg s; s.g = g0;
-    while (s.g + 1 < n_prefixes && u >= px.unit0[s.g + 1]) ++s.g;          // prefixes without units begin where the next one does
-    const int64_t rem = u - px.unit0[s.g];
-    const int kt = px.key_tiles[s.g], i = (int)(rem / kt);
-    s.k0 = (int)(rem - (int64_t)i * kt); s.k1 = (int)min((int64_t)kt, s.k0 + left);
-    s.kvh = i / px.tiles[s.g]; s.tile = i - s.kvh * px.tiles[s.g]; s.item = px.item0[s.g] + i;
+struct PrePiece { int g, kvh, tile, k0, k1; };
+OA_DEVINL PrePiece pre_piece(const PrefixPieces& px, int piece, int n_prefixes) {
+    PrePiece s; s.g = 0;
+    while (s.g + 1 < n_prefixes && piece >= px.piece0[s.g + 1]) ++s.g;     // prefixes without pieces begin where the next one does
+    const int rem = piece - px.piece0[s.g], split = px.split[s.g], i = rem / split, k = rem - i * split;
+    s.k0 = (int)quotient((int64_t)px.key_tiles[s.g] * k, split); s.k1 = (int)quotient((int64_t)px.key_tiles[s.g] * (k + 1), split);
+    s.kvh = i / px.tiles[s.g]; s.tile = i - s.kvh * px.tiles[s.g];
     return s;
 }
 
-template <int D>
-__global__ void __launch_bounds__(PRE_THREADS, 1) prefix_part_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ PrefixAttnArgs a) {
-    using Cfg = PreCfg<D>;
-    constexpr int HALVES = Cfg::HALVES, NK = Cfg::NK, NV = Cfg::NV;
+template <int D, int SLOTS>
+__global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ PrefixAttnArgs a) {
+    using Cfg = PreCfg<D, SLOTS>;
+    constexpr int HALVES = Cfg::HALVES;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* q_s = smem;
-    uint8_t* k_s = q_s + Cfg::TILE_BYTES;
-    uint8_t* v_s = k_s + NK * Cfg::TILE_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + NV * Cfg::TILE_BYTES);
-    uint64_t *q_full = bars, *s_full = bars + 1, *p_full = bars + 3, *t_full = bars + 5, *o_full = bars + 6;
-    uint64_t *k_full = bars + 7, *k_empty = k_full + NK, *v_full = k_empty + NK, *v_empty = v_full + NV;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + NV);
-    __shared__ Prefixes px;
+    uint8_t* kv_s = q_s + Cfg::TILE_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(kv_s + SLOTS * Cfg::TILE_BYTES);
+    uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_full = bars + 4, *t_full = bars + 6, *o_full = bars + 7, *full = bars + 8, *empty = full + SLOTS;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(empty + SLOTS);
+    float* xch = reinterpret_cast<float*>(kv_s + SLOTS * Cfg::TILE_BYTES + 256);
+    __shared__ PrefixPieces px;
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int grp = a.n_heads / a.n_kv, tile_tokens = KEY_TILE / grp;
+    const int grp = a.n_heads / a.n_kv, tile_tokens = KEY_TILE / grp;      // tokens of a row tile
     if (warp == 0 && lane == 0) {
-        tma_prefetch_desc(&tm_kv);
-        mbar_init(q_full, 4); mbar_init(t_full, 1); mbar_init(o_full, 1);
-        for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
-        for (int i = 0; i < NK; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
-        for (int i = 0; i < NV; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
+        tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_kv);
+        mbar_init(q_full, 1); mbar_init(q_empty, 1); mbar_init(t_full, 1); mbar_init(o_full, 1);
+        for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], PRE_SOFTMAX / 32); }
+        for (int i = 0; i < SLOTS; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         fence_barrier_init();
     }
     if (warp == 1) tmem_alloc<512>(tmem_slot);
     griddep_wait();
     griddep_launch();            // behind the wait: what the own part's kernel reads ahead of its own wait was written by kernels that have ended
-    if (warp == 0) read_prefixes(a, px, tile_tokens, lane);
-    for (int i = blockIdx.x * PRE_THREADS + threadIdx.x; i < a.own_ctas; i += gridDim.x * PRE_THREADS) a.counters[i] = 0;
+    if (warp == 0) cut_prefixes(a, px, lane);
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-    const int64_t total = px.units, busy = busy_ctas(gridDim.x, total);
-    const int64_t u_begin = first_unit(blockIdx.x, busy, total), u_end = first_unit(blockIdx.x + 1, busy, total);
-
+    // Keys and values share one ring in the order of their products: K_0, then K_(j+1) and V_j
     if (warp == 0) {
-        uint32_t n = 0;                                          // tiles loaded
-        int g = 0;
-        for (int64_t u = u_begin; u < u_end;) {
-            const PreSeg sg = pre_segment(px, u, u_end - u, g, a.n_prefixes); g = sg.g; u += sg.k1 - sg.k0;
-            const int32_t* bt = a.prefix_tables + (size_t)sg.g * a.max_prefix_pages;
-            const int pages = (px.len[sg.g] + CACHE_PAGE - 1) / CACHE_PAGE;
-            for (int kt = sg.k0; kt < sg.k1; ++kt, ++n) {
-                const int two = 2 * kt + 1 < pages;              // a missing second page is not loaded: its scores are masked, its values set to zero
-                int page[2] = {bt[2 * kt], two ? bt[2 * kt + 1] : 0};
+        uint32_t n = 0, seg = 0;                                 // tiles and pieces loaded
+        for (int piece = blockIdx.x; piece < px.pieces; piece += gridDim.x, ++seg) {
+            const PrePiece sg = pre_piece(px, piece, a.n_prefixes);
+            mbar_wait(q_empty, (seg & 1) ^ 1);
+            if (elect_one()) {                                   // rows of a tile: tokens, and the group's heads within; tokens behind the last sequence are zeros, other prefixes' are not looked at
+                mbar_expect_tx(q_full, HALVES * tile_tokens * grp * 128);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) if (page[i] < 0 || page[i] >= a.num_pages) { if (lane == 0) report(a); page[i] = 0; }
+                for (int h = 0; h < HALVES; ++h)
+                    tma_load_3d(q_s + h * Cfg::HALF_BYTES, &tm_q, q_full, h * 64, sg.kvh * grp, px.row0[sg.g] + sg.tile * tile_tokens, kEvictNormal);
+            }
+            __syncwarp();
+            const int32_t* bt = a.prefix_tables + (size_t)sg.g * a.max_prefix_pages;
+            const int pages = pages_of(px.len[sg.g]);
+            int page[2] = {0, 0}, prev[2] = {0, 0};
+            for (int j = 0; j <= sg.k1 - sg.k0; ++j) {
+                const int kt = sg.k0 + j;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    prev[i] = page[i];
+                    page[i] = kt < sg.k1 && 2 * kt + i < pages ? bt[2 * kt + i] : 0;
+                    if (page[i] < 0 || page[i] >= a.num_pages) { if (lane == 0) report(a); page[i] = 0; }
+                }
 #pragma unroll
                 for (int v = 0; v < 2; ++v) {
-                    const uint32_t slot = n % (v ? NV : NK), turn = n / (v ? NV : NK);
-                    uint64_t* full = (v ? v_full : k_full) + slot;
-                    mbar_wait((v ? v_empty : k_empty) + slot, (turn & 1) ^ 1);
+                    const int t = kt - v;                        // K of this tile, V of the one before
+                    if (t < sg.k0 || t >= sg.k1) continue;
+                    const uint32_t slot = n % SLOTS;
+                    mbar_wait(&empty[slot], ((n / SLOTS) & 1) ^ 1);
                     if (elect_one()) {
-                        uint8_t* dst = (v ? v_s : k_s) + slot * Cfg::TILE_BYTES;
-                        mbar_expect_tx(full, two ? Cfg::TILE_BYTES : Cfg::TILE_BYTES / 2);
+                        const int two = 2 * t + 1 < pages;       // a missing second page is not loaded: its scores are masked, its values set to zero
+                        uint8_t* dst = kv_s + slot * Cfg::TILE_BYTES;
+                        mbar_expect_tx(&full[slot], two ? Cfg::TILE_BYTES : Cfg::TILE_BYTES / 2);
                         for (int i = 0; i <= two; ++i) {
-                            const int row = ((v ? a.num_pages : 0) + page[i]) * a.n_kv * CACHE_PAGE + sg.kvh * CACHE_PAGE;
+                            const int row = ((v ? a.num_pages + prev[i] : page[i]) * a.n_kv + sg.kvh) * CACHE_PAGE;
 #pragma unroll
-                            for (int h = 0; h < HALVES; ++h) tma_load_2d(dst + h * Cfg::HALF_BYTES + i * 8192, &tm_kv, full, h * 64, row, kEvictLast);
+                            for (int h = 0; h < HALVES; ++h) tma_load_2d(dst + h * Cfg::HALF_BYTES + i * 8192, &tm_kv, &full[slot], h * 64, row, kEvictLast);
                         }
                     }
                     __syncwarp();
+                    ++n;
                 }
             }
         }
     } else if (warp == 1) {
         // the whole warp walks the loop, an elected lane issues: descriptors stay in uniform registers
         constexpr uint32_t idesc_s = umma_idesc_bf16(128, KEY_TILE), idesc_o = umma_idesc_bf16_bmn(128, D);
-        const uint64_t q_desc = umma_desc_sw128(smem_u32(q_s)), k_desc = umma_desc_sw128(smem_u32(k_s));
-        const uint64_t v_desc = umma_desc_sw128_mn(smem_u32(v_s), (uint32_t)Cfg::HALF_BYTES, 1024u);
-        auto issue_s = [&](uint32_t n) {
-            const uint32_t slot = n % NK;
-            mbar_wait(&k_full[slot], (n / NK) & 1);
+        const uint64_t q_desc = umma_desc_sw128(smem_u32(q_s)), k_desc = umma_desc_sw128(smem_u32(kv_s));
+        const uint64_t v_desc = umma_desc_sw128_mn(smem_u32(kv_s), (uint32_t)Cfg::HALF_BYTES, 1024u);
+        uint32_t n = 0, r = 0, seg = 0;                          // tiles, tiles of the ring, pieces
+        auto issue_s = [&](uint32_t n, bool last) {
+            const uint32_t slot = r % SLOTS;
+            mbar_wait(&full[slot], (r / SLOTS) & 1);
+            ++r;
             tcgen05_fence_after();
             if (elect_one()) {
                 const uint64_t b = k_desc + (uint64_t)(slot * (Cfg::TILE_BYTES >> 4));
@@ -173,22 +197,24 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) prefix_part_kernel(const __gri
                     umma_bf16(tmem_base + (n & 1) * 128, q_desc + off, b + off, idesc_s, ks > 0 ? 1u : 0u);
                 }
                 umma_commit(&s_full[n & 1]);
-                umma_commit(&k_empty[slot]);
+                umma_commit(&empty[slot]);
+                if (last) umma_commit(q_empty);
             }
             __syncwarp();
         };
-        uint32_t n = 0, seg = 0; int g = 0;
-        for (int64_t u = u_begin; u < u_end; ++seg) {
-            const PreSeg sg = pre_segment(px, u, u_end - u, g, a.n_prefixes); g = sg.g; u += sg.k1 - sg.k0;
+        // products of one thread are carried out in the order of their issue: S of a tile goes over scores whose P a product ahead of it reads
+        for (int piece = blockIdx.x; piece < px.pieces; piece += gridDim.x, ++seg) {
+            const PrePiece sg = pre_piece(px, piece, a.n_prefixes);
             const int tiles = sg.k1 - sg.k0;
             mbar_wait(q_full, seg & 1);
             tcgen05_fence_after();
-            issue_s(n);
+            issue_s(n, tiles == 1);
             for (int j = 0; j < tiles; ++j, ++n) {
-                if (j + 1 < tiles) issue_s(n + 1);               // S of the next tile goes over the scores of the one before, whose P the tensor core has been told to read
-                const uint32_t slot = n % NV;
+                if (j + 1 < tiles) issue_s(n + 1, j + 2 == tiles);               // the next tile's scores under this one's softmax
+                const uint32_t slot = r % SLOTS;
                 mbar_wait(&p_full[n & 1], (n >> 1) & 1);
-                mbar_wait(&v_full[slot], (n / NV) & 1);
+                mbar_wait(&full[slot], (r / SLOTS) & 1);
+                ++r;
                 tcgen05_fence_after();
                 if (elect_one()) {
                     const uint64_t b = v_desc + (uint64_t)(slot * (Cfg::TILE_BYTES >> 4));
@@ -196,79 +222,74 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) prefix_part_kernel(const __gri
                     for (int ks = 0; ks < KEY_TILE / 16; ++ks)
                         umma_bf16_ta(tmem_base + Cfg::O_COL, tmem_base + (n & 1) * 128 + ks * 8, b + (uint64_t)(ks * (2048 >> 4)), idesc_o, (j > 0 || ks > 0) ? 1u : 0u);
                     umma_commit(j + 1 < tiles ? t_full : o_full);
-                    umma_commit(&v_empty[slot]);
+                    umma_commit(&empty[slot]);
                 }
                 __syncwarp();
             }
         }
     } else {
-        const int quarter = warp & 3, row = quarter * 32 + lane;                 // this thread's row, TMEM lane of the same number
-        const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+        // Warps w and w + 4 of the eight hold the same 32 rows and half of every tile's keys each (and of O's columns where those are rescaled or written), 64 scores a thread
+        const int quarter = warp & 3, row = quarter * 32 + lane, wg = (warp - 2) >> 2;
+        const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16, o_addr = tmem_base + lane_addr + Cfg::O_COL;
+        auto meet = [] { asm volatile("bar.sync 2, %0;" ::"n"(PRE_SOFTMAX) : "memory"); };
         constexpr float kRaise = 8.0f;                                           // log2 units a score may pass the reference by
-        uint32_t n = 0, seg = 0, rescaled0 = 0; int g = 0;                       // rescaled0: completions of t_full before this segment
-        for (int64_t u = u_begin; u < u_end; ++seg) {
-            const PreSeg sg = pre_segment(px, u, u_end - u, g, a.n_prefixes); g = sg.g; u += sg.k1 - sg.k0;
+        constexpr int KEYS = KEY_TILE / 2, COLS = D / 2;
+        uint32_t n = 0, r = 0, seg = 0, landed = 0;                              // landed: completions of t_full before this piece
+        for (int piece = blockIdx.x; piece < px.pieces; piece += gridDim.x, ++seg) {
+            const PrePiece sg = pre_piece(px, piece, a.n_prefixes);
+            const bool live = row < tile_tokens * grp && sg.tile * tile_tokens + row / grp < px.rows[sg.g];
             const int tiles = sg.k1 - sg.k0, len = px.len[sg.g];
-            const int token = sg.tile * tile_tokens + row / grp;
-            const bool live = row < tile_tokens * grp && token < px.rows[sg.g];
-            {   // Q: a row of 128 or 256 bytes a thread, zeros where there is none
-                const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(px.row0[sg.g] + (live ? token : 0)) * a.ldq +
-                                                                  (int64_t)(sg.kvh * grp + (live ? row % grp : 0)) * D);
-#pragma unroll
-                for (int c = 0; c < D / 8; ++c) {
-                    const uint4 w = live ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-                    *reinterpret_cast<uint4*>(q_s + (c >> 3) * Cfg::HALF_BYTES + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = w;
-                }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(q_full);
-            }
             float m_ref = -INFINITY, l_run = 0.f;
             for (int j = 0; j < tiles; ++j, ++n) {
                 const uint32_t sb = n & 1;
-                const int valid = len - (sg.k0 + j) * KEY_TILE;                 // keys of this tile
+                const int valid = len - (sg.k0 + j) * KEY_TILE;                  // keys of this tile
                 mbar_wait(&s_full[sb], (n >> 1) & 1);
                 tcgen05_fence_after();
-                uint32_t v[4][32];
+                uint32_t v[2][32];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(tmem_base + lane_addr + sb * 128 + c * 32, v[c]);
+                for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(tmem_base + lane_addr + sb * 128 + wg * KEYS + c * 32, v[c]);
                 tmem_ld_wait();
                 if (valid < KEY_TILE) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 2; ++c)
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) if (c * 32 + i >= valid) v[c][i] = 0xff800000u;
-                    // values behind the end may be anything, and 0 x inf is not 0
-                    const uint32_t slot = n % NV;
-                    mbar_wait(&v_full[slot], (n / NV) & 1);
+                        for (int i = 0; i < 32; ++i) if (wg * KEYS + c * 32 + i >= valid) v[c][i] = 0xff800000u;
+                    // values behind the end may be anything, and 0 x inf is not 0; only the last tile of a prefix ends early, and its V is the last of the piece's 2 tiles
+                    const uint32_t at = r + 2 * tiles - 1, slot = at % SLOTS;
+                    mbar_wait(&full[slot], (at / SLOTS) & 1);
                     if (row >= valid) {
 #pragma unroll
-                        for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-                            for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(v_s + slot * Cfg::TILE_BYTES + h * Cfg::HALF_BYTES + row * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        for (int c = 0; c < D / 16; ++c) {
+                            const int chunk = wg * (D / 16) + c;
+                            *reinterpret_cast<uint4*>(kv_s + slot * Cfg::TILE_BYTES + (chunk >> 3) * Cfg::HALF_BYTES + row * 128 + (chunk & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        }
                     }
                     fence_proxy_async();
                 }
                 float mraw = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) mraw = fmaxf(mraw, __uint_as_float(v[c][i]));
+                float* maxima = xch + (n & 1) * 256;
+                maxima[wg * 128 + row] = mraw;
+                meet();                                                          // and both halves of S are in registers: P may go over them
+                mraw = fmaxf(mraw, maxima[(wg ^ 1) * 128 + row]);
                 const float mx = mraw * a.scale_log2e;
-                const bool raise = mx > m_ref + kRaise;
+                const bool raise = mx > m_ref + kRaise;                          // the same in both warps of a row
                 if (__any_sync(0xffffffffu, raise)) {
                     if (j > 0) {
-                        mbar_wait(t_full, (rescaled0 + j - 1) & 1);             // O has the products of the tile before; this tile's are not issued before p_full
+                        mbar_wait(t_full, (landed + j - 1) & 1);                 // O has the products of the tile before; this tile's are not issued before p_full
                         tcgen05_fence_after();
                         const float alpha = raise ? exp2f(m_ref - mx) : 1.0f;
 #pragma unroll 1
-                        for (int c = 0; c < D; c += 32) {
-                            uint32_t o[32];
-                            tmem_ld_32x32b_x32(tmem_base + lane_addr + Cfg::O_COL + c, o);
+                        for (int c = 0; c < COLS; c += 16) {                     // the scores stay in registers meanwhile
+                            uint32_t o[16];
+                            tmem_ld_32x32b_x16(o_addr + wg * COLS + c, o);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                            tmem_st_32x32b_x32(tmem_base + lane_addr + Cfg::O_COL + c, o);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            tmem_st_32x32b_x16(o_addr + wg * COLS + c, o);
                         }
                         l_run *= alpha;
                     }
@@ -277,16 +298,15 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) prefix_part_kernel(const __gri
                 const float neg_ref = -finite_or_zero(m_ref);
                 uint64_t sum = 0;
 #pragma unroll
-                for (int c = 0; c < 4; c += 2) {
-                    uint32_t w[32];
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t w[16];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float x = ex2_approx(fmaf(__uint_as_float(v[c + (i >> 4)][(2 * i) & 31]), a.scale_log2e, neg_ref));
-                        const float y = ex2_approx(fmaf(__uint_as_float(v[c + (i >> 4)][(2 * i + 1) & 31]), a.scale_log2e, neg_ref));
+                    for (int i = 0; i < 16; ++i) {
+                        const float x = ex2_approx(fmaf(__uint_as_float(v[c][2 * i]), a.scale_log2e, neg_ref)), y = ex2_approx(fmaf(__uint_as_float(v[c][2 * i + 1]), a.scale_log2e, neg_ref));
                         sum = add_f32x2(sum, pack_f32x2(x, y));
                         w[i] = pack_bf16x2(x, y);
                     }
-                    tmem_st_32x32b_x32(tmem_base + lane_addr + sb * 128 + c * 16, w);
+                    tmem_st_32x32b_x16(tmem_base + lane_addr + sb * 128 + wg * 32 + c * 16, w);
                 }
                 tmem_st_wait();
                 tcgen05_fence_before();
@@ -295,23 +315,24 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) prefix_part_kernel(const __gri
                 float even, odd; unpack_f32x2(sum, even, odd);
                 l_run += even + odd;
             }
-            rescaled0 += tiles - 1;
+            landed += tiles - 1; r += 2 * tiles;
+            xch[512 + wg * 128 + row] = l_run;                                   // the piece's before was read ahead of this one's tiles' barriers
             mbar_wait(o_full, seg & 1);
             tcgen05_fence_after();
-            const int64_t slot = (int64_t)blockIdx.x + sg.item;
-            float* po = a.pre_o + slot * (KEY_TILE * D) + row * 4;               // [D / 4][128 rows][4]: a warp's rows lie next to each other
+            float* po = a.pre_o + (int64_t)piece * (KEY_TILE * D) + row * 4;     // [D / 4][128 rows][4]: a warp's rows lie next to each other
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
+            for (int c = wg * COLS; c < (wg + 1) * COLS; c += 32) {
                 uint32_t o[32];
-                tmem_ld_32x32b_x32(tmem_base + lane_addr + Cfg::O_COL + c, o);
+                tmem_ld_32x32b_x32(o_addr + c, o);
                 tmem_ld_wait();
                 if (live)
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
                         *reinterpret_cast<float4*>(po + (c + i) / 4 * (KEY_TILE * 4)) = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
             }
-            if (live) *reinterpret_cast<float2*>(a.pre_ml + (slot * KEY_TILE + row) * 2) = make_float2(m_ref, l_run);
             tcgen05_fence_before();
+            meet();
+            if (live && wg == 0) *reinterpret_cast<float2*>(a.pre_ml + ((int64_t)piece * KEY_TILE + row) * 2) = make_float2(m_ref, l_run + xch[512 + 128 + row]);
         }
     }
     __syncthreads();
@@ -321,157 +342,135 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) prefix_part_kernel(const __gri
 // =============================================================================================
 // the sequences' own part, and the join
 // =============================================================================================
-template <int D, bool WIDE>              // WIDE: 9 to 16 heads a group, both halves of the 16-row tile
+template <int D, bool WIDE, int STAGES>  // WIDE: 9 to 16 heads a group, two blocks of 8 columns; STAGES: pages in the ring
 struct OwnCfg {
     static constexpr int HALVES = D / 64;
     static constexpr int TILE_BYTES = CACHE_PAGE * 128;
     static constexpr int KV_BYTES = HALVES * TILE_BYTES;
     static constexpr int STAGE_BYTES = 2 * KV_BYTES;
-    static constexpr int STAGES = D == 128 ? 2 : 4;
-    static constexpr int ROWS = WIDE ? 16 : 8;
-    static constexpr int REGS = D / 4 * (WIDE ? 2 : 1);                          // output values of a lane
+    static constexpr int BLOCKS = WIDE ? 2 : 1, ROWS = 8 * BLOCKS, REGS = D / 4 * BLOCKS;      // output values of a lane and its twin's in the other half
+    static constexpr int Q_PITCH = D * 2 + 16, Q_BYTES = ROWS * Q_PITCH;         // queries of an item, rows 16 bytes further apart than they are long: no bank conflicts
     static constexpr int SCRATCH_BYTES = 4 * REGS * 32 * 4 + 4 * ROWS * 2 * 4;
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + SCRATCH_BYTES + 2 * STAGES * 8;
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 2 * Q_BYTES + SCRATCH_BYTES + (2 * STAGES + 6) * 8;
 };
 template <int D>
 OA_DEVINL uint32_t own_off(int r, int d) { return (uint32_t)((d >> 6) * (CACHE_PAGE * 128) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4)); }
 
-// position in the list of (sequence, key/value head) items
+// transpose of an 8 x 8 matrix of 16-bit values, a row in four lanes
+OA_DEVINL uint32_t transpose_8x8(uint32_t v) { uint32_t r; asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v)); return r; }
+// untiled copy of 16-byte pieces from global to shared memory, completing on an mbarrier
+OA_DEVINL void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(smem_dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+// Position in the list of (sequence, key/value head) items.  An item's units are one for the item itself (its states have to meet, which takes about as long as a page)
+// and one for each of its pages: those of its prefix first, where prefixes are not a kernel of their own, then its own
+struct Runs { int row0[PREFIX_MAX], rows[PREFIX_MAX], len[PREFIX_MAX]; };
 struct OwnAt {
-    int seq, kvh, len, pages; int64_t unit0;                                     // unit0: first unit of this item
-    OA_DEVINL void read(const PrefixAttnArgs& a) {
-        len = __ldcg(a.own_lens + seq);
-        len = (int)min((int64_t)max(len, 0), (int64_t)a.max_own_pages * CACHE_PAGE);
-        pages = own_pages(len);
+    int seq, kvh, len, run, pre_len, pre_pages, pages, next_len; int64_t unit0;              // next_len: the next sequence's, read ahead (ahead()); unit0: first unit of this item
+    OA_DEVINL static int length(const PrefixAttnArgs& a, int seq) { return seq < a.n_seqs ? __ldcg(a.own_lens + seq) : 0; }
+    OA_DEVINL void take(const PrefixAttnArgs& a, const Runs& runs, int raw) {
+        len = (int)min((int64_t)max(raw, 0), (int64_t)a.max_own_pages * CACHE_PAGE);
+        run = pre_len = pre_pages = 0;
+        if (a.pre_ctas == 0)
+            for (int r = 0; r < a.n_prefixes; ++r)
+                if (seq >= runs.row0[r] && seq < runs.row0[r] + runs.rows[r]) { run = r; pre_len = runs.len[r]; pre_pages = pages_of(pre_len); }
+        pages = pre_pages + pages_of(len);
     }
-    OA_DEVINL void next(const PrefixAttnArgs& a) {
-        unit0 += pages;
-        if (++kvh == a.n_kv) { kvh = 0; if (++seq < a.n_seqs) read(a); }
+    OA_DEVINL OwnAt& ahead(const PrefixAttnArgs& a) { next_len = length(a, seq + 1); return *this; }
+    OA_DEVINL void next(const PrefixAttnArgs& a, const Runs& runs) {
+        unit0 += 1 + pages;
+        if (++kvh == a.n_kv) { kvh = 0; ++seq; take(a, runs, next_len); ahead(a); }
+    }
+    OA_DEVINL int tokens(int c) const { return c < pre_pages ? pre_len - c * CACHE_PAGE : len - (c - pre_pages) * CACHE_PAGE; }      // from page c on, in its part
+    OA_DEVINL const int32_t* entry(const PrefixAttnArgs& a, int c) const {
+        return c < pre_pages ? a.prefix_tables + (int64_t)run * a.max_prefix_pages + c : a.own_tables + (int64_t)seq * a.max_own_pages + (c - pre_pages);
     }
 };
 
-// joins the parts of one item's rows and writes them; one warp, RP rows at a time, 32 / RP lanes a row
-template <int D, int RP>
-OA_DEVINL void join_item(const PrefixAttnArgs& a, const Prefixes& px, const OwnAt& at, int c_first, int c_last, int grp, int tile_tokens, int lane) {
-    constexpr int LANES = 32 / RP, ITERS = D / 4 / LANES;
-    const int part = lane / RP;
-    // the row's prefix, if it has one
-    int mine = -1;
-    { const bool in = px.rows[lane] > 0 && at.seq >= px.row0[lane] && at.seq < px.row0[lane] + px.rows[lane]; const unsigned who = __ballot_sync(0xffffffffu, in); if (who) mine = __ffs(who) - 1; }
-    int n_pre = 0, first_row = 0; int64_t pre_slot = 0;
-    if (mine >= 0) {
-        const int token = at.seq - px.row0[mine], tile = token / tile_tokens, i = at.kvh * px.tiles[mine] + tile;
-        const int64_t u = px.unit0[mine] + (int64_t)i * px.key_tiles[mine];
-        const int64_t busy = busy_ctas(a.pre_ctas, px.units);
-        const int c0 = cta_of(u, busy, px.units), c1 = cta_of(u + px.key_tiles[mine] - 1, busy, px.units);
-        n_pre = c1 - c0 + 1; pre_slot = (int64_t)c0 + px.item0[mine] + i; first_row = (token - tile * tile_tokens) * grp;
-    }
-    const int n_own = c_last - c_first + 1;
-    const int64_t own_slot = (int64_t)c_first + (int64_t)at.seq * a.n_kv + at.kvh;
-    const bool nothing = at.len == 0 && mine < 0;
-    for (int r0 = 0; r0 < grp; r0 += RP) {
-        const int row = r0 + lane % RP, r = row < grp ? row : grp - 1;          // lanes beyond the group go along for the shuffles
-        const float2* pre_ml = reinterpret_cast<const float2*>(a.pre_ml) + pre_slot * KEY_TILE + first_row + r;
-        const float2* own_ml = reinterpret_cast<const float2*>(a.own_ml) + own_slot * grp + r;
-        const float* pre_o = a.pre_o + pre_slot * (KEY_TILE * D) + (first_row + r) * 4 + part * (KEY_TILE * 4);
-        const float* own_o = a.own_o + own_slot * (grp * D) + r * 4 + part * (grp * 4);
-        float M = -INFINITY;
-        for (int i = part; i < n_pre; i += LANES) M = fmaxf(M, __ldcg(pre_ml + (int64_t)i * KEY_TILE).x);
-        for (int i = part; i < n_own; i += LANES) M = fmaxf(M, __ldcg(own_ml + (int64_t)i * grp).x);
-#pragma unroll
-        for (int o = RP; o < 32; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        M = finite_or_zero(M);
-        float l = 0.f; float4 acc[ITERS];
-#pragma unroll
-        for (int k = 0; k < ITERS; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto add = [&](float2 ml, const float* o, int step) {
-            const float f = exp2f(ml.x - M);
-            l += f * ml.y;
-#pragma unroll
-            for (int k = 0; k < ITERS; ++k) {
-                const float4 x = __ldcg(reinterpret_cast<const float4*>(o + (int64_t)k * LANES * step));
-                acc[k].x += f * x.x; acc[k].y += f * x.y; acc[k].z += f * x.z; acc[k].w += f * x.w;
-            }
-        };
-#pragma unroll 2
-        for (int i = 0; i < n_pre; ++i) add(__ldcg(pre_ml + (int64_t)i * KEY_TILE), pre_o + (int64_t)i * (KEY_TILE * D), KEY_TILE * 4);
-#pragma unroll 2
-        for (int i = 0; i < n_own; ++i) add(__ldcg(own_ml + (int64_t)i * grp), own_o + (int64_t)i * (grp * D), grp * 4);
-        if (row < grp) {
-            const float inv = nothing ? 0.f : 1.0f / l;
-            uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)at.seq * a.ldo + (int64_t)(at.kvh * grp + row) * D + part * 4;
-#pragma unroll
-            for (int k = 0; k < ITERS; ++k)
-                *reinterpret_cast<uint2*>(out + k * LANES * 4) = make_uint2(pack_bf16x2(acc[k].x * inv, acc[k].y * inv), pack_bf16x2(acc[k].z * inv, acc[k].w * inv));
-        }
-    }
-}
-
-template <int D, bool WIDE>
-__global__ void __launch_bounds__(OWN_THREADS, 2) own_part_kernel(const __grid_constant__ CUtensorMap tm_page, const __grid_constant__ CUtensorMap tm_part, const __grid_constant__ PrefixAttnArgs a) {
-    using Cfg = OwnCfg<D, WIDE>;
-    constexpr int STAGES = Cfg::STAGES, KS = D / 16, NT = D / 8, ROWS = Cfg::ROWS, VALS = WIDE ? 4 : 2;
+template <int D, bool WIDE, int STAGES>
+__global__ void __maxnreg__(WIDE ? 168 : 104) own_part_kernel(const __grid_constant__ CUtensorMap tm_page, const __grid_constant__ CUtensorMap tm_part, const __grid_constant__ PrefixAttnArgs a) {
+    using Cfg = OwnCfg<D, WIDE, STAGES>;
+    constexpr int KS = D / 16, ROWS = Cfg::ROWS, NB = Cfg::BLOCKS;
     extern __shared__ __align__(1024) uint8_t smem[];
-    float* scratch = reinterpret_cast<float*>(smem + STAGES * Cfg::STAGE_BYTES);             // [4 warps][values][32 lanes]
-    float* ml_s = scratch + 4 * Cfg::REGS * 32;                                              // [4 warps][rows][2]
+    uint8_t* q_s = smem + STAGES * Cfg::STAGE_BYTES;                                         // [2 items][rows]
+    float* scratch = reinterpret_cast<float*>(q_s + 2 * Cfg::Q_BYTES);                       // [4 quarters][values][32 lanes]
+    float* ml_s = scratch + 4 * Cfg::REGS * 32;                                              // [4 quarters][rows][2]
     uint64_t* full_bar = reinterpret_cast<uint64_t*>(ml_s + 4 * ROWS * 2);
-    uint64_t* empty_bar = full_bar + STAGES;
-    __shared__ Prefixes px;
+    uint64_t *empty_bar = full_bar + STAGES, *q_full = empty_bar + STAGES, *q_empty = q_full + 2, *states_full = q_empty + 2, *states_empty = states_full + 1;
+    __shared__ Runs runs;
     __shared__ int64_t sums[OWN_THREADS / 32];
     __shared__ OwnAt start;
-    __shared__ int joins[2];                                                                 // whether this CTA came last for its first and its last item
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int grp = a.n_heads / a.n_kv, tile_tokens = KEY_TILE / grp;
-    if (threadIdx.x == 0) {
-        tma_prefetch_desc(&tm_page); tma_prefetch_desc(&tm_part);
-        for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 4); }
-        fence_barrier_init();
-    }
-    griddep_launch();
+    const int grp = a.n_heads / a.n_kv;
+    if (a.pre_ctas == 0) griddep_wait();
     // ---- the plan: everything read here was written before the prefixes' kernel let this one start ----
     const int per = (a.n_seqs + OWN_THREADS - 1) / OWN_THREADS, s0 = threadIdx.x * per, s1 = min(a.n_seqs, s0 + per);
-    int64_t pages = 0; bool wrong = false;
-    for (int s = s0; s < s1; ++s) {
-        const int len = __ldcg(a.own_lens + s);
+    const int first_len = OwnAt::length(a, s0);
+    if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tm_page); tma_prefetch_desc(&tm_part);
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], OWN_CONSUMERS / 32); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], OWN_CONSUMERS / 32); }
+        mbar_init(states_full, OWN_CONSUMERS / 32); mbar_init(states_empty, 1);
+        fence_barrier_init();
+    }
+    if (a.pre_ctas == 0) {
+        if (warp == 8) { int row0, rows, len; read_runs(a, lane, row0, rows, len); runs.row0[lane] = row0; runs.rows[lane] = rows; runs.len[lane] = len; }
+        __syncthreads();
+    }
+    OwnAt at;
+    int64_t units = 0; bool wrong = false;
+    for (at.seq = s0; at.seq < s1; ++at.seq) {
+        const int len = at.seq == s0 ? first_len : OwnAt::length(a, at.seq);
         wrong = wrong || len < 0 || len > (int64_t)a.max_own_pages * CACHE_PAGE;
-        pages += own_pages((int)min((int64_t)max(len, 0), (int64_t)a.max_own_pages * CACHE_PAGE));
+        at.take(a, runs, len);
+        units += 1 + at.pages;
     }
     if (wrong) report(a);
-    int64_t before = pages;
+    int64_t before = units;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int64_t x = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += x; }
     if (lane == 31) sums[warp] = before;
-    if (warp == 4) read_prefixes(a, px, tile_tokens, lane);
     __syncthreads();
-    before -= pages;
+    before -= units;
     int64_t total = 0;
 #pragma unroll
     for (int w = 0; w < OWN_THREADS / 32; ++w) { if (w < warp) before += sums[w]; total += sums[w]; }
     before *= a.n_kv; total *= a.n_kv;
     const int64_t busy = busy_ctas(gridDim.x, total), u_begin = first_unit(blockIdx.x, busy, total), u_end = first_unit(blockIdx.x + 1, busy, total);
-    if (u_begin < u_end && u_begin >= before && u_begin < before + pages * a.n_kv) {         // one thread
-        OwnAt at; at.seq = s0; at.unit0 = before;
-        for (at.read(a); u_begin >= at.unit0 + (int64_t)at.pages * a.n_kv;) { at.unit0 += (int64_t)at.pages * a.n_kv; ++at.seq; at.read(a); }
-        at.kvh = (int)((u_begin - at.unit0) / at.pages); at.unit0 += (int64_t)at.kvh * at.pages;
+    if (u_begin < u_end && u_begin >= before && u_begin < before + units * a.n_kv) {         // one thread
+        at.seq = s0; at.unit0 = before;
+        for (at.take(a, runs, first_len); u_begin >= at.unit0 + (int64_t)(1 + at.pages) * a.n_kv;) { at.unit0 += (int64_t)(1 + at.pages) * a.n_kv; ++at.seq; at.take(a, runs, OwnAt::length(a, at.seq)); }
+        at.kvh = (int)quotient(u_begin - at.unit0, 1 + at.pages); at.unit0 += (int64_t)at.kvh * (1 + at.pages);
         start = at;
     }
     __syncthreads();
-    if (u_begin >= u_end) { griddep_wait(); return; }
+    if (u_begin >= u_end) { griddep_launch(); griddep_wait(); return; }
 
-    if (warp == 4) {
+    if (warp == 8) {
         if (lane == 0) {
-            int s = 0; uint32_t ph = 0;
-            OwnAt at = start;
-            for (int64_t u = u_begin; u < u_end; at.next(a)) {
-                const int c0 = (int)(u - at.unit0), c1 = (int)min((int64_t)at.pages, u_end - at.unit0);
-                u = at.unit0 + c1;
-                const int32_t* bt = a.own_tables + (int64_t)at.seq * a.max_own_pages;
-                int page = at.len > 0 ? __ldcg(bt + c0) : 0;
+            int s = 0; uint32_t ph = 0, k = 0;
+            at = start;
+            at.ahead(a);
+            auto first_page = [&](int seq) { return seq < a.n_seqs ? __ldcg(a.own_tables + (int64_t)seq * a.max_own_pages) : 0; };
+            int page0 = first_page(at.seq), next_page0 = first_page(at.seq + 1), seq = at.seq;      // read ahead, like lengths
+            for (int64_t u = u_begin; u < u_end; at.next(a, runs), ++k) {
+                if (at.seq != seq) { page0 = next_page0; seq = at.seq; next_page0 = first_page(seq + 1); }
+                const int c0 = (int)max(u - at.unit0 - 1, (int64_t)0), c1 = (int)min((int64_t)at.pages, u_end - at.unit0 - 1);
+                u = at.unit0 + 1 + c1;
+                mbar_wait(&q_empty[k & 1], ((k >> 1) & 1) ^ 1);
+                if (c1 > c0) {
+                    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)at.seq * a.ldq + (int64_t)at.kvh * grp * D;
+                    mbar_expect_tx(&q_full[k & 1], grp * D * 2);
+                    for (int r = 0; r < grp; ++r) bulk_load(q_s + (k & 1) * Cfg::Q_BYTES + r * Cfg::Q_PITCH, q + r * D, D * 2, &q_full[k & 1]);
+                } else mbar_arrive(&q_full[k & 1]);
+                int page = c1 <= c0 ? 0 : c0 == 0 && at.pre_pages == 0 ? page0 : __ldcg(at.entry(a, c0));
                 for (int c = c0; c < c1; ++c) {
-                    const int next_page = c + 1 < c1 ? __ldcg(bt + c + 1) : 0;               // looked up while this one's slot is waited for
+                    const int next_page = c + 1 < c1 ? __ldcg(at.entry(a, c + 1)) : 0;       // looked up while this one's slot is waited for
+                    const int valid = min(CACHE_PAGE, at.tokens(c));
                     if (page < 0 || page >= a.num_pages) { report(a); page = 0; }
-                    const int valid = min(CACHE_PAGE, at.len - c * CACHE_PAGE);
                     mbar_wait(&empty_bar[s], ph ^ 1);
                     uint8_t* kdst = smem + s * Cfg::STAGE_BYTES;
                     uint8_t* vdst = kdst + Cfg::KV_BYTES;
@@ -483,7 +482,7 @@ __global__ void __launch_bounds__(OWN_THREADS, 2) own_part_kernel(const __grid_c
                             tma_load_2d(kdst + h * Cfg::TILE_BYTES, &tm_page, &full_bar[s], h * 64, krow, kEvictFirst);
                             tma_load_2d(vdst + h * Cfg::TILE_BYTES, &tm_page, &full_bar[s], h * 64, vrow, kEvictFirst);
                         }
-                    } else if (valid > 0) {                                                  // a page that ends early: pieces of 16 tokens
+                    } else {                                                                 // a page that ends early: pieces of 16 tokens
                         const int n = (valid + 15) / 16;
                         mbar_expect_tx(&full_bar[s], n * 2 * Cfg::HALVES * 16 * 128);
                         for (int i = 0; i < n; ++i)
@@ -492,79 +491,133 @@ __global__ void __launch_bounds__(OWN_THREADS, 2) own_part_kernel(const __grid_c
                                 tma_load_2d(kdst + h * Cfg::TILE_BYTES + i * 2048, &tm_part, &full_bar[s], h * 64, krow + i * 16, kEvictFirst);
                                 tma_load_2d(vdst + h * Cfg::TILE_BYTES + i * 2048, &tm_part, &full_bar[s], h * 64, vrow + i * 16, kEvictFirst);
                             }
-                    } else mbar_arrive(&full_bar[s]);
+                    }
                     page = next_page;
                     if (++s == STAGES) { s = 0; ph ^= 1; }
                 }
             }
         }
         __syncwarp();
+        griddep_launch();
+        griddep_wait();
+        return;
+    }
+    if (warp == 9) {
+        // An item's part: O and l of the four quarters under one maximum.  The part with an item's first unit goes to the item's own place, a later one (a CTA has at most one,
+        // its first) to the CTA's
+        at = start;
+        at.ahead(a);
+        const int g = lane >> 2, t = lane & 3;
+        uint32_t k = 0;
+        for (int64_t u = u_begin; u < u_end; at.next(a, runs), ++k) {
+            const int64_t end = at.unit0 + 1 + at.pages, item = (int64_t)at.seq * a.n_kv + at.kvh;
+            const bool first = at.unit0 >= u_begin, tokens = min(end, u_end) > max(u, at.unit0 + 1);
+            u = min(end, u_end);
+            if (lane == 0 && first) a.own_parts[item] = make_int2(blockIdx.x + 1, end <= u_end ? 0 : cta_of(end - 1, busy, total) - (int)blockIdx.x);      // for the join: later parts, from which CTA on
+            float* po = first ? a.own_o + item * grp * D : a.more_o + (int64_t)blockIdx.x * grp * D;
+            float2* ml = reinterpret_cast<float2*>(first ? a.own_ml + item * grp * 2 : a.more_ml + (int64_t)blockIdx.x * grp * 2);
+            mbar_wait(states_full, k & 1);
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int row = b * 8 + 2 * t + h;
+                    float2 st[4]; float m = -INFINITY, l = 0.f;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) { st[w] = *reinterpret_cast<const float2*>(ml_s + (w * ROWS + row) * 2); m = fmaxf(m, st[w].x); }
+                    const float ref = finite_or_zero(m);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) { st[w].x = ex2_approx(st[w].x - ref); l += st[w].x * st[w].y; }
+                    if (row >= grp) continue;
+                    if (g == 0) ml[row] = make_float2(m, tokens ? l : -1.0f);                // -1: a part without tokens
+#pragma unroll 4
+                    for (int r = 0; r < KS * 2; ++r) {                                       // channel block r / 2 and its upper or lower 8 channels
+                        const int i = r >> 1, up = r & 1, reg = (i / (KS / 2)) * (Cfg::REGS / 2) + (b * (KS / 2) + i % (KS / 2)) * 4 + 2 * up + h;
+                        float o = 0.f;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) o += st[w].x * scratch[(w * Cfg::REGS + reg) * 32 + lane];
+                        po[row * D + i * 16 + 8 * up + g] = o;                               // [heads][D]
+                    }
+                }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(states_empty);
+        }
+        griddep_launch();
         griddep_wait();
         return;
     }
 
-    const int g = lane >> 2, t = lane & 3;
-    int s = 0; uint32_t ph = 0; int n_items = 0;
+    // Warps w and w + 4 take the same 16 tokens of every page and half of the channels each: scores and probabilities twice, which costs less than states of eight warps that have
+    // to meet.  Tokens are the 16 rows of the first product and channels those of the second, heads the 8 columns of both: S^T = K Q^T, O^T = V^T P^T
+    constexpr int KH = KS / 2;
+    const int g = lane >> 2, t = lane & 3, quarter = warp & 3, half = warp >> 2;
+    int s = 0, n_items = 0; uint32_t ph = 0;
     {
-        OwnAt at = start;
-        for (int64_t u = u_begin; u < u_end; at.next(a), ++n_items) {
-            const int c0 = (int)(u - at.unit0), c1 = (int)min((int64_t)at.pages, u_end - at.unit0);
-            u = at.unit0 + c1;
-            uint32_t qa[KS][VALS];                                                           // rows = heads of the group, zeros beyond it
-            {
-                const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)at.seq * a.ldq + (int64_t)(at.kvh * grp + g) * D;
+        at = start;
+        at.ahead(a);
+        for (int64_t u = u_begin; u < u_end; at.next(a, runs), ++n_items) {
+            const int c0 = (int)max(u - at.unit0 - 1, (int64_t)0), c1 = (int)min((int64_t)at.pages, u_end - at.unit0 - 1);
+            u = at.unit0 + 1 + c1;
+            float oacc[NB][KH][4], m_run[NB][2], l_run[NB][2];                               // O^T: channels 16 i + g and + 8, heads 2 t and 2 t + 1; maxima and sums of these heads
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
+            for (int b = 0; b < NB; ++b) {
 #pragma unroll
-                    for (int v = 0; v < VALS; ++v) {                                         // v: columns + 8, then rows + 8
-                        const int up = WIDE ? v & 1 : 0, right = WIDE ? v >> 1 : v;
-                        qa[ks][v] = g + 8 * up < grp ? __ldcg(reinterpret_cast<const uint32_t*>(q + up * 8 * D + ks * 16 + right * 8 + 2 * t)) : 0u;
-                    }
+                for (int i = 0; i < KH; ++i) oacc[b][i][0] = oacc[b][i][1] = oacc[b][i][2] = oacc[b][i][3] = 0.f;
+                m_run[b][0] = m_run[b][1] = -INFINITY; l_run[b][0] = l_run[b][1] = 0.f;
             }
-            float oacc[NT][4];
-#pragma unroll
-            for (int j = 0; j < NT; ++j) { oacc[j][0] = oacc[j][1] = oacc[j][2] = oacc[j][3] = 0.f; }
-            float m_run[VALS / 2], l_run[VALS / 2];
-#pragma unroll
-            for (int h = 0; h < VALS / 2; ++h) { m_run[h] = -INFINITY; l_run[h] = 0.f; }
+            const uint32_t qbase = smem_u32(q_s + (n_items & 1) * Cfg::Q_BYTES) + (lane & 7) * Cfg::Q_PITCH + (lane >> 3) * 16;      // rows beyond the group hold anything: columns of no head
+            mbar_wait(&q_full[n_items & 1], (n_items >> 1) & 1);
             for (int c = c0; c < c1; ++c) {
+                const int valid = at.tokens(c) - quarter * 16;                               // tokens of this warp's quarter
                 mbar_wait(&full_bar[s], ph);
-                const int valid = at.len - c * CACHE_PAGE - warp * 16;                       // tokens of this warp's quarter
                 if (valid > 0) {
                     const uint32_t kbase = smem_u32(smem + s * Cfg::STAGE_BYTES), vbase = kbase + Cfg::KV_BYTES;
-                    float sacc[2][4];
+                    float sacc[NB][2][4];                                                    // even and odd steps apart: two chains of products
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) { sacc[j][0] = sacc[j][1] = sacc[j][2] = sacc[j][3] = 0.f; }
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sacc[b][0][e] = sacc[b][1][e] = 0.f;
                     {
-                        const int r = warp * 16 + ((lane >> 4) << 3) + (lane & 7), dsel = ((lane >> 3) & 1) << 3;
+                        const int r = quarter * 16 + (((lane >> 3) & 1) << 3) + (lane & 7), dsel = (lane >> 4) << 3;
 #pragma unroll
-                        for (int ks = 0; ks < KS; ++ks) {
-                            uint32_t b0, b1, b2, b3;
-                            ldmatrix_x4(kbase + own_off<D>(r, ks * 16 + dsel), b0, b1, b2, b3);
-                            const uint32_t a0 = qa[ks][0], a1 = WIDE ? qa[ks][1] : 0u, a2 = qa[ks][WIDE ? 2 : 1], a3 = WIDE ? qa[ks][VALS - 1] : 0u;
-                            mma_bf16_16816(sacc[0], a0, a1, a2, a3, b0, b1);
-                            mma_bf16_16816(sacc[1], a0, a1, a2, a3, b2, b3);
+                        for (int ks = 0; ks < KS; ks += 2) {
+                            uint32_t qf[NB][4], a0, a1, a2, a3;
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) ldmatrix_x4(qbase + b * 8 * Cfg::Q_PITCH + ks * 32, qf[b][0], qf[b][1], qf[b][2], qf[b][3]);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                ldmatrix_x4(kbase + own_off<D>(r, (ks + h) * 16 + dsel), a0, a1, a2, a3);
+#pragma unroll
+                                for (int b = 0; b < NB; ++b) mma_bf16_16816(sacc[b][h], a0, a1, a2, a3, qf[b][2 * h], qf[b][2 * h + 1]);
+                            }
                         }
                     }
-                    uint32_t pa[4] = {0u, 0u, 0u, 0u}; float alpha[VALS / 2];
+                    uint32_t pb[NB][2]; float alpha[NB][2];
+                    bool same = true;
 #pragma unroll
-                    for (int h = 0; h < VALS / 2; ++h) {                                     // rows g, and g + 8
-                        float sc[4];
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) sc[j * 2 + e] = j * 8 + 2 * t + e < valid ? sacc[j][2 * h + e] * a.scale_log2e : -INFINITY;
-                        float mx = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                        const float m_new = fmaxf(m_run[h], mx), ref = finite_or_zero(m_new);
-                        alpha[h] = exp2f(m_run[h] - ref);
+                    for (int b = 0; b < NB; ++b) {
                         float pr[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) pr[e] = exp2f(sc[e] - ref);
-                        l_run[h] = l_run[h] * alpha[h] + (pr[0] + pr[1] + pr[2] + pr[3]);
-                        m_run[h] = m_new;
-                        pa[h] = pack_bf16x2(pr[0], pr[1]); pa[2 + h] = pack_bf16x2(pr[2], pr[3]);
+                        for (int h = 0; h < 2; ++h) {
+                            const float lo = g < valid ? (sacc[b][0][h] + sacc[b][1][h]) * a.scale_log2e : -INFINITY;
+                            const float hi = g + 8 < valid ? (sacc[b][0][2 + h] + sacc[b][1][2 + h]) * a.scale_log2e : -INFINITY;
+                            float mx = fmaxf(lo, hi);
+#pragma unroll
+                            for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                            const float m_new = fmaxf(m_run[b][h], mx), ref = finite_or_zero(m_new);
+                            alpha[b][h] = ex2_approx(m_run[b][h] - ref);
+                            pr[h] = ex2_approx(lo - ref); pr[2 + h] = ex2_approx(hi - ref);
+                            l_run[b][h] = l_run[b][h] * alpha[b][h] + (pr[h] + pr[2 + h]);
+                            same = same && m_new == m_run[b][h];
+                            m_run[b][h] = m_new;
+                        }
+                        pb[b][0] = transpose_8x8(pack_bf16x2(pr[0], pr[1])); pb[b][1] = transpose_8x8(pack_bf16x2(pr[2], pr[3]));
+                    }
+                    if (!__all_sync(0xffffffffu, same)) {
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+#pragma unroll
+                            for (int i = 0; i < KH; ++i) { oacc[b][i][0] *= alpha[b][0]; oacc[b][i][1] *= alpha[b][1]; oacc[b][i][2] *= alpha[b][0]; oacc[b][i][3] *= alpha[b][1]; }
                     }
                     // values behind the end may be anything, and 0 x inf is not 0
                     uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
@@ -572,132 +625,205 @@ __global__ void __launch_bounds__(OWN_THREADS, 2) own_part_kernel(const __grid_c
                         keep0 = (2 * t < valid ? 0xffffu : 0u) | (2 * t + 1 < valid ? 0xffff0000u : 0u);
                         keep1 = (2 * t + 8 < valid ? 0xffffu : 0u) | (2 * t + 9 < valid ? 0xffff0000u : 0u);
                     }
-                    {
-                        const int r = warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7), dsel = (lane >> 4) << 3;
+                    const int r = quarter * 16 + ((lane >> 4) << 3) + (lane & 7), dsel = ((lane >> 3) & 1) << 3;
 #pragma unroll
-                        for (int j = 0; j < NT; j += 2) {
-                            uint32_t b0, b1, b2, b3;
-                            ldmatrix_x4_trans(vbase + own_off<D>(r, j * 8 + dsel), b0, b1, b2, b3);
+                    for (int i = 0; i < KH; ++i) {
+                        uint32_t a0, a1, a2, a3;
+                        ldmatrix_x4_trans(vbase + own_off<D>(r, (half * KH + i) * 16 + dsel), a0, a1, a2, a3);
 #pragma unroll
-                            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                                for (int e = 0; e < VALS; ++e) oacc[j + i][e] *= alpha[e >> 1];
-                            mma_bf16_16816(oacc[j], pa[0], pa[1], pa[2], pa[3], b0 & keep0, b1 & keep1);
-                            mma_bf16_16816(oacc[j + 1], pa[0], pa[1], pa[2], pa[3], b2 & keep0, b3 & keep1);
-                        }
+                        for (int b = 0; b < NB; ++b) mma_bf16_16816(oacc[b][i], a0 & keep0, a1 & keep0, a2 & keep1, a3 & keep1, pb[b][0], pb[b][1]);
                     }
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&empty_bar[s]);
                 if (++s == STAGES) { s = 0; ph ^= 1; }
             }
-            // ---- the four warps' states meet: each warp adds up a quarter of the columns ----
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_empty[n_items & 1]);
+            // the four quarters' states, for the warp that brings them together while this one goes on
+            mbar_wait(states_empty, (n_items & 1) ^ 1);
+            float* mine = scratch + (quarter * Cfg::REGS + half * (Cfg::REGS / 2)) * 32 + lane;          // value [half][b][i][e]
 #pragma unroll
-            for (int h = 0; h < VALS / 2; ++h) {
-                l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
-                l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
-                if (t == 0) { ml_s[(warp * ROWS + g + 8 * h) * 2] = m_run[h]; ml_s[(warp * ROWS + g + 8 * h) * 2 + 1] = l_run[h]; }
-            }
+            for (int b = 0; b < NB; ++b) {
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+                for (int h = 0; h < 2; ++h) {
+                    float l = l_run[b][h];
 #pragma unroll
-                for (int e = 0; e < VALS; ++e) scratch[(warp * Cfg::REGS + j * VALS + e) * 32 + lane] = oacc[j][e];
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            const int64_t slot = (int64_t)blockIdx.x + (int64_t)at.seq * a.n_kv + at.kvh;
-#pragma unroll
-            for (int h = 0; h < VALS / 2; ++h) {
-                const int row = g + 8 * h;
-                float f[4], m = -INFINITY, l = 0.f;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) { f[w] = ml_s[(w * ROWS + row) * 2]; m = fmaxf(m, f[w]); }
-                const float ref = finite_or_zero(m);
-#pragma unroll
-                for (int w = 0; w < 4; ++w) { f[w] = exp2f(f[w] - ref); l += f[w] * ml_s[(w * ROWS + row) * 2 + 1]; }
-                if (row >= grp) continue;
-                float* po = a.own_o + slot * (grp * D) + row * 4;                            // [D / 4][heads][4]
-#pragma unroll
-                for (int j = 0; j < NT / 4; ++j) {
-                    const int jj = warp * (NT / 4) + j, col = jj * 8 + 2 * t;
-                    float o[2];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        o[e] = 0.f;
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) o[e] += f[w] * scratch[(w * Cfg::REGS + jj * VALS + 2 * h + e) * 32 + lane];
-                    }
-                    *reinterpret_cast<float2*>(po + (col >> 2) * (grp * 4) + (col & 3)) = make_float2(o[0], o[1]);
+                    for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+                    if (half == 0 && g == 0) *reinterpret_cast<float2*>(ml_s + (quarter * ROWS + b * 8 + 2 * t + h) * 2) = make_float2(m_run[b][h], l);
                 }
-                if (warp == 0 && t == 0) *reinterpret_cast<float2*>(a.own_ml + (slot * grp + row) * 2) = make_float2(m, l);
+#pragma unroll
+                for (int i = 0; i < KH; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mine[((b * KH + i) * 4 + e) * 32] = oacc[b][i][e];
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");                                   // scratch is free for the next item
+            __syncwarp();
+            if (lane == 0) mbar_arrive(states_full);
         }
     }
 
-    // ---- the join.  Items that lie in this CTA alone are its own; of one cut between CTAs (at most the first and the last here) the CTA that comes last joins all parts ----
-    griddep_wait();                                                                          // the prefixes' parts are there, and the counters are zero
-    fence_acq_rel_gpu();
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    if (threadIdx.x == 0) {
-        OwnAt at = start;
-        for (int k = 0; k < n_items; ++k, at.next(a)) {
-            if (k > 0 && k + 1 < n_items) continue;
-            const int c0 = cta_of(at.unit0, busy, total), c1 = cta_of(at.unit0 + at.pages - 1, busy, total);
-            bool last = true;
-            if (c0 != c1) {
-                last = atomicAdd(a.counters + c0, 1) == c1 - c0;
-                if (last) fence_acq_rel_gpu();
-            }
-            joins[k > 0] = last;
+    griddep_launch();                            // not before: the next kernels' CTAs would crowd onto the SMs that are done first
+    griddep_wait();                              // the join waits for this kernel alone
+}
+
+// =============================================================================================
+// the join
+// =============================================================================================
+// One warp an item (or one of SPLIT pieces of its columns), RP rows at a time, 32 / RP lanes a row.  One pass over the parts, 16 loads of 16 bytes of eight of them in flight per
+// lane; what is summed up follows a maximum that rises from batch to batch.  A kernel of its own: at the end of own_part_kernel, whose CTAs have from 2 to 20 items each, the same
+// sums took 3 to 11 us, and a CTA that came last for an item had to be found by a counter.
+template <int D, int RP>
+__global__ void __launch_bounds__(JOIN_THREADS) join_parts_kernel(const __grid_constant__ PrefixAttnArgs a) {
+    constexpr int SPLIT = D * RP / 256 > 1 ? D * RP / 256 : 1, LANES = 32 / RP, ITERS = D / 4 / LANES / SPLIT, MP = 8;
+    const int lane = threadIdx.x & 31, grp = a.n_heads / a.n_kv, tile_tokens = KEY_TILE / grp;
+    const int64_t task = (int64_t)blockIdx.x * (JOIN_THREADS / 32) + (threadIdx.x >> 5), item = task / SPLIT;
+    const int seq = (int)(item / a.n_kv), kvh = (int)(item - (int64_t)seq * a.n_kv), part = (int)(task % SPLIT) * (D / 4 / SPLIT) + lane / RP;
+    griddep_launch();
+    int n_pre = 0, first_row = 0; int64_t pre_slot = 0;
+    if (a.pre_ctas > 0) {                        // the row's prefix, if it has one: from the call's arguments, while the parts are being made
+        __shared__ PrefixPieces px;
+        if (threadIdx.x < 32) cut_prefixes(a, px, lane);
+        __syncthreads();
+        const unsigned who = __ballot_sync(0xffffffffu, px.rows[lane] > 0 && seq >= px.row0[lane] && seq < px.row0[lane] + px.rows[lane]);
+        if (who) {
+            const int run = __ffs(who) - 1, token = seq - px.row0[run], tile = token / tile_tokens;
+            n_pre = px.split[run]; first_row = (token - tile * tile_tokens) * grp;
+            pre_slot = (int64_t)px.piece0[run] + (int64_t)(kvh * px.tiles[run] + tile) * n_pre;
         }
     }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    OwnAt at = start;
-    for (int k = 0; k < n_items; ++k, at.next(a)) {
-        if ((k & 3) != warp || (k == 0 && !joins[0]) || (k > 0 && k + 1 == n_items && !joins[1])) continue;
-        const int c0 = cta_of(at.unit0, busy, total), c1 = cta_of(at.unit0 + at.pages - 1, busy, total);
-        if (grp > 4) join_item<D, 8>(a, px, at, c0, c1, grp, tile_tokens, lane);
-        else if (grp > 2) join_item<D, 4>(a, px, at, c0, c1, grp, tile_tokens, lane);
-        else join_item<D, 2>(a, px, at, c0, c1, grp, tile_tokens, lane);
+    griddep_wait();
+    if (seq >= a.n_seqs) return;
+    const int2 later = __ldcg(a.own_parts + item);
+    const int n = n_pre + 1;                     // the prefix's parts and the first own one: where they lie is known; later own ones follow
+    for (int r0 = 0; r0 < grp; r0 += RP) {
+        const int row = r0 + lane % RP, r = row < grp ? row : grp - 1;          // lanes beyond the group go along
+        const float2* pre_ml = reinterpret_cast<const float2*>(a.pre_ml) + pre_slot * KEY_TILE + first_row + r;
+        const float2* own_ml = reinterpret_cast<const float2*>(a.own_ml) + item * grp + r;
+        const float2* more_ml = reinterpret_cast<const float2*>(a.more_ml) + (int64_t)later.x * grp + r;
+        const float* pre_o = a.pre_o + pre_slot * (KEY_TILE * D) + (first_row + r) * 4 + part * (KEY_TILE * 4);
+        const float* own_o = a.own_o + (item * grp + r) * D + part * 4;
+        const float* more_o = a.more_o + ((int64_t)later.x * grp + r) * D + part * 4;
+        float M = -INFINITY, l = 0.f; float4 acc[ITERS]; bool some = false;
+#pragma unroll
+        for (int k = 0; k < ITERS; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        int i0 = 0;
+        do {
+            float2 ml[MP]; float4 o[MP][ITERS];
+#pragma unroll
+            for (int p = 0; p < MP; ++p) {
+                const int i = i0 + p;
+                ml[p] = make_float2(-INFINITY, -1.f);
+                if (i >= n && i >= n + later.y) continue;
+                const float2* m = i < n_pre ? pre_ml + (int64_t)i * KEY_TILE : i < n ? own_ml : more_ml + (int64_t)(i - n) * grp;
+                const float* src = i < n_pre ? pre_o + (int64_t)i * (KEY_TILE * D) : i < n ? own_o : more_o + (int64_t)(i - n) * (grp * D);
+                const int step = i < n_pre ? KEY_TILE * 4 * LANES : 4 * LANES;
+                ml[p] = __ldcg(m);
+#pragma unroll
+                for (int k = 0; k < ITERS; ++k) o[p][k] = __ldcg(reinterpret_cast<const float4*>(src + k * step));
+            }
+            float m = M;
+#pragma unroll
+            for (int p = 0; p < MP; ++p) m = fmaxf(m, ml[p].x);
+            const float ref = finite_or_zero(m), f0 = ex2_approx(M - ref);
+            M = m; l *= f0;
+#pragma unroll
+            for (int k = 0; k < ITERS; ++k) { acc[k].x *= f0; acc[k].y *= f0; acc[k].z *= f0; acc[k].w *= f0; }
+#pragma unroll
+            for (int p = 0; p < MP; ++p) {
+                if (ml[p].y < 0.f) continue;                                     // a part without tokens
+                const float f = ex2_approx(ml[p].x - ref);
+                l += f * ml[p].y; some = true;
+#pragma unroll
+                for (int k = 0; k < ITERS; ++k) { acc[k].x += f * o[p][k].x; acc[k].y += f * o[p][k].y; acc[k].z += f * o[p][k].z; acc[k].w += f * o[p][k].w; }
+            }
+            i0 += MP;
+        } while (i0 < n + later.y);
+        if (row < grp) {
+            const float inv = some ? 1.0f / l : 0.f;
+            uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)seq * a.ldo + (int64_t)(kvh * grp + row) * D + part * 4;
+#pragma unroll
+            for (int k = 0; k < ITERS; ++k)
+                *reinterpret_cast<uint2*>(out + k * LANES * 4) = make_uint2(pack_bf16x2(acc[k].x * inv, acc[k].y * inv), pack_bf16x2(acc[k].z * inv, acc[k].w * inv));
+        }
     }
 }
 
 // =============================================================================================
 // host
 // =============================================================================================
+constexpr int PREFIX_LONG_UNITS = 8, PREFIX_INLINE_ROWS = 4, PREFIX_INLINE_UNITS = 4;
 PrefixAttnPlan prefix_attn_plan(int n_seqs, int n_heads, int n_kv, int head_dim, int n_prefixes, int max_prefix_pages, int max_own_pages, int sms) {
     PrefixAttnPlan p{};
-    const int grp = n_heads / n_kv, tile_tokens = KEY_TILE / grp;
-    const int64_t items = n_prefixes > 0 ? ((int64_t)n_seqs / tile_tokens + n_prefixes) * n_kv : 0;                // no more row tiles than that, however rows fall on prefixes
-    const int64_t units = items * ((max_prefix_pages + 1) / 2), own_units = (int64_t)n_seqs * n_kv * max_own_pages;
-    p.pre_ctas = (int)(units < 1 ? 1 : units < sms ? units : sms);
-    p.own_ctas = (int)(own_units < 2 * sms ? own_units : 2 * sms);
-    p.pre_slots = (size_t)(items + p.pre_ctas); p.own_slots = (size_t)((int64_t)n_seqs * n_kv + p.own_ctas);
+    const int grp = n_heads / n_kv;
+    const int tile_tokens = KEY_TILE / grp;
+    const int64_t work = ((int64_t)n_seqs + tile_tokens - 1) / tile_tokens * n_kv * ((max_prefix_pages + 1) / 2);       // units, if one prefix has all rows
+    const bool apart = n_prefixes > 0 && !(n_seqs <= PREFIX_INLINE_ROWS && (int64_t)n_seqs * n_kv * max_prefix_pages <= PREFIX_INLINE_UNITS * (int64_t)sms);
+    const int64_t items = apart ? ((int64_t)n_seqs / tile_tokens + n_prefixes) * n_kv : 0;                              // no more row tiles than that, however rows fall on prefixes
+    const int64_t units = items * ((max_prefix_pages + 1) / 2), own_units = (int64_t)n_seqs * n_kv * (1 + (int64_t)max_own_pages + (apart ? 0 : max_prefix_pages));
+    p.pre_ctas = (int)(units < sms ? units : sms);                                                                      // 0: prefixes are read with the sequences' own parts
+    p.own_ctas = (int)(own_units < sms ? own_units : sms);
+    p.long_prefix = work >= PREFIX_LONG_UNITS * (int64_t)sms;
+    p.pre_slots = (size_t)(items + p.pre_ctas);
     auto take = [&](size_t bytes) { const size_t at = p.bytes; p.bytes += (bytes + 255) & ~size_t(255); return at; };
     p.pre_o = take(p.pre_slots * KEY_TILE * head_dim * 4); p.pre_ml = take(p.pre_slots * KEY_TILE * 8);
-    p.own_o = take(p.own_slots * grp * head_dim * 4); p.own_ml = take(p.own_slots * grp * 8);
-    p.counters = take((size_t)p.own_ctas * 4);
+    const size_t own_items = (size_t)n_seqs * n_kv;
+    p.own_o = take(own_items * grp * head_dim * 4); p.own_ml = take(own_items * grp * 8); p.own_parts = take(own_items * 8);
+    p.more_o = take((size_t)p.own_ctas * grp * head_dim * 4); p.more_ml = take((size_t)p.own_ctas * grp * 8);
     return p;
 }
 
-template <int D, bool WIDE>
+// The first two kernels' CTAs share SMs: both ask for the whole carve-out, or an SM would have to be empty before it takes the other kernel's (2 us between the kernels)
+template <typename K>
+static cudaError_t raise_smem(K kern, int bytes, bool (&done)[16]) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev >= 0 && dev < 16 && done[dev])) return e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    return e == cudaSuccess ? ensure_dynamic_smem(kern, bytes, done) : e;
+}
+template <int D, bool WIDE, int STAGES>
 static cudaError_t launch_own(const CUtensorMap* tm_page, const CUtensorMap* tm_part, const PrefixAttnArgs& a, cudaStream_t s) {
-    auto kern = own_part_kernel<D, WIDE>;
+    auto kern = own_part_kernel<D, WIDE, STAGES>;
     static bool attr_done[16] = {};
-    { const cudaError_t e = ensure_dynamic_smem(kern, OwnCfg<D, WIDE>::SMEM_BYTES, attr_done); if (e != cudaSuccess) return e; }
-    return launch_k(kern, dim3(a.own_ctas), dim3(OWN_THREADS), OwnCfg<D, WIDE>::SMEM_BYTES, s, *tm_page, *tm_part, a);
+    { const cudaError_t e = raise_smem(kern, OwnCfg<D, WIDE, STAGES>::SMEM_BYTES, attr_done); if (e != cudaSuccess) return e; }
+    return launch_k(kern, dim3(a.own_ctas), dim3(OWN_THREADS), OwnCfg<D, WIDE, STAGES>::SMEM_BYTES, s, *tm_page, *tm_part, a);
+}
+template <int D, int SLOTS>
+static cudaError_t launch_prefixes(const CUtensorMap* tm_q, const CUtensorMap* tm_page, const PrefixAttnArgs& a, cudaStream_t s) {
+    auto kern = prefix_part_kernel<D, SLOTS>;
+    static bool attr_done[16] = {};
+    { const cudaError_t e = raise_smem(kern, PreCfg<D, SLOTS>::SMEM_BYTES, attr_done); if (e != cudaSuccess) return e; }
+    return launch_k(kern, dim3(a.pre_ctas), dim3(PreCfg<D, SLOTS>::THREADS), PreCfg<D, SLOTS>::SMEM_BYTES, s, *tm_q, *tm_page, a);
+}
+template <int D, int RP>
+static cudaError_t launch_join(const PrefixAttnArgs& a, cudaStream_t s) {
+    const int64_t tasks = (int64_t)a.n_seqs * a.n_kv * (D * RP / 256 > 1 ? D * RP / 256 : 1);
+    return launch_k(join_parts_kernel<D, RP>, dim3((unsigned)((tasks + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32))), dim3(JOIN_THREADS), 0, s, a);
 }
 template <int D>
-static cudaError_t launch_both(const CUtensorMap* tm_page, const CUtensorMap* tm_part, const PrefixAttnArgs& a, cudaStream_t s) {
-    auto kern = prefix_part_kernel<D>;
-    static bool attr_done[16] = {};
-    { const cudaError_t e = ensure_dynamic_smem(kern, PreCfg<D>::SMEM_BYTES, attr_done); if (e != cudaSuccess) return e; }
-    const cudaError_t e = launch_k(kern, dim3(a.pre_ctas), dim3(PRE_THREADS), PreCfg<D>::SMEM_BYTES, s, *tm_page, a);
-    if (e != cudaSuccess) return e;
-    return a.n_heads / a.n_kv > 8 ? launch_own<D, true>(tm_page, tm_part, a, s) : launch_own<D, false>(tm_page, tm_part, a, s);
+static cudaError_t launch_all(const CUtensorMap* tm_q, const CUtensorMap* tm_page, const CUtensorMap* tm_part, bool long_prefix, const PrefixAttnArgs& a, cudaStream_t s) {
+    const int grp = a.n_heads / a.n_kv;
+    cudaError_t e = cudaSuccess;
+    // An SM's shared memory goes to both kernels: long prefixes take three tiles of the first's ring and leave two pages to the second's, others two and three (heads of 64: 4 and 5)
+    constexpr int RING = D == 128 ? 2 : 4, PAGES = D == 128 ? 3 : 5;
+    bool done = false;
+    if constexpr (D == 128) {
+        if (long_prefix && a.pre_ctas > 0) {
+            e = launch_prefixes<D, 3>(tm_q, tm_page, a, s);
+            if (e == cudaSuccess && grp <= 8) { e = launch_own<D, false, 2>(tm_page, tm_part, a, s); done = true; }
+            else if (e == cudaSuccess) { e = launch_own<D, true, PAGES>(tm_page, tm_part, a, s); done = true; }
+        }
+    }
+    if (!done && e == cudaSuccess) {
+        if (a.pre_ctas > 0) e = launch_prefixes<D, RING>(tm_q, tm_page, a, s);
+        if (e == cudaSuccess) e = grp > 8 ? launch_own<D, true, PAGES>(tm_page, tm_part, a, s) : launch_own<D, false, PAGES>(tm_page, tm_part, a, s);
+    }
+    if (e == cudaSuccess) e = grp > 4 ? launch_join<D, 8>(a, s) : grp > 2 ? launch_join<D, 4>(a, s) : launch_join<D, 2>(a, s);
+    return e;
 }
-cudaError_t launch_prefix_attention(const CUtensorMap* tm_page, const CUtensorMap* tm_part, int head_dim, const PrefixAttnArgs& a, cudaStream_t s) {
-    if (head_dim == 128) return launch_both<128>(tm_page, tm_part, a, s);
-    if (head_dim == 64) return launch_both<64>(tm_page, tm_part, a, s);
+cudaError_t launch_prefix_attention(const CUtensorMap* tm_q, const CUtensorMap* tm_page, const CUtensorMap* tm_part, int head_dim, bool long_prefix, const PrefixAttnArgs& a, cudaStream_t s) {
+    if (head_dim == 128) return launch_all<128>(tm_q, tm_page, tm_part, long_prefix, a, s);
+    if (head_dim == 64) return launch_all<64>(tm_q, tm_page, tm_part, long_prefix, a, s);
     return cudaErrorInvalidValue;
 }
 
