@@ -27,8 +27,8 @@ namespace oa {
 
 constexpr int PRE_SOFTMAX = 256;        // threads of a row tile: two softmax warpgroups
 constexpr int OWN_CONSUMERS = 256, OWN_THREADS = OWN_CONSUMERS + 64;        // eight consumer warps, producer, a warp that brings an item's states together
-constexpr int KEY_TILE = 128;
-constexpr int JOIN_THREADS = 256;
+constexpr int ROW_TILE = 128;          // rows of a prefix's products
+constexpr int JOIN_THREADS = 128;
 
 OA_DEVINL float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }        // nothing seen: any reference will do, 2^(-inf - 0) is 0
 OA_DEVINL int pages_of(int len) { return (len + CACHE_PAGE - 1) / CACHE_PAGE; }
@@ -60,15 +60,14 @@ struct PrefixPieces { int row0[PREFIX_MAX], rows[PREFIX_MAX], len[PREFIX_MAX], t
 OA_DEVINL void cut_prefixes(const PrefixAttnArgs& a, PrefixPieces& px, int lane) {      // one warp
     int row0, rows, len;
     read_runs(a, lane, row0, rows, len);
-    const int tile_tokens = KEY_TILE / (a.n_heads / a.n_kv), tiles = (rows + tile_tokens - 1) / tile_tokens, key_tiles = (len + KEY_TILE - 1) / KEY_TILE, items = tiles * a.n_kv;
-    // Pieces of at most `most` key tiles, as many as make the CTA with most work end first, where a piece costs what PIECE_COST tiles do besides its own; every lane weighs
+    const int tile_tokens = ROW_TILE / (a.n_heads / a.n_kv), tiles = (rows + tile_tokens - 1) / tile_tokens, key_tiles = (len + a.key_tile - 1) / a.key_tile, items = tiles * a.n_kv;
+    // Pieces of at most `most` key tiles, as many as make the CTA with most work end first, where a piece costs what 384 keys do besides its own; every lane weighs
     // one number of them, up to 144 for the longest prefix.  No more pieces than CTAs and items together: the scratch has that many slots.
-    constexpr int PIECE_COST = 3;
     const int longest = __reduce_max_sync(0xffffffffu, key_tiles), all_items = __reduce_add_sync(0xffffffffu, items);
     const int want = lane < 16 ? lane + 1 : 16 + 8 * (lane - 15), most = (max(longest, 1) + want - 1) / want;
     int64_t n = 0;
     for (int p = 0; p < a.n_prefixes; ++p) n += (int64_t)__shfl_sync(0xffffffffu, items, p) * ((__shfl_sync(0xffffffffu, key_tiles, p) + most - 1) / most);
-    const int64_t cost = quotient(n + a.pre_ctas - 1, a.pre_ctas) * (most + PIECE_COST);
+    const int64_t cost = quotient(n + a.pre_ctas - 1, a.pre_ctas) * (most + 384 / a.key_tile);
     const unsigned key = n > (int64_t)a.pre_ctas + all_items ? 0xffffffffu : (unsigned)min(cost, (int64_t)0x3ffffff) << 5 | (unsigned)lane;
     const unsigned best = __reduce_min_sync(0xffffffffu, key);
     const int cut = __shfl_sync(0xffffffffu, most, (int)(best & 31u)), split = (key_tiles + cut - 1) / cut;
@@ -83,14 +82,14 @@ OA_DEVINL void cut_prefixes(const PrefixAttnArgs& a, PrefixPieces& px, int lane)
 // =============================================================================================
 // the prefixes' part
 // =============================================================================================
-template <int D, int SLOTS>          // SLOTS: tiles of 128 keys or values in the ring
+template <int D, int KEYS, int SLOTS>          // KEYS: of a tile; SLOTS: tiles of keys or values in the ring
 struct PreCfg {
     static constexpr int HALVES = D / 64;
-    static constexpr int HALF_BYTES = 128 * 128;                 // 128 rows x 64 bf16 columns under the 128-byte swizzle
-    static constexpr int TILE_BYTES = HALVES * HALF_BYTES;       // Q of a row tile, and K or V of 128 keys
+    static constexpr int Q_HALF = ROW_TILE * 128, KV_HALF = KEYS * 128;          // rows x 64 bf16 columns under the 128-byte swizzle
+    static constexpr int Q_BYTES = HALVES * Q_HALF, TILE_BYTES = HALVES * KV_HALF;
     static constexpr int THREADS = 64 + PRE_SOFTMAX;             // producer, issuer, softmax warps
     static constexpr int XCH_BYTES = (2 * 2 + 2) * 128 * 4;      // a row's two maxima of a tile, [tile parity][warpgroup][row], and its two sums of a piece
-    static constexpr int SMEM_BYTES = (1 + SLOTS) * TILE_BYTES + 256 + XCH_BYTES;
+    static constexpr int SMEM_BYTES = Q_BYTES + SLOTS * TILE_BYTES + 256 + XCH_BYTES;
     static constexpr uint32_t O_COL = 256;                       // TMEM: S and P of the tiles in turn at 0 and 128, O at 256
 };
 struct PrePiece { int g, kvh, tile, k0, k1; };
@@ -103,13 +102,13 @@ OA_DEVINL PrePiece pre_piece(const PrefixPieces& px, int piece, int n_prefixes) 
     return s;
 }
 
-template <int D, int SLOTS>
+template <int D, int KEYS, int SLOTS>
 __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ PrefixAttnArgs a) {
-    using Cfg = PreCfg<D, SLOTS>;
-    constexpr int HALVES = Cfg::HALVES;
+    using Cfg = PreCfg<D, KEYS, SLOTS>;
+    constexpr int HALVES = Cfg::HALVES, PAGES = KEYS / CACHE_PAGE;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* q_s = smem;
-    uint8_t* kv_s = q_s + Cfg::TILE_BYTES;
+    uint8_t* kv_s = q_s + Cfg::Q_BYTES;
     uint64_t* bars = reinterpret_cast<uint64_t*>(kv_s + SLOTS * Cfg::TILE_BYTES);
     uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_full = bars + 4, *t_full = bars + 6, *o_full = bars + 7, *full = bars + 8, *empty = full + SLOTS;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(empty + SLOTS);
@@ -117,7 +116,7 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
     __shared__ PrefixPieces px;
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int grp = a.n_heads / a.n_kv, tile_tokens = KEY_TILE / grp;      // tokens of a row tile
+    const int grp = a.n_heads / a.n_kv, tile_tokens = ROW_TILE / grp;      // tokens of a row tile
     if (warp == 0 && lane == 0) {
         tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_kv);
         mbar_init(q_full, 1); mbar_init(q_empty, 1); mbar_init(t_full, 1); mbar_init(o_full, 1);
@@ -143,18 +142,18 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
                 mbar_expect_tx(q_full, HALVES * tile_tokens * grp * 128);
 #pragma unroll
                 for (int h = 0; h < HALVES; ++h)
-                    tma_load_3d(q_s + h * Cfg::HALF_BYTES, &tm_q, q_full, h * 64, sg.kvh * grp, px.row0[sg.g] + sg.tile * tile_tokens, kEvictNormal);
+                    tma_load_3d(q_s + h * Cfg::Q_HALF, &tm_q, q_full, h * 64, sg.kvh * grp, px.row0[sg.g] + sg.tile * tile_tokens, kEvictNormal);
             }
             __syncwarp();
             const int32_t* bt = a.prefix_tables + (size_t)sg.g * a.max_prefix_pages;
             const int pages = pages_of(px.len[sg.g]);
-            int page[2] = {0, 0}, prev[2] = {0, 0};
+            int page[PAGES] = {}, prev[PAGES] = {};
             for (int j = 0; j <= sg.k1 - sg.k0; ++j) {
                 const int kt = sg.k0 + j;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < PAGES; ++i) {
                     prev[i] = page[i];
-                    page[i] = kt < sg.k1 && 2 * kt + i < pages ? bt[2 * kt + i] : 0;
+                    page[i] = kt < sg.k1 && PAGES * kt + i < pages ? bt[PAGES * kt + i] : 0;
                     if (page[i] < 0 || page[i] >= a.num_pages) { if (lane == 0) report(a); page[i] = 0; }
                 }
 #pragma unroll
@@ -164,13 +163,15 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
                     const uint32_t slot = n % SLOTS;
                     mbar_wait(&empty[slot], ((n / SLOTS) & 1) ^ 1);
                     if (elect_one()) {
-                        const int two = 2 * t + 1 < pages;       // a missing second page is not loaded: its scores are masked, its values set to zero
+                        const int there = min(PAGES, pages - PAGES * t);         // a missing second page is not loaded: its scores are masked, its values set to zero
                         uint8_t* dst = kv_s + slot * Cfg::TILE_BYTES;
-                        mbar_expect_tx(&full[slot], two ? Cfg::TILE_BYTES : Cfg::TILE_BYTES / 2);
-                        for (int i = 0; i <= two; ++i) {
+                        mbar_expect_tx(&full[slot], there * HALVES * 8192);
+#pragma unroll
+                        for (int i = 0; i < PAGES; ++i) {
+                            if (i >= there) break;
                             const int row = ((v ? a.num_pages + prev[i] : page[i]) * a.n_kv + sg.kvh) * CACHE_PAGE;
 #pragma unroll
-                            for (int h = 0; h < HALVES; ++h) tma_load_2d(dst + h * Cfg::HALF_BYTES + i * 8192, &tm_kv, &full[slot], h * 64, row, kEvictLast);
+                            for (int h = 0; h < HALVES; ++h) tma_load_2d(dst + h * Cfg::KV_HALF + i * 8192, &tm_kv, &full[slot], h * 64, row, kEvictLast);
                         }
                     }
                     __syncwarp();
@@ -180,9 +181,9 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
         }
     } else if (warp == 1) {
         // the whole warp walks the loop, an elected lane issues: descriptors stay in uniform registers
-        constexpr uint32_t idesc_s = umma_idesc_bf16(128, KEY_TILE), idesc_o = umma_idesc_bf16_bmn(128, D);
+        constexpr uint32_t idesc_s = umma_idesc_bf16(128, KEYS), idesc_o = umma_idesc_bf16_bmn(128, D);
         const uint64_t q_desc = umma_desc_sw128(smem_u32(q_s)), k_desc = umma_desc_sw128(smem_u32(kv_s));
-        const uint64_t v_desc = umma_desc_sw128_mn(smem_u32(kv_s), (uint32_t)Cfg::HALF_BYTES, 1024u);
+        const uint64_t v_desc = umma_desc_sw128_mn(smem_u32(kv_s), (uint32_t)Cfg::KV_HALF, 1024u);
         uint32_t n = 0, r = 0, seg = 0;                          // tiles, tiles of the ring, pieces
         auto issue_s = [&](uint32_t n, bool last) {
             const uint32_t slot = r % SLOTS;
@@ -193,8 +194,8 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
                 const uint64_t b = k_desc + (uint64_t)(slot * (Cfg::TILE_BYTES >> 4));
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) {
-                    const uint64_t off = (uint64_t)(((ks >> 2) * Cfg::HALF_BYTES + (ks & 3) * 32) >> 4);
-                    umma_bf16(tmem_base + (n & 1) * 128, q_desc + off, b + off, idesc_s, ks > 0 ? 1u : 0u);
+                    const int half = ks >> 2, in = (ks & 3) * 32;
+                    umma_bf16(tmem_base + (n & 1) * 128, q_desc + (uint64_t)((half * Cfg::Q_HALF + in) >> 4), b + (uint64_t)((half * Cfg::KV_HALF + in) >> 4), idesc_s, ks > 0 ? 1u : 0u);
                 }
                 umma_commit(&s_full[n & 1]);
                 umma_commit(&empty[slot]);
@@ -219,7 +220,7 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
                 if (elect_one()) {
                     const uint64_t b = v_desc + (uint64_t)(slot * (Cfg::TILE_BYTES >> 4));
 #pragma unroll
-                    for (int ks = 0; ks < KEY_TILE / 16; ++ks)
+                    for (int ks = 0; ks < KEYS / 16; ++ks)
                         umma_bf16_ta(tmem_base + Cfg::O_COL, tmem_base + (n & 1) * 128 + ks * 8, b + (uint64_t)(ks * (2048 >> 4)), idesc_o, (j > 0 || ks > 0) ? 1u : 0u);
                     umma_commit(j + 1 < tiles ? t_full : o_full);
                     umma_commit(&empty[slot]);
@@ -228,12 +229,12 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
             }
         }
     } else {
-        // Warps w and w + 4 of the eight hold the same 32 rows and half of every tile's keys each (and of O's columns where those are rescaled or written), 64 scores a thread
+        // Warps w and w + 4 of the eight hold the same 32 rows and half of every tile's keys each (and of O's columns where those are rescaled or written)
         const int quarter = warp & 3, row = quarter * 32 + lane, wg = (warp - 2) >> 2;
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16, o_addr = tmem_base + lane_addr + Cfg::O_COL;
         auto meet = [] { asm volatile("bar.sync 2, %0;" ::"n"(PRE_SOFTMAX) : "memory"); };
         constexpr float kRaise = 8.0f;                                           // log2 units a score may pass the reference by
-        constexpr int KEYS = KEY_TILE / 2, COLS = D / 2;
+        constexpr int MINE = KEYS / 2, CH = MINE / 32, COLS = D / 2;               // keys and 32-key chunks of a thread
         uint32_t n = 0, r = 0, seg = 0, landed = 0;                              // landed: completions of t_full before this piece
         for (int piece = blockIdx.x; piece < px.pieces; piece += gridDim.x, ++seg) {
             const PrePiece sg = pre_piece(px, piece, a.n_prefixes);
@@ -242,33 +243,33 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
             float m_ref = -INFINITY, l_run = 0.f;
             for (int j = 0; j < tiles; ++j, ++n) {
                 const uint32_t sb = n & 1;
-                const int valid = len - (sg.k0 + j) * KEY_TILE;                  // keys of this tile
+                const int valid = len - (sg.k0 + j) * KEYS;                      // keys of this tile
                 mbar_wait(&s_full[sb], (n >> 1) & 1);
                 tcgen05_fence_after();
-                uint32_t v[2][32];
+                uint32_t v[CH][32];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(tmem_base + lane_addr + sb * 128 + wg * KEYS + c * 32, v[c]);
+                for (int c = 0; c < CH; ++c) tmem_ld_32x32b_x32(tmem_base + lane_addr + sb * 128 + wg * MINE + c * 32, v[c]);
                 tmem_ld_wait();
-                if (valid < KEY_TILE) {
+                if (valid < KEYS) {
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
+                    for (int c = 0; c < CH; ++c)
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) if (wg * KEYS + c * 32 + i >= valid) v[c][i] = 0xff800000u;
+                        for (int i = 0; i < 32; ++i) if (wg * MINE + c * 32 + i >= valid) v[c][i] = 0xff800000u;
                     // values behind the end may be anything, and 0 x inf is not 0; only the last tile of a prefix ends early, and its V is the last of the piece's 2 tiles
                     const uint32_t at = r + 2 * tiles - 1, slot = at % SLOTS;
                     mbar_wait(&full[slot], (at / SLOTS) & 1);
-                    if (row >= valid) {
+                    if (row >= valid && row < KEYS) {
 #pragma unroll
                         for (int c = 0; c < D / 16; ++c) {
                             const int chunk = wg * (D / 16) + c;
-                            *reinterpret_cast<uint4*>(kv_s + slot * Cfg::TILE_BYTES + (chunk >> 3) * Cfg::HALF_BYTES + row * 128 + (chunk & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                            *reinterpret_cast<uint4*>(kv_s + slot * Cfg::TILE_BYTES + (chunk >> 3) * Cfg::KV_HALF + row * 128 + (chunk & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
                         }
                     }
                     fence_proxy_async();
                 }
                 float mraw = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
+                for (int c = 0; c < CH; ++c)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) mraw = fmaxf(mraw, __uint_as_float(v[c][i]));
                 float* maxima = xch + (n & 1) * 256;
@@ -298,7 +299,7 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
                 const float neg_ref = -finite_or_zero(m_ref);
                 uint64_t sum = 0;
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
+                for (int c = 0; c < CH; ++c) {
                     uint32_t w[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
@@ -306,7 +307,7 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
                         sum = add_f32x2(sum, pack_f32x2(x, y));
                         w[i] = pack_bf16x2(x, y);
                     }
-                    tmem_st_32x32b_x16(tmem_base + lane_addr + sb * 128 + wg * 32 + c * 16, w);
+                    tmem_st_32x32b_x16(tmem_base + lane_addr + sb * 128 + wg * (MINE / 2) + c * 16, w);
                 }
                 tmem_st_wait();
                 tcgen05_fence_before();
@@ -319,7 +320,7 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
             xch[512 + wg * 128 + row] = l_run;                                   // the piece's before was read ahead of this one's tiles' barriers
             mbar_wait(o_full, seg & 1);
             tcgen05_fence_after();
-            float* po = a.pre_o + (int64_t)piece * (KEY_TILE * D) + row * 4;     // [D / 4][128 rows][4]: a warp's rows lie next to each other
+            float* po = a.pre_o + (int64_t)piece * (ROW_TILE * D) + row * 4;     // [D / 4][128 rows][4]: a warp's rows lie next to each other
 #pragma unroll 1
             for (int c = wg * COLS; c < (wg + 1) * COLS; c += 32) {
                 uint32_t o[32];
@@ -328,11 +329,11 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
                 if (live)
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<float4*>(po + (c + i) / 4 * (KEY_TILE * 4)) = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+                        *reinterpret_cast<float4*>(po + (c + i) / 4 * (ROW_TILE * 4)) = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
             }
             tcgen05_fence_before();
             meet();
-            if (live && wg == 0) *reinterpret_cast<float2*>(a.pre_ml + ((int64_t)piece * KEY_TILE + row) * 2) = make_float2(m_ref, l_run + xch[512 + 128 + row]);
+            if (live && wg == 0) *reinterpret_cast<float2*>(a.pre_ml + ((int64_t)piece * ROW_TILE + row) * 2) = make_float2(m_ref, l_run + xch[512 + 128 + row]);
         }
     }
     __syncthreads();
@@ -450,28 +451,43 @@ __global__ void __maxnreg__(WIDE ? 168 : 104) own_part_kernel(const __grid_const
     if (u_begin >= u_end) { griddep_launch(); griddep_wait(); return; }
 
     if (warp == 8) {
-        if (lane == 0) {
-            int s = 0; uint32_t ph = 0, k = 0;
-            at = start;
-            at.ahead(a);
-            auto first_page = [&](int seq) { return seq < a.n_seqs ? __ldcg(a.own_tables + (int64_t)seq * a.max_own_pages) : 0; };
-            int page0 = first_page(at.seq), next_page0 = first_page(at.seq + 1), seq = at.seq;      // read ahead, like lengths
-            for (int64_t u = u_begin; u < u_end; at.next(a, runs), ++k) {
-                if (at.seq != seq) { page0 = next_page0; seq = at.seq; next_page0 = first_page(seq + 1); }
-                const int c0 = (int)max(u - at.unit0 - 1, (int64_t)0), c1 = (int)min((int64_t)at.pages, u_end - at.unit0 - 1);
-                u = at.unit0 + 1 + c1;
-                mbar_wait(&q_empty[k & 1], ((k >> 1) & 1) ^ 1);
+        int s = 0; uint32_t ph = 0, k = 0;
+        at = start;
+        at.ahead(a);
+        // Page numbers come 32 at a time, one a lane, and the next 32 that will be wanted are on their way meanwhile (a look one page ahead is a chain of one latency a page: 1300 cycles, as
+        // long as a page takes to arrive)
+        auto block_of = [&](int seq, int block, int pages) {
+            const int c = block * 32 + lane;
+            if (seq == at.seq) return c < at.pages ? __ldcg(at.entry(a, c)) : 0;
+            return seq < a.n_seqs && c < pages ? __ldcg(a.own_tables + (int64_t)seq * a.max_own_pages + c) : 0;
+        };
+        int have = 0, next = 0, have_seq = -1, have_block = 0, next_seq = -1, next_block = 0;
+        for (int64_t u = u_begin; u < u_end; at.next(a, runs), ++k) {
+            const int c0 = (int)max(u - at.unit0 - 1, (int64_t)0), c1 = (int)min((int64_t)at.pages, u_end - at.unit0 - 1);
+            u = at.unit0 + 1 + c1;
+            mbar_wait(&q_empty[k & 1], ((k >> 1) & 1) ^ 1);
+            if (lane == 0) {
                 if (c1 > c0) {
                     const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)at.seq * a.ldq + (int64_t)at.kvh * grp * D;
                     mbar_expect_tx(&q_full[k & 1], grp * D * 2);
                     for (int r = 0; r < grp; ++r) bulk_load(q_s + (k & 1) * Cfg::Q_BYTES + r * Cfg::Q_PITCH, q + r * D, D * 2, &q_full[k & 1]);
                 } else mbar_arrive(&q_full[k & 1]);
-                int page = c1 <= c0 ? 0 : c0 == 0 && at.pre_pages == 0 ? page0 : __ldcg(at.entry(a, c0));
-                for (int c = c0; c < c1; ++c) {
-                    const int next_page = c + 1 < c1 ? __ldcg(at.entry(a, c + 1)) : 0;       // looked up while this one's slot is waited for
-                    const int valid = min(CACHE_PAGE, at.tokens(c));
-                    if (page < 0 || page >= a.num_pages) { report(a); page = 0; }
-                    mbar_wait(&empty_bar[s], ph ^ 1);
+            }
+            for (int c = c0; c < c1; ++c) {
+                const int block = c >> 5;
+                if (have_seq != at.seq || have_block != block) {
+                    have = next_seq == at.seq && next_block == block ? next : block_of(at.seq, block, 0);
+                    have_seq = at.seq; have_block = block;
+                    if (block < (c1 - 1) >> 5) { next_seq = at.seq; next_block = block + 1; }
+                    else if (block > 0 && at.kvh + 1 < a.n_kv) { next_seq = at.seq; next_block = 0; }
+                    else { next_seq = a.pre_ctas > 0 || a.n_prefixes == 0 ? at.seq + 1 : -1; next_block = 0; }      // with prefixes' pages first, the next sequence's are not known yet
+                    if (next_seq >= 0) next = block_of(next_seq, next_block, a.max_own_pages);
+                }
+                int page = __shfl_sync(0xffffffffu, have, c & 31);
+                const int valid = min(CACHE_PAGE, at.tokens(c));
+                if (page < 0 || page >= a.num_pages) { if (lane == 0) report(a); page = 0; }
+                mbar_wait(&empty_bar[s], ph ^ 1);
+                if (lane == 0) {
                     uint8_t* kdst = smem + s * Cfg::STAGE_BYTES;
                     uint8_t* vdst = kdst + Cfg::KV_BYTES;
                     const int krow = (page * a.n_kv + at.kvh) * CACHE_PAGE, vrow = krow + a.num_pages * a.n_kv * CACHE_PAGE;
@@ -492,9 +508,9 @@ __global__ void __maxnreg__(WIDE ? 168 : 104) own_part_kernel(const __grid_const
                                 tma_load_2d(vdst + h * Cfg::TILE_BYTES + i * 2048, &tm_part, &full_bar[s], h * 64, vrow + i * 16, kEvictFirst);
                             }
                     }
-                    page = next_page;
-                    if (++s == STAGES) { s = 0; ph ^= 1; }
                 }
+                __syncwarp();
+                if (++s == STAGES) { s = 0; ph ^= 1; }
             }
         }
         __syncwarp();
@@ -580,16 +596,18 @@ __global__ void __maxnreg__(WIDE ? 168 : 104) own_part_kernel(const __grid_const
                     {
                         const int r = quarter * 16 + (((lane >> 3) & 1) << 3) + (lane & 7), dsel = (lane >> 4) << 3;
 #pragma unroll
-                        for (int ks = 0; ks < KS; ks += 2) {
-                            uint32_t qf[NB][4], a0, a1, a2, a3;
+                        for (int k0 = 0; k0 < KS; k0 += 4) {                                 // loads of four steps ahead of their products
+                            uint32_t qf[NB][2][4], kf[4][4];
 #pragma unroll
-                            for (int b = 0; b < NB; ++b) ldmatrix_x4(qbase + b * 8 * Cfg::Q_PITCH + ks * 32, qf[b][0], qf[b][1], qf[b][2], qf[b][3]);
+                            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                ldmatrix_x4(kbase + own_off<D>(r, (ks + h) * 16 + dsel), a0, a1, a2, a3);
+                                for (int b = 0; b < NB; ++b) ldmatrix_x4(qbase + b * 8 * Cfg::Q_PITCH + (k0 + 2 * h) * 32, qf[b][h][0], qf[b][h][1], qf[b][h][2], qf[b][h][3]);
 #pragma unroll
-                                for (int b = 0; b < NB; ++b) mma_bf16_16816(sacc[b][h], a0, a1, a2, a3, qf[b][2 * h], qf[b][2 * h + 1]);
-                            }
+                            for (int ks = 0; ks < 4; ++ks) ldmatrix_x4(kbase + own_off<D>(r, (k0 + ks) * 16 + dsel), kf[ks][0], kf[ks][1], kf[ks][2], kf[ks][3]);
+#pragma unroll
+                            for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                                for (int b = 0; b < NB; ++b) mma_bf16_16816(sacc[b][ks & 1], kf[ks][0], kf[ks][1], kf[ks][2], kf[ks][3], qf[b][ks >> 1][2 * (ks & 1)], qf[b][ks >> 1][2 * (ks & 1) + 1]);
                         }
                     }
                     uint32_t pb[NB][2]; float alpha[NB][2];
@@ -619,20 +637,19 @@ __global__ void __maxnreg__(WIDE ? 168 : 104) own_part_kernel(const __grid_const
 #pragma unroll
                             for (int i = 0; i < KH; ++i) { oacc[b][i][0] *= alpha[b][0]; oacc[b][i][1] *= alpha[b][1]; oacc[b][i][2] *= alpha[b][0]; oacc[b][i][3] *= alpha[b][1]; }
                     }
-                    // values behind the end may be anything, and 0 x inf is not 0
-                    uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-                    if (valid < 16) {
-                        keep0 = (2 * t < valid ? 0xffffu : 0u) | (2 * t + 1 < valid ? 0xffff0000u : 0u);
-                        keep1 = (2 * t + 8 < valid ? 0xffffu : 0u) | (2 * t + 9 < valid ? 0xffff0000u : 0u);
-                    }
                     const int r = quarter * 16 + ((lane >> 4) << 3) + (lane & 7), dsel = ((lane >> 3) & 1) << 3;
+                    uint32_t vf[KH][4];
 #pragma unroll
-                    for (int i = 0; i < KH; ++i) {
-                        uint32_t a0, a1, a2, a3;
-                        ldmatrix_x4_trans(vbase + own_off<D>(r, (half * KH + i) * 16 + dsel), a0, a1, a2, a3);
+                    for (int i = 0; i < KH; ++i) ldmatrix_x4_trans(vbase + own_off<D>(r, (half * KH + i) * 16 + dsel), vf[i][0], vf[i][1], vf[i][2], vf[i][3]);
+                    if (valid < 16) {                                                        // values behind the end may be anything, and 0 x inf is not 0
+                        const uint32_t keep0 = (2 * t < valid ? 0xffffu : 0u) | (2 * t + 1 < valid ? 0xffff0000u : 0u), keep1 = (2 * t + 8 < valid ? 0xffffu : 0u) | (2 * t + 9 < valid ? 0xffff0000u : 0u);
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) mma_bf16_16816(oacc[b][i], a0 & keep0, a1 & keep0, a2 & keep1, a3 & keep1, pb[b][0], pb[b][1]);
+                        for (int i = 0; i < KH; ++i) { vf[i][0] &= keep0; vf[i][1] &= keep0; vf[i][2] &= keep1; vf[i][3] &= keep1; }
                     }
+#pragma unroll
+                    for (int i = 0; i < KH; ++i)
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) mma_bf16_16816(oacc[b][i], vf[i][0], vf[i][1], vf[i][2], vf[i][3], pb[b][0], pb[b][1]);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&empty_bar[s]);
@@ -675,7 +692,7 @@ __global__ void __maxnreg__(WIDE ? 168 : 104) own_part_kernel(const __grid_const
 template <int D, int RP>
 __global__ void __launch_bounds__(JOIN_THREADS) join_parts_kernel(const __grid_constant__ PrefixAttnArgs a) {
     constexpr int SPLIT = D * RP / 256 > 1 ? D * RP / 256 : 1, LANES = 32 / RP, ITERS = D / 4 / LANES / SPLIT, MP = 8;
-    const int lane = threadIdx.x & 31, grp = a.n_heads / a.n_kv, tile_tokens = KEY_TILE / grp;
+    const int lane = threadIdx.x & 31, grp = a.n_heads / a.n_kv, tile_tokens = ROW_TILE / grp;
     const int64_t task = (int64_t)blockIdx.x * (JOIN_THREADS / 32) + (threadIdx.x >> 5), item = task / SPLIT;
     const int seq = (int)(item / a.n_kv), kvh = (int)(item - (int64_t)seq * a.n_kv), part = (int)(task % SPLIT) * (D / 4 / SPLIT) + lane / RP;
     griddep_launch();
@@ -697,10 +714,10 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_parts_kernel(const __grid_c
     const int n = n_pre + 1;                     // the prefix's parts and the first own one: where they lie is known; later own ones follow
     for (int r0 = 0; r0 < grp; r0 += RP) {
         const int row = r0 + lane % RP, r = row < grp ? row : grp - 1;          // lanes beyond the group go along
-        const float2* pre_ml = reinterpret_cast<const float2*>(a.pre_ml) + pre_slot * KEY_TILE + first_row + r;
+        const float2* pre_ml = reinterpret_cast<const float2*>(a.pre_ml) + pre_slot * ROW_TILE + first_row + r;
         const float2* own_ml = reinterpret_cast<const float2*>(a.own_ml) + item * grp + r;
         const float2* more_ml = reinterpret_cast<const float2*>(a.more_ml) + (int64_t)later.x * grp + r;
-        const float* pre_o = a.pre_o + pre_slot * (KEY_TILE * D) + (first_row + r) * 4 + part * (KEY_TILE * 4);
+        const float* pre_o = a.pre_o + pre_slot * (ROW_TILE * D) + (first_row + r) * 4 + part * (ROW_TILE * 4);
         const float* own_o = a.own_o + (item * grp + r) * D + part * 4;
         const float* more_o = a.more_o + ((int64_t)later.x * grp + r) * D + part * 4;
         float M = -INFINITY, l = 0.f; float4 acc[ITERS]; bool some = false;
@@ -714,9 +731,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_parts_kernel(const __grid_c
                 const int i = i0 + p;
                 ml[p] = make_float2(-INFINITY, -1.f);
                 if (i >= n && i >= n + later.y) continue;
-                const float2* m = i < n_pre ? pre_ml + (int64_t)i * KEY_TILE : i < n ? own_ml : more_ml + (int64_t)(i - n) * grp;
-                const float* src = i < n_pre ? pre_o + (int64_t)i * (KEY_TILE * D) : i < n ? own_o : more_o + (int64_t)(i - n) * (grp * D);
-                const int step = i < n_pre ? KEY_TILE * 4 * LANES : 4 * LANES;
+                const float2* m = i < n_pre ? pre_ml + (int64_t)i * ROW_TILE : i < n ? own_ml : more_ml + (int64_t)(i - n) * grp;
+                const float* src = i < n_pre ? pre_o + (int64_t)i * (ROW_TILE * D) : i < n ? own_o : more_o + (int64_t)(i - n) * (grp * D);
+                const int step = i < n_pre ? ROW_TILE * 4 * LANES : 4 * LANES;
                 ml[p] = __ldcg(m);
 #pragma unroll
                 for (int k = 0; k < ITERS; ++k) o[p][k] = __ldcg(reinterpret_cast<const float4*>(src + k * step));
@@ -751,21 +768,22 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_parts_kernel(const __grid_c
 // =============================================================================================
 // host
 // =============================================================================================
-constexpr int PREFIX_LONG_UNITS = 8, PREFIX_INLINE_ROWS = 4, PREFIX_INLINE_UNITS = 4;
+constexpr int PREFIX_LONG_UNITS = 16, PREFIX_INLINE_ROWS = 4, PREFIX_INLINE_UNITS = 4;
 PrefixAttnPlan prefix_attn_plan(int n_seqs, int n_heads, int n_kv, int head_dim, int n_prefixes, int max_prefix_pages, int max_own_pages, int sms) {
     PrefixAttnPlan p{};
     const int grp = n_heads / n_kv;
-    const int tile_tokens = KEY_TILE / grp;
-    const int64_t work = ((int64_t)n_seqs + tile_tokens - 1) / tile_tokens * n_kv * ((max_prefix_pages + 1) / 2);       // units, if one prefix has all rows
+    const int tile_tokens = ROW_TILE / grp;
+    const int64_t work = ((int64_t)n_seqs + tile_tokens - 1) / tile_tokens * n_kv * max_prefix_pages;       // pages, if one prefix has all rows
     const bool apart = n_prefixes > 0 && !(n_seqs <= PREFIX_INLINE_ROWS && (int64_t)n_seqs * n_kv * max_prefix_pages <= PREFIX_INLINE_UNITS * (int64_t)sms);
     const int64_t items = apart ? ((int64_t)n_seqs / tile_tokens + n_prefixes) * n_kv : 0;                              // no more row tiles than that, however rows fall on prefixes
-    const int64_t units = items * ((max_prefix_pages + 1) / 2), own_units = (int64_t)n_seqs * n_kv * (1 + (int64_t)max_own_pages + (apart ? 0 : max_prefix_pages));
+    const int64_t units = items * max_prefix_pages, own_units = (int64_t)n_seqs * n_kv * (1 + (int64_t)max_own_pages + (apart ? 0 : max_prefix_pages));
     p.pre_ctas = (int)(units < sms ? units : sms);                                                                      // 0: prefixes are read with the sequences' own parts
     p.own_ctas = (int)(own_units < sms ? own_units : sms);
-    p.long_prefix = work >= PREFIX_LONG_UNITS * (int64_t)sms;
+    p.long_prefix = apart && work >= PREFIX_LONG_UNITS * (int64_t)sms;
+    p.key_tile = head_dim == 64 || p.long_prefix ? 128 : 64;
     p.pre_slots = (size_t)(items + p.pre_ctas);
     auto take = [&](size_t bytes) { const size_t at = p.bytes; p.bytes += (bytes + 255) & ~size_t(255); return at; };
-    p.pre_o = take(p.pre_slots * KEY_TILE * head_dim * 4); p.pre_ml = take(p.pre_slots * KEY_TILE * 8);
+    p.pre_o = take(p.pre_slots * ROW_TILE * head_dim * 4); p.pre_ml = take(p.pre_slots * ROW_TILE * 8);
     const size_t own_items = (size_t)n_seqs * n_kv;
     p.own_o = take(own_items * grp * head_dim * 4); p.own_ml = take(own_items * grp * 8); p.own_parts = take(own_items * 8);
     p.more_o = take((size_t)p.own_ctas * grp * head_dim * 4); p.more_ml = take((size_t)p.own_ctas * grp * 8);
@@ -788,43 +806,40 @@ static cudaError_t launch_own(const CUtensorMap* tm_page, const CUtensorMap* tm_
     { const cudaError_t e = raise_smem(kern, OwnCfg<D, WIDE, STAGES>::SMEM_BYTES, attr_done); if (e != cudaSuccess) return e; }
     return launch_k(kern, dim3(a.own_ctas), dim3(OWN_THREADS), OwnCfg<D, WIDE, STAGES>::SMEM_BYTES, s, *tm_page, *tm_part, a);
 }
-template <int D, int SLOTS>
+template <int D, int KEYS, int SLOTS>
 static cudaError_t launch_prefixes(const CUtensorMap* tm_q, const CUtensorMap* tm_page, const PrefixAttnArgs& a, cudaStream_t s) {
-    auto kern = prefix_part_kernel<D, SLOTS>;
+    using Cfg = PreCfg<D, KEYS, SLOTS>;
+    auto kern = prefix_part_kernel<D, KEYS, SLOTS>;
     static bool attr_done[16] = {};
-    { const cudaError_t e = raise_smem(kern, PreCfg<D, SLOTS>::SMEM_BYTES, attr_done); if (e != cudaSuccess) return e; }
-    return launch_k(kern, dim3(a.pre_ctas), dim3(PreCfg<D, SLOTS>::THREADS), PreCfg<D, SLOTS>::SMEM_BYTES, s, *tm_q, *tm_page, a);
+    { const cudaError_t e = raise_smem(kern, Cfg::SMEM_BYTES, attr_done); if (e != cudaSuccess) return e; }
+    return launch_k(kern, dim3(a.pre_ctas), dim3(Cfg::THREADS), Cfg::SMEM_BYTES, s, *tm_q, *tm_page, a);
 }
 template <int D, int RP>
 static cudaError_t launch_join(const PrefixAttnArgs& a, cudaStream_t s) {
+    auto kern = join_parts_kernel<D, RP>;
+    static bool attr_done[16] = {};
+    { const cudaError_t e = raise_smem(kern, 0, attr_done); if (e != cudaSuccess) return e; }
     const int64_t tasks = (int64_t)a.n_seqs * a.n_kv * (D * RP / 256 > 1 ? D * RP / 256 : 1);
-    return launch_k(join_parts_kernel<D, RP>, dim3((unsigned)((tasks + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32))), dim3(JOIN_THREADS), 0, s, a);
+    return launch_k(kern, dim3((unsigned)((tasks + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32))), dim3(JOIN_THREADS), 0, s, a);
 }
-template <int D>
-static cudaError_t launch_all(const CUtensorMap* tm_q, const CUtensorMap* tm_page, const CUtensorMap* tm_part, bool long_prefix, const PrefixAttnArgs& a, cudaStream_t s) {
-    const int grp = a.n_heads / a.n_kv;
+// KEYS, SLOTS: tiles and ring of the prefixes' kernel; PAGES: ring of the own parts'
+template <int D, int KEYS, int SLOTS, int PAGES>
+static cudaError_t launch_parts(const CUtensorMap* tm_q, const CUtensorMap* tm_page, const CUtensorMap* tm_part, const PrefixAttnArgs& a, cudaStream_t s) {
     cudaError_t e = cudaSuccess;
-    // An SM's shared memory goes to both kernels: long prefixes take three tiles of the first's ring and leave two pages to the second's, others two and three (heads of 64: 4 and 5)
-    constexpr int RING = D == 128 ? 2 : 4, PAGES = D == 128 ? 3 : 5;
-    bool done = false;
-    if constexpr (D == 128) {
-        if (long_prefix && a.pre_ctas > 0) {
-            e = launch_prefixes<D, 3>(tm_q, tm_page, a, s);
-            if (e == cudaSuccess && grp <= 8) { e = launch_own<D, false, 2>(tm_page, tm_part, a, s); done = true; }
-            else if (e == cudaSuccess) { e = launch_own<D, true, PAGES>(tm_page, tm_part, a, s); done = true; }
-        }
-    }
-    if (!done && e == cudaSuccess) {
-        if (a.pre_ctas > 0) e = launch_prefixes<D, RING>(tm_q, tm_page, a, s);
-        if (e == cudaSuccess) e = grp > 8 ? launch_own<D, true, PAGES>(tm_page, tm_part, a, s) : launch_own<D, false, PAGES>(tm_page, tm_part, a, s);
-    }
-    if (e == cudaSuccess) e = grp > 4 ? launch_join<D, 8>(a, s) : grp > 2 ? launch_join<D, 4>(a, s) : launch_join<D, 2>(a, s);
+    if (a.pre_ctas > 0) e = launch_prefixes<D, KEYS, SLOTS>(tm_q, tm_page, a, s);
+    if (e == cudaSuccess) e = a.n_heads / a.n_kv > 8 ? launch_own<D, true, PAGES>(tm_page, tm_part, a, s) : launch_own<D, false, PAGES>(tm_page, tm_part, a, s);
     return e;
 }
 cudaError_t launch_prefix_attention(const CUtensorMap* tm_q, const CUtensorMap* tm_page, const CUtensorMap* tm_part, int head_dim, bool long_prefix, const PrefixAttnArgs& a, cudaStream_t s) {
-    if (head_dim == 128) return launch_all<128>(tm_q, tm_page, tm_part, long_prefix, a, s);
-    if (head_dim == 64) return launch_all<64>(tm_q, tm_page, tm_part, long_prefix, a, s);
-    return cudaErrorInvalidValue;
+    if (head_dim != 64 && head_dim != 128) return cudaErrorInvalidValue;
+    // An SM's shared memory goes to both kernels: heads of 128 give the prefixes three tiles of 128 keys and the own parts two pages where prefixes are most of the work, two tiles
+    // of 64 keys and four pages elsewhere
+    const cudaError_t e = head_dim == 64 ? launch_parts<64, 128, 3, 8>(tm_q, tm_page, tm_part, a, s)
+                        : long_prefix ? launch_parts<128, 128, 3, 2>(tm_q, tm_page, tm_part, a, s) : launch_parts<128, 64, 2, 4>(tm_q, tm_page, tm_part, a, s);
+    if (e != cudaSuccess) return e;
+    const int grp = a.n_heads / a.n_kv;
+    if (head_dim == 64) return grp > 4 ? launch_join<64, 8>(a, s) : grp > 2 ? launch_join<64, 4>(a, s) : launch_join<64, 2>(a, s);
+    return grp > 4 ? launch_join<128, 8>(a, s) : grp > 2 ? launch_join<128, 4>(a, s) : launch_join<128, 2>(a, s);
 }
 
 }  // namespace oa

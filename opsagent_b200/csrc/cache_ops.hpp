@@ -42,9 +42,9 @@ struct PrefixAttnArgs {
     int32_t* status;
     // scratch (prefix_attn_plan): parts of the prefixes, each item's first own part, later ones by the CTA that makes them, and how many of those an item has
     float *pre_o, *pre_ml, *own_o, *own_ml, *more_o, *more_ml; int2* own_parts;
-    int32_t pre_ctas, own_ctas;                    // pre_ctas 0: prefixes have no kernel of their own
+    int32_t pre_ctas, own_ctas, key_tile;          // pre_ctas 0: prefixes have no kernel of their own; key_tile: keys of its tiles
 };
-struct PrefixAttnPlan { int pre_ctas, own_ctas; bool long_prefix; size_t pre_slots, pre_o, pre_ml, own_o, own_ml, more_o, more_ml, own_parts, bytes; };      // CTAs, slots, byte offsets
+struct PrefixAttnPlan { int pre_ctas, own_ctas, key_tile; bool long_prefix; size_t pre_slots, pre_o, pre_ml, own_o, own_ml, more_o, more_ml, own_parts, bytes; };      // CTAs, slots, byte offsets
 PrefixAttnPlan prefix_attn_plan(int n_seqs, int n_heads, int n_kv, int head_dim, int n_prefixes, int max_prefix_pages, int max_own_pages, int sms);
 // tm_q: box of 128 / group tokens by a group's heads over q; tm_page: box of 64 rows, tm_part: box of 16 rows over the layer's cache [2 * num_pages * n_kv * 64, head_dim]
 cudaError_t launch_prefix_attention(const CUtensorMap* tm_q, const CUtensorMap* tm_page, const CUtensorMap* tm_part, int head_dim, bool long_prefix, const PrefixAttnArgs& a, cudaStream_t s);
