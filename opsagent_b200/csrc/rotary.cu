@@ -16,105 +16,126 @@
 
 namespace oa {
 
-constexpr int ROT_THREADS = 128;
+constexpr int ROT_THREADS = 128;         // at least ROTARY_MAX_PAIRS: a pair's angle a thread
 constexpr int ROT_UNROLL = 4;            // units of two pieces in flight per thread
+constexpr int ROT_CTAS = 6;              // of an SM: 80 registers a thread
+static_assert(ROT_THREADS >= ROTARY_MAX_PAIRS);
 
-OA_DEVINL void rot_read(const float* p, float (&v)[4]) { const float4 x = *reinterpret_cast<const float4*>(p); v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; }
-OA_DEVINL void rot_read(const float* p, float (&v)[1]) { v[0] = *p; }
-OA_DEVINL void rot_read(const uint16_t* p, float (&v)[8]) {
-    const uint4 x = *reinterpret_cast<const uint4*>(p);
-    v[0] = bf16lo(x.x); v[1] = bf16hi(x.x); v[2] = bf16lo(x.y); v[3] = bf16hi(x.y); v[4] = bf16lo(x.z); v[5] = bf16hi(x.z); v[6] = bf16lo(x.w); v[7] = bf16hi(x.w);
+template <typename E, int VEC> struct RotPiece { E v; };
+template <> struct RotPiece<uint16_t, 8> { uint4 v; };
+template <> struct RotPiece<float, 4> { float4 v; };
+
+OA_DEVINL void rot_unpack(const RotPiece<float, 4>& p, float (&v)[4]) { v[0] = p.v.x; v[1] = p.v.y; v[2] = p.v.z; v[3] = p.v.w; }
+OA_DEVINL void rot_unpack(const RotPiece<float, 1>& p, float (&v)[1]) { v[0] = p.v; }
+OA_DEVINL void rot_unpack(const RotPiece<uint16_t, 8>& p, float (&v)[8]) {
+    v[0] = bf16lo(p.v.x); v[1] = bf16hi(p.v.x); v[2] = bf16lo(p.v.y); v[3] = bf16hi(p.v.y); v[4] = bf16lo(p.v.z); v[5] = bf16hi(p.v.z); v[6] = bf16lo(p.v.w); v[7] = bf16hi(p.v.w);
 }
-OA_DEVINL void rot_read(const uint16_t* p, float (&v)[1]) { v[0] = bf16_bits_to_f32(*p); }
-OA_DEVINL void rot_write(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
-OA_DEVINL void rot_write(float* p, const float (&v)[1]) { *p = v[0]; }
-OA_DEVINL void rot_write(uint16_t* p, const float (&v)[8]) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+OA_DEVINL void rot_unpack(const RotPiece<uint16_t, 1>& p, float (&v)[1]) { v[0] = bf16_bits_to_f32(p.v); }
+OA_DEVINL void rot_pack(RotPiece<float, 4>& p, const float (&v)[4]) { p.v = make_float4(v[0], v[1], v[2], v[3]); }
+OA_DEVINL void rot_pack(RotPiece<float, 1>& p, const float (&v)[1]) { p.v = v[0]; }
+OA_DEVINL void rot_pack(RotPiece<uint16_t, 8>& p, const float (&v)[8]) { p.v = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])); }
+OA_DEVINL void rot_pack(RotPiece<uint16_t, 1>& p, const float (&v)[1]) { p.v = (uint16_t)(pack_bf16x2(v[0], 0.f) & 0xffffu); }
+
+template <int VEC>
+OA_DEVINL void rot_angles(const float* from, float (&v)[VEC]) {
+    if constexpr (VEC == 1) v[0] = *from;
+    else {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) { const float4 x = *reinterpret_cast<const float4*>(from + i); v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w; }
+    }
 }
-OA_DEVINL void rot_write(uint16_t* p, const float (&v)[1]) { *p = (uint16_t)(pack_bf16x2(v[0], 0.f) & 0xffffu); }
 
 // E: uint16_t (bf16 bits) or float; VEC: elements of a piece, 16 bytes or 1 where rows, heads or halves are not aligned to pieces.  A unit is two pieces:
-// the a and the b of VEC pairs (HALVES: pairs apart; else 2 VEC channels side by side), or 2 VEC channels that are copied.
+// the a and the b of VEC pairs (HALVES: pairs apart; else 2 VEC channels side by side), or 2 VEC channels that are copied.  A thread keeps its place in a head
+// and walks over heads, so that it reads its cos and sin once a token.
 template <typename E, int VEC, bool HALVES, bool CACHE>
-__global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const __grid_constant__ RotaryArgs a) {
-    __shared__ float2 cs[ROTARY_MAX_PAIRS];
-    const int t = blockIdx.x;
+__global__ void __launch_bounds__(ROT_THREADS, ROT_CTAS) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+    using Piece = RotPiece<E, VEC>;
+    __shared__ __align__(16) float cosines[2][ROTARY_MAX_PAIRS], sines[2][ROTARY_MAX_PAIRS];
     const int D = a.head_dim, pairs = a.pairs;
     const int per_head = D / (2 * VEC), turned = pairs / VEC;
-    const int heads = a.n_heads + (CACHE ? 2 * a.n_kv : 0), units = heads * per_head;
+    const int heads = a.n_heads + (CACHE ? 2 * a.n_kv : 0);
+    const int across = per_head < ROT_THREADS ? per_head : ROT_THREADS, down = ROT_THREADS / across;     // threads on a head, heads at a time
+    const int r0 = threadIdx.x % across, row = threadIdx.x / across;
+    const int head0 = row < down ? blockIdx.y * down + row : heads, head_step = gridDim.y * down;
+    const double turns = threadIdx.x < pairs ? a.turns[threadIdx.x] : 0.0;
     griddep_launch();
     griddep_wait();
-    const double p = (double)a.positions[t];
-    int64_t page_row = -1;                                      // the token's row of head 0 in a plane of the cache
-    if (CACHE) {
-        const int slot = a.slots[t];
-        if (slot >= 0 && slot / CACHE_PAGE < a.num_pages) page_row = (int64_t)(slot / CACHE_PAGE) * a.n_kv * CACHE_PAGE + slot % CACHE_PAGE;
-        else if (slot >= 0 && a.status && threadIdx.x == 0) *a.status = 400;
-    }
-    bool first = true;
-    const int stride = gridDim.y * ROT_THREADS;
-    for (int u0 = blockIdx.y * ROT_THREADS; u0 < units; u0 += stride * ROT_UNROLL) {
-        float lo[ROT_UNROLL][VEC], hi[ROT_UNROLL][VEC];
-        E* dst[ROT_UNROLL]; int step[ROT_UNROLL], angle[ROT_UNROLL];
-#pragma unroll
-        for (int k = 0; k < ROT_UNROLL; ++k) {
-            const int u = u0 + k * stride + threadIdx.x;
-            dst[k] = nullptr;
-            if (u >= units) continue;
-            const int head = u / per_head, r = u - head * per_head;
-            const E* src; E* to;
-            bool turn = r < turned;
-            if (!CACHE || head < a.n_heads) {
-                src = reinterpret_cast<const E*>(a.x) + (int64_t)t * a.ldx + (int64_t)head * D;
-                to = reinterpret_cast<E*>(a.out) + (int64_t)t * a.ldo + (int64_t)head * D;
-            } else {
-                const int kv = (head - a.n_heads) % a.n_kv;
-                const bool value = head >= a.n_heads + a.n_kv;
-                if (page_row < 0) continue;
-                src = reinterpret_cast<const E*>(value ? a.v : a.k) + (int64_t)t * a.ldkv + (int64_t)kv * D;
-                to = reinterpret_cast<E*>(a.cache) + (page_row + (int64_t)kv * CACHE_PAGE + (value ? (int64_t)a.num_pages * a.n_kv * CACHE_PAGE : 0)) * D;
-                turn = turn && !value;
-            }
+    int position = a.positions[blockIdx.x], slot = CACHE ? a.slots[blockIdx.x] : -1;
+    int phase = 0;
+    for (int t = blockIdx.x; t < a.T; t += gridDim.x, phase ^= 1) {
+        const int64_t plane = CACHE ? (int64_t)a.num_pages * a.n_kv * CACHE_PAGE : 0;
+        int64_t page_row = -1;                                  // the token's row of head 0 in a plane of the cache
+        if (CACHE) {
+            if (slot >= 0 && slot / CACHE_PAGE < a.num_pages) page_row = (int64_t)(slot / CACHE_PAGE) * a.n_kv * CACHE_PAGE + slot % CACHE_PAGE;
+            else if (slot >= 0 && a.status && threadIdx.x == 0) *a.status = 400;
+        }
+        const double p = (double)position;
+        if (t + (int)gridDim.x < a.T) { position = a.positions[t + gridDim.x]; if (CACHE) slot = a.slots[t + gridDim.x]; }
+        const E* x = reinterpret_cast<const E*>(a.x) + (int64_t)t * a.ldx;
+        E* out = reinterpret_cast<E*>(a.out) + (int64_t)t * a.ldo;
+        // head h's source and place, nullptr where it is not written; values are neither turned nor in out
+        auto source = [&](int h) -> const E* {
+            if (!CACHE || h < a.n_heads) return x + (int64_t)h * D;
+            const bool value = h >= a.n_heads + a.n_kv;
+            return reinterpret_cast<const E*>(value ? a.v : a.k) + (int64_t)t * a.ldkv + (int64_t)(h - a.n_heads - (value ? a.n_kv : 0)) * D;
+        };
+        auto place = [&](int h) -> E* {
+            if (!CACHE || h < a.n_heads) return out + (int64_t)h * D;
+            const bool value = h >= a.n_heads + a.n_kv;
+            return reinterpret_cast<E*>(a.cache) + (page_row + (int64_t)(h - a.n_heads - (value ? a.n_kv : 0)) * CACHE_PAGE + (value ? plane : 0)) * D;
+        };
+        const int last = CACHE && page_row < 0 ? a.n_heads : heads;
+        bool angles = false;
+        for (int r = r0; r < per_head; r += across) {
             const bool apart = HALVES && r < turned;            // values too: their pieces only have to be all of the head's
-            const int at = apart ? r * VEC : r * 2 * VEC;
-            step[k] = apart ? pairs : VEC; angle[k] = turn ? r * VEC : -1;
-            dst[k] = to + at;
-            rot_read(src + at, lo[k]); rot_read(src + at + step[k], hi[k]);
-        }
-        if (first) {
-            for (int i = threadIdx.x; i < pairs; i += ROT_THREADS) {
-                const double turns = p * a.turns[i];
-                float sn, cn;
-                sincospif((float)(2.0 * (turns - rint(turns))), &sn, &cn);
-                cs[i] = make_float2(cn * a.amplitude, sn * a.amplitude);
-            }
-            __syncthreads();
-            first = false;
-        }
+            const int at = apart ? r * VEC : r * 2 * VEC, step = apart ? pairs : VEC;
+            float cn[VEC], sn[VEC];
+            int h = head0;
+            do {
+                Piece lo[ROT_UNROLL], hi[ROT_UNROLL];
 #pragma unroll
-        for (int k = 0; k < ROT_UNROLL; ++k) {
-            if (!dst[k]) continue;
-            if (angle[k] >= 0) {
-                if (HALVES) {
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) {
-                        const float2 c = cs[angle[k] + i]; const float x = lo[k][i], y = hi[k][i];
-                        lo[k][i] = x * c.x - y * c.y; hi[k][i] = x * c.y + y * c.x;
-                    }
-                } else if constexpr (VEC == 1) {
-                    const float2 c = cs[angle[k]]; const float x = lo[k][0], y = hi[k][0];
-                    lo[k][0] = x * c.x - y * c.y; hi[k][0] = x * c.y + y * c.x;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < VEC; i += 2) {
-                        const float2 c = cs[angle[k] + i / 2], d = cs[angle[k] + VEC / 2 + i / 2];
-                        const float x = lo[k][i], y = lo[k][i + 1], z = hi[k][i], w = hi[k][i + 1];
-                        lo[k][i] = x * c.x - y * c.y; lo[k][i + 1] = x * c.y + y * c.x;
-                        hi[k][i] = z * d.x - w * d.y; hi[k][i + 1] = z * d.y + w * d.x;
-                    }
+                for (int k = 0; k < ROT_UNROLL; ++k) {
+                    const int hk = h + k * head_step;
+                    if (hk < last) { const E* src = source(hk) + at; lo[k] = *reinterpret_cast<const Piece*>(src); hi[k] = *reinterpret_cast<const Piece*>(src + step); }
                 }
-            }
-            rot_write(dst[k], lo[k]); rot_write(dst[k] + step[k], hi[k]);
+                if (!angles) {
+                    if (threadIdx.x < pairs) {
+                        const double full = p * turns;
+                        float s, c;
+                        sincospif((float)(2.0 * (full - rint(full))), &s, &c);
+                        cosines[phase][threadIdx.x] = c * a.amplitude; sines[phase][threadIdx.x] = s * a.amplitude;
+                    }
+                    __syncthreads();                            // of the other phase's readers too: they are through with the token before
+                    angles = true;
+                }
+                if (h == head0 && r < turned) { rot_angles<VEC>(&cosines[phase][r * VEC], cn); rot_angles<VEC>(&sines[phase][r * VEC], sn); }
+#pragma unroll
+                for (int k = 0; k < ROT_UNROLL; ++k) {
+                    const int hk = h + k * head_step;
+                    if (hk >= last) continue;
+                    if (r < turned && (!CACHE || hk < a.n_heads + a.n_kv)) {
+                        float u[VEC], w[VEC];
+                        rot_unpack(lo[k], u); rot_unpack(hi[k], w);
+                        if constexpr (HALVES || VEC == 1) {
+#pragma unroll
+                            for (int i = 0; i < VEC; ++i) { const float m = u[i], n = w[i]; u[i] = m * cn[i] - n * sn[i]; w[i] = m * sn[i] + n * cn[i]; }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < VEC; i += 2) {
+                                const int j = i / 2, l = VEC / 2 + j;
+                                const float m = u[i], n = u[i + 1], o = w[i], q = w[i + 1];
+                                u[i] = m * cn[j] - n * sn[j]; u[i + 1] = m * sn[j] + n * cn[j];
+                                w[i] = o * cn[l] - q * sn[l]; w[i + 1] = o * sn[l] + q * cn[l];
+                            }
+                        }
+                        rot_pack(lo[k], u); rot_pack(hi[k], w);
+                    }
+                    E* dst = place(hk) + at;
+                    *reinterpret_cast<Piece*>(dst) = lo[k]; *reinterpret_cast<Piece*>(dst + step) = hi[k];
+                }
+                h += ROT_UNROLL * head_step;
+            } while (h < last);
         }
     }
 }
@@ -124,10 +145,15 @@ static cudaError_t launch_rotary_e(const RotaryArgs& a, bool halves, cudaStream_
     const bool cache = a.cache != nullptr;
     auto kern = halves ? rotary_kernel<E, VEC, true, false> : rotary_kernel<E, VEC, false, false>;
     if constexpr (sizeof(E) == 2) if (cache) kern = halves ? rotary_kernel<E, VEC, true, true> : rotary_kernel<E, VEC, false, true>;      // a cache of pages is bf16
-    const int64_t units = (int64_t)(a.n_heads + (cache ? 2 * a.n_kv : 0)) * (a.head_dim / (2 * VEC));
-    // few tokens: a token's heads over several CTAs, so that each thread has one unit or two
-    const int64_t parts = a.T >= 148 ? 1 : (units + ROT_THREADS - 1) / ROT_THREADS;
-    return launch_k(kern, dim3(a.T, (unsigned)(parts < 1 ? 1 : parts > 64 ? 64 : parts)), dim3(ROT_THREADS), 0, s, a);
+    const int per_head = a.head_dim / (2 * VEC), down = ROT_THREADS / (per_head < ROT_THREADS ? per_head : ROT_THREADS);
+    const int heads = a.n_heads + (cache ? 2 * a.n_kv : 0);
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return e;
+    // few tokens: a token's heads over several CTAs, a unit a thread
+    const int parts = a.T >= sms ? 1 : (heads + down - 1) / down;
+    return launch_k(kern, dim3(a.T < ROT_CTAS * sms ? a.T : ROT_CTAS * sms, parts > 64 ? 64 : parts), dim3(ROT_THREADS), 0, s, a);
 }
 
 cudaError_t launch_rotary(const RotaryArgs& a, int layout, bool f32, cudaStream_t s) {
