@@ -88,9 +88,9 @@ struct PreCfg {
     static constexpr int Q_HALF = ROW_TILE * 128, KV_HALF = KEYS * 128;          // rows x 64 bf16 columns under the 128-byte swizzle
     static constexpr int Q_BYTES = HALVES * Q_HALF, TILE_BYTES = HALVES * KV_HALF;
     static constexpr int THREADS = 64 + PRE_SOFTMAX;             // producer, issuer, softmax warps
-    static constexpr int XCH_BYTES = (2 * 2 + 2) * 128 * 4;      // a row's two maxima of a tile, [tile parity][warpgroup][row], and its two sums of a piece
+    static constexpr int XCH_BYTES = 3 * 128 * 4;                // a row's reference maximum, and its two sums of a piece
     static constexpr int SMEM_BYTES = Q_BYTES + SLOTS * TILE_BYTES + 256 + XCH_BYTES;
-    static constexpr uint32_t O_COL = 256;                       // TMEM: S and P of the tiles in turn at 0 and 128, O at 256
+    static constexpr uint32_t O_COL = 384;                       // TMEM: S and P of the tiles in turn at 0, 128 and 256, O at 384
 };
 struct PrePiece { int g, kvh, tile, k0, k1; };
 OA_DEVINL PrePiece pre_piece(const PrefixPieces& px, int piece, int n_prefixes) {
@@ -110,7 +110,7 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
     uint8_t* q_s = smem;
     uint8_t* kv_s = q_s + Cfg::Q_BYTES;
     uint64_t* bars = reinterpret_cast<uint64_t*>(kv_s + SLOTS * Cfg::TILE_BYTES);
-    uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_full = bars + 4, *t_full = bars + 6, *o_full = bars + 7, *full = bars + 8, *empty = full + SLOTS;
+    uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_full = bars + 5, *o_full = bars + 8, *full = bars + 12, *empty = full + SLOTS;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(empty + SLOTS);
     float* xch = reinterpret_cast<float*>(kv_s + SLOTS * Cfg::TILE_BYTES + 256);
     __shared__ PrefixPieces px;
@@ -119,8 +119,9 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
     const int grp = a.n_heads / a.n_kv, tile_tokens = ROW_TILE / grp;      // tokens of a row tile
     if (warp == 0 && lane == 0) {
         tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_kv);
-        mbar_init(q_full, 1); mbar_init(q_empty, 1); mbar_init(t_full, 1); mbar_init(o_full, 1);
-        for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], PRE_SOFTMAX / 32); }
+        mbar_init(q_full, 1); mbar_init(q_empty, 1);
+        for (int i = 0; i < 3; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], PRE_SOFTMAX / 64); }
+        for (int i = 0; i < 4; ++i) mbar_init(&o_full[i], 1);
         for (int i = 0; i < SLOTS; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         fence_barrier_init();
     }
@@ -132,7 +133,7 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
     __syncthreads();
     tcgen05_fence_after();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-    // Keys and values share one ring in the order of their products: K_0, then K_(j+1) and V_j
+    // Keys and values share one ring in the order of their products: K_0 and K_1, then K_(j+2) and V_j
     if (warp == 0) {
         uint32_t n = 0, seg = 0;                                 // tiles and pieces loaded
         for (int piece = blockIdx.x; piece < px.pieces; piece += gridDim.x, ++seg) {
@@ -147,18 +148,17 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
             __syncwarp();
             const int32_t* bt = a.prefix_tables + (size_t)sg.g * a.max_prefix_pages;
             const int pages = pages_of(px.len[sg.g]);
-            int page[PAGES] = {}, prev[PAGES] = {};
-            for (int j = 0; j <= sg.k1 - sg.k0; ++j) {
-                const int kt = sg.k0 + j;
+            int page[3][PAGES] = {};                             // of this tile and of the two before
+            for (int kt = sg.k0; kt < sg.k1 + 2; ++kt) {
 #pragma unroll
                 for (int i = 0; i < PAGES; ++i) {
-                    prev[i] = page[i];
-                    page[i] = kt < sg.k1 && PAGES * kt + i < pages ? bt[PAGES * kt + i] : 0;
-                    if (page[i] < 0 || page[i] >= a.num_pages) { if (lane == 0) report(a); page[i] = 0; }
+                    page[2][i] = page[1][i]; page[1][i] = page[0][i];
+                    page[0][i] = kt < sg.k1 && PAGES * kt + i < pages ? bt[PAGES * kt + i] : 0;
+                    if (page[0][i] < 0 || page[0][i] >= a.num_pages) { if (lane == 0) report(a); page[0][i] = 0; }
                 }
 #pragma unroll
                 for (int v = 0; v < 2; ++v) {
-                    const int t = kt - v;                        // K of this tile, V of the one before
+                    const int t = kt - 2 * v;                    // K of this tile, V of the one two before
                     if (t < sg.k0 || t >= sg.k1) continue;
                     const uint32_t slot = n % SLOTS;
                     mbar_wait(&empty[slot], ((n / SLOTS) & 1) ^ 1);
@@ -169,7 +169,7 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
 #pragma unroll
                         for (int i = 0; i < PAGES; ++i) {
                             if (i >= there) break;
-                            const int row = ((v ? a.num_pages + prev[i] : page[i]) * a.n_kv + sg.kvh) * CACHE_PAGE;
+                            const int row = ((v ? a.num_pages + page[2][i] : page[0][i]) * a.n_kv + sg.kvh) * CACHE_PAGE;
 #pragma unroll
                             for (int h = 0; h < HALVES; ++h) tma_load_2d(dst + h * Cfg::KV_HALF + i * 8192, &tm_kv, &full[slot], h * 64, row, kEvictLast);
                         }
@@ -184,24 +184,13 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
         constexpr uint32_t idesc_s = umma_idesc_bf16(128, KEYS), idesc_o = umma_idesc_bf16_bmn(128, D);
         const uint64_t q_desc = umma_desc_sw128(smem_u32(q_s)), k_desc = umma_desc_sw128(smem_u32(kv_s));
         const uint64_t v_desc = umma_desc_sw128_mn(smem_u32(kv_s), (uint32_t)Cfg::KV_HALF, 1024u);
-        uint32_t n = 0, r = 0, seg = 0;                          // tiles, tiles of the ring, pieces
-        auto issue_s = [&](uint32_t n, bool last) {
+        uint32_t n = 0, r = 0, seg = 0;                          // tiles of the pieces before, tiles of the ring, pieces
+        auto await = [&] {                                       // the ring's next tile
             const uint32_t slot = r % SLOTS;
             mbar_wait(&full[slot], (r / SLOTS) & 1);
             ++r;
             tcgen05_fence_after();
-            if (elect_one()) {
-                const uint64_t b = k_desc + (uint64_t)(slot * (Cfg::TILE_BYTES >> 4));
-#pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks) {
-                    const int half = ks >> 2, in = (ks & 3) * 32;
-                    umma_bf16(tmem_base + (n & 1) * 128, q_desc + (uint64_t)((half * Cfg::Q_HALF + in) >> 4), b + (uint64_t)((half * Cfg::KV_HALF + in) >> 4), idesc_s, ks > 0 ? 1u : 0u);
-                }
-                umma_commit(&s_full[n & 1]);
-                umma_commit(&empty[slot]);
-                if (last) umma_commit(q_empty);
-            }
-            __syncwarp();
+            return slot;
         };
         // products of one thread are carried out in the order of their issue: S of a tile goes over scores whose P a product ahead of it reads
         for (int piece = blockIdx.x; piece < px.pieces; piece += gridDim.x, ++seg) {
@@ -209,120 +198,158 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
             const int tiles = sg.k1 - sg.k0;
             mbar_wait(q_full, seg & 1);
             tcgen05_fence_after();
-            issue_s(n, tiles == 1);
-            for (int j = 0; j < tiles; ++j, ++n) {
-                if (j + 1 < tiles) issue_s(n + 1, j + 2 == tiles);               // the next tile's scores under this one's softmax
-                const uint32_t slot = r % SLOTS;
-                mbar_wait(&p_full[n & 1], (n >> 1) & 1);
-                mbar_wait(&full[slot], (r / SLOTS) & 1);
-                ++r;
-                tcgen05_fence_after();
-                if (elect_one()) {
-                    const uint64_t b = v_desc + (uint64_t)(slot * (Cfg::TILE_BYTES >> 4));
+            for (int j = -2; j < tiles; ++j) {
+                if (j + 2 < tiles) {                                             // scores two tiles ahead, under the softmaxes of the tiles before
+                    const uint32_t slot = await(), at = (n + j + 2) % 3;
+                    if (elect_one()) {
+                        const uint64_t b = k_desc + (uint64_t)(slot * (Cfg::TILE_BYTES >> 4));
 #pragma unroll
-                    for (int ks = 0; ks < KEYS / 16; ++ks)
-                        umma_bf16_ta(tmem_base + Cfg::O_COL, tmem_base + (n & 1) * 128 + ks * 8, b + (uint64_t)(ks * (2048 >> 4)), idesc_o, (j > 0 || ks > 0) ? 1u : 0u);
-                    umma_commit(j + 1 < tiles ? t_full : o_full);
-                    umma_commit(&empty[slot]);
+                        for (int ks = 0; ks < D / 16; ++ks) {
+                            const int half = ks >> 2, in = (ks & 3) * 32;
+                            umma_bf16(tmem_base + at * 128, q_desc + (uint64_t)((half * Cfg::Q_HALF + in) >> 4), b + (uint64_t)((half * Cfg::KV_HALF + in) >> 4), idesc_s, ks > 0 ? 1u : 0u);
+                        }
+                        umma_commit(&s_full[at]);
+                        umma_commit(&empty[slot]);
+                        if (j + 3 == tiles) umma_commit(q_empty);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
+                if (j >= 0) {
+                    const uint32_t m = n + j, at = m % 3;
+                    mbar_wait(&p_full[at], (m / 3) & 1);
+                    const uint32_t slot = await();
+                    if (elect_one()) {
+                        const uint64_t b = v_desc + (uint64_t)(slot * (Cfg::TILE_BYTES >> 4));
+#pragma unroll
+                        for (int ks = 0; ks < KEYS / 16; ++ks)
+                            umma_bf16_ta(tmem_base + Cfg::O_COL, tmem_base + at * 128 + ks * 8, b + (uint64_t)(ks * (2048 >> 4)), idesc_o, (j > 0 || ks > 0) ? 1u : 0u);
+                        umma_commit(&o_full[m & 3]);
+                        umma_commit(&empty[slot]);
+                    }
+                    __syncwarp();
+                }
             }
+            n += tiles;
         }
     } else {
-        // Warps w and w + 4 of the eight hold the same 32 rows and half of every tile's keys each (and of O's columns where those are rescaled or written)
-        const int quarter = warp & 3, row = quarter * 32 + lane, wg = (warp - 2) >> 2;
-        const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16, o_addr = tmem_base + lane_addr + Cfg::O_COL;
+        // Two warpgroups take the tiles in turn, a row a thread: one's exponentials run under the other's loads and maxima.  A row's reference maximum goes from one to the other
+        // with each tile, as soon as the tile's own maximum is known; sums stay with either, O is one for both
+        const int quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t wg = (warp - 2) >> 2, lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16), o_addr = lane_addr + Cfg::O_COL;
+        float *m_s = xch, *l_s = xch + 128;
         auto meet = [] { asm volatile("bar.sync 2, %0;" ::"n"(PRE_SOFTMAX) : "memory"); };
+        auto take_turn = [](uint32_t n) {                                        // tile n - 1 has left its reference
+            if (n & 1) asm volatile("bar.sync 3, %0;" ::"n"(PRE_SOFTMAX) : "memory"); else asm volatile("bar.sync 4, %0;" ::"n"(PRE_SOFTMAX) : "memory");
+        };
+        auto pass_turn = [](uint32_t n) {                                        // to tile n
+            if (n & 1) asm volatile("bar.arrive 3, %0;" ::"n"(PRE_SOFTMAX) : "memory"); else asm volatile("bar.arrive 4, %0;" ::"n"(PRE_SOFTMAX) : "memory");
+        };
         constexpr float kRaise = 8.0f;                                           // log2 units a score may pass the reference by
-        constexpr int MINE = KEYS / 2, CH = MINE / 32, COLS = D / 2;               // keys and 32-key chunks of a thread
-        uint32_t n = 0, r = 0, seg = 0, landed = 0;                              // landed: completions of t_full before this piece
-        for (int piece = blockIdx.x; piece < px.pieces; piece += gridDim.x, ++seg) {
+        constexpr int COLS = D / 2;
+        uint32_t n0 = 0;                                                         // tiles of the pieces before
+        for (int piece = blockIdx.x; piece < px.pieces; piece += gridDim.x) {
             const PrePiece sg = pre_piece(px, piece, a.n_prefixes);
             const bool live = row < tile_tokens * grp && sg.tile * tile_tokens + row / grp < px.rows[sg.g];
             const int tiles = sg.k1 - sg.k0, len = px.len[sg.g];
-            float m_ref = -INFINITY, l_run = 0.f;
-            for (int j = 0; j < tiles; ++j, ++n) {
-                const uint32_t sb = n & 1;
-                const int valid = len - (sg.k0 + j) * KEYS;                      // keys of this tile
-                mbar_wait(&s_full[sb], (n >> 1) & 1);
+            const uint32_t n1 = n0 + tiles;
+            float m_mine = -INFINITY, l_run = 0.f;                               // the sum so far and the reference that it is under
+            for (uint32_t n = n0 + ((n0 ^ wg) & 1); n < n1; n += 2) {
+                const int valid = len - (sg.k0 + (int)(n - n0)) * KEYS;          // keys of this tile
+                const uint32_t at = n % 3, s_addr = lane_addr + at * 128;
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};     // four chains
+                mbar_wait(&s_full[at], (n / 3) & 1);
                 tcgen05_fence_after();
-                uint32_t v[CH][32];
+#pragma unroll 1
+                for (int k = 0; k < KEYS; k += 64) {
+                    uint32_t v[2][32];
+                    tmem_ld_32x32b_x32(s_addr + k, v[0]);
+                    tmem_ld_32x32b_x32(s_addr + k + 32, v[1]);
+                    tmem_ld_wait();
+                    if (valid < k + 64) {                                        // keys behind the end: -inf, also for the second reading
 #pragma unroll
-                for (int c = 0; c < CH; ++c) tmem_ld_32x32b_x32(tmem_base + lane_addr + sb * 128 + wg * MINE + c * 32, v[c]);
-                tmem_ld_wait();
+                        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) if (c * 32 + i >= valid - k) v[c][i] = 0xff800000u;
+                            tmem_st_32x32b_x32(s_addr + k + c * 32, v[c]);
+                        }
+                    }
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[c][i]));
+                }
+                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2e;
+                if (n > 0) take_turn(n);
+                // A barrier's phases are seen one by one: PV of the tile three before is the last one that this tile can be sure of without a wait
+                if (n > 2) mbar_wait(&o_full[(n - 3) & 3], ((n - 3) >> 2) & 1);
+                const float m_last = n > n0 ? m_s[row] : -INFINITY;
+                const bool raise = mx > m_last + kRaise;
+                const float m_ref = raise ? mx : m_last;
+                m_s[row] = m_ref;
+                if (n + 1 < n1 || piece + (int)gridDim.x < px.pieces) pass_turn(n + 1);
+                if (n > n0 && (valid < KEYS || __any_sync(0xffffffffu, raise))) {
+                    mbar_wait(&o_full[(n - 1) & 3], ((n - 1) >> 2) & 1);         // O has the products of all tiles before; this tile's are not issued before p_full
+                    tcgen05_fence_after();
+                    const float alpha = raise ? exp2f(m_last - m_ref) : 1.0f;
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 16) {
+                        uint32_t o[16];
+                        tmem_ld_32x32b_x16(o_addr + c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        tmem_st_32x32b_x16(o_addr + c, o);
+                    }
+                }
                 if (valid < KEYS) {
-#pragma unroll
-                    for (int c = 0; c < CH; ++c)
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) if (wg * MINE + c * 32 + i >= valid) v[c][i] = 0xff800000u;
-                    // values behind the end may be anything, and 0 x inf is not 0; only the last tile of a prefix ends early, and its V is the last of the piece's 2 tiles
-                    const uint32_t at = r + 2 * tiles - 1, slot = at % SLOTS;
-                    mbar_wait(&full[slot], (at / SLOTS) & 1);
+                    tmem_st_wait();
+                    // values behind the end may be anything, and 0 x inf is not 0; only the last tile of a prefix ends early, and its V is the last of the pieces' tiles so far
+                    const uint32_t last = 2 * n1 - 1, slot = last % SLOTS;
+                    mbar_wait(&full[slot], (last / SLOTS) & 1);
                     if (row >= valid && row < KEYS) {
 #pragma unroll
-                        for (int c = 0; c < D / 16; ++c) {
-                            const int chunk = wg * (D / 16) + c;
-                            *reinterpret_cast<uint4*>(kv_s + slot * Cfg::TILE_BYTES + (chunk >> 3) * Cfg::KV_HALF + row * 128 + (chunk & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                        }
+                        for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(kv_s + slot * Cfg::TILE_BYTES + (c >> 3) * Cfg::KV_HALF + row * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
                     }
                     fence_proxy_async();
                 }
-                float mraw = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < CH; ++c)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) mraw = fmaxf(mraw, __uint_as_float(v[c][i]));
-                float* maxima = xch + (n & 1) * 256;
-                maxima[wg * 128 + row] = mraw;
-                meet();                                                          // and both halves of S are in registers: P may go over them
-                mraw = fmaxf(mraw, maxima[(wg ^ 1) * 128 + row]);
-                const float mx = mraw * a.scale_log2e;
-                const bool raise = mx > m_ref + kRaise;                          // the same in both warps of a row
-                if (__any_sync(0xffffffffu, raise)) {
-                    if (j > 0) {
-                        mbar_wait(t_full, (landed + j - 1) & 1);                 // O has the products of the tile before; this tile's are not issued before p_full
-                        tcgen05_fence_after();
-                        const float alpha = raise ? exp2f(m_ref - mx) : 1.0f;
-#pragma unroll 1
-                        for (int c = 0; c < COLS; c += 16) {                     // the scores stay in registers meanwhile
-                            uint32_t o[16];
-                            tmem_ld_32x32b_x16(o_addr + wg * COLS + c, o);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                            tmem_st_32x32b_x16(o_addr + wg * COLS + c, o);
-                        }
-                        l_run *= alpha;
-                    }
-                    if (raise) m_ref = mx;
-                }
+                if (m_mine != m_ref) { l_run *= ex2_approx(m_mine - m_ref); m_mine = m_ref; }
                 const float neg_ref = -finite_or_zero(m_ref);
                 uint64_t sum = 0;
+#pragma unroll 1
+                for (int k = 0; k < KEYS; k += 64) {                             // read again: P of the keys before lies over their own scores
+                    uint32_t v[2][32];
+                    tmem_ld_32x32b_x32(s_addr + k, v[0]);
+                    tmem_ld_32x32b_x32(s_addr + k + 32, v[1]);
+                    tmem_ld_wait();
 #pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                    uint32_t w[16];
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t w[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float x = ex2_approx(fmaf(__uint_as_float(v[c][2 * i]), a.scale_log2e, neg_ref)), y = ex2_approx(fmaf(__uint_as_float(v[c][2 * i + 1]), a.scale_log2e, neg_ref));
-                        sum = add_f32x2(sum, pack_f32x2(x, y));
-                        w[i] = pack_bf16x2(x, y);
+                        for (int i = 0; i < 16; ++i) {
+                            const float x = ex2_approx(fmaf(__uint_as_float(v[c][2 * i]), a.scale_log2e, neg_ref)), y = ex2_approx(fmaf(__uint_as_float(v[c][2 * i + 1]), a.scale_log2e, neg_ref));
+                            sum = add_f32x2(sum, pack_f32x2(x, y));
+                            w[i] = pack_bf16x2(x, y);
+                        }
+                        tmem_st_32x32b_x16(s_addr + k / 2 + c * 16, w);
                     }
-                    tmem_st_32x32b_x16(tmem_base + lane_addr + sb * 128 + wg * (MINE / 2) + c * 16, w);
                 }
                 tmem_st_wait();
                 tcgen05_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[sb]);
-                float even, odd; unpack_f32x2(sum, even, odd);
-                l_run += even + odd;
+                if (lane == 0) mbar_arrive(&p_full[at]);
+                float lo, hi; unpack_f32x2(sum, lo, hi);
+                l_run += lo + hi;
             }
-            landed += tiles - 1; r += 2 * tiles;
-            xch[512 + wg * 128 + row] = l_run;                                   // the piece's before was read ahead of this one's tiles' barriers
-            mbar_wait(o_full, seg & 1);
+            n0 = n1;
+            meet();                                                              // the last tile's reference is there
+            const float m_ref = m_s[row];
+            if (m_mine != m_ref) l_run *= ex2_approx(m_mine - m_ref);
+            l_s[wg * 128 + row] = l_run;
+            mbar_wait(&o_full[(n1 - 1) & 3], ((n1 - 1) >> 2) & 1);
             tcgen05_fence_after();
             float* po = a.pre_o + (int64_t)piece * (ROW_TILE * D) + row * 4;     // [D / 4][128 rows][4]: a warp's rows lie next to each other
 #pragma unroll 1
-            for (int c = wg * COLS; c < (wg + 1) * COLS; c += 32) {
+            for (int c = wg * COLS; c < (int)(wg + 1) * COLS; c += 32) {
                 uint32_t o[32];
                 tmem_ld_32x32b_x32(o_addr + c, o);
                 tmem_ld_wait();
@@ -332,8 +359,8 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
                         *reinterpret_cast<float4*>(po + (c + i) / 4 * (ROW_TILE * 4)) = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
             }
             tcgen05_fence_before();
-            meet();
-            if (live && wg == 0) *reinterpret_cast<float2*>(a.pre_ml + ((int64_t)piece * ROW_TILE + row) * 2) = make_float2(m_ref, l_run + xch[512 + 128 + row]);
+            meet();                                                              // O may be written again, and both sums are there
+            if (live && wg == 0) *reinterpret_cast<float2*>(a.pre_ml + ((int64_t)piece * ROW_TILE + row) * 2) = make_float2(m_ref, l_run + l_s[128 + row]);
         }
     }
     __syncthreads();

@@ -215,13 +215,13 @@ def test_cache_copy(L, planes, pages, n_kv, dim, dtype, n, tokens):
 class Batch:
     """Pages anywhere in a cache whose unused places hold NaN."""
 
-    def __init__(self, heads, n_kv, dim, prefixes, runs, own, seed=0, spare=3, pad=0, scale_q=1.0):
+    def __init__(self, heads, n_kv, dim, prefixes, runs, own, seed=0, spare=3, pad=0, scale_q=1.0, wide=1):
         self.heads, self.n_kv, self.dim, self.prefixes, self.runs, self.own = heads, n_kv, dim, list(prefixes), list(runs), list(own)
         n, rng = len(self.own), np.random.default_rng(seed)
         need = [-(-x // PAGE) for x in self.prefixes + self.own]
         self.pages = sum(need) + spare
         order, at = rng.permutation(self.pages), 0
-        width = [max([1] + need[: len(prefixes)]), max(need[len(prefixes):] + [1]) + 1]
+        width = [max([wide] + need[: len(prefixes)]), max(need[len(prefixes):] + [1]) + 1]
         self.pt, self.ot = np.full((max(1, len(prefixes)), width[0]), -7, np.int32), np.full((max(1, n), width[1]), 10 ** 9, np.int32)
         for i, k in enumerate(need):
             (self.pt[i] if i < len(prefixes) else self.ot[i - len(prefixes)])[:k] = order[at:at + k]
@@ -341,6 +341,19 @@ def test_batches(L, heads, n_kv, dim, n, prefix, top):
     for _ in range(5):                                                           # the same call gives the same bits
         run(L, b)
         assert torch.equal(b.out.view(torch.int16), first.view(torch.int16))
+
+
+# tables with room for prefixes far longer than these: rows are taken two tiles at a time, whose second one may have no rows
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,n_kv,prefixes,runs,wide", [
+    (32, 2, [1000], [0, 17], 400), (5, 1, [64, 0, 129, 700], [0, 9, 9, 36, 63], 900), (12, 12, [300, 257], [1, 130, 140], 120), (16, 4, [1, 2000, 63], [0, 33, 97, 104], 200), (48, 3, [640], [2, 11], 400)])
+def test_tables_with_room_for_long_prefixes(L, heads, n_kv, prefixes, runs, wide, dim):
+    b = Batch(heads, n_kv, dim, prefixes, runs, [(i * 31) % 140 for i in range(runs[-1] + 1)], seed=heads, wide=wide)
+    run(L, b)
+    b.check()
+    first = b.out.clone()
+    run(L, b)
+    assert torch.equal(first, b.out) and b.status.item() == 0
 
 
 def test_one_long_sequence(L):
