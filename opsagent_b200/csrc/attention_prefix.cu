@@ -103,7 +103,9 @@ OA_DEVINL PrePiece pre_piece(const PrefixPieces& px, int piece, int n_prefixes) 
 }
 
 template <int D, int KEYS, int SLOTS>
-__global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ PrefixAttnArgs a) {
+// 104 registers: one CTA and one of the own parts' (96) fill an SM's file, two of this kernel do not fit (of 96 they would).  Started while the kernel before it leaves the SMs one by one, two
+// CTAs on one SM would have the second wait for the first one's TMEM, and the own parts' CTA go elsewhere: 8 to 15 us of a call of 45
+__global__ void __maxnreg__(104) prefix_part_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ PrefixAttnArgs a) {
     using Cfg = PreCfg<D, KEYS, SLOTS>;
     constexpr int HALVES = Cfg::HALVES, PAGES = KEYS / CACHE_PAGE;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -259,9 +261,9 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};     // four chains
                 mbar_wait(&s_full[at], (n / 3) & 1);
                 tcgen05_fence_after();
+                uint32_t v[2][32];
 #pragma unroll 1
-                for (int k = 0; k < KEYS; k += 64) {
-                    uint32_t v[2][32];
+                for (int k = KEYS - 64; k >= 0; k -= 64) {                       // the lower keys last: they stay in registers
                     tmem_ld_32x32b_x32(s_addr + k, v[0]);
                     tmem_ld_32x32b_x32(s_addr + k + 32, v[1]);
                     tmem_ld_wait();
@@ -316,11 +318,12 @@ __global__ void __maxnreg__(96) prefix_part_kernel(const __grid_constant__ CUten
                 const float neg_ref = -finite_or_zero(m_ref);
                 uint64_t sum = 0;
 #pragma unroll 1
-                for (int k = 0; k < KEYS; k += 64) {                             // read again: P of the keys before lies over their own scores
-                    uint32_t v[2][32];
-                    tmem_ld_32x32b_x32(s_addr + k, v[0]);
-                    tmem_ld_32x32b_x32(s_addr + k + 32, v[1]);
-                    tmem_ld_wait();
+                for (int k = 0; k < KEYS; k += 64) {
+                    if (k > 0) {                                                 // read again: P of the keys before lies over their own scores
+                        tmem_ld_32x32b_x32(s_addr + k, v[0]);
+                        tmem_ld_32x32b_x32(s_addr + k + 32, v[1]);
+                        tmem_ld_wait();
+                    }
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         uint32_t w[16];
@@ -418,7 +421,7 @@ struct OwnAt {
 };
 
 template <int D, bool WIDE, int STAGES>
-__global__ void __maxnreg__(WIDE ? 168 : 104) own_part_kernel(const __grid_constant__ CUtensorMap tm_page, const __grid_constant__ CUtensorMap tm_part, const __grid_constant__ PrefixAttnArgs a) {
+__global__ void __maxnreg__(WIDE ? 168 : 96) own_part_kernel(const __grid_constant__ CUtensorMap tm_page, const __grid_constant__ CUtensorMap tm_part, const __grid_constant__ PrefixAttnArgs a) {
     using Cfg = OwnCfg<D, WIDE, STAGES>;
     constexpr int KS = D / 16, ROWS = Cfg::ROWS, NB = Cfg::BLOCKS;
     extern __shared__ __align__(1024) uint8_t smem[];
