@@ -421,7 +421,7 @@ struct OwnAt {
 };
 
 template <int D, bool WIDE, int STAGES>
-__global__ void __maxnreg__(WIDE ? 168 : 96) own_part_kernel(const __grid_constant__ CUtensorMap tm_page, const __grid_constant__ CUtensorMap tm_part, const __grid_constant__ PrefixAttnArgs a) {
+__global__ void __maxnreg__(WIDE ? 168 : 96) own_part_kernel(const __grid_constant__ CUtensorMap tm_page, const __grid_constant__ PrefixAttnArgs a) {
     using Cfg = OwnCfg<D, WIDE, STAGES>;
     constexpr int KS = D / 16, ROWS = Cfg::ROWS, NB = Cfg::BLOCKS;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -441,7 +441,7 @@ __global__ void __maxnreg__(WIDE ? 168 : 96) own_part_kernel(const __grid_consta
     const int per = (a.n_seqs + OWN_THREADS - 1) / OWN_THREADS, s0 = threadIdx.x * per, s1 = min(a.n_seqs, s0 + per);
     const int first_len = OwnAt::length(a, s0);
     if (threadIdx.x == 0) {
-        tma_prefetch_desc(&tm_page); tma_prefetch_desc(&tm_part);
+        tma_prefetch_desc(&tm_page);
         for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], OWN_CONSUMERS / 32); }
         for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], OWN_CONSUMERS / 32); }
         mbar_init(states_full, OWN_CONSUMERS / 32); mbar_init(states_empty, 1);
@@ -514,29 +514,17 @@ __global__ void __maxnreg__(WIDE ? 168 : 96) own_part_kernel(const __grid_consta
                     if (next_seq >= 0) next = block_of(next_seq, next_block, a.max_own_pages);
                 }
                 int page = __shfl_sync(0xffffffffu, have, c & 31);
-                const int valid = min(CACHE_PAGE, at.tokens(c));
                 if (page < 0 || page >= a.num_pages) { if (lane == 0) report(a); page = 0; }
                 mbar_wait(&empty_bar[s], ph ^ 1);
                 if (lane == 0) {
                     uint8_t* kdst = smem + s * Cfg::STAGE_BYTES;
                     uint8_t* vdst = kdst + Cfg::KV_BYTES;
                     const int krow = (page * a.n_kv + at.kvh) * CACHE_PAGE, vrow = krow + a.num_pages * a.n_kv * CACHE_PAGE;
-                    if (valid > 48) {
-                        mbar_expect_tx(&full_bar[s], Cfg::STAGE_BYTES);
+                    mbar_expect_tx(&full_bar[s], Cfg::STAGE_BYTES);                          // whole pages, also those that end early: pieces of 16 tokens were 0.7 us of 40 faster for own parts of 64 to 512 tokens, 0.5 us of 25 slower for 1 to 40
 #pragma unroll
-                        for (int h = 0; h < Cfg::HALVES; ++h) {
-                            tma_load_2d(kdst + h * Cfg::TILE_BYTES, &tm_page, &full_bar[s], h * 64, krow, kEvictFirst);
-                            tma_load_2d(vdst + h * Cfg::TILE_BYTES, &tm_page, &full_bar[s], h * 64, vrow, kEvictFirst);
-                        }
-                    } else {                                                                 // a page that ends early: pieces of 16 tokens
-                        const int n = (valid + 15) / 16;
-                        mbar_expect_tx(&full_bar[s], n * 2 * Cfg::HALVES * 16 * 128);
-                        for (int i = 0; i < n; ++i)
-#pragma unroll
-                            for (int h = 0; h < Cfg::HALVES; ++h) {
-                                tma_load_2d(kdst + h * Cfg::TILE_BYTES + i * 2048, &tm_part, &full_bar[s], h * 64, krow + i * 16, kEvictFirst);
-                                tma_load_2d(vdst + h * Cfg::TILE_BYTES + i * 2048, &tm_part, &full_bar[s], h * 64, vrow + i * 16, kEvictFirst);
-                            }
+                    for (int h = 0; h < Cfg::HALVES; ++h) {
+                        tma_load_2d(kdst + h * Cfg::TILE_BYTES, &tm_page, &full_bar[s], h * 64, krow, kEvictFirst);
+                        tma_load_2d(vdst + h * Cfg::TILE_BYTES, &tm_page, &full_bar[s], h * 64, vrow, kEvictFirst);
                     }
                 }
                 __syncwarp();
@@ -798,13 +786,18 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_parts_kernel(const __grid_c
 // =============================================================================================
 // host
 // =============================================================================================
-constexpr int PREFIX_LONG_UNITS = 16, PREFIX_INLINE_ROWS = 4, PREFIX_INLINE_UNITS = 4;
+// Prefixes are read with the sequences' own parts, once for each sequence, where that is few pages: two launches instead of three.  us with one kernel / two, heads of 64, own parts of
+// 50 to 200 tokens, rows x prefix: 4 x 256 9.0 / 10.0, 8 x 1024 11.5 / 13.1, 8 x 4096 20.1 / 15.2; 16 x 256 10.6 / 11.2, 32 x 128 12.2 / 13.0, 16 x 512 11.9 / 10.8, 32 x 256 13.5 / 12.8 (128 the same way)
+constexpr int PREFIX_INLINE_UNITS = 4, PREFIX_FEW_ROWS = 8;           // pages an SM; up to so many rows twice as many
+// Heads of 128: an SM's shared memory holds tiles of 64 keys beside four of the own parts' pages, or tiles of 128 beside two.  us with 64 / 128, own parts of 20 to 600 tokens: 128 rows of
+// 4 heads a group on a prefix of 1024 41.2 / 45.7, 4096 44.5 / 48.5, 8192 48.9 / 51.8; 64 rows of 8 heads a group 1024 30.6 / 31.6, 4096 33.1 / 34.1, 6144 34.9 / 35.6, 8192 40.2 / 37.1
+constexpr int PREFIX_LONG_UNITS = 24;                                 // pages an SM
 PrefixAttnPlan prefix_attn_plan(int n_seqs, int n_heads, int n_kv, int head_dim, int n_prefixes, int max_prefix_pages, int max_own_pages, int sms) {
     PrefixAttnPlan p{};
     const int grp = n_heads / n_kv;
     const int tile_tokens = ROW_TILE / grp;
     const int64_t work = ((int64_t)n_seqs + tile_tokens - 1) / tile_tokens * n_kv * max_prefix_pages;       // pages, if one prefix has all rows
-    const bool apart = n_prefixes > 0 && !(n_seqs <= PREFIX_INLINE_ROWS && (int64_t)n_seqs * n_kv * max_prefix_pages <= PREFIX_INLINE_UNITS * (int64_t)sms);
+    const bool apart = n_prefixes > 0 && (int64_t)n_seqs * n_kv * max_prefix_pages > (n_seqs <= PREFIX_FEW_ROWS ? 2 : 1) * PREFIX_INLINE_UNITS * (int64_t)sms;
     const int64_t items = apart ? ((int64_t)n_seqs / tile_tokens + n_prefixes) * n_kv : 0;                              // no more row tiles than that, however rows fall on prefixes
     const int64_t units = items * max_prefix_pages, own_units = (int64_t)n_seqs * n_kv * (1 + (int64_t)max_own_pages + (apart ? 0 : max_prefix_pages));
     p.pre_ctas = (int)(units < sms ? units : sms);                                                                      // 0: prefixes are read with the sequences' own parts
@@ -830,11 +823,11 @@ static cudaError_t raise_smem(K kern, int bytes, bool (&done)[16]) {
     return e == cudaSuccess ? ensure_dynamic_smem(kern, bytes, done) : e;
 }
 template <int D, bool WIDE, int STAGES>
-static cudaError_t launch_own(const CUtensorMap* tm_page, const CUtensorMap* tm_part, const PrefixAttnArgs& a, cudaStream_t s) {
+static cudaError_t launch_own(const CUtensorMap* tm_page, const PrefixAttnArgs& a, cudaStream_t s) {
     auto kern = own_part_kernel<D, WIDE, STAGES>;
     static bool attr_done[16] = {};
     { const cudaError_t e = raise_smem(kern, OwnCfg<D, WIDE, STAGES>::SMEM_BYTES, attr_done); if (e != cudaSuccess) return e; }
-    return launch_k(kern, dim3(a.own_ctas), dim3(OWN_THREADS), OwnCfg<D, WIDE, STAGES>::SMEM_BYTES, s, *tm_page, *tm_part, a);
+    return launch_k(kern, dim3(a.own_ctas), dim3(OWN_THREADS), OwnCfg<D, WIDE, STAGES>::SMEM_BYTES, s, *tm_page, a);
 }
 template <int D, int KEYS, int SLOTS>
 static cudaError_t launch_prefixes(const CUtensorMap* tm_q, const CUtensorMap* tm_page, const PrefixAttnArgs& a, cudaStream_t s) {
@@ -854,18 +847,18 @@ static cudaError_t launch_join(const PrefixAttnArgs& a, cudaStream_t s) {
 }
 // KEYS, SLOTS: tiles and ring of the prefixes' kernel; PAGES: ring of the own parts'
 template <int D, int KEYS, int SLOTS, int PAGES>
-static cudaError_t launch_parts(const CUtensorMap* tm_q, const CUtensorMap* tm_page, const CUtensorMap* tm_part, const PrefixAttnArgs& a, cudaStream_t s) {
+static cudaError_t launch_parts(const CUtensorMap* tm_q, const CUtensorMap* tm_page, const PrefixAttnArgs& a, cudaStream_t s) {
     cudaError_t e = cudaSuccess;
     if (a.pre_ctas > 0) e = launch_prefixes<D, KEYS, SLOTS>(tm_q, tm_page, a, s);
-    if (e == cudaSuccess) e = a.n_heads / a.n_kv > 8 ? launch_own<D, true, PAGES>(tm_page, tm_part, a, s) : launch_own<D, false, PAGES>(tm_page, tm_part, a, s);
+    if (e == cudaSuccess) e = a.n_heads / a.n_kv > 8 ? launch_own<D, true, PAGES>(tm_page, a, s) : launch_own<D, false, PAGES>(tm_page, a, s);
     return e;
 }
-cudaError_t launch_prefix_attention(const CUtensorMap* tm_q, const CUtensorMap* tm_page, const CUtensorMap* tm_part, int head_dim, bool long_prefix, const PrefixAttnArgs& a, cudaStream_t s) {
+cudaError_t launch_prefix_attention(const CUtensorMap* tm_q, const CUtensorMap* tm_page, int head_dim, bool long_prefix, const PrefixAttnArgs& a, cudaStream_t s) {
     if (head_dim != 64 && head_dim != 128) return cudaErrorInvalidValue;
     // An SM's shared memory goes to both kernels: heads of 128 give the prefixes three tiles of 128 keys and the own parts two pages where prefixes are most of the work, two tiles
     // of 64 keys and four pages elsewhere
-    const cudaError_t e = head_dim == 64 ? launch_parts<64, 128, 3, 8>(tm_q, tm_page, tm_part, a, s)
-                        : long_prefix ? launch_parts<128, 128, 3, 2>(tm_q, tm_page, tm_part, a, s) : launch_parts<128, 64, 2, 4>(tm_q, tm_page, tm_part, a, s);
+    const cudaError_t e = head_dim == 64 ? launch_parts<64, 128, 3, 8>(tm_q, tm_page, a, s)
+                        : long_prefix ? launch_parts<128, 128, 3, 2>(tm_q, tm_page, a, s) : launch_parts<128, 64, 2, 4>(tm_q, tm_page, a, s);
     if (e != cudaSuccess) return e;
     const int grp = a.n_heads / a.n_kv;
     if (head_dim == 64) return grp > 4 ? launch_join<64, 8>(a, s) : grp > 2 ? launch_join<64, 4>(a, s) : launch_join<64, 2>(a, s);

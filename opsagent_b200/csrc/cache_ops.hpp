@@ -46,7 +46,7 @@ struct PrefixAttnArgs {
 };
 struct PrefixAttnPlan { int pre_ctas, own_ctas, key_tile; bool long_prefix; size_t pre_slots, pre_o, pre_ml, own_o, own_ml, more_o, more_ml, own_parts, bytes; };      // CTAs, slots, byte offsets
 PrefixAttnPlan prefix_attn_plan(int n_seqs, int n_heads, int n_kv, int head_dim, int n_prefixes, int max_prefix_pages, int max_own_pages, int sms);
-// tm_q: box of 128 / group tokens by a group's heads over q; tm_page: box of 64 rows, tm_part: box of 16 rows over the layer's cache [2 * num_pages * n_kv * 64, head_dim]
-cudaError_t launch_prefix_attention(const CUtensorMap* tm_q, const CUtensorMap* tm_page, const CUtensorMap* tm_part, int head_dim, bool long_prefix, const PrefixAttnArgs& a, cudaStream_t s);
+// tm_q: box of 128 / group tokens by a group's heads over q; tm_page: box of 64 rows over the layer's cache [2 * num_pages * n_kv * 64, head_dim]
+cudaError_t launch_prefix_attention(const CUtensorMap* tm_q, const CUtensorMap* tm_page, int head_dim, bool long_prefix, const PrefixAttnArgs& a, cudaStream_t s);
 
 }  // namespace oa

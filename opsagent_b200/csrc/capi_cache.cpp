@@ -167,12 +167,11 @@ int oa_k_prefix_attention(const void* q, int64_t ldq, void* out, int64_t ldo, co
     if (!apart_or_same(q, ldq, out, ldo, n_seqs, width, 2)) return bad("prefix attention: out overlaps q without being q");
     if (n_prefixes == 0) { prefix_tables = prefix_lens = prefix_rows = nullptr; max_prefix_pages = 0; }
     OA_ON_DEVICE_OF(kv_cache, q, out, prefix_tables, prefix_lens, prefix_rows, own_tables, own_lens, status);
-    CUtensorMap tm_q, tm_page, tm_part;
+    CUtensorMap tm_q, tm_page;
     const int group = n_heads / n_kv;
     if (make_tmap_bf16_heads(&tm_q, q, (uint64_t)n_seqs, (uint64_t)n_heads, (uint64_t)head_dim, (uint64_t)ldq, 128 / group, group) != 0) return call_failed(OA_ERR_INTERNAL, "prefix attention: no tensor map of the queries");
     const uint64_t rows = 2ull * num_pages * n_kv * CACHE_PAGE;
-    if (make_tmap_bf16_2d(&tm_page, kv_cache, rows, head_dim, head_dim, 64, 64) != 0 || make_tmap_bf16_2d(&tm_part, kv_cache, rows, head_dim, head_dim, 16, 64) != 0)
-        return call_failed(OA_ERR_INTERNAL, "prefix attention: no tensor map of the cache");
+    if (make_tmap_bf16_2d(&tm_page, kv_cache, rows, head_dim, head_dim, 64, 64) != 0) return call_failed(OA_ERR_INTERNAL, "prefix attention: no tensor map of the cache");
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -188,7 +187,7 @@ int oa_k_prefix_attention(const void* q, int64_t ldq, void* out, int64_t ldo, co
     a.scale_log2e = (scale > 0 ? scale : 1.0f / std::sqrt((float)head_dim)) * 1.4426950408889634f;
     a.pre_o = (float*)(base + plan.pre_o); a.pre_ml = (float*)(base + plan.pre_ml); a.own_o = (float*)(base + plan.own_o); a.own_ml = (float*)(base + plan.own_ml);
     a.more_o = (float*)(base + plan.more_o); a.more_ml = (float*)(base + plan.more_ml); a.own_parts = (int2*)(base + plan.own_parts); a.pre_ctas = plan.pre_ctas; a.own_ctas = plan.own_ctas; a.key_tile = plan.key_tile;
-    return device_rc(launch_prefix_attention(&tm_q, &tm_page, &tm_part, head_dim, plan.long_prefix, a, (cudaStream_t)stream));
+    return device_rc(launch_prefix_attention(&tm_q, &tm_page, head_dim, plan.long_prefix, a, (cudaStream_t)stream));
 }
 
 }  // extern "C"

@@ -212,6 +212,11 @@ def test_cache_copy(L, planes, pages, n_kv, dim, dtype, n, tokens):
 
 
 # ---- decode attention over shared prefixes -------------------------------------------------------
+def apart(n, n_kv):
+    """A table of prefixes so wide that prefixes are work of their own."""
+    return (1200 if n <= 8 else 600) // (n * n_kv) + 1
+
+
 class Batch:
     """Pages anywhere in a cache whose unused places hold NaN."""
 
@@ -287,8 +292,9 @@ SHAPES = [  # heads, key/value heads, head size
 
 @pytest.mark.parametrize("heads,n_kv,dim", SHAPES)
 @pytest.mark.parametrize("prefix,own", [(1, [1]), (64, [0, 1]), (130, [5, 64, 65, 0, 200]), (500, [3] * 40)])
-def test_prefix_attention(L, heads, n_kv, dim, prefix, own):
-    b = Batch(heads, n_kv, dim, [prefix], [0, len(own)], own, seed=heads + prefix)
+@pytest.mark.parametrize("wide", [False, True])
+def test_prefix_attention(L, heads, n_kv, dim, prefix, own, wide):
+    b = Batch(heads, n_kv, dim, [prefix], [0, len(own)], own, seed=heads + prefix, wide=apart(len(own), n_kv) if wide else 1)
     run(L, b)
     b.check()
     assert b.status.item() == 0
@@ -296,8 +302,9 @@ def test_prefix_attention(L, heads, n_kv, dim, prefix, own):
 
 @pytest.mark.parametrize("prefix", [63, 65, 127, 128, 129, 192, 255, 256, 257, 1000])
 @pytest.mark.parametrize("dim", [64, 128])
-def test_prefixes_that_end_anywhere(L, prefix, dim):
-    b = Batch(4, 1, dim, [prefix], [0, 3], [0, 17, 16], seed=prefix)
+@pytest.mark.parametrize("wide", [1, apart(3, 1), 4000])
+def test_prefixes_that_end_anywhere(L, prefix, dim, wide):
+    b = Batch(4, 1, dim, [prefix], [0, 3], [0, 17, 16], seed=prefix, wide=wide)
     run(L, b)
     b.check()
 
@@ -310,8 +317,9 @@ def test_own_parts_that_end_anywhere(L, own, dim):
     b.check()
 
 
-def test_rows_without_a_prefix_and_rows_that_see_nothing(L):
-    b = Batch(8, 2, 128, [100, 0, 300], [1, 3, 5, 9], [0, 0, 7, 0, 9, 0, 80, 0, 0, 0, 4], seed=5)      # rows 0, 9 and 10 have no prefix, 3 and 4 an empty one
+@pytest.mark.parametrize("wide", [1, apart(11, 2), 2000])
+def test_rows_without_a_prefix_and_rows_that_see_nothing(L, wide):
+    b = Batch(8, 2, 128, [100, 0, 300], [1, 3, 5, 9], [0, 0, 7, 0, 9, 0, 80, 0, 0, 0, 4], seed=5, wide=wide)      # rows 0, 9 and 10 have no prefix, 3 and 4 an empty one
     run(L, b)
     b.check()
     assert not b.out[[0, 3, 9], :1024].any() and b.out[10, :1024].any()
@@ -323,10 +331,11 @@ def test_no_prefix_at_all(L):
     b.check()
 
 
-def test_many_prefixes(L):
+@pytest.mark.parametrize("wide", [1, apart(75, 1), 3000])
+def test_many_prefixes(L, wide):
     lens = [(i * 37) % 211 for i in range(32)]
     runs = [0] + [min(70, 2 * i + (i % 3)) for i in range(1, 33)]
-    b = Batch(8, 1, 64, lens, runs, [(i * 13) % 90 for i in range(75)], seed=7)
+    b = Batch(8, 1, 64, lens, runs, [(i * 13) % 90 for i in range(75)], seed=7, wide=wide)
     run(L, b)
     b.check()
 
@@ -362,9 +371,10 @@ def test_one_long_sequence(L):
     b.check()
 
 
-def test_scores_that_grow_along_the_keys(L):
+@pytest.mark.parametrize("wide", [1, apart(6, 2), 2000])
+def test_scores_that_grow_along_the_keys(L, wide):
     """Every tile raises the maximum by far more than the reference may lag behind."""
-    b = Batch(8, 2, 128, [700], [0, 6], [200] * 6, seed=9)
+    b = Batch(8, 2, 128, [700], [0, 6], [200] * 6, seed=9, wide=wide)
     ramp = torch.arange(700, device="cuda", dtype=torch.float32) / 40
     direction = torch.nn.functional.normalize(randn(3, (128,), torch.float32), dim=0)
     for i, page in enumerate(b.pt[0, :11]):
@@ -384,9 +394,10 @@ def test_strides_scale_and_in_place(L):
     assert torch.equal(b.q[:, :1024], b.out[:9, :1024]) and torch.equal(b.q[:, 1024:], q[:, 1024:])
 
 
-def test_infinities_and_nan_that_are_seen(L):
+@pytest.mark.parametrize("wide", [1, apart(3, 2), 2000])
+def test_infinities_and_nan_that_are_seen(L, wide):
     """-inf scores leave a key out, a NaN or +inf key makes its rows NaN, as the plain softmax does; other heads stay."""
-    b = Batch(4, 2, 64, [150], [0, 3], [70, 3, 0], seed=11)
+    b = Batch(4, 2, 64, [150], [0, 3], [70, 3, 0], seed=11, wide=wide)
     b.q[:, 0], b.q[:, 64] = 1.0, 1.0
     b.q[:, 128 + 1] = 1.0
     b.cache[0, b.pt[0, 0], 0, 3, 0] = -math.inf                                   # head 0 of the cache: a score of -inf (or inf where q is negative: q is 1 there)
@@ -411,13 +422,14 @@ def test_infinities_and_nan_that_are_seen(L):
     assert bool(((out[0, 0].double() - p @ v).abs() <= tol).all()) and torch.isnan(out[2, 0]).all()
 
 
-def test_bad_tables_set_the_status_and_spare_the_others(L):
+@pytest.mark.parametrize("wide", [1, apart(4, 2), 2000])
+def test_bad_tables_set_the_status_and_spare_the_others(L, wide):
     own = [30, 70, 64, 5]
-    good = Batch(8, 2, 128, [200], [0, 4], own, seed=12)
+    good = Batch(8, 2, 128, [200], [0, 4], own, seed=12, wide=wide)
     run(L, good)
     assert good.status.item() == 0
     for what in ("own page", "own page below", "own length", "negative length", "prefix page", "prefix length", "runs fall", "runs beyond"):
-        b = Batch(8, 2, 128, [200], [0, 4], own, seed=12)
+        b = Batch(8, 2, 128, [200], [0, 4], own, seed=12, wide=wide)
         b.cache.nan_to_num_(0.0)
         rows = [0, 2, 3]
         if what == "own page":
@@ -445,9 +457,10 @@ def test_bad_tables_set_the_status_and_spare_the_others(L):
         assert (b.out[4:] == 5.0).all()
 
 
-def test_a_captured_call_follows_its_tables(L):
+@pytest.mark.parametrize("wide", [1, apart(6, 2), 2000])
+def test_a_captured_call_follows_its_tables(L, wide):
     """Two graphs and eager calls in between; lengths change between replays (a row ends, another grows, the prefix grows)."""
-    b, c = Batch(8, 2, 128, [300], [0, 6], [11, 1, 64, 90, 2, 65], seed=13), Batch(8, 2, 64, [90, 64], [0, 2, 5], [100, 3, 0, 0, 700], seed=14)
+    b, c = Batch(8, 2, 128, [300], [0, 6], [11, 1, 64, 90, 2, 65], seed=13, wide=wide), Batch(8, 2, 64, [90, 64], [0, 2, 5], [100, 3, 0, 0, 700], seed=14)
     run(L, b), run(L, c)
     graphs = []
     side = torch.cuda.Stream()
