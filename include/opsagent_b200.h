@@ -172,7 +172,7 @@ OA_API int oa_host_rotary_freqs(int32_t rot_dims, double base, int32_t scaling, 
  * from row to row; out is x itself or does not overlap it.  head_dim even, any alignment of the elements (rows of whole 16-byte pieces are faster) */
 OA_API int oa_k_rotary(const void* x, int64_t ldx, void* out, int64_t ldo, const int32_t* positions, int32_t T, int32_t n_heads, int32_t head_dim, int32_t rot_dims, int32_t layout,
                        const double* freqs, float amplitude, int32_t transpose, int32_t f32, void* stream);
-/* the same for T new tokens of a layer (bf16): q [T, n_heads, head_dim] -> q_out (q itself or apart from it), k turned and v as it is -> row slots[t] % 64 of page
+/* the same for T new tokens of a layer (bf16): q [T, n_heads, head_dim] -> q_out (q itself or apart from it, and apart from k and v), k turned and v as it is -> row slots[t] % 64 of page
  * slots[t] / 64 (slots: device; negative: the token is not written; distinct otherwise).  Other places of the cache stay as they are */
 OA_API int oa_k_rotary_cache(const void* q, int64_t ldq, const void* k, const void* v, int64_t ldkv, void* q_out, int64_t ldqo, void* kv_cache, int32_t num_pages,
                              const int32_t* positions, const int32_t* slots, int32_t T, int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t rot_dims, int32_t layout,

@@ -66,6 +66,7 @@ static cudaError_t launch_copy(void* cache, int planes, int num_pages, int n_kv,
     a.cache = reinterpret_cast<uint4*>(cache); a.planes = planes; a.num_pages = num_pages; a.n_kv = n_kv; a.row16 = row_bytes / 16; a.n = n;
     int most = 0, again = 0;
     for (int i = 0; i < n; ++i) { a.moves[i] = moves[i]; if (moves[i].tokens > most) most = moves[i].tokens; if (i && moves[i].src == moves[i - 1].src) ++again; }
+    if (most == 0) return cudaSuccess;
     a.parts = (n_kv * most * a.row16 + COPY_CHUNKS - 1) / COPY_CHUNKS;
     const int64_t ctas = (int64_t)n * planes * a.parts;
     const int64_t share = again * 2 >= n ? ctas / COPY_SHARE_CTAS : 1;

@@ -37,15 +37,21 @@ const char* rotary_wrong(int64_t T, int64_t heads, int32_t head_dim, int32_t rot
     if (ldx < heads * head_dim || ldo < heads * head_dim) return "rotary: a row is longer than its pitch";
     return nullptr;
 }
-// out is x itself or apart from it: other rows' memory, or other columns of the same rows
+// rows of T x wa and T x wb elements share no memory: they are other memory, or other columns of the same rows
+bool apart(const void* x, int64_t ldx, int64_t wa, const void* y, int64_t ldy, int64_t wb, int64_t T, int64_t esz) {
+    const uintptr_t a = (uintptr_t)x, b = (uintptr_t)y;
+    if (a + ((T - 1) * ldx + wa) * esz <= b || b + ((T - 1) * ldy + wb) * esz <= a) return true;
+    if (ldx != ldy) return false;
+    const int64_t pitch = ldx * esz, off = b >= a ? (int64_t)((b - a) % (uintptr_t)pitch) : (pitch - (int64_t)((a - b) % (uintptr_t)pitch)) % pitch;
+    return off >= wa * esz && off + wb * esz <= pitch;
+}
 bool apart_or_same(const void* x, int64_t ldx, const void* out, int64_t ldo, int64_t T, int64_t cols, int64_t esz) {
-    if (T == 0 || (x == out && ldx == ldo)) return true;
-    const uintptr_t a = (uintptr_t)x, b = (uintptr_t)out;
-    const uintptr_t a1 = a + ((T - 1) * ldx + cols) * esz, b1 = b + ((T - 1) * ldo + cols) * esz;
-    if (a1 <= b || b1 <= a) return true;
-    if (ldx != ldo) return false;
-    const int64_t pitch = ldx * esz, w = cols * esz, off = (int64_t)((b > a ? b - a : a - b) % (uintptr_t)pitch);
-    return off >= w && off + w <= pitch;
+    return (x == out && ldx == ldo) || apart(x, ldx, cols, out, ldo, cols, T, esz);
+}
+// rows of bf16 have nothing of a layer's two planes
+bool outside_cache(const void* cache, int64_t num_pages, int64_t n_kv, int64_t head_dim, const void* x, int64_t ldx, int64_t cols, int64_t T) {
+    const uintptr_t c = (uintptr_t)cache, p = (uintptr_t)x;
+    return p + ((T - 1) * ldx + cols) * 2 <= c || c + 2 * num_pages * n_kv * CACHE_PAGE * head_dim * 2 <= p;
 }
 void rotary_turns(RotaryArgs& a, const double* freqs, int32_t rot_dims, float amplitude, bool transpose) {
     a.pairs = rot_dims / 2; a.amplitude = amplitude;
@@ -105,7 +111,11 @@ int oa_k_rotary_cache(const void* q, int64_t ldq, const void* k, const void* v, 
     if (T == 0) return OA_OK;
     if (!q || !k || !v || !q_out || !kv_cache || !positions || !slots) return bad("rotary: null pointer");
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)kv_cache) % 2 || ((uintptr_t)positions | (uintptr_t)slots | (uintptr_t)status) % 4) return bad("rotary: a pointer is not aligned to its elements");
-    if (!apart_or_same(q, ldq, q_out, ldqo, T, (int64_t)n_heads * head_dim, 2)) return bad("rotary: q_out overlaps q without being q");
+    const int64_t cols = (int64_t)n_heads * head_dim, kv_cols = (int64_t)n_kv * head_dim;
+    if (!apart_or_same(q, ldq, q_out, ldqo, T, cols, 2)) return bad("rotary: q_out overlaps q without being q");
+    if (!apart(k, ldkv, kv_cols, q_out, ldqo, cols, T, 2) || !apart(v, ldkv, kv_cols, q_out, ldqo, cols, T, 2)) return bad("rotary: q_out overlaps the keys or values");
+    auto out_of_cache = [&](const void* x, int64_t ld, int64_t w) { return outside_cache(kv_cache, num_pages, n_kv, head_dim, x, ld, w, T); };
+    if (!out_of_cache(q, ldq, cols) || !out_of_cache(q_out, ldqo, cols) || !out_of_cache(k, ldkv, kv_cols) || !out_of_cache(v, ldkv, kv_cols)) return bad("rotary: rows overlap the cache");
     OA_ON_DEVICE_OF(q, k, v, q_out, kv_cache, positions, slots, status);
     RotaryArgs a{};
     a.x = q; a.ldx = ldq; a.out = q_out; a.ldo = ldqo; a.positions = positions; a.T = T; a.n_heads = n_heads; a.head_dim = head_dim;
@@ -165,6 +175,7 @@ int oa_k_prefix_attention(const void* q, int64_t ldq, void* out, int64_t ldo, co
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)kv_cache) % 16 || ((uintptr_t)own_tables | (uintptr_t)own_lens | (uintptr_t)status) % 4 ||
         (n_prefixes > 0 && ((uintptr_t)prefix_tables | (uintptr_t)prefix_lens | (uintptr_t)prefix_rows) % 4)) return bad("prefix attention: a pointer is not aligned");
     if (!apart_or_same(q, ldq, out, ldo, n_seqs, width, 2)) return bad("prefix attention: out overlaps q without being q");
+    if (!outside_cache(kv_cache, num_pages, n_kv, head_dim, out, ldo, width, n_seqs)) return bad("prefix attention: out overlaps the cache");
     if (n_prefixes == 0) { prefix_tables = prefix_lens = prefix_rows = nullptr; max_prefix_pages = 0; }
     OA_ON_DEVICE_OF(kv_cache, q, out, prefix_tables, prefix_lens, prefix_rows, own_tables, own_lens, status);
     CUtensorMap tm_q, tm_page;

@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(ROT_THREADS, ROT_CTAS) rotary_kernel(const __g
     griddep_wait();
     int position = a.positions[blockIdx.x], slot = CACHE ? a.slots[blockIdx.x] : -1;
     int phase = 0;
-    for (int t = blockIdx.x; t < a.T; t += gridDim.x, phase ^= 1) {
+    for (unsigned t = blockIdx.x; t < (unsigned)a.T; t += gridDim.x, phase ^= 1) {
         const int64_t plane = CACHE ? (int64_t)a.num_pages * a.n_kv * CACHE_PAGE : 0;
         int64_t page_row = -1;                                  // the token's row of head 0 in a plane of the cache
         if (CACHE) {
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(ROT_THREADS, ROT_CTAS) rotary_kernel(const __g
             else if (slot >= 0 && a.status && threadIdx.x == 0) *a.status = 400;
         }
         const double p = (double)position;
-        if (t + (int)gridDim.x < a.T) { position = a.positions[t + gridDim.x]; if (CACHE) slot = a.slots[t + gridDim.x]; }
+        if (t + gridDim.x < (unsigned)a.T) { position = a.positions[t + gridDim.x]; if (CACHE) slot = a.slots[t + gridDim.x]; }
         const E* x = reinterpret_cast<const E*>(a.x) + (int64_t)t * a.ldx;
         E* out = reinterpret_cast<E*>(a.out) + (int64_t)t * a.ldo;
         // head h's source and place, nullptr where it is not written; values are neither turned nor in out

@@ -192,6 +192,45 @@ def test_rotary_cache(L, tokens, heads, n_kv, dim, rot, layout):
     assert status.item() == (400 if tokens > 4 else 0)
 
 
+@pytest.mark.parametrize("heads,dim,rot,layout,f32,pad", [(2, 64, 64, 1, False, 0), (3, 128, 96, 0, False, 8), (2, 66, 30, 1, False, 6), (1, 600, 256, 0, False, 0), (2, 520, 256, 1, True, 1), (1, 2048, 64, 1, False, 0),
+                                                           (17, 64, 32, 0, True, 0)])
+def test_rotary_of_more_rows_than_run_at_once(L, heads, dim, rot, layout, f32, pad):
+    """Every CTA takes several rows; heads of more pieces than a CTA has threads, too."""
+    tokens, dtype, width = 2003, torch.float32 if f32 else torch.bfloat16, heads * dim
+    freqs, _ = frequencies(L, rot)
+    x, positions = randn(dim, (tokens, width + pad), dtype), cuda_i32((np.arange(tokens) * 7919) % 4099)
+    out = torch.empty_like(x)
+    assert L.oa_k_rotary(ptr(x), width + pad, ptr(out), width + pad, ptr(positions), tokens, heads, dim, rot, layout, freqs.ctypes.data, 1.0, 0, int(f32), now()) == 0
+    torch.cuda.synchronize()
+    rows = x[:, :width].reshape(tokens, heads, dim)
+    got = out[:, :width].reshape(tokens, heads, dim)
+    want, mag = turned(rows, positions, freqs, 1.0, rot, layout)
+    assert_turned(got, want, mag, dtype, 2.0 ** -52 * 4099)
+    assert torch.equal(got[..., rot:], rows[..., rot:])
+
+
+@pytest.mark.parametrize("layout", [0, 1])
+def test_rotary_cache_in_place_on_fused_rows(L, layout):
+    """q, k and v next to each other in a row, q turned in place: what the two calls apart give, and k and v stay."""
+    tokens, heads, n_kv, dim, pages = 1500, 4, 2, 64, 30
+    width = (heads + 2 * n_kv) * dim
+    freqs, _ = frequencies(L, dim)
+    qkv, cache = randn(1, (tokens, width)), randn(2, (2, pages, n_kv, PAGE, dim))
+    slots, positions = np.random.default_rng(3).permutation(pages * PAGE)[:tokens], cuda_i32(np.arange(tokens) % 777)
+    want_q, want_k = torch.empty(tokens, heads * dim, dtype=torch.bfloat16, device="cuda"), torch.empty(tokens, n_kv * dim, dtype=torch.bfloat16, device="cuda")
+    k0 = qkv.data_ptr() + 2 * heads * dim
+    assert L.oa_k_rotary(ptr(qkv), width, ptr(want_q), heads * dim, ptr(positions), tokens, heads, dim, dim, layout, freqs.ctypes.data, 1.0, 0, 0, now()) == 0
+    assert L.oa_k_rotary(k0, width, ptr(want_k), n_kv * dim, ptr(positions), tokens, n_kv, dim, dim, layout, freqs.ctypes.data, 1.0, 0, 0, now()) == 0
+    before = qkv.clone()
+    assert L.oa_k_rotary_cache(ptr(qkv), width, k0, k0 + 2 * n_kv * dim, width, ptr(qkv), width, ptr(cache), pages, ptr(positions), ptr(cuda_i32(slots)), tokens, heads, n_kv, dim, dim, layout,
+                               freqs.ctypes.data, 1.0, None, now()) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(qkv[:, :heads * dim], want_q) and torch.equal(qkv[:, heads * dim:], before[:, heads * dim:])
+    s = torch.tensor(slots, device="cuda")
+    assert torch.equal(cache[0, s // PAGE, :, s % PAGE].reshape(tokens, -1), want_k)
+    assert torch.equal(cache[1, s // PAGE, :, s % PAGE].reshape(tokens, -1), before[:, (heads + n_kv) * dim:])
+
+
 # ---- copies of pages -----------------------------------------------------------------------------
 @pytest.mark.parametrize("planes,pages,n_kv,dim,dtype,n,tokens", [
     (2, 9, 1, 8, torch.bfloat16, 3, (64,)), (4, 40, 8, 128, torch.bfloat16, 17, (64,)), (6, 30, 8, 64, torch.bfloat16, 13, (1, 63, 20, 0)), (2, 30, 3, 80, torch.bfloat16, 12, (5, 64)),
@@ -209,6 +248,32 @@ def test_cache_copy(L, planes, pages, n_kv, dim, dtype, n, tokens):
     assert L.oa_k_cache_copy(ptr(cache), planes, pages, n_kv, dim, cache.element_size(), moves, n, now()) == 0
     torch.cuda.synchronize()
     assert torch.equal(cache.view(torch.int16), want.view(torch.int16))
+
+
+@pytest.mark.parametrize("runs", [(70,), (20, 13, 1, 30, 6), (2,) * 35])
+def test_cache_copy_of_pages_that_go_to_many(L, runs):
+    """Enough work that a CTA writes what it has read to several pages; sources change and lengths differ within its share."""
+    planes, n_kv, dim = 16, 8, 128
+    n, pages = sum(runs), sum(runs) + len(runs)
+    order, cache = np.random.default_rng(len(runs)).permutation(pages), randn(len(runs), (planes, pages, n_kv, PAGE, dim))
+    want, moves, at = cache.clone(), (_lib.OaPageMove * n)(), 0
+    for r, count in enumerate(runs):
+        for i in range(count):
+            k, dst = (64, 49, 64, 0, 1)[(at + i) % 5] if r % 2 else 49, int(order[len(runs) + at + i])
+            moves[at + i] = _lib.OaPageMove(int(order[r]), dst, k)
+            want[:, dst, :, :k] = cache[:, order[r], :, :k]
+        at += count
+    assert L.oa_k_cache_copy(ptr(cache), planes, pages, n_kv, dim, 2, moves, n, now()) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(cache.view(torch.int16), want.view(torch.int16))
+
+
+def test_cache_copy_of_no_places(L):
+    cache = randn(1, (2, 4, 1, PAGE, 8))
+    want, moves = cache.clone(), (_lib.OaPageMove * 2)(_lib.OaPageMove(0, 1, 0), _lib.OaPageMove(0, 2, 0))
+    assert L.oa_k_cache_copy(ptr(cache), 2, 4, 1, 8, 2, moves, 2, now()) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(cache, want)
 
 
 # ---- decode attention over shared prefixes -------------------------------------------------------

@@ -272,6 +272,31 @@ def test_prefix_attention_refuses(L):
         assert "prefix attention" in _lib.last_error()
 
 
+def test_rows_that_overlap_are_refused(L):
+    """Addresses alone: nothing behind them is touched before a device is found."""
+    f, far = np.ones(64), 1 << 40
+
+    def rotary(q=far, ldq=512, k=far + 512, v=far + 768, ldkv=512, qo=far, ldqo=512, cache=2 * far, T=5):
+        _rc = L.oa_k_rotary_cache(q, ldq, k, v, ldkv, qo, ldqo, cache, 4, P, P, T, 2, 1, 128, 128, 1, f.ctypes.data, 1.0, None, None)
+        return _rc, _lib.last_error()
+
+    assert "overlap" not in rotary()[1]                                       # rows of q, k and v next to each other, q turned in place
+    assert "overlap" not in rotary(T=1, qo=far + 1024)[1] and "overlap" not in rotary(qo=far + 10240, ldqo=256)[1]
+    for case in [dict(qo=far + 512), dict(qo=far + 256), dict(k=far + 510), dict(v=far + 256), dict(qo=far + 1024 + 896), dict(qo=far + 3 * 1024 - 128), dict(qo=far - 16), dict(qo=far + 768, ldqo=256),
+                 dict(cache=far), dict(cache=far - 4 * 2 * 64 * 128 * 2 + 16), dict(qo=2 * far + 64), dict(k=2 * far + 65536, ldkv=128)]:
+        code, text = rotary(**case)
+        assert code == 400 and "overlap" in text, case
+
+    def attention(out, cache=2 * far):
+        _rc = L.oa_k_prefix_attention(far, 1024, out, 1024, cache, 8, P, 2, P, P, 1, P, 2, P, 3, 8, 2, 128, 0.0, None, None)
+        return _rc, _lib.last_error()
+
+    assert "overlap" not in attention(far)[1] and "overlap" not in attention(far + 6144)[1] and "overlap" not in attention(2 * far - 6144)[1]
+    for out in (far + 16, far + 6128, 2 * far - 6128, 2 * far, 2 * far + 8 * 2 * 2 * 64 * 128 * 2 - 16):
+        code, text = attention(out)
+        assert code == 400 and "overlap" in text, out
+
+
 def test_host_memory_is_not_run_on(L):
     """Arguments in order, memory that is not a device's: an error, with or without a GPU, and no launch."""
     f = np.ones(64)
