@@ -28,7 +28,7 @@ namespace oa {
 constexpr int PRE_SOFTMAX = 256;        // threads of a row tile: two softmax warpgroups
 constexpr int OWN_CONSUMERS = 256, OWN_THREADS = OWN_CONSUMERS + 64;        // eight consumer warps, producer, a warp that brings an item's states together
 constexpr int ROW_TILE = 128;          // rows of a prefix's products
-constexpr int JOIN_THREADS = 128;
+constexpr int JOIN_THREADS = 128, JOIN_CTAS = 4;         // of an SM: 128 registers a thread
 
 OA_DEVINL float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }        // nothing seen: any reference will do, 2^(-inf - 0) is 0
 OA_DEVINL int pages_of(int len) { return (len + CACHE_PAGE - 1) / CACHE_PAGE; }
@@ -708,77 +708,85 @@ __global__ void __maxnreg__(WIDE ? 168 : 96) own_part_kernel(const __grid_consta
 // lane; what is summed up follows a maximum that rises from batch to batch.  A kernel of its own: at the end of own_part_kernel, whose CTAs have from 2 to 20 items each, the same
 // sums took 3 to 11 us, and a CTA that came last for an item had to be found by a counter.
 template <int D, int RP>
-__global__ void __launch_bounds__(JOIN_THREADS) join_parts_kernel(const __grid_constant__ PrefixAttnArgs a) {
+__global__ void __launch_bounds__(JOIN_THREADS, JOIN_CTAS) join_parts_kernel(const __grid_constant__ PrefixAttnArgs a) {
     constexpr int SPLIT = D * RP / 256 > 1 ? D * RP / 256 : 1, LANES = 32 / RP, ITERS = D / 4 / LANES / SPLIT, MP = 8;
     const int lane = threadIdx.x & 31, grp = a.n_heads / a.n_kv, tile_tokens = ROW_TILE / grp;
-    const int64_t task = (int64_t)blockIdx.x * (JOIN_THREADS / 32) + (threadIdx.x >> 5), item = task / SPLIT;
-    const int seq = (int)(item / a.n_kv), kvh = (int)(item - (int64_t)seq * a.n_kv), part = (int)(task % SPLIT) * (D / 4 / SPLIT) + lane / RP;
+    __shared__ PrefixPieces px;
     griddep_launch();
-    int n_pre = 0, first_row = 0; int64_t pre_slot = 0;
-    if (a.pre_ctas > 0) {                        // the row's prefix, if it has one: from the call's arguments, while the parts are being made
-        __shared__ PrefixPieces px;
+    if (a.pre_ctas > 0) {                        // from the call's arguments, while the parts are being made
         if (threadIdx.x < 32) cut_prefixes(a, px, lane);
         __syncthreads();
+    }
+    const int64_t tasks = (int64_t)a.n_seqs * a.n_kv * SPLIT;
+    int64_t task = (int64_t)blockIdx.x * (JOIN_THREADS / 32) + (threadIdx.x >> 5), item = 0, pre_slot = 0;
+    int seq = 0, kvh = 0, part = 0, n_pre = 0, first_row = 0;
+    auto look = [&] {                            // where the task's row and its prefix's parts are
+        if (task >= tasks) return;
+        item = task / SPLIT; seq = (int)quotient(item, a.n_kv); kvh = (int)(item - (int64_t)seq * a.n_kv); part = (int)(task % SPLIT) * (D / 4 / SPLIT) + lane / RP;
+        n_pre = 0;
+        if (a.pre_ctas == 0) return;
         const unsigned who = __ballot_sync(0xffffffffu, px.rows[lane] > 0 && seq >= px.row0[lane] && seq < px.row0[lane] + px.rows[lane]);
         if (who) {
             const int run = __ffs(who) - 1, token = seq - px.row0[run], tile = token / tile_tokens;
             n_pre = px.split[run]; first_row = (token - tile * tile_tokens) * grp;
             pre_slot = (int64_t)px.piece0[run] + (int64_t)(kvh * px.tiles[run] + tile) * n_pre;
         }
-    }
+    };
+    look();
     griddep_wait();
-    if (seq >= a.n_seqs) return;
-    const int2 later = __ldcg(a.own_parts + item);
-    const int n = n_pre + 1;                     // the prefix's parts and the first own one: where they lie is known; later own ones follow
-    for (int r0 = 0; r0 < grp; r0 += RP) {
-        const int row = r0 + lane % RP, r = row < grp ? row : grp - 1;          // lanes beyond the group go along
-        const float2* pre_ml = reinterpret_cast<const float2*>(a.pre_ml) + pre_slot * ROW_TILE + first_row + r;
-        const float2* own_ml = reinterpret_cast<const float2*>(a.own_ml) + item * grp + r;
-        const float2* more_ml = reinterpret_cast<const float2*>(a.more_ml) + (int64_t)later.x * grp + r;
-        const float* pre_o = a.pre_o + pre_slot * (ROW_TILE * D) + (first_row + r) * 4 + part * (ROW_TILE * 4);
-        const float* own_o = a.own_o + (item * grp + r) * D + part * 4;
-        const float* more_o = a.more_o + ((int64_t)later.x * grp + r) * D + part * 4;
-        float M = -INFINITY, l = 0.f; float4 acc[ITERS]; bool some = false;
+    for (; task < tasks; task += (int64_t)gridDim.x * (JOIN_THREADS / 32), look()) {
+        const int2 later = __ldcg(a.own_parts + item);
+        const int n = n_pre + 1;                     // the prefix's parts and the first own one: where they lie is known; later own ones follow
+        for (int r0 = 0; r0 < grp; r0 += RP) {
+            const int row = r0 + lane % RP, r = row < grp ? row : grp - 1;          // lanes beyond the group go along
+            const float2* pre_ml = reinterpret_cast<const float2*>(a.pre_ml) + pre_slot * ROW_TILE + first_row + r;
+            const float2* own_ml = reinterpret_cast<const float2*>(a.own_ml) + item * grp + r;
+            const float2* more_ml = reinterpret_cast<const float2*>(a.more_ml) + (int64_t)later.x * grp + r;
+            const float* pre_o = a.pre_o + pre_slot * (ROW_TILE * D) + (first_row + r) * 4 + part * (ROW_TILE * 4);
+            const float* own_o = a.own_o + (item * grp + r) * D + part * 4;
+            const float* more_o = a.more_o + ((int64_t)later.x * grp + r) * D + part * 4;
+            float M = -INFINITY, l = 0.f; float4 acc[ITERS]; bool some = false;
 #pragma unroll
-        for (int k = 0; k < ITERS; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        int i0 = 0;
-        do {
-            float2 ml[MP]; float4 o[MP][ITERS];
+            for (int k = 0; k < ITERS; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            int i0 = 0;
+            do {
+                float2 ml[MP]; float4 o[MP][ITERS];
 #pragma unroll
-            for (int p = 0; p < MP; ++p) {
-                const int i = i0 + p;
-                ml[p] = make_float2(-INFINITY, -1.f);
-                if (i >= n && i >= n + later.y) continue;
-                const float2* m = i < n_pre ? pre_ml + (int64_t)i * ROW_TILE : i < n ? own_ml : more_ml + (int64_t)(i - n) * grp;
-                const float* src = i < n_pre ? pre_o + (int64_t)i * (ROW_TILE * D) : i < n ? own_o : more_o + (int64_t)(i - n) * (grp * D);
-                const int step = i < n_pre ? ROW_TILE * 4 * LANES : 4 * LANES;
-                ml[p] = __ldcg(m);
+                for (int p = 0; p < MP; ++p) {
+                    const int i = i0 + p;
+                    ml[p] = make_float2(-INFINITY, -1.f);
+                    if (i >= n && i >= n + later.y) continue;
+                    const float2* m = i < n_pre ? pre_ml + (int64_t)i * ROW_TILE : i < n ? own_ml : more_ml + (int64_t)(i - n) * grp;
+                    const float* src = i < n_pre ? pre_o + (int64_t)i * (ROW_TILE * D) : i < n ? own_o : more_o + (int64_t)(i - n) * (grp * D);
+                    const int step = i < n_pre ? ROW_TILE * 4 * LANES : 4 * LANES;
+                    ml[p] = __ldcg(m);
 #pragma unroll
-                for (int k = 0; k < ITERS; ++k) o[p][k] = __ldcg(reinterpret_cast<const float4*>(src + k * step));
+                    for (int k = 0; k < ITERS; ++k) o[p][k] = __ldcg(reinterpret_cast<const float4*>(src + k * step));
+                }
+                float m = M;
+#pragma unroll
+                for (int p = 0; p < MP; ++p) m = fmaxf(m, ml[p].x);
+                const float ref = finite_or_zero(m), f0 = ex2_approx(M - ref);
+                M = m; l *= f0;
+#pragma unroll
+                for (int k = 0; k < ITERS; ++k) { acc[k].x *= f0; acc[k].y *= f0; acc[k].z *= f0; acc[k].w *= f0; }
+#pragma unroll
+                for (int p = 0; p < MP; ++p) {
+                    if (ml[p].y < 0.f) continue;                                     // a part without tokens
+                    const float f = ex2_approx(ml[p].x - ref);
+                    l += f * ml[p].y; some = true;
+#pragma unroll
+                    for (int k = 0; k < ITERS; ++k) { acc[k].x += f * o[p][k].x; acc[k].y += f * o[p][k].y; acc[k].z += f * o[p][k].z; acc[k].w += f * o[p][k].w; }
+                }
+                i0 += MP;
+            } while (i0 < n + later.y);
+            if (row < grp) {
+                const float inv = some ? 1.0f / l : 0.f;
+                uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)seq * a.ldo + (int64_t)(kvh * grp + row) * D + part * 4;
+#pragma unroll
+                for (int k = 0; k < ITERS; ++k)
+                    *reinterpret_cast<uint2*>(out + k * LANES * 4) = make_uint2(pack_bf16x2(acc[k].x * inv, acc[k].y * inv), pack_bf16x2(acc[k].z * inv, acc[k].w * inv));
             }
-            float m = M;
-#pragma unroll
-            for (int p = 0; p < MP; ++p) m = fmaxf(m, ml[p].x);
-            const float ref = finite_or_zero(m), f0 = ex2_approx(M - ref);
-            M = m; l *= f0;
-#pragma unroll
-            for (int k = 0; k < ITERS; ++k) { acc[k].x *= f0; acc[k].y *= f0; acc[k].z *= f0; acc[k].w *= f0; }
-#pragma unroll
-            for (int p = 0; p < MP; ++p) {
-                if (ml[p].y < 0.f) continue;                                     // a part without tokens
-                const float f = ex2_approx(ml[p].x - ref);
-                l += f * ml[p].y; some = true;
-#pragma unroll
-                for (int k = 0; k < ITERS; ++k) { acc[k].x += f * o[p][k].x; acc[k].y += f * o[p][k].y; acc[k].z += f * o[p][k].z; acc[k].w += f * o[p][k].w; }
-            }
-            i0 += MP;
-        } while (i0 < n + later.y);
-        if (row < grp) {
-            const float inv = some ? 1.0f / l : 0.f;
-            uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)seq * a.ldo + (int64_t)(kvh * grp + row) * D + part * 4;
-#pragma unroll
-            for (int k = 0; k < ITERS; ++k)
-                *reinterpret_cast<uint2*>(out + k * LANES * 4) = make_uint2(pack_bf16x2(acc[k].x * inv, acc[k].y * inv), pack_bf16x2(acc[k].z * inv, acc[k].w * inv));
         }
     }
 }
@@ -843,7 +851,8 @@ static cudaError_t launch_join(const PrefixAttnArgs& a, cudaStream_t s) {
     static bool attr_done[16] = {};
     { const cudaError_t e = raise_smem(kern, 0, attr_done); if (e != cudaSuccess) return e; }
     const int64_t tasks = (int64_t)a.n_seqs * a.n_kv * (D * RP / 256 > 1 ? D * RP / 256 : 1);
-    return launch_k(kern, dim3((unsigned)((tasks + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32))), dim3(JOIN_THREADS), 0, s, a);
+    const int64_t ctas = (tasks + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32), most = (int64_t)JOIN_CTAS * a.sms;
+    return launch_k(kern, dim3((unsigned)(ctas < most ? ctas : most)), dim3(JOIN_THREADS), 0, s, a);
 }
 // KEYS, SLOTS: tiles and ring of the prefixes' kernel; PAGES: ring of the own parts'
 template <int D, int KEYS, int SLOTS, int PAGES>

@@ -42,7 +42,7 @@ struct PrefixAttnArgs {
     int32_t* status;
     // scratch (prefix_attn_plan): parts of the prefixes, each item's first own part, later ones by the CTA that makes them, and how many of those an item has
     float *pre_o, *pre_ml, *own_o, *own_ml, *more_o, *more_ml; int2* own_parts;
-    int32_t pre_ctas, own_ctas, key_tile;          // pre_ctas 0: prefixes have no kernel of their own; key_tile: keys of its tiles
+    int32_t pre_ctas, own_ctas, key_tile, sms;     // pre_ctas 0: prefixes have no kernel of their own; key_tile: keys of its tiles
 };
 struct PrefixAttnPlan { int pre_ctas, own_ctas, key_tile; bool long_prefix; size_t pre_slots, pre_o, pre_ml, own_o, own_ml, more_o, more_ml, own_parts, bytes; };      // CTAs, slots, byte offsets
 PrefixAttnPlan prefix_attn_plan(int n_seqs, int n_heads, int n_kv, int head_dim, int n_prefixes, int max_prefix_pages, int max_own_pages, int sms);

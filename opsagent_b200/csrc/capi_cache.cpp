@@ -197,7 +197,7 @@ int oa_k_prefix_attention(const void* q, int64_t ldq, void* out, int64_t ldo, co
     a.n_seqs = n_seqs; a.n_heads = n_heads; a.n_kv = n_kv; a.num_pages = num_pages; a.status = status;
     a.scale_log2e = (scale > 0 ? scale : 1.0f / std::sqrt((float)head_dim)) * 1.4426950408889634f;
     a.pre_o = (float*)(base + plan.pre_o); a.pre_ml = (float*)(base + plan.pre_ml); a.own_o = (float*)(base + plan.own_o); a.own_ml = (float*)(base + plan.own_ml);
-    a.more_o = (float*)(base + plan.more_o); a.more_ml = (float*)(base + plan.more_ml); a.own_parts = (int2*)(base + plan.own_parts); a.pre_ctas = plan.pre_ctas; a.own_ctas = plan.own_ctas; a.key_tile = plan.key_tile;
+    a.more_o = (float*)(base + plan.more_o); a.more_ml = (float*)(base + plan.more_ml); a.own_parts = (int2*)(base + plan.own_parts); a.pre_ctas = plan.pre_ctas; a.own_ctas = plan.own_ctas; a.key_tile = plan.key_tile; a.sms = sms;
     return device_rc(launch_prefix_attention(&tm_q, &tm_page, head_dim, plan.long_prefix, a, (cudaStream_t)stream));
 }
 
