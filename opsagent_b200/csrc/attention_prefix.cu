@@ -3,25 +3,29 @@
 //   out_i = softmax(scale q_i [K_prefix; K_own(i)]^T) [V_prefix; V_own(i)]
 //
 // The softmax splits over any partition of the keys: a part leaves its maximum m, l = sum 2^(s - m) and O = sum 2^(s - m) v, and parts join as
-// O = sum_i 2^(m_i - M) O_i, l likewise, M = max m_i.  Two kernels make the parts, the second also joins them:
+// O = sum_i 2^(m_i - M) O_i, l likewise, M = max m_i.  Scores, maxima, sums, O and parts are fp32; the weights 2^(s - m) are rounded to bf16 for the second product (2^-9 of a weight, of
+// either sign; l sums them unrounded) and the result once more.  Two kernels make the parts, a third joins them:
 //
-//  prefix_part_kernel: all rows of a prefix against its keys is a product of matrices (128 conversations of 4 heads a group: 512 rows a key/value head), so it
-//    runs on tcgen05: 128 rows (as many tokens' heads of a group as fit) x 128 keys a unit, S = Q K^T in two TMEM buffers, P over S's own columns as the second
-//    product's operand, O in TMEM.  One row a thread, reference maximum raised (and O rescaled) only where a score passes it by 2^8.
-//  own_part_kernel: a sequence's own keys have only its few heads as rows: streamed through shared memory by TMA and multiplied on the warp path of 16 x 8 x 16
-//    products, a page's 64 tokens over four warps, with tokens and channels as the 16 rows and the heads as the 8 columns (nothing of a product is empty for 8 heads a
-//    group, and O takes D / 4 registers a lane).
+//  prefix_part_kernel: all rows of a prefix against its keys is a product of matrices (128 conversations of 4 heads a group: 512 rows a key/value head), so it runs on tcgen05: 128 rows (as
+//    many tokens' heads of a group as fit) x 64 or 128 keys a tile, S = Q K^T in three TMEM buffers, two tiles ahead, P over S's own columns as the second product's operand, O in TMEM.  Two
+//    softmax warpgroups take the tiles in turn, one row a thread; the reference maximum rises (and O is rescaled) only where a score passes it by 2^8.  16384 keys under 4 x 8 row tiles of
+//    128: 29 us, 1680 cycles a tile of 128 x 128 x 128 for 1024 of the tensor pipe's and 1024 of the exponentials' (all eight warps on one tile, as before: 1900).
+//  own_part_kernel: a sequence's own keys have only its few heads as rows: streamed through shared memory by TMA and multiplied on the warp path of 16 x 8 x 16 products, a page's 64
+//    tokens over four warps (and either half of its channels on one of two), with tokens and channels as the 16 rows and the heads as the 8 columns: nothing of a product is empty for 8 heads a
+//    group, and O takes D / 8 registers a lane.  128 sequences of 64 to 512 tokens, 170 MB, in 28 us: 6.1 TB/s.
+//  join_parts_kernel: 3 us and as much to begin.
 //
-// Both deal their units (128 keys of a row tile; a page of a sequence and key/value head) out contiguously, the same number to every CTA: unit u is CTA
-// floor(((u + 1) G - 1) / total)'s, so what parts an item has, and in which slot (CTA + item) each of them lies, follows from lengths alone.  The plan is made on the
-// device, by every CTA for itself: lengths may come from the kernel before, a captured call serves other lengths when it is replayed, and the host waits for nothing.
-// Parts are joined in one order, whatever came first: the same call gives the same bits.
+// Row tiles and key/value heads are items; the prefixes' are cut into pieces of equally many key tiles, the own parts (a unit a page, and one an item) dealt out contiguously, the same number
+// to every CTA: unit u is CTA floor(((u + 1) G - 1) / total)'s, so what parts an item has, and where each of them lies, follows from lengths alone.  The plan is made on the device, by every
+// CTA for itself: lengths may come from the kernel before, a captured call serves other lengths when it is replayed, and the host waits for nothing.  Parts are joined in one order, whatever
+// came first: the same call gives the same bits.
 //
-// The second kernel starts beside the first (it needs nothing of it until it joins): it streams own keys from memory while the first is busy with products.
+// The second kernel starts beside the first (it needs nothing of it): it streams own keys from memory while the first is busy with products, and their shared memory and registers are cut so
+// that an SM holds one CTA of each.  Whole calls: 128 rows of 4 x 8 heads on a prefix of 1536 40 us (162 MB; 25 at the copy rate): 3 to begin, 28 of stream, 3 between the first CTA's end and the last
+// one's, 5 for the join with its start; 8 rows of 4000 to 9000 own tokens 42 us for 221 MB.
 #include "common.cuh"
 #include "kernels.hpp"
 #include "cache_ops.hpp"
-
 
 namespace oa {
 
@@ -705,8 +709,9 @@ __global__ void __maxnreg__(WIDE ? 168 : 96) own_part_kernel(const __grid_consta
 // the join
 // =============================================================================================
 // One warp an item (or one of SPLIT pieces of its columns), RP rows at a time, 32 / RP lanes a row.  One pass over the parts, 16 loads of 16 bytes of eight of them in flight per
-// lane; what is summed up follows a maximum that rises from batch to batch.  A kernel of its own: at the end of own_part_kernel, whose CTAs have from 2 to 20 items each, the same
-// sums took 3 to 11 us, and a CTA that came last for an item had to be found by a counter.
+// lane; what is summed up follows a maximum that rises from batch to batch.  Bound by latency: four parts a batch in fewer registers were 2 to 8 us slower (two batches one after the other),
+// two rows at a time for any group 1 us (16 bytes of a row here and there).  A kernel of its own: at the end of own_part_kernel, whose CTAs have from 2 to 20 items each, the same sums took 3 to
+// 11 us, and a CTA that came last for an item had to be found by a counter.
 template <int D, int RP>
 __global__ void __launch_bounds__(JOIN_THREADS, JOIN_CTAS) join_parts_kernel(const __grid_constant__ PrefixAttnArgs a) {
     constexpr int SPLIT = D * RP / 256 > 1 ? D * RP / 256 : 1, LANES = 32 / RP, ITERS = D / 4 / LANES / SPLIT, MP = 8;
