@@ -8,7 +8,7 @@
 // product in 32 bits would be whole turns off), and only then rounded to fp32.  cos and sin of it, times s, in fp32; products and sums in fp32; one rounding
 // at the end.
 //
-// Bound by memory.  A CTA walks over tokens with ROT_CTAS of them on an SM: a thread holds its pair's frequency throughout, takes the pair's cos and sin of the
+// Bound by memory.  A CTA walks over tokens (where one does not fill it) with ROT_CTAS of them on an SM: a thread holds its pair's frequency throughout, takes the pair's cos and sin of the
 // token under the loads of its first units, and reads those of its place in a head once a token; the next token's position comes a token ahead.  Pieces stay packed
 // until they turn: 80 registers a thread, four units of 32 bytes in flight each.  8192 tokens of 32 + 2 x 8 heads of 128 channels, 201 MB, take 33 us (6.1 TB/s; a
 // CTA for each token, with its cos and sin in shared memory and unpacked pieces, 70 us), 1337 tokens of 40 + 2 x 8 heads 7.7 us (10.3 us).
@@ -153,9 +153,12 @@ static cudaError_t launch_rotary_e(const RotaryArgs& a, bool halves, cudaStream_
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return e;
-    // few tokens: a token's heads over several CTAs, a unit a thread
+    // Few tokens: a token's heads over several CTAs, a unit a thread (us with one CTA a token / several, 48 heads of 128: 6 tokens 2.1 / 1.8, 100 2.3 / 2.2, 300 3.1 / 3.5).
     const int parts = a.T >= sms ? 1 : (heads + down - 1) / down;
-    return launch_k(kern, dim3(a.T < ROT_CTAS * sms ? a.T : ROT_CTAS * sms, parts > 64 ? 64 : parts), dim3(ROT_THREADS), 0, s, a);
+    // CTAs walk over tokens that do not fill their threads' loads in flight: 8192 tokens of 32 + 2 x 8 heads of 128 in bf16 33.3 us (a CTA a token 36.8), of 32 heads 23.3 (26.7), of 8 heads in
+    // fp32 15.4 (19.8).  Tokens that do have a CTA each, as many as registers allow: 32 heads in fp32 40.3 (walking 44.9), 64 heads in bf16 41.3 (47.5), 64 + 2 x 8 56
+    const bool walk = (int64_t)heads * per_head < ROT_THREADS * ROT_UNROLL;
+    return launch_k(kern, dim3(walk && a.T > ROT_CTAS * sms ? ROT_CTAS * sms : a.T, parts > 64 ? 64 : parts), dim3(ROT_THREADS), 0, s, a);
 }
 
 cudaError_t launch_rotary(const RotaryArgs& a, int layout, bool f32, cudaStream_t s) {
