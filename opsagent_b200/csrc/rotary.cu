@@ -5,8 +5,8 @@
 // the same with -f_i.
 //
 // The angle is taken in 64 bits, in turns: p (f_i / 2 pi) less its nearest whole number is below 1/2 with an error of 2^-22 turns for positions of 31 bits (a
-// product in 32 bits would be whole turns off), and only then rounded to fp32.  cos and sin of it, times s, in fp32; products and sums in fp32; one rounding
-// at the end.
+// product in 32 bits would be whole turns off), and only then rounded to fp32; what that rounding leaves (up to 1e-7, more than a result's own) turns cos and
+// sin of it by its first order.  These, times s, in fp32; products and sums in fp32; one rounding at the end.
 //
 // Bound by memory.  A CTA walks over tokens (where one does not fill it) with ROT_CTAS of them on an SM: a thread holds its pair's frequency throughout, takes the pair's cos and sin of the
 // token under the loads of its first units, and reads those of its place in a head once a token; the next token's position comes a token ahead.  Pieces stay packed
@@ -103,10 +103,11 @@ __global__ void __launch_bounds__(ROT_THREADS, ROT_CTAS) rotary_kernel(const __g
                 }
                 if (!angles) {
                     if (threadIdx.x < pairs) {
-                        const double full = p * turns;
+                        const double full = p * turns, half = 2.0 * (full - rint(full));
+                        const float near = (float)half, rest = (float)(half - (double)near) * 3.14159265f;
                         float s, c;
-                        sincospif((float)(2.0 * (full - rint(full))), &s, &c);
-                        cosines[phase][threadIdx.x] = c * a.amplitude; sines[phase][threadIdx.x] = s * a.amplitude;
+                        sincospif(near, &s, &c);
+                        cosines[phase][threadIdx.x] = (c - s * rest) * a.amplitude; sines[phase][threadIdx.x] = (s + c * rest) * a.amplitude;
                     }
                     __syncthreads();                            // of the other phase's readers too: they are through with the token before
                     angles = true;
