@@ -430,6 +430,46 @@ def test_tables_with_room_for_long_prefixes(L, heads, n_kv, prefixes, runs, wide
     assert torch.equal(first, b.out) and b.status.item() == 0
 
 
+# more rows than one tile has, with such a table
+@pytest.mark.parametrize("prefix", [1, 63, 64, 65, 127, 128, 129, 191, 192, 193, 255, 256, 257, 1000, 5000])
+@pytest.mark.parametrize("heads,n_kv,rows", [(8, 2, 40), (5, 1, 77)])
+def test_rows_of_several_tiles(L, heads, n_kv, rows, prefix):
+    b = Batch(heads, n_kv, 128, [prefix], [0, rows], [(i * 31) % 140 for i in range(rows)], seed=prefix + heads, wide=2000, scale_q=1.5)
+    run(L, b)
+    b.check()
+    first = b.out.clone()
+    run(L, b)
+    assert torch.equal(first, b.out) and b.status.item() == 0
+
+
+def test_rows_of_several_tiles_on_many_prefixes(L):
+    """Runs of one row, of one tile, of a tile and a row, of three tiles; prefixes of one place and of many; pieces of one tile and of several for a CTA."""
+    rows, lens = [1, 32, 33, 96, 2, 64, 130], [700, 1, 3000, 65, 129, 0, 257]
+    runs = np.concatenate([[3], 3 + np.cumsum(rows)]).tolist()
+    b = Batch(16, 4, 128, lens, runs, [(i * 13) % 90 for i in range(runs[-1] + 2)], seed=23, wide=1000)
+    run(L, b)
+    b.check()
+    assert b.status.item() == 0
+
+
+def test_rows_of_several_tiles_keep_what_masks_and_maxima_ask_for(L):
+    """Scores that rise along the keys, then tables with a page that there is not."""
+    b = Batch(8, 2, 128, [700], [0, 50], [5] * 50, seed=24, wide=2000)
+    ramp = torch.arange(700, device="cuda", dtype=torch.float32) / 40
+    direction = torch.nn.functional.normalize(randn(3, (128,), torch.float32), dim=0)
+    for i, page in enumerate(b.pt[0, :11]):
+        n = min(PAGE, 700 - i * PAGE)
+        b.cache[0, page, :, :n] = (ramp[i * PAGE:i * PAGE + n, None] * direction * 8).bfloat16()
+    b.q[:] = (direction * 8).bfloat16().repeat(8)
+    run(L, b)
+    b.check()
+    b.cache.nan_to_num_(0.0)
+    b.pt[0, 3] = b.pages
+    b.upload()
+    run(L, b)
+    assert b.status.item() == 400 and torch.isfinite(b.out).all() and (b.out[50:] == 5.0).all()
+
+
 def test_one_long_sequence(L):
     b = Batch(8, 2, 128, [40], [0, 1], [20011], seed=8)
     run(L, b)
