@@ -1,16 +1,17 @@
 // cache_copy.cu — copies of pages (or of a page's first places) of a paged cache, in all its planes and heads, by one launch.
 //
 // The pairs of pages travel in the launch's own parameters: no copy to the device ahead of the kernel, nothing to keep alive behind the call, and a captured
-// call holds its own.  Up to 64 pairs go with 0.8 KB of parameters, up to 2560 with 30 KB; beyond that another launch.
+// call holds its own.  Up to 64 pairs go with 0.8 KB of parameters (a call takes the host 3.9 us; with 30 KB 5.9 us), up to
+// 2560 with 30 KB; beyond that another launch.
 //
 // Bound by memory.  The places of a head of a page are one piece of up to 16 KB in each plane; a CTA copies up to 16 KB of a plane of a page, eight loads of 16
 // bytes in flight per thread, whose heads lie next to each other where whole pages are copied and a stride apart otherwise.  515 MB of whole pages (257 MB read, as
 // many written) take 78 us, 6.6 TB/s.
 //
-// A fork writes one page to many.  A CTA then keeps what it has read in registers and writes it to several pages: up to COPY_SHARE, as many as leave every SM its
-// COPY_SHARE_CTAS / 148 CTAs, where at least every other pair's source is that of the pair before.  The bytes that come out of L2 are what it saves.  us for a
-// page of 49 places in 64 planes of 8 x 128 channels written to 64 / 32 / 16 / 8 pages, a CTA for each pair: 103 / 53 / 25.6 / 10.3, four pairs a CTA 84 / 43 /
-// 20.0 / 10.8, by this rule (16, 8, 4, 2) 73 / 39 / 20.0 / 9.4, all 64 in one CTA 118; floors 64 / 32 / 17 / 9.
+// A fork writes one page to many.  A CTA then keeps what it has read in registers and writes it to several pages: as many as leave every SM the CTAs that it runs at
+// once, where at least every other pair's source is that of the pair before.  The bytes that come out of L2 are what it saves.  us for a page of 49 places in 64 planes
+// of 8 x 128 channels written to 64 / 32 / 16 / 8 pages, a CTA for each pair: 103 / 53 / 25.6 / 10.3, by this rule (24, 12, 6, 3) 69 / 36 / 18.1 / 9.5, fewer (up to
+// 16, 12 CTAs an SM) 73 / 39 / 20.0 / 9.4, more (6 CTAs) 77 / 39 / 19.5 / 10.7; floors 64 / 32 / 17 / 9.
 #include "common.cuh"
 #include "kernels.hpp"
 #include "cache_ops.hpp"
@@ -18,7 +19,7 @@
 namespace oa {
 
 constexpr int COPY_THREADS = 128, COPY_UNROLL = 8, COPY_CHUNKS = COPY_THREADS * COPY_UNROLL;
-constexpr int COPY_SHARE = 16, COPY_SHARE_CTAS = 12 * 148;    // pairs of a CTA, CTAs that stay
+constexpr int COPY_SHARE_CTAS = 8 * 148;                      // as many as run at once
 
 template <int CAP>
 struct CopyArgs {
@@ -54,9 +55,10 @@ __global__ void __launch_bounds__(COPY_THREADS) cache_copy_kernel(const __grid_c
             }
         }
         uint4* dst = base + (int64_t)m.dst * a.n_kv * page16;
+        // what is copied leaves L2 first: 69.0 us instead of 70.6 for the 64 pages above, 83.3 instead of 84.3 for 515 MB of whole pages over three sets of inputs
 #pragma unroll
         for (int i = 0; i < COPY_UNROLL; ++i)
-            if (mine >> i & 1) dst[at[i]] = v[i];
+            if (mine >> i & 1) __stcs(dst + at[i], v[i]);
     }
 }
 
@@ -70,7 +72,7 @@ static cudaError_t launch_copy(void* cache, int planes, int num_pages, int n_kv,
     a.parts = (n_kv * most * a.row16 + COPY_CHUNKS - 1) / COPY_CHUNKS;
     const int64_t ctas = (int64_t)n * planes * a.parts;
     const int64_t share = again * 2 >= n ? ctas / COPY_SHARE_CTAS : 1;
-    a.share = share < 1 ? 1 : share > COPY_SHARE ? COPY_SHARE : (int)share;
+    a.share = share < 1 ? 1 : (int)share;
     return launch_k(cache_copy_kernel<CAP>, dim3((unsigned)((n + a.share - 1) / a.share * (int64_t)planes * a.parts)), dim3(COPY_THREADS), 0, s, a);
 }
 
