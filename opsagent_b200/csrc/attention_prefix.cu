@@ -26,6 +26,7 @@
 #include "common.cuh"
 #include "kernels.hpp"
 #include "cache_ops.hpp"
+#include "work_units.hpp"
 
 namespace oa {
 
@@ -36,11 +37,6 @@ constexpr int JOIN_THREADS = 128, JOIN_CTAS = 4;         // of an SM: 128 regist
 
 OA_DEVINL float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }        // nothing seen: any reference will do, 2^(-inf - 0) is 0
 OA_DEVINL int pages_of(int len) { return (len + CACHE_PAGE - 1) / CACHE_PAGE; }
-// of a grid's CTAs the first min(grid, total) have units, each at least one: an item's parts are those of consecutive CTAs
-OA_DEVINL int64_t busy_ctas(int64_t grid, int64_t total) { return total < grid ? (total > 0 ? total : 1) : grid; }
-OA_DEVINL int64_t quotient(int64_t a, int64_t b) { return (uint64_t)a >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b); }      // a >= 0, b > 0; a 64-bit division takes several times as long
-OA_DEVINL int64_t first_unit(int64_t cta, int64_t busy, int64_t total) { return cta < busy ? quotient(total * cta, busy) : total; }
-OA_DEVINL int cta_of(int64_t unit, int64_t busy, int64_t total) { return (int)quotient((unit + 1) * busy - 1, total); }
 OA_DEVINL void report(const PrefixAttnArgs& a) { if (a.status) *a.status = 400; }
 
 // The runs of rows that share a prefix: bounds that never fall, lengths that fit their tables (0 where nobody sees it)

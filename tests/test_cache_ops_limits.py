@@ -1,0 +1,58 @@
+"""The operators on a caller's paged cache at the limits of what their entry points accept, no GPU: the arithmetic that deals out units of work, rows whose lengths
+come near 31 bits, and arguments at the edge of a refusal."""
+import ctypes as C
+import os
+import random
+import subprocess
+
+import numpy as np
+import pytest
+
+from opsagent_b200 import _lib
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+PAGE = 64
+
+
+@pytest.fixture(scope="module")
+def L():
+    return _lib.load()
+
+
+# ---- units of work -----------------------------------------------------------------------------
+SRC_UNITS = r'''
+#include <cstdio>
+#include "opsagent_b200/csrc/work_units.hpp"
+int main() {                                             // lines of (grid, total, unit) -> busy CTAs, the unit's CTA, that CTA's first unit and the next one's
+    long long grid, total, unit;
+    while (std::scanf("%lld %lld %lld", &grid, &total, &unit) == 3) {
+        const long long busy = oa::busy_ctas(grid, total); const int cta = oa::cta_of(unit, busy, total);
+        std::printf("%lld %d %lld %lld\n", busy, cta, (long long)oa::first_unit(cta, busy, total), (long long)oa::first_unit(cta + 1, busy, total));
+    }
+    return 0;
+}
+'''
+
+
+def test_units_are_dealt_out_exactly_beyond_32_bits(tmp_path):
+    """Whole-number arithmetic of any length says whose a unit is, from one unit up to the most that prefix attention accepts (2^20 sequences of 2^10 heads and 2^24 pages a table):
+    a dividend below 2^32 over a divisor beyond it is 0, not what is left of the divisor."""
+    src, exe, rng = tmp_path / "units.cpp", tmp_path / "units", random.Random(1)
+    src.write_text(SRC_UNITS)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-fsanitize=undefined", "-fno-sanitize-recover", f"-I{ROOT}", str(src), "-o", str(exe)], check=True)
+    most = 2 ** 20 * 2 ** 10 * (1 + 2 * 2 ** 24)
+    totals = [1, 2, 147, 148, 149, 2 ** 31 - 1, 2 ** 31, 2 ** 32 - 1, 2 ** 32, 2 ** 32 + 1, 2 ** 34 + 1024, 2 ** 40 + 3, most] + [int(2 ** rng.uniform(0, 55)) for _ in range(200)]
+    asked = []
+    for total in totals:
+        for grid in (1, 7, 132, 148):
+            busy, page_units = min(grid, total), min(total, 2 ** 24 + 1)
+            edges = {total * c // busy + d for c in (0, 1, busy // 2, busy - 1, busy) for d in (-1, 0, 1)} | {page_units - 1, page_units, rng.randrange(total)}
+            asked += [(grid, total, u) for u in sorted(edges) if 0 <= u < total]
+    r = subprocess.run([str(exe)], input="\n".join("%d %d %d" % x for x in asked), capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr[-500:]
+    got = [tuple(map(int, line.split())) for line in r.stdout.splitlines()]
+    assert len(got) == len(asked)
+    for (grid, total, unit), g in zip(asked, got):
+        busy = min(grid, total)
+        cta = next(c for c in range(busy) if total * c // busy <= unit < total * (c + 1) // busy)
+        assert g == (busy, cta, total * cta // busy, total * (cta + 1) // busy), (grid, total, unit, g)
