@@ -42,7 +42,7 @@ inline PageResult table_grow(const oa_page_table* tp, int row, int n_tokens) {
     const oa_page_table& t = *tp;
     if ((r = check_row(t, row)).rc) return r;
     const int len = t.lens[row], have = table_pages_of(len);
-    if (n_tokens < 0 || (int64_t)len + n_tokens > (int64_t)t.max_pages_per_seq * TABLE_PAGE) return page_bad("page table: a row holds no more than its pages");
+    if (n_tokens < 0 || (int64_t)len + n_tokens > INT32_MAX || (int64_t)len + n_tokens > (int64_t)t.max_pages_per_seq * TABLE_PAGE) return page_bad("page table: a row holds no more than its pages, and fewer than 2^31 tokens");
     int32_t* pages = t.block_tables + (size_t)row * t.max_pages_per_seq;
     if (n_tokens > 0 && len % TABLE_PAGE != 0 && t.refs[pages[have - 1]] > 1) return page_bad("page table: the last page is shared and not full (a fork copies it)");
     std::vector<int32_t> fresh;

@@ -56,3 +56,18 @@ def test_units_are_dealt_out_exactly_beyond_32_bits(tmp_path):
         busy = min(grid, total)
         cta = next(c for c in range(busy) if total * c // busy <= unit < total * (c + 1) // busy)
         assert g == (busy, cta, total * cta // busy, total * (cta + 1) // busy), (grid, total, unit, g)
+
+
+# ---- pages -------------------------------------------------------------------------------------
+def test_a_row_that_would_pass_31_bits_is_not_grown(L):
+    """A table with room for more tokens than a length can count: the last ones that fit are given, one more is refused and changes nothing."""
+    width, full = 2 ** 25 + 8, 2 ** 31 - PAGE                             # a row of one page named over and over
+    tables, lens, refs = np.zeros((1, width), np.int32), np.array([full], np.int32), np.array([2 ** 30, 0], np.int32)
+    tables[0, full // PAGE:] = -1
+    t = _lib.OaPageTable(tables.ctypes.data, lens.ctypes.data, refs.ctypes.data, 1, width, 2)
+    for more in (PAGE, 200, 2 ** 31 - 1):
+        assert L.oa_host_cache_grow(t, 0, more) == 400
+        assert "page table" in _lib.last_error() and lens.tolist() == [full] and refs.tolist() == [2 ** 30, 0] and (tables[0, full // PAGE:] == -1).all()
+    assert L.oa_host_cache_grow(t, 0, PAGE - 1) == 0
+    assert lens.tolist() == [2 ** 31 - 1] and refs.tolist() == [2 ** 30, 1] and tables[0, full // PAGE] == 1 and (tables[0, full // PAGE + 1:] == -1).all()
+    assert L.oa_host_cache_grow(t, 0, 1) == 400 and L.oa_host_cache_grow(t, 0, 0) == 0 and lens.tolist() == [2 ** 31 - 1]
