@@ -129,7 +129,9 @@ __global__ void __maxnreg__(104) prefix_part_kernel(const __grid_constant__ CUte
     }
     if (warp == 1) tmem_alloc<512>(tmem_slot);
     griddep_wait();
-    griddep_launch();            // behind the wait: what the own part's kernel reads ahead of its own wait was written by kernels that have ended
+    // Behind the wait: what the own part's kernel reads ahead of its own wait was written by kernels that have ended.  From the warp that allocates (one warp's signal is its CTA's): a later kernel
+    // of the stream that takes tensor memory ahead of its own wait finds every CTA of this one with its columns
+    if (warp == 1) griddep_launch();
     if (warp == 0) cut_prefixes(a, px, lane);
     tcgen05_fence_before();
     __syncthreads();

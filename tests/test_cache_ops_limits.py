@@ -1,8 +1,10 @@
 """The operators on a caller's paged cache at the limits of what their entry points accept, no GPU: the arithmetic that deals out units of work, rows whose lengths
 come near 31 bits, and arguments at the edge of a refusal."""
 import ctypes as C
+import glob
 import os
 import random
+import re
 import subprocess
 
 import numpy as np
@@ -71,3 +73,35 @@ def test_a_row_that_would_pass_31_bits_is_not_grown(L):
     assert L.oa_host_cache_grow(t, 0, PAGE - 1) == 0
     assert lens.tolist() == [2 ** 31 - 1] and refs.tolist() == [2 ** 30, 1] and tables[0, full // PAGE] == 1 and (tables[0, full // PAGE + 1:] == -1).all()
     assert L.oa_host_cache_grow(t, 0, 1) == 400 and L.oa_host_cache_grow(t, 0, 0) == 0 and lens.tolist() == [2 ** 31 - 1]
+
+
+# ---- order of a kernel's first steps ---------------------------------------------------------------
+def _kernels(source):
+    """Bodies of the __global__ functions of a CUDA source, without comments."""
+    text = re.sub(r"//[^\n]*|/\*.*?\*/", "", source, flags=re.S)
+    for part in text.split("__global__")[1:]:
+        at = depth = part.index("{")
+        depth = 0
+        for i in range(at, len(part)):
+            depth += {"{": 1, "}": -1}.get(part[i], 0)
+            if depth == 0:
+                yield part[:at], part[at:i + 1]
+                break
+
+
+def test_tensor_memory_is_held_before_the_next_kernel_may_start():
+    """A kernel that lets its successor start while one of its own CTAs still waits for tensor memory could wait for columns that the successor, which waits for it, has taken.  The signal comes
+    behind the allocation: behind a barrier of the whole CTA, or from the warp that allocates and no other."""
+    seen = 0
+    for path in sorted(glob.glob(os.path.join(ROOT, "opsagent_b200", "csrc", "*.cu"))):
+        for head, body in _kernels(open(path).read()):
+            alloc = re.search(r"tmem_alloc<|tcgen05\.alloc", body)
+            if not alloc:
+                continue
+            seen += 1
+            first = body.find("griddep_launch()")
+            assert first > alloc.start(), (path, head.strip()[-200:])
+            behind_barrier = "__syncthreads()" in body[alloc.start():first]
+            same_warp = body[:alloc.start()].endswith("if (warp == 1) ") and body[:first].endswith("if (warp == 1) ")
+            assert behind_barrier or same_warp, (path, head.strip()[-200:])
+    assert seen >= 8
