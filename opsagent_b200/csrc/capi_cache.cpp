@@ -37,11 +37,13 @@ const char* rotary_wrong(int64_t T, int64_t heads, int32_t head_dim, int32_t rot
     if (ldx < heads * head_dim || ldo < heads * head_dim) return "rotary: a row is longer than its pitch";
     return nullptr;
 }
+// T rows whose last one no device's memory holds beside the first: 2^39 elements, below which products of rows, pitches and element sizes stay in 64 bits and a tensor map takes the pitch
+bool beyond_memory(int64_t T, int64_t ld) { return T > 1 && ld >= ((int64_t)1 << 39) / (T - 1); }
 // rows of T x wa and T x wb elements share no memory: they are other memory, or other columns of the same rows
 bool apart(const void* x, int64_t ldx, int64_t wa, const void* y, int64_t ldy, int64_t wb, int64_t T, int64_t esz) {
     const uintptr_t a = (uintptr_t)x, b = (uintptr_t)y;
     if (a + ((T - 1) * ldx + wa) * esz <= b || b + ((T - 1) * ldy + wb) * esz <= a) return true;
-    if (ldx != ldy) return false;
+    if (ldx != ldy || T == 1) return false;                  // a single row has no pitch
     const int64_t pitch = ldx * esz, off = b >= a ? (int64_t)((b - a) % (uintptr_t)pitch) : (pitch - (int64_t)((a - b) % (uintptr_t)pitch)) % pitch;
     return off >= wa * esz && off + wb * esz <= pitch;
 }
@@ -91,6 +93,7 @@ int oa_k_rotary(const void* x, int64_t ldx, void* out, int64_t ldo, const int32_
     const char* wrong = rotary_wrong(T, n_heads, head_dim, rot_dims, layout, freqs, amplitude, ldx, ldo);
     if (wrong) return bad(wrong);
     if (T == 0) return OA_OK;
+    if (beyond_memory(T, ldx) || beyond_memory(T, ldo)) return bad("rotary: rows further apart than memory reaches");
     const int64_t esz = f32 ? 4 : 2;
     if (!x || !out || !positions) return bad("rotary: null pointer");
     if (((uintptr_t)x | (uintptr_t)out) % esz || (uintptr_t)positions % 4) return bad("rotary: a pointer is not aligned to its elements");
@@ -111,6 +114,7 @@ int oa_k_rotary_cache(const void* q, int64_t ldq, const void* k, const void* v, 
     if (T == 0) return OA_OK;
     if (!q || !k || !v || !q_out || !kv_cache || !positions || !slots) return bad("rotary: null pointer");
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)kv_cache) % 2 || ((uintptr_t)positions | (uintptr_t)slots | (uintptr_t)status) % 4) return bad("rotary: a pointer is not aligned to its elements");
+    if (beyond_memory(T, ldq) || beyond_memory(T, ldqo) || beyond_memory(T, ldkv)) return bad("rotary: rows further apart than memory reaches");
     const int64_t cols = (int64_t)n_heads * head_dim, kv_cols = (int64_t)n_kv * head_dim;
     if (!apart_or_same(q, ldq, q_out, ldqo, T, cols, 2)) return bad("rotary: q_out overlaps q without being q");
     if (!apart(k, ldkv, kv_cols, q_out, ldqo, cols, T, 2) || !apart(v, ldkv, kv_cols, q_out, ldqo, cols, T, 2)) return bad("rotary: q_out overlaps the keys or values");
@@ -174,6 +178,8 @@ int oa_k_prefix_attention(const void* q, int64_t ldq, void* out, int64_t ldo, co
     if (!q || !out || !kv_cache || !own_tables || !own_lens || (n_prefixes > 0 && (!prefix_tables || !prefix_lens || !prefix_rows))) return bad("prefix attention: null pointer");
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)kv_cache) % 16 || ((uintptr_t)own_tables | (uintptr_t)own_lens | (uintptr_t)status) % 4 ||
         (n_prefixes > 0 && ((uintptr_t)prefix_tables | (uintptr_t)prefix_lens | (uintptr_t)prefix_rows) % 4)) return bad("prefix attention: a pointer is not aligned");
+    if (beyond_memory(n_seqs, ldq) || beyond_memory(n_seqs, ldo)) return bad("prefix attention: rows further apart than memory reaches");
+    if (n_seqs == 1) ldq = ldo = width;                      // a single row has no pitch, and a tensor map takes none of 2^40 bytes
     if (!apart_or_same(q, ldq, out, ldo, n_seqs, width, 2)) return bad("prefix attention: out overlaps q without being q");
     if (!outside_cache(kv_cache, num_pages, n_kv, head_dim, out, ldo, width, n_seqs)) return bad("prefix attention: out overlaps the cache");
     if (n_prefixes == 0) { prefix_tables = prefix_lens = prefix_rows = nullptr; max_prefix_pages = 0; }

@@ -105,3 +105,48 @@ def test_tensor_memory_is_held_before_the_next_kernel_may_start():
             same_warp = body[:alloc.start()].endswith("if (warp == 1) ") and body[:first].endswith("if (warp == 1) ")
             assert behind_barrier or same_warp, (path, head.strip()[-200:])
     assert seen >= 8
+
+
+# ---- pitches and rows ------------------------------------------------------------------------------
+BUF, FREQS = np.zeros(4096, np.int32), np.ones(128)
+P, FAR = (BUF.ctypes.data + 15) // 16 * 16, 1 << 40                       # addresses alone: nothing behind them is touched before a device is found
+
+
+def rotary(L, x=P, ldx=256, out=P, ldo=256, T=2, f32=0):
+    return L.oa_k_rotary(x, ldx, out, ldo, P, T, 2, 128, 64, 1, FREQS.ctypes.data, 1.0, 0, f32, None), _lib.last_error()
+
+
+def rotary_cache(L, q=FAR, ldq=512, k=FAR + 512, v=FAR + 768, ldkv=512, out=FAR, ldo=512, T=5):
+    return L.oa_k_rotary_cache(q, ldq, k, v, ldkv, out, ldo, 2 * FAR, 4, P, P, T, 2, 1, 128, 128, 1, FREQS.ctypes.data, 1.0, None, None), _lib.last_error()
+
+
+def attention(L, q=FAR, ldq=1024, out=FAR, ldo=1024, n=3, scale=0.0):
+    return L.oa_k_prefix_attention(q, ldq, out, ldo, 2 * FAR, 8, P, 2, P, P, 1, P, 2, P, n, 8, 2, 128, scale, None, None), _lib.last_error()
+
+
+PITCHES = [2 ** 39, 2 ** 45, 2 ** 61, 2 ** 62, 2 ** 63 - 8]
+
+
+@pytest.mark.parametrize("pitch", PITCHES)
+def test_pitches_that_no_memory_has_are_refused(L, pitch):
+    """Two rows so far apart that their addresses leave 64 bits, or that no device holds both: refused, and the process goes on."""
+    for f32 in (0, 1):
+        assert rotary(L, ldx=pitch, ldo=pitch, f32=f32)[0] == 400 and "apart" in _lib.last_error()
+        for case in [dict(ldx=pitch, out=P + 2 ** 20), dict(ldo=pitch, out=P + 2 ** 20), dict(ldx=pitch // 64, ldo=pitch // 64, T=100), dict(ldx=pitch, ldo=pitch, out=P + 16)]:
+            assert rotary(L, **case, f32=f32)[0] == 400 and "rotary" in _lib.last_error(), case
+    for case in [dict(ldq=pitch), dict(ldkv=pitch), dict(ldo=pitch, out=3 * FAR), dict(ldq=pitch, ldo=pitch), dict(ldq=pitch, ldo=pitch, ldkv=pitch)]:
+        assert rotary_cache(L, **case)[0] == 400 and "apart" in _lib.last_error(), case
+    for case in [dict(ldq=pitch), dict(ldo=pitch, out=3 * FAR), dict(ldq=pitch, ldo=pitch)]:
+        assert attention(L, **case)[0] == 400 and "apart" in _lib.last_error(), case
+
+
+@pytest.mark.parametrize("pitch", PITCHES)
+def test_a_single_row_may_have_any_pitch(L, pitch):
+    """Nothing lies a pitch away from a single row.  Only overlaps are judged here: without a device the call ends behind that."""
+    for f32 in (0, 1):
+        assert rotary(L, ldx=pitch, ldo=pitch, T=1, f32=f32)[0] != 400 or "device" in _lib.last_error()
+        code, text = rotary(L, ldx=pitch, out=P + 16, ldo=pitch, T=1, f32=f32)
+        assert code == 400 and "overlap" in text
+        assert "overlap" not in rotary(L, ldx=pitch, out=P + 1024, ldo=pitch, T=1, f32=f32)[1]
+    assert "overlap" not in rotary_cache(L, ldq=pitch, ldkv=pitch, ldo=pitch, T=1)[1] and "apart" not in rotary_cache(L, ldq=pitch, ldkv=pitch, ldo=pitch, T=1)[1]
+    assert "overlap" not in attention(L, ldq=pitch, ldo=pitch, n=1)[1] and "apart" not in attention(L, ldq=pitch, ldo=pitch, n=1)[1]
