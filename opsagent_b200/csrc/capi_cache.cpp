@@ -48,7 +48,7 @@ bool apart(const void* x, int64_t ldx, int64_t wa, const void* y, int64_t ldy, i
     return off >= wa * esz && off + wb * esz <= pitch;
 }
 bool apart_or_same(const void* x, int64_t ldx, const void* out, int64_t ldo, int64_t T, int64_t cols, int64_t esz) {
-    return (x == out && ldx == ldo) || apart(x, ldx, cols, out, ldo, cols, T, esz);
+    return (x == out && (ldx == ldo || T == 1)) || apart(x, ldx, cols, out, ldo, cols, T, esz);
 }
 // rows of bf16 have nothing of a layer's two planes
 bool outside_cache(const void* cache, int64_t num_pages, int64_t n_kv, int64_t head_dim, const void* x, int64_t ldx, int64_t cols, int64_t T) {

@@ -150,3 +150,11 @@ def test_a_single_row_may_have_any_pitch(L, pitch):
         assert "overlap" not in rotary(L, ldx=pitch, out=P + 1024, ldo=pitch, T=1, f32=f32)[1]
     assert "overlap" not in rotary_cache(L, ldq=pitch, ldkv=pitch, ldo=pitch, T=1)[1] and "apart" not in rotary_cache(L, ldq=pitch, ldkv=pitch, ldo=pitch, T=1)[1]
     assert "overlap" not in attention(L, ldq=pitch, ldo=pitch, n=1)[1] and "apart" not in attention(L, ldq=pitch, ldo=pitch, n=1)[1]
+
+
+def test_a_single_row_is_turned_in_place_under_any_two_pitches(L):
+    """out is x itself, whatever the pitches of the one row are; two rows under two pitches are not the same rows."""
+    assert "overlap" not in rotary(L, ldo=264, T=1)[1] and "overlap" not in rotary(L, ldx=1024, T=1, f32=1)[1]
+    assert "overlap" not in rotary_cache(L, ldo=256, T=1)[1] and "overlap" not in attention(L, ldo=2048, n=1)[1]
+    for code, text in (rotary(L, ldo=264), rotary_cache(L, ldo=256, T=2), attention(L, ldo=2048, n=2), rotary(L, out=P + 16, ldo=264, T=1)):
+        assert code == 400 and "overlap" in text
