@@ -171,7 +171,8 @@ int oa_k_prefix_attention(const void* q, int64_t ldq, void* out, int64_t ldo, co
     if (n_seqs < 0 || n_seqs > (1 << 20) || max_own_pages < 1 || max_own_pages > (1 << 24)) return bad("prefix attention: bad number of sequences or of their pages");
     if (n_prefixes < 0 || n_prefixes > PREFIX_MAX || (n_prefixes > 0 && (max_prefix_pages < 1 || max_prefix_pages > (1 << 24)))) return bad("prefix attention: up to 32 prefixes, each with a page or more of room");
     if (num_pages < 1 || (int64_t)num_pages * n_kv * 2 * CACHE_PAGE > INT32_MAX) return bad("prefix attention: the cache's rows are counted in 31 bits");
-    if (!std::isfinite(scale) || scale < 0) return bad("prefix attention: the scale is positive, or 0 for 1 / sqrt(head_dim)");
+    const float scale_log2e = (scale > 0 ? scale : 1.0f / std::sqrt((float)head_dim)) * 1.4426950408889634f;
+    if (!std::isfinite(scale_log2e) || !(scale >= 0)) return bad("prefix attention: the scale is positive, and finite times log2(e), or 0 for 1 / sqrt(head_dim)");
     const int64_t width = (int64_t)n_heads * head_dim;
     if (ldq < width || ldo < width || ldq % 8 || ldo % 8) return bad("prefix attention: pitches hold a row and are multiples of 16 bytes");
     if (n_seqs == 0) return OA_OK;
@@ -201,7 +202,7 @@ int oa_k_prefix_attention(const void* q, int64_t ldq, void* out, int64_t ldo, co
     a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo; a.prefix_tables = prefix_tables; a.prefix_lens = prefix_lens; a.prefix_rows = prefix_rows; a.n_prefixes = n_prefixes;
     a.max_prefix_pages = max_prefix_pages; a.own_tables = own_tables; a.own_lens = own_lens; a.max_own_pages = max_own_pages;
     a.n_seqs = n_seqs; a.n_heads = n_heads; a.n_kv = n_kv; a.num_pages = num_pages; a.status = status;
-    a.scale_log2e = (scale > 0 ? scale : 1.0f / std::sqrt((float)head_dim)) * 1.4426950408889634f;
+    a.scale_log2e = scale_log2e;
     a.pre_o = (float*)(base + plan.pre_o); a.pre_ml = (float*)(base + plan.pre_ml); a.own_o = (float*)(base + plan.own_o); a.own_ml = (float*)(base + plan.own_ml);
     a.more_o = (float*)(base + plan.more_o); a.more_ml = (float*)(base + plan.more_ml); a.own_parts = (int2*)(base + plan.own_parts); a.pre_ctas = plan.pre_ctas; a.own_ctas = plan.own_ctas; a.key_tile = plan.key_tile; a.sms = sms;
     return device_rc(launch_prefix_attention(&tm_q, &tm_page, head_dim, plan.long_prefix, a, (cudaStream_t)stream));

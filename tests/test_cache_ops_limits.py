@@ -158,3 +158,12 @@ def test_a_single_row_is_turned_in_place_under_any_two_pitches(L):
     assert "overlap" not in rotary_cache(L, ldo=256, T=1)[1] and "overlap" not in attention(L, ldo=2048, n=1)[1]
     for code, text in (rotary(L, ldo=264), rotary_cache(L, ldo=256, T=2), attention(L, ldo=2048, n=2), rotary(L, out=P + 16, ldo=264, T=1)):
         assert code == 400 and "overlap" in text
+
+
+def test_a_scale_beyond_fp32_in_powers_of_two_is_refused(L):
+    """Scores are taken times scale log2(e) in fp32: where that is infinite, a score of 0 would become NaN."""
+    largest = np.nextafter(np.float32(np.finfo(np.float32).max / 1.4426950408889634), np.float32(0))
+    assert attention(L, scale=float(largest))[0] != 400 or "device" in _lib.last_error()
+    for scale in (2.4e38, float(np.finfo(np.float32).max)):
+        code, text = attention(L, scale=scale)
+        assert code == 400 and "scale" in text
