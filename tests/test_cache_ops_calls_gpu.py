@@ -1,0 +1,217 @@
+"""Calls of the operators on a caller's paged cache as a program makes them on the B200: tables that ask for what there is not (and what is cut to what there is), captured calls,
+calls from two threads on two streams.  Values against the 64-bit oracles and tolerances of test_cache_ops_gpu.py, or against an eager call's bits."""
+import ctypes as C
+import threading
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from opsagent_b200 import _lib  # noqa: E402
+from test_cache_ops_gpu import PAGE, Batch, apart, assert_turned, cuda_i32, frequencies, now, ptr, randn, run, turned  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def L():
+    return _lib.load()
+
+
+def same_bits(a, b):
+    return torch.equal(a.view(torch.int16 if a.element_size() == 2 else torch.int32), b.view(torch.int16 if b.element_size() == 2 else torch.int32))
+
+
+# ---- tables that ask for what there is not -----------------------------------------------------------
+def full_tables(b, seed):
+    """Every entry of both tables names a page of the cache, and every place holds a number: a row that is cut to its table sees only those."""
+    rng = np.random.default_rng(seed)
+    for table in (b.pt, b.ot):
+        bad = (table < 0) | (table >= b.pages)
+        table[bad] = rng.integers(0, b.pages, int(bad.sum()))
+    b.cache.nan_to_num_(0.25)
+    return b
+
+
+# what is asked for, and the lengths and bounds that the header's cut leaves of it (None: as they were); the runs that fall are those of three prefixes
+CUTS = {
+    "own length": (dict(own=(1, 10 ** 6)), dict(own=(1, "width"))),
+    "longest own length": (dict(own=(3, 2 ** 31 - 1)), dict(own=(3, "width"))),
+    "negative length": (dict(own=(1, -5)), dict(own=(1, 0))),
+    "prefix length": (dict(prefix=(0, 2 ** 31 - 1)), dict(prefix=(0, "width"))),
+    "negative prefix length": (dict(prefix=(1, -1)), dict(prefix=(1, 0))),
+    "runs fall": (dict(runs=[0, 4, 2, 6]), dict(runs=[0, 4, 4, 6])),
+    "runs fall at once": (dict(runs=[5, 1, 0, 0]), dict(runs=[5, 5, 5, 5])),
+    "runs beyond": (dict(runs=[-2, 3, 5, 90]), dict(runs=[0, 3, 5, 6])),
+    "runs all beyond": (dict(runs=[9, 10, 11, 12]), dict(runs=[6, 6, 6, 6])),
+}
+
+
+@pytest.mark.parametrize("wide", [1, apart(6, 2), 600])
+@pytest.mark.parametrize("what", list(CUTS))
+@pytest.mark.parametrize("dim", [64, 128])
+def test_lengths_and_runs_are_cut_to_what_there_is(L, what, wide, dim):
+    """Every row's value, the cut ones' among them, is that of the cut lengths and runs, and the status says that something was cut."""
+    b = full_tables(Batch(8, 2, dim, [200, 64, 130], [0, 3, 5, 6], [30, 70, 64, 5, 0, 17], seed=12, wide=wide), 5)
+    run(L, b)
+    b.check()
+    assert b.status.item() == 0
+    asked, left = CUTS[what]
+
+    def put(change):
+        for name, value in change.items():
+            if name == "runs":
+                b.runs = list(value)
+            else:
+                lens, table = (b.own, b.ot) if name == "own" else (b.prefixes, b.pt)
+                lens[value[0]] = table.shape[1] * PAGE if value[1] == "width" else value[1]
+
+    put(asked)
+    b.upload()
+    b.out.fill_(5.0)
+    run(L, b)
+    assert b.status.item() == 400
+    put(left)
+    b.check()
+
+
+@pytest.mark.parametrize("wide", [1, apart(4, 2), 600])
+@pytest.mark.parametrize("page", [-1, -2 ** 31, 2 ** 31 - 1, "pages"])
+def test_pages_that_there_are_not_leave_the_other_rows_right(L, page, wide):
+    """A bad page of one row, then of one of two prefixes: rows that do not read it have their values, and nothing behind the rows is written."""
+    for which in ("own", "prefix"):
+        b = full_tables(Batch(8, 2, 128, [200, 300], [0, 2, 4], [30, 70, 64, 5], seed=13, wide=wide), 6)
+        bad = b.pages if page == "pages" else page
+        table = b.ot if which == "own" else b.pt
+        table[1, 1] = bad
+        b.upload()
+        run(L, b)
+        assert b.status.item() == 400
+        table[1, 1] = 0
+        b.check(rows=[0, 2, 3] if which == "own" else [0, 1])
+        assert torch.isfinite(b.out[:4]).all() and (b.out[4:] == 5.0).all()
+
+
+# ---- rows ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("f32", [False, True])
+def test_a_single_row_in_place_under_two_pitches(L, f32):
+    dtype = torch.float32 if f32 else torch.bfloat16
+    x, positions = randn(4, (1, 3, 128), dtype), cuda_i32([70001])
+    freqs, _ = frequencies(L, 128)
+    want, mag = turned(x, positions, freqs, 1.0, 128, 1)
+    assert L.oa_k_rotary(ptr(x), 384, ptr(x), 2 ** 62, ptr(positions), 1, 3, 128, 128, 1, freqs.ctypes.data, 1.0, 0, int(f32), now()) == 0
+    torch.cuda.synchronize()
+    assert_turned(x, want, mag, dtype, 2.0 ** -52 * 70001)
+    b = Batch(8, 2, 128, [100], [0, 1], [7], seed=3)
+    run(L, b)
+    pt, pl, pr, ot, ol = b.d
+    q = b.q.clone()
+    assert L.oa_k_prefix_attention(ptr(q), 2 ** 61, ptr(q), 1024, ptr(b.cache), b.pages, ptr(pt), b.pt.shape[1], ptr(pl), ptr(pr), 1, ptr(ot), b.ot.shape[1], ptr(ol), 1, 8, 2, 128, 0.0, None, now()) == 0
+    torch.cuda.synchronize()
+    assert same_bits(q, b.out[:1])
+
+
+# ---- captured calls -------------------------------------------------------------------------------------
+class Appends:
+    """q, k and v of new tokens, rotated and written to a cache; the transposed rotation of q in fp32; copies of two pages."""
+
+    def __init__(self, L, tokens, seed):
+        self.L, self.tokens, self.heads, self.n_kv, self.dim, self.pages = L, tokens, 8, 2, 128, tokens // PAGE + 9
+        self.width = (self.heads + 2 * self.n_kv) * self.dim
+        self.freqs, self.amp = frequencies(L, 128, 1e6, 3, 4.0, 32.0, 1.0, 32768)
+        self.qkv, self.g = randn(seed, (tokens, self.width)), randn(seed + 1, (tokens, 8 * 128), torch.float32)
+        self.start = randn(seed + 2, (2, self.pages, self.n_kv, PAGE, self.dim))
+        self.cache, self.q, self.dx = self.start.clone(), torch.empty(tokens, 1024, dtype=torch.bfloat16, device="cuda"), torch.empty(tokens, 1024, dtype=torch.float32, device="cuda")
+        free = self.pages - 4                                                       # the last four pages are for the copies
+        self.rng = np.random.default_rng(seed)
+        self.positions, self.slots = cuda_i32(self.rng.integers(0, 30000, tokens)), cuda_i32(self.rng.permutation(free * PAGE)[:tokens])
+        self.moves = (_lib.OaPageMove * 3)(*[_lib.OaPageMove(s, free + i, n) for i, (s, n) in enumerate([(0, 64), (0, 17), (1, 64)])])
+        self.status = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def call(self, stream=None):
+        L, s, f, k0 = self.L, stream or now(), self.freqs.ctypes.data, self.qkv.data_ptr() + 2 * 1024
+        rc = L.oa_k_rotary_cache(ptr(self.qkv), self.width, k0, k0 + 512, self.width, ptr(self.q), 1024, ptr(self.cache), self.pages, ptr(self.positions), ptr(self.slots), self.tokens, self.heads,
+                                 self.n_kv, self.dim, 128, 1, f, self.amp, ptr(self.status), s)
+        rc = rc or L.oa_k_rotary(ptr(self.g), 1024, ptr(self.dx), 1024, ptr(self.positions), self.tokens, 8, 128, 128, 0, f, self.amp, 1, 1, s)
+        return rc or L.oa_k_cache_copy(ptr(self.cache), 2, self.pages, self.n_kv, self.dim, 2, self.moves, 3, s)
+
+    def outputs(self):
+        return [self.cache.clone(), self.q.clone(), self.dx.clone(), self.status.clone()]
+
+    def reset(self):
+        self.cache.copy_(self.start), self.q.zero_(), self.dx.zero_(), self.status.zero_()
+
+    def change(self):
+        """Other positions, slots and rows, where the device arrays lie."""
+        free = self.pages - 4
+        self.positions.copy_(cuda_i32(self.rng.integers(0, 30000, self.tokens))), self.slots.copy_(cuda_i32(self.rng.permutation(free * PAGE)[: self.tokens]))
+        self.qkv.neg_(), self.g.mul_(0.5)
+
+
+@pytest.mark.parametrize("tokens", [1, 6, 130, 2003])
+def test_captured_calls_keep_host_arrays_and_follow_device_arrays(L, tokens):
+    """A replay has the frequencies and moves that the call was captured with, whatever lies in their arrays now, and the positions, slots and rows of the replay."""
+    a = Appends(L, tokens, seed=tokens)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert a.call() == 0
+    a.reset()
+    freqs, moves = a.freqs.copy(), [(m.src, m.dst, m.tokens) for m in a.moves]
+    for replay in range(3):
+        if replay:
+            a.change()
+        a.freqs[:] = freqs
+        for m, (src, dst, n) in zip(a.moves, moves):
+            m.src, m.dst, m.tokens = src, dst, n
+        a.reset()
+        assert a.call() == 0
+        torch.cuda.synchronize()
+        want = a.outputs()
+        a.freqs[:] = 1e9
+        for m in a.moves:
+            m.src, m.dst, m.tokens = 10 ** 6, -1, 99
+        a.reset()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(same_bits(x, y) for x, y in zip(a.outputs(), want)), replay
+    assert not same_bits(a.start, a.cache) and a.status.item() == 0
+
+
+# ---- threads ----------------------------------------------------------------------------------------------
+def test_two_threads_on_two_streams(L):
+    """Each thread has a cache, tables, a stream and errors of its own; every result is the one that the calls give alone."""
+    wanted = []
+    for t in range(2):
+        b = Batch(32, 8, 128, [900], [0, 30], [(i * 29) % 300 for i in range(30)], seed=15) if t else Batch(8, 2, 64, [5000], [0, 50], [(i * 17) % 90 for i in range(50)], seed=16)
+        a = Appends(L, 700 + 600 * t, seed=t)
+        run(L, b), a.reset()
+        assert a.call() == 0
+        torch.cuda.synchronize()
+        wanted.append((b, b.out.clone(), a, a.outputs()))
+    failures, start = [], threading.Barrier(2)
+
+    def work(t):
+        try:
+            b, first, a, outputs = wanted[t]
+            side = torch.cuda.Stream()
+            stream = C.c_void_p(side.cuda_stream)
+            start.wait()
+            with torch.cuda.stream(side):
+                for i in range(30):
+                    b.out.fill_(5.0), a.reset()
+                    assert b.call(L, stream=stream) == 0 and a.call(stream) == 0
+                    assert L.oa_k_cache_copy(ptr(a.cache), 0 if t else 2, a.pages, 2, 128, 2 if t else 3, a.moves, 1, stream) == 400 and "cache copy" in _lib.last_error()
+                    assert L.oa_k_prefix_attention(None, 0, None, 0, None, 1, None, 1, None, None, 0, None, 1, None, 1, 8, 2, 96 + t, 0.0, None, stream) == 400 and "64 or 128" in _lib.last_error()
+                    if i % 10 == 9:
+                        side.synchronize()
+                        assert same_bits(b.out, first) and all(same_bits(x, y) for x, y in zip(a.outputs(), outputs)), (t, i)
+        except BaseException as e:      # noqa: BLE001
+            failures.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(t,)) for t in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failures, failures
