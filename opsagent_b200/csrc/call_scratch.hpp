@@ -7,6 +7,19 @@
 
 namespace oa {
 
+// Making the pool is no work of a stream, and a stream that is being captured, here or on another thread, would refuse it and lose its capture: it is allowed on this thread for as long as
+// this lives.
+class BesideCaptures {
+public:
+    BesideCaptures() { if (cudaThreadExchangeStreamCaptureMode(&mode_) != cudaSuccess) known_ = false; }
+    BesideCaptures(const BesideCaptures&) = delete;
+    ~BesideCaptures() { if (known_) cudaThreadExchangeStreamCaptureMode(&mode_); }
+
+private:
+    cudaStreamCaptureMode mode_ = cudaStreamCaptureModeRelaxed;
+    bool known_ = true;
+};
+
 // Scratch of one call (partials, plans, tables) comes from a stream-ordered pool of this library's own, one per device, made at the first use:
 // cudaMalloc and cudaFree stop the whole device and cost 0.1 ms to several ms a call, more than most kernels here (paged attention of 6 x 3000
 // tokens: 10 us of kernels in a call of 0.7 ms and more; from the pool 0.05 ms).  An allocation is ordered on the call's stream, so calls on
@@ -21,6 +34,7 @@ inline cudaMemPool_t scratch_pool() {
     std::lock_guard<std::mutex> lk(mu);
     cudaMemPool_t& pool = pools[dev];
     if (!pool) {
+        const BesideCaptures making_the_pool;
         cudaMemPoolProps props{};
         props.allocType = cudaMemAllocationTypePinned; props.handleTypes = cudaMemHandleTypeNone;
         props.location.type = cudaMemLocationTypeDevice; props.location.id = dev;

@@ -1,6 +1,9 @@
-"""Calls of the operators on a caller's paged cache as a program makes them on the B200: tables that ask for what there is not (and what is cut to what there is), captured calls,
-calls from two threads on two streams.  Values against the 64-bit oracles and tolerances of test_cache_ops_gpu.py, or against an eager call's bits."""
+"""Calls of the operators on a caller's paged cache as a program makes them on the B200: tables that ask for what there is not (and what is cut to what there is), captured calls, a first call that
+is captured, calls from two threads on two streams.  Values against the 64-bit oracles and tolerances of test_cache_ops_gpu.py, or against an eager call's bits."""
 import ctypes as C
+import os
+import subprocess
+import sys
 import threading
 
 import numpy as np
@@ -11,6 +14,8 @@ pytestmark = pytest.mark.gpu
 
 from opsagent_b200 import _lib  # noqa: E402
 from test_cache_ops_gpu import PAGE, Batch, apart, assert_turned, cuda_i32, frequencies, now, ptr, randn, run, turned  # noqa: E402
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.fixture(scope="module")
@@ -175,6 +180,51 @@ def test_captured_calls_keep_host_arrays_and_follow_device_arrays(L, tokens):
         torch.cuda.synchronize()
         assert all(same_bits(x, y) for x, y in zip(a.outputs(), want)), replay
     assert not same_bits(a.start, a.cache) and a.status.item() == 0
+
+
+FIRST = r'''
+import sys
+sys.path[:0] = [sys.argv[1], sys.argv[1] + "/tests"]
+import torch
+torch.zeros(8, device="cuda").normal_()
+from test_cache_ops_calls_gpu import Appends, Batch, _lib, run, same_bits
+L, what = _lib.load(), sys.argv[2]
+if what == "attention":
+    b = Batch(8, 2, 128, [300], [0, 6], [11, 1, 64, 90, 2, 65], seed=13, wide=int(sys.argv[3]))
+else:
+    b = Appends(L, 130, 7)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    rc = b.call(L) if what == "attention" else b.call()
+assert rc == 0, (rc, _lib.last_error())
+if what == "attention":
+    for _ in range(2):
+        b.out.fill_(5.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        b.check()
+    first = b.out.clone()
+    run(L, b)
+    assert same_bits(first, b.out)
+else:
+    b.reset()
+    graph.replay()
+    torch.cuda.synchronize()
+    first = b.outputs()
+    b.reset()
+    assert b.call() == 0
+    torch.cuda.synchronize()
+    assert all(same_bits(x, y) for x, y in zip(first, b.outputs()))
+print("same")
+'''
+
+
+@pytest.mark.parametrize("what,wide", [("attention", 1), ("attention", 600), ("appends", 0)])
+def test_a_process_may_capture_its_first_call(L, what, wide):
+    """Nothing that the library makes at its first use (its pool of scratch memory, attributes of its kernels) ends a capture."""
+    r = subprocess.run([sys.executable, "-c", FIRST, ROOT, what, str(wide)], capture_output=True, text=True, timeout=300, cwd=ROOT)
+    assert r.returncode == 0 and r.stdout.strip().endswith("same"), (r.stdout[-500:], r.stderr[-3000:])
 
 
 # ---- threads ----------------------------------------------------------------------------------------------
