@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(COPY_THREADS) cache_copy_kernel(const __grid_c
                 const unsigned c = first + i * COPY_THREADS + threadIdx.x;
                 const unsigned head = tokens == CACHE_PAGE ? 0 : c / piece;
                 at[i] = c + head * (page16 - piece);
-                if (c < stop) { mine |= 1u << i; v[i] = ld_nc_16(src + at[i]); }
+                if (c < stop) { mine |= 1u << i; v[i] = ld_once_16(src + at[i]); }
             }
         }
         uint4* dst = base + (int64_t)m.dst * a.n_kv * page16;

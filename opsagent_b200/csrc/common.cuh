@@ -311,10 +311,10 @@ OA_DEVINL float warp_sum(float v) {
     return v;
 }
 
-// 16-byte global accesses
-OA_DEVINL uint4 ld_nc_16(const void* p) {
+// 16 bytes that a thread reads once.  Not by the read-only path, which asks that nothing writes them while the kernel lives: it may live before the kernel that writes them has ended
+OA_DEVINL uint4 ld_once_16(const void* p) {
     uint4 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
     return r;
 }
 

@@ -227,6 +227,38 @@ def test_a_process_may_capture_its_first_call(L, what, wide):
     assert r.returncode == 0 and r.stdout.strip().endswith("same"), (r.stdout[-500:], r.stderr[-3000:])
 
 
+# ---- calls one after the other --------------------------------------------------------------------------
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("n_kv,tokens", [(8, 64), (2, 3), (32, 64)])
+def test_a_copy_has_what_the_calls_before_it_wrote(L, n_kv, tokens, captured):
+    """Page 0 is written, copied, written again, copied, two hundred times without a wait on the host: every kernel may start before the one ahead of it has ended, and each copy holds its own step's
+    keys and values."""
+    steps, dim, heads = 200, 64, n_kv
+    width = 3 * heads * dim
+    rows, freqs = randn(9, (steps, tokens, width)), np.zeros(dim // 2)                # angles of 0: keys come out as they are
+    cache = torch.zeros((2, steps + 1, n_kv, PAGE, dim), dtype=torch.bfloat16, device="cuda")
+    q, positions, slots = torch.empty(tokens, heads * dim, dtype=torch.bfloat16, device="cuda"), cuda_i32(np.arange(tokens)), cuda_i32(np.arange(tokens))
+    moves = [(_lib.OaPageMove * 1)(_lib.OaPageMove(0, i + 1, tokens)) for i in range(steps)]
+
+    def chain():
+        for i in range(steps):
+            at = rows[i].data_ptr()
+            assert L.oa_k_rotary_cache(at, width, at + 2 * heads * dim, at + 4 * heads * dim, width, ptr(q), heads * dim, ptr(cache), steps + 1, ptr(positions), ptr(slots), tokens, heads, n_kv, dim,
+                                       dim, 1, freqs.ctypes.data, 1.0, None, now()) == 0
+            assert L.oa_k_cache_copy(ptr(cache), 2, steps + 1, n_kv, dim, 2, moves[i], 1, now()) == 0
+
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            chain()
+    for _ in range(5):
+        cache.zero_(), q.zero_()
+        graph.replay() if captured else chain()
+        torch.cuda.synchronize()
+        kv = rows.view(steps, tokens, 3, n_kv, dim)[:, :, 1:].permute(2, 0, 3, 1, 4)        # [planes, steps, heads, tokens, channels]
+        assert torch.equal(cache[:, 1:, :, :tokens], kv) and not cache[:, :, :, tokens:].any() and torch.equal(q, rows[-1, :, :heads * dim])
+
+
 # ---- threads ----------------------------------------------------------------------------------------------
 def test_two_threads_on_two_streams(L):
     """Each thread has a cache, tables, a stream and errors of its own; every result is the one that the calls give alone."""

@@ -107,6 +107,13 @@ def test_tensor_memory_is_held_before_the_next_kernel_may_start():
     assert seen >= 8
 
 
+def test_copies_do_not_read_by_the_read_only_path():
+    """A page may have been written by the kernel ahead, which has not ended when the copy's CTAs start: loads that ask for memory nobody writes while their kernel lives are not for it."""
+    for name in ("cache_copy.cu", "common.cuh"):
+        text = re.sub(r"//[^\n]*", "", open(os.path.join(ROOT, "opsagent_b200", "csrc", name)).read())
+        assert not re.search(r"ld\.global\.nc|__ldg\(", text), name
+
+
 # ---- pitches and rows ------------------------------------------------------------------------------
 BUF, FREQS = np.zeros(4096, np.int32), np.ones(128)
 P, FAR = (BUF.ctypes.data + 15) // 16 * 16, 1 << 40                       # addresses alone: nothing behind them is touched before a device is found
