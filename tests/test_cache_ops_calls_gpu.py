@@ -259,6 +259,89 @@ def test_a_copy_has_what_the_calls_before_it_wrote(L, n_kv, tokens, captured):
         assert torch.equal(cache[:, 1:, :, :tokens], kv) and not cache[:, :, :, tokens:].any() and torch.equal(q, rows[-1, :, :heads * dim])
 
 
+@pytest.mark.parametrize("wide", [1, apart(12, 2), 600])
+@pytest.mark.parametrize("captured", [False, True])
+def test_steps_without_a_wait_are_those_with_one(L, wide, captured):
+    """Sixty decoding steps: lengths rise on the device, a new token is rotated into its page, attention reads it, in place.  Nothing waits between them, and no step reads what a later one writes or misses
+    what an earlier one wrote."""
+    steps, n, heads, n_kv, dim = 60, 12, 8, 2, 128
+    own = [0, 1, 30, 63, 64, 100, 3, 0, 127, 65, 10, 5]
+    b = Batch(heads, n_kv, dim, [200, 300], [0, 5, 11], own, seed=21, wide=wide)
+    at, b.ot = 0, np.full((n, 4), -1, np.int32)                                        # room for sixty tokens more, in pages of their own
+    free = np.random.default_rng(2).permutation(200).astype(np.int32)
+    cache = torch.full((2, 200, n_kv, PAGE, dim), float("nan"), dtype=torch.bfloat16, device="cuda")
+    for table, lens, room in ((b.pt, b.prefixes, 0), (b.ot, own, steps)):
+        for i, x in enumerate(lens):
+            k = -(-(x + room) // PAGE)
+            table[i, :k] = free[at:at + k]
+            at += k
+            for j in range(-(-x // PAGE)):
+                cache[:, int(table[i, j]), :, : min(PAGE, x - j * PAGE)] = randn(i * 10 + j + room, (2, n_kv, min(PAGE, x - j * PAGE), dim))
+    b.cache, b.pages, b.pad = cache, 200, 0
+    b.upload()
+    rows, freqs = randn(5, (steps, n, (heads + 2 * n_kv) * dim)), frequencies(L, dim)[0]
+    tables, outs, start = cuda_i32(b.ot).long(), torch.empty(steps, n, heads * dim, dtype=torch.bfloat16, device="cuda"), cuda_i32(own)
+    positions, slots, width = start.clone(), start.clone(), rows.shape[2]
+
+    def steps_of(wait):
+        for i in range(steps):
+            positions.copy_(b.d[4])
+            slots.copy_(torch.gather(tables, 1, (b.d[4] // PAGE).long()[:, None])[:, 0] * PAGE + b.d[4] % PAGE)
+            k0 = rows[i].data_ptr() + 2 * heads * dim
+            assert L.oa_k_rotary_cache(ptr(rows[i]), width, k0, k0 + 2 * n_kv * dim, width, ptr(outs[i]), heads * dim, ptr(cache), 200, ptr(positions), ptr(slots), n, heads, n_kv, dim, dim, 1,
+                                       freqs.ctypes.data, 1.0, ptr(b.status), now()) == 0
+            b.d[4].add_(1)
+            if wait:
+                torch.cuda.synchronize()
+            assert b.call(L, q=outs[i], out=outs[i]) == 0
+            if wait:
+                torch.cuda.synchronize()
+
+    def again():
+        cache.copy_(before), b.d[4].copy_(start), outs.zero_()
+
+    before = cache.clone()
+    steps_of(wait=True)
+    want, last = outs.clone(), cache.clone()
+    assert b.status.item() == 0 and torch.isfinite(want).all() and b.d[4].tolist() == [x + steps for x in own]
+    if captured:
+        again()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            steps_of(wait=False)
+    for _ in range(4):
+        again()
+        graph.replay() if captured else steps_of(wait=False)
+        torch.cuda.synchronize()
+        assert same_bits(outs, want) and same_bits(cache, last)
+    b.own = [x + steps for x in own]
+    q = torch.empty(n, heads * dim, dtype=torch.bfloat16, device="cuda")
+    assert L.oa_k_rotary(ptr(rows[-1]), width, ptr(q), heads * dim, ptr(positions), n, heads, dim, dim, 1, freqs.ctypes.data, 1.0, 0, 0, now()) == 0
+    b.check(out=outs[-1], q=q)
+
+
+def test_two_captured_calls_at_once(L):
+    """Two graphs on two streams, replayed over one another: neither has the other's scratch."""
+    bs = [Batch(32, 8, 128, [900], [0, 30], [(i * 29) % 300 for i in range(30)], seed=15), Batch(8, 2, 64, [5000], [0, 50], [(i * 17) % 90 for i in range(50)], seed=16)]
+    streams, graphs = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for b in bs:
+        run(L, b)
+        b.first = b.out.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(3):
+                assert b.call(L) == 0
+        graphs.append(graph)
+    for _ in range(20):
+        for b, s, g in zip(bs, streams, graphs):
+            with torch.cuda.stream(s):
+                b.out.fill_(5.0)
+                g.replay()
+    torch.cuda.synchronize()
+    for b in bs:
+        assert same_bits(b.out, b.first)
+
+
 # ---- threads ----------------------------------------------------------------------------------------------
 def test_two_threads_on_two_streams(L):
     """Each thread has a cache, tables, a stream and errors of its own; every result is the one that the calls give alone."""
