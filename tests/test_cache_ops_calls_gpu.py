@@ -342,6 +342,48 @@ def test_two_captured_calls_at_once(L):
         assert same_bits(b.out, b.first)
 
 
+@pytest.mark.parametrize("heads,n_kv,dim", [(8, 2, 128), (8, 2, 64), (5, 1, 128)])
+def test_prompts_on_a_cache_that_was_cleared_once(L, heads, n_kv, dim):
+    """Prompts of any length grow into pages, are rotated and written by one call and attended to by oa_k_paged_attention, whose tables name nothing (-1) behind a row's end; then pages are freed,
+    handed on as they are and grown into again by shorter prompts.  The one condition is a cache that was cleared after its allocation."""
+    width, pages = 8, 64
+    cache = torch.zeros((2, pages, n_kv, PAGE, dim), dtype=torch.bfloat16, device="cuda")
+    rng, (freqs, amp) = np.random.default_rng(5), frequencies(L, dim)
+    for lens in ([1, 63, 64, 65, 127, 128, 129, 200, 300], [300, 17, 64, 1, 100, 129, 5, 65, 191], [2, 3, 1, 66, 70, 190, 130, 64, 63]):
+        n = len(lens)
+        tables, have, refs = np.full((n, width), -1, np.int32), np.zeros(n, np.int32), np.zeros(pages, np.int32)
+        refs[rng.permutation(pages)[:20]] = 1                                          # pages that another part of a program holds
+        table = _lib.OaPageTable(tables.ctypes.data, have.ctypes.data, refs.ctypes.data, n, width, pages)
+        for r, x in enumerate(lens):
+            assert L.oa_host_cache_grow(table, r, x) == 0
+        at = [(r, i) for r, x in enumerate(lens) for i in range(x)]
+        qkv = randn(sum(lens) + dim, (len(at), (heads + 2 * n_kv) * dim))
+        q, out = (torch.empty((len(at), heads * dim), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        k0, slots, where = qkv.data_ptr() + 2 * heads * dim, [int(tables[r, i // PAGE]) * PAGE + i % PAGE for r, i in at], cuda_i32([i for _, i in at])
+        assert L.oa_k_rotary_cache(ptr(qkv), qkv.shape[1], k0, k0 + 2 * n_kv * dim, qkv.shape[1], ptr(q), heads * dim, ptr(cache), pages, ptr(where), ptr(cuda_i32(slots)), len(at), heads, n_kv, dim, dim,
+                                   1, freqs.ctypes.data, amp, None, now()) == 0
+        ctx = np.array(lens, np.int32)
+        assert L.oa_k_paged_attention(ptr(q), ptr(out), ptr(cache), pages, tables.ctypes.data, width, ctx.ctypes.data, ctx.ctypes.data, n, heads, n_kv, dim, 0, now()) == 0
+        torch.cuda.synchronize()
+        first = 0
+        for r, x in enumerate(lens):
+            rows = torch.tensor(tables[r, : -(-x // PAGE)].astype(np.int64), device="cuda")
+            k, v = (cache[p, rows].double().transpose(1, 2).reshape(-1, n_kv, dim)[:x] for p in (0, 1))
+            y = q[first:first + x].double().view(x, n_kv, -1, dim)
+            s = torch.einsum("tkhd,pkd->tkhp", y, k) / dim ** 0.5
+            seen = (torch.arange(x, device="cuda")[None] <= torch.arange(x, device="cuda")[:, None])[:, None, None]
+            p = torch.softmax(s.masked_fill(~seen, -float("inf")), -1)
+            want, size = torch.einsum("tkhp,pkd->tkhd", p, v), torch.einsum("tkhp,pkd->tkhd", p, v.abs())
+            got = out[first:first + x].double().view(want.shape)
+            # a weight rounded to bf16, scores as sums of products in fp32 that move a weight by twice that, the result's own rounding
+            score = torch.einsum("tkhd,pkd->tkhp", y.abs(), k.abs()).amax(-1, keepdim=True) / dim ** 0.5
+            tol = size * (2.0 ** -8 + 2 * (dim + 4) * 2.0 ** -24 * score + 2.0 ** -18) + want.abs() * 2.0 ** -8 * (1 + 2.0 ** -7) + 2.0 ** -133
+            assert bool(((got - want).abs() <= tol).all()), (lens, r, ((got - want).abs() / tol).max().item())
+            first += x
+        everyone = np.arange(n, dtype=np.int32)
+        assert L.oa_host_cache_free(table, everyone.ctypes.data, n) == 0 and (have == 0).all() and (tables == -1).all() and refs.sum() == 20
+
+
 # ---- threads ----------------------------------------------------------------------------------------------
 def test_two_threads_on_two_streams(L):
     """Each thread has a cache, tables, a stream and errors of its own; every result is the one that the calls give alone."""
