@@ -138,7 +138,7 @@ OA_API int oa_bench_decode(oa_engine*, int32_t batch, int32_t ctx_len, int32_t s
 /* in-situ per-kernel-class timings accumulated while OA_PROFILE_ALL=1 (JSON name -> [total ms, launches]) */
 OA_API int oa_debug_kernel_times(oa_engine*, char* buf, size_t n, int32_t reset);
 
-/* kernel-level entry points on raw device pointers (tests call these with torch-allocated memory) */
+/* kernel-level entry points on raw device pointers, for programs that bring their own tensors (torch's, say) */
 OA_API int oa_k_rmsnorm(const void* x, const void* gain, void* y, int32_t T, int32_t H, float eps, void* stream);
 OA_API int oa_k_gemm(const void* A, const void* B, int32_t M, int32_t N, int32_t K, int32_t epilogue, int32_t block_n, void* out,
               const void* bias, const void* resid, float* logits, int32_t* argmax_out, void* stream);
@@ -155,13 +155,16 @@ OA_API int oa_k_hybrid_gemm(int32_t mode, const void* A, int32_t lda, const void
 OA_API int oa_k_init_weight(void* dst, uint64_t seed, uint64_t tensor_id, int64_t tensor_id_b, int64_t rows, int64_t cols, float std,
                      float mean, void* stream);
 /* paged attention on a caller-provided cache [2(K,V)][num_pages][n_kv][64][D] (one layer): decode when q has one
- * row per sequence (n_q_rows == n_seqs), otherwise causal prefill of `q_lens[i]` new rows per sequence */
+ * row per sequence (n_q_rows == n_seqs), otherwise causal prefill of `q_lens[i]` new rows per sequence.  Whole pages are read and what lies behind a
+ * sequence's end is weighted with 0: the cache holds finite values everywhere (cleared once after its allocation, whatever calls leave in it later
+ * may stay), or NaN behind an end comes out.  Waits for the stream */
 OA_API int oa_k_paged_attention(const void* q, void* out, const void* kv_cache, int32_t num_pages, const int32_t* block_tables,
                          int32_t max_pages_per_seq, const int32_t* ctx_lens, const int32_t* q_lens, int32_t n_seqs,
                          int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t force_splits, void* stream);
 /* ---- operators on a caller's paged cache: [planes][num_pages][n_kv][64][head_dim], planes = K and V of each layer (a layer's two planes are the kv_cache
- * of oa_k_paged_attention).  All of them only enqueue on `stream` of the device that holds the cache, whichever device is current, never synchronise and can be
- * captured; a captured call keeps the host arrays' values.  400 with a text in oa_last_error() where an argument cannot be served; nothing has been enqueued then.
+ * of oa_k_paged_attention: clear it once if that entry is to read it; the operators here ignore what lies behind an end, and copy it with whole pages).  All of them only enqueue on `stream` of the device that holds the cache, whichever device is current, never synchronise and can be
+ * captured, a process's first call too; a captured call keeps the host arrays' values.  Rows of one or more heads are `pitch` elements apart, of which a single row has none; rows of two
+ * pitches in one stretch of memory count as overlapping, and 2^39 elements from the first row to the last are refused.  400 with a text in oa_last_error() where an argument cannot be served; nothing has been enqueued then.
  * `status` (device int32, or NULL): set to 400 where a device array asks for what there is not; never cleared. ---- */
 /* frequencies of rotary positions: base^(-2i / rot_dims), i < rot_dims / 2, in 64 bits.  scaling 0: as they are; 1: / factor; 2 (llama3): / factor below `first`
  * turns in `original` positions, as they are above `second` turns, blended in between; 3 (YaRN): blended along a ramp over i between where `first` (fast) and
@@ -169,11 +172,11 @@ OA_API int oa_k_paged_attention(const void* q, void* out, const void* kv_cache, 
 OA_API int oa_host_rotary_freqs(int32_t rot_dims, double base, int32_t scaling, double factor, double first, double second, int32_t original, double* freqs_out, float* amplitude_out);
 /* out[t, h, :] = x[t, h, :] with the first rot_dims of head_dim channels turned by positions[t] (device) times freqs (host): layout 0: channel 2i with 2i + 1,
  * 1: channel i with i + rot_dims / 2; cos and sin times amplitude.  transpose != 0: the transposed map (the gradient's).  bf16, or fp32 where f32 != 0; sums fp32.  ldx, ldo: elements
- * from row to row; out is x itself or does not overlap it.  head_dim even, any alignment of the elements (rows of whole 16-byte pieces are faster) */
+ * from row to row; out is x itself or does not overlap it.  head_dim even, up to 2^16 channels and as many heads, any alignment of the elements (rows of whole 16-byte pieces are faster) */
 OA_API int oa_k_rotary(const void* x, int64_t ldx, void* out, int64_t ldo, const int32_t* positions, int32_t T, int32_t n_heads, int32_t head_dim, int32_t rot_dims, int32_t layout,
                        const double* freqs, float amplitude, int32_t transpose, int32_t f32, void* stream);
 /* the same for T new tokens of a layer (bf16): q [T, n_heads, head_dim] -> q_out (q itself or apart from it, and apart from k and v), k turned and v as it is -> row slots[t] % 64 of page
- * slots[t] / 64 (slots: device; negative: the token is not written; distinct otherwise).  Other places of the cache stay as they are */
+ * slots[t] / 64 (slots: device; negative: the token is not written; distinct otherwise).  Up to 2^14 key/value heads.  Other places of the cache stay as they are */
 OA_API int oa_k_rotary_cache(const void* q, int64_t ldq, const void* k, const void* v, int64_t ldkv, void* q_out, int64_t ldqo, void* kv_cache, int32_t num_pages,
                              const int32_t* positions, const int32_t* slots, int32_t T, int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t rot_dims, int32_t layout,
                              const double* freqs, float amplitude, int32_t* status, void* stream);
@@ -186,19 +189,23 @@ typedef struct {
     int32_t n_rows, max_pages_per_seq, num_pages;
 } oa_page_table;
 typedef struct { int32_t src, dst, tokens; } oa_page_move; /* the first `tokens` places of page src belong in page dst */
-OA_API int oa_host_cache_grow(const oa_page_table*, int32_t row, int32_t n_tokens);                  /* room for n_tokens more, in the lowest-numbered free pages */
+OA_API int oa_host_cache_grow(const oa_page_table*, int32_t row, int32_t n_tokens);                  /* room for n_tokens more (up to 2^31 - 1 in all), in the lowest-numbered free pages */
 OA_API int oa_host_cache_free(const oa_page_table*, const int32_t* rows, int32_t n);                 /* rows end: length 0, entries -1, references back */
 /* empty rows `children` become copies of `parent`: its full pages are shared, a last page that is not full is to be copied (a move per child, in their order) */
 OA_API int oa_host_cache_fork(const oa_page_table*, int32_t parent, const int32_t* children, int32_t n, oa_page_move* moves_out, int32_t cap, int32_t* n_moves_out);
-/* the pages in use become the lowest-numbered ones, in the order they had; rows name the new pages.  What else names a page by number has to follow the moves */
+/* the pages in use become the lowest-numbered ones: the i-th of them beyond their count moves to the i-th free one below it, the others stay; rows name the new pages.  What else names
+ * a page by number has to follow the moves */
 OA_API int oa_host_cache_compact(const oa_page_table*, oa_page_move* moves_out, int32_t cap, int32_t* n_moves_out);
-/* carries moves (host) out in all planes of a cache of elem_bytes 2 or 4: no page may be the target of two moves, or a target and a source */
+/* carries moves (host) out in all planes of a cache of elem_bytes 2 or 4: no page may be the target of two moves, or a target and a source.  The cache starts on a 16-byte boundary, a
+ * token's row of a head is a multiple of 16 bytes up to 4096, up to 4096 heads */
 OA_API int oa_k_cache_copy(void* kv_cache, int32_t planes, int32_t num_pages, int32_t n_kv, int32_t head_dim, int32_t elem_bytes, const oa_page_move* moves, int32_t n_moves, void* stream);
 /* attention of one new token of each of n_seqs sequences (bf16) over a prefix that a run of sequences shares, read once for all of them, and over the sequence's own
  * tokens behind it: rows prefix_rows[p] .. prefix_rows[p + 1] - 1 see the first prefix_lens[p] places of the pages prefix_tables[p, :], and row i the first own_lens[i]
  * places of own_tables[i, :] (its new token among them, if it is to be seen).  A row without a prefix (before, behind or between the runs, or of a prefix of length 0) sees its
  * own tokens alone, one that sees nothing gets zeros.  All tables and lengths are on the device.  scale 0: 1 / sqrt(head_dim).  head_dim 64 or 128, up to 16 query heads of a key/value head, up to 32
- * prefixes.  out is q itself (same pitch) or apart from it; pitches and addresses are multiples of 16 bytes.  A page number beyond the cache, a length beyond its table or run
+ * prefixes, 2^20 sequences, 2^10 key/value heads and 2^24 pages a table; 2 num_pages n_kv 64 rows of the cache are counted in 31 bits.  out is q itself (same pitch) or apart from it; pitches and
+ * addresses are multiples of 16 bytes.  Softmax weights are rounded to bf16 for their product with the values, sums are fp32.  The host, which knows no length, divides the work by max_prefix_pages
+ * and max_own_pages: tables much wider than their prefixes cost time (128 rows on 1536 tokens: 41 us with 24 or 64 entries a prefix, 45 with 128).  A page number beyond the cache, a length beyond its table or run
  * bounds that fall set *status; rows that read such a page hold no meaningful value, lengths and bounds are cut to what there is */
 OA_API int oa_k_prefix_attention(const void* q, int64_t ldq, void* out, int64_t ldo, const void* kv_cache, int32_t num_pages, const int32_t* prefix_tables, int32_t max_prefix_pages,
                                  const int32_t* prefix_lens, const int32_t* prefix_rows, int32_t n_prefixes, const int32_t* own_tables, int32_t max_own_pages, const int32_t* own_lens,

@@ -20,9 +20,10 @@
 // CTA for itself: lengths may come from the kernel before, a captured call serves other lengths when it is replayed, and the host waits for nothing.  Parts are joined in one order, whatever
 // came first: the same call gives the same bits.
 //
-// The second kernel starts beside the first (it needs nothing of it): it streams own keys from memory while the first is busy with products, and their shared memory and registers are cut so
-// that an SM holds one CTA of each.  Whole calls: 128 rows of 4 x 8 heads on a prefix of 1536 40 us (162 MB; 25 at the copy rate): 3 to begin, 28 of stream, 3 between the first CTA's end and the last
-// one's, 5 for the join with its start; 8 rows of 4000 to 9000 own tokens 42 us for 221 MB.
+// The second kernel starts beside the first (it needs nothing of it): it streams own keys from memory while the first is busy with products, and for up to 8 heads a group their shared memory and
+// registers are cut so that an SM holds one CTA of each.  For 9 to 16 heads a group they are not (the own parts' kernel has 112 to 158 registers a thread): on an SM the own parts come after the
+// prefixes; 128 rows of 16 heads a group on 1536 tokens, own parts of 64 to 512: 46 us with 4 key/value heads of 128 (bytes 12.8 at the copy rate), 79 with 8 (25.6), 35 with 4 of 64 (6.4).
+// Whole calls: 128 rows of 4 x 8 heads on a prefix of 1536 40 us (162 MB; 25 at the copy rate): 3 to begin, 28 of stream, 3 between the first CTA's end and the last one's, 5 for the join with its start; 8 rows of 4000 to 9000 own tokens 42 us for 221 MB.
 #include "common.cuh"
 #include "kernels.hpp"
 #include "cache_ops.hpp"
@@ -103,7 +104,7 @@ OA_DEVINL PrePiece pre_piece(const PrefixPieces& px, int piece, int n_prefixes) 
 }
 
 template <int D, int KEYS, int SLOTS>
-// 104 registers: one CTA and one of the own parts' (96) fill an SM's file, two of this kernel do not fit (of 96 they would).  Started while the kernel before it leaves the SMs one by one, two
+// 104 registers: one CTA and one of the own parts' (96, up to 8 heads a group) fill an SM's file, two of this kernel do not fit (of 96 they would).  Started while the kernel before it leaves the SMs one by one, two
 // CTAs on one SM would have the second wait for the first one's TMEM, and the own parts' CTA go elsewhere: 8 to 15 us of a call of 45
 __global__ void __maxnreg__(104) prefix_part_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ PrefixAttnArgs a) {
     using Cfg = PreCfg<D, KEYS, SLOTS>;
@@ -798,7 +799,8 @@ __global__ void __launch_bounds__(JOIN_THREADS, JOIN_CTAS) join_parts_kernel(con
 // host
 // =============================================================================================
 // Prefixes are read with the sequences' own parts, once for each sequence, where that is few pages: two launches instead of three.  us with one kernel / two, heads of 64, own parts of
-// 50 to 200 tokens, rows x prefix: 4 x 256 9.0 / 10.0, 8 x 1024 11.5 / 13.1, 8 x 4096 20.1 / 15.2; 16 x 256 10.6 / 11.2, 32 x 128 12.2 / 13.0, 16 x 512 11.9 / 10.8, 32 x 256 13.5 / 12.8 (128 the same way)
+// 50 to 200 tokens, rows x prefix: 4 x 256 9.0 / 10.0, 8 x 1024 11.5 / 13.1, 8 x 4096 20.1 / 15.2; 16 x 256 10.6 / 11.2, 32 x 128 12.2 / 13.0, 16 x 512 11.9 / 10.8, 32 x 256 13.5 / 12.8 (128 the same way); 9 to 15
+// rows were not measured
 constexpr int PREFIX_INLINE_UNITS = 4, PREFIX_FEW_ROWS = 8;           // pages an SM; up to so many rows twice as many
 // Heads of 128: an SM's shared memory holds tiles of 64 keys beside four of the own parts' pages, or tiles of 128 beside two.  us with 64 / 128, own parts of 20 to 600 tokens: 128 rows of
 // 4 heads a group on a prefix of 1024 41.2 / 45.7, 4096 44.5 / 48.5, 8192 48.9 / 51.8; 64 rows of 8 heads a group 1024 30.6 / 31.6, 4096 33.1 / 34.1, 6144 34.9 / 35.6, 8192 40.2 / 37.1

@@ -6,12 +6,13 @@
 //
 // Bound by memory.  The places of a head of a page are one piece of up to 16 KB in each plane; a CTA copies up to 16 KB of a plane of a page, eight loads of 16
 // bytes in flight per thread, whose heads lie next to each other where whole pages are copied and a stride apart otherwise.  515 MB of whole pages (257 MB read, as
-// many written) take 78 us, 6.6 TB/s.
+// many written) take 83.3 us over three sets of inputs, 6.2 TB/s (78 with one, whose last pages L2 still holds).
 //
 // A fork writes one page to many.  A CTA then keeps what it has read in registers and writes it to several pages: as many as leave every SM the CTAs that it runs at
-// once, where at least every other pair's source is that of the pair before.  The bytes that come out of L2 are what it saves.  us for a page of 49 places in 64 planes
+// once (9 at 56 registers), where at least every other pair's source is that of the pair before.  The bytes that come out of L2 are what it saves.  us for a page of 49 places in 64 planes
 // of 8 x 128 channels written to 64 / 32 / 16 / 8 pages, a CTA for each pair: 103 / 53 / 25.6 / 10.3, by this rule (24, 12, 6, 3) 69 / 36 / 18.1 / 9.5, fewer (up to
-// 16, 12 CTAs an SM) 73 / 39 / 20.0 / 9.4, more (6 CTAs) 77 / 39 / 19.5 / 10.7; floors 64 / 32 / 17 / 9.
+// 16, 12 CTAs an SM) 73 / 39 / 20.0 / 9.4, more (6 CTAs) 77 / 39 / 19.5 / 10.7; floors 64 / 32 / 17 / 9.  A CTA's
+// pairs are rounded down and the groups of pairs up: each of these four launches has 1344 CTAs, where 1332 run at once, and its last group may have fewer pairs.
 #include "common.cuh"
 #include "kernels.hpp"
 #include "cache_ops.hpp"
@@ -19,7 +20,7 @@
 namespace oa {
 
 constexpr int COPY_THREADS = 128, COPY_UNROLL = 8, COPY_CHUNKS = COPY_THREADS * COPY_UNROLL;
-constexpr int COPY_SHARE_CTAS = 8 * 148;                      // as many as run at once
+constexpr int COPY_SHARE_CTAS = 8 * 148;                      // eight of an SM's nine: rounded up to groups, about as many as run at once
 
 template <int CAP>
 struct CopyArgs {

@@ -56,7 +56,7 @@ struct DevBuf {
     ~DevBuf() { if (p) cudaFreeAsync(p, s); }
 };
 
-// The device that holds a call's memory, current for as long as this lives.  ok(): every pointer is device (or managed) memory of that one device.
+// The device that holds a call's memory, current for as long as this lives, if foreign() is false and error() is none: then every pointer is device (or managed) memory of that one device.
 class CallDevice {
 public:
     explicit CallDevice(std::initializer_list<const void*> pointers) {

@@ -11,7 +11,8 @@
 // Bound by memory.  A CTA walks over tokens (where one does not fill it) with ROT_CTAS of them on an SM: a thread holds its pair's frequency throughout, takes the pair's cos and sin of the
 // token under the loads of its first units, and reads those of its place in a head once a token; the next token's position comes a token ahead.  Pieces stay packed
 // until they turn: 80 registers a thread, four units of 32 bytes in flight each.  8192 tokens of 32 + 2 x 8 heads of 128 channels, 201 MB, take 33 us (6.1 TB/s; a
-// CTA for each token, with its cos and sin in shared memory and unpacked pieces, 70 us), 1337 tokens of 40 + 2 x 8 heads 7.7 us (10.3 us).
+// CTA for each token, with its cos and sin in shared memory and unpacked pieces, 70 us), 1337 tokens of 40 + 2 x 8 heads 7.7 us with
+// one set of inputs, which L2 holds (10.3 us), 8.7 over three.
 #include "common.cuh"
 #include "kernels.hpp"
 #include "cache_ops.hpp"
