@@ -44,13 +44,14 @@ inline cudaMemPool_t scratch_pool() {
     }
     return pool;
 }
+// p is null where there is no memory.  The call says so by its code: the runtime's error does not stay behind for whoever asks next, which may be another library's check of its own launch.
 struct DevBuf {
     void* p = nullptr;
     cudaStream_t s;
     DevBuf(size_t n, cudaStream_t stream) : s(stream) {
         if (n == 0) return;
         cudaMemPool_t pool = scratch_pool();
-        if (!pool || cudaMallocFromPoolAsync(&p, n, pool, s) != cudaSuccess) p = nullptr;
+        if (!pool || cudaMallocFromPoolAsync(&p, n, pool, s) != cudaSuccess) { p = nullptr; cudaGetLastError(); }
     }
     DevBuf(const DevBuf&) = delete;
     ~DevBuf() { if (p) cudaFreeAsync(p, s); }

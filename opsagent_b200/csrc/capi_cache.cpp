@@ -18,7 +18,11 @@ static_assert(sizeof(oa_page_move) == sizeof(PageMove) && TABLE_PAGE == CACHE_PA
 
 namespace {
 int bad(const char* why) { return call_failed(OA_ERR_BAD_REQUEST, why); }
-int device_rc(cudaError_t e) { return e == cudaSuccess ? OA_OK : call_failed(OA_ERR_INTERNAL, cudaGetErrorString(e)); }
+int device_rc(cudaError_t e) {
+    if (e == cudaSuccess) return OA_OK;
+    cudaGetLastError();                          // told by the code: it does not stay behind for whoever asks next
+    return call_failed(OA_ERR_INTERNAL, cudaGetErrorString(e));
+}
 int page_rc(const PageResult& r) { return r.rc == OA_OK ? OA_OK : call_failed(r.rc, r.why); }
 #define OA_ON_DEVICE_OF(...)                                                                                 \
     CallDevice on_device({__VA_ARGS__});                                                                     \

@@ -384,6 +384,23 @@ def test_prompts_on_a_cache_that_was_cleared_once(L, heads, n_kv, dim):
         assert L.oa_host_cache_free(table, everyone.ctypes.data, n) == 0 and (have == 0).all() and (tables == -1).all() and refs.sum() == 20
 
 
+# ---- errors ---------------------------------------------------------------------------------------------
+def test_a_call_that_found_no_memory_leaves_no_error_behind(L):
+    """Scratch of over a terabyte: the call says so with its code and text, nothing is launched, and the program's next CUDA call does not meet the error again."""
+    buf = torch.zeros(9 << 20, dtype=torch.bfloat16, device="cuda")                     # a cache of one page, and the first of q's rows behind it
+    ints, before = torch.zeros(64, dtype=torch.int32, device="cuda"), L.oa_kernel_launches()
+    n, heads, n_kv, dim = 2 ** 18, 16384, 1024, 64
+    q = C.c_void_p(buf.data_ptr() + 2 * n_kv * PAGE * dim * 2)                          # in place; nothing is launched that could go beyond it
+    for again in range(2):
+        code = L.oa_k_prefix_attention(q, heads * dim, q, heads * dim, ptr(buf), 1, ptr(ints), 10 ** 4, ptr(ints), ptr(ints), 1, ptr(ints), 8, ptr(ints), n, heads, n_kv, dim, 0.0, None, now())
+        assert code == 500 and "scratch" in _lib.last_error(), (code, _lib.last_error())
+        assert L.oa_kernel_launches() == before
+        assert torch.ones(8, device="cuda").mul_(2).sum().item() == 16.0
+    b = Batch(8, 2, 128, [100], [0, 1], [7], seed=3)
+    run(L, b)
+    b.check()
+
+
 # ---- threads ----------------------------------------------------------------------------------------------
 def test_two_threads_on_two_streams(L):
     """Each thread has a cache, tables, a stream and errors of its own; every result is the one that the calls give alone."""
