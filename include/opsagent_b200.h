@@ -162,9 +162,10 @@ OA_API int oa_k_paged_attention(const void* q, void* out, const void* kv_cache, 
                          int32_t max_pages_per_seq, const int32_t* ctx_lens, const int32_t* q_lens, int32_t n_seqs,
                          int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t force_splits, void* stream);
 /* ---- operators on a caller's paged cache: [planes][num_pages][n_kv][64][head_dim], planes = K and V of each layer (a layer's two planes are the kv_cache
- * of oa_k_paged_attention: clear it once if that entry is to read it; the operators here ignore what lies behind an end, and copy it with whole pages).  All of them only enqueue on `stream` of the device that holds the cache, whichever device is current, never synchronise and can be
- * captured, a process's first call too; a captured call keeps the host arrays' values.  Rows of one or more heads are `pitch` elements apart, of which a single row has none; rows of two
- * pitches in one stretch of memory count as overlapping, and 2^39 elements from the first row to the last are refused.  400 with a text in oa_last_error() where an argument cannot be served; nothing has been enqueued then.
+ * of oa_k_paged_attention: clear it once if that entry is to read it; the operators here ignore what lies behind an end, and copy it with whole pages).
+ * All of them only enqueue on `stream` of the device that holds the cache, whichever device is current, never synchronise and can be captured, a process's first
+ * call too; a captured call keeps the host arrays' values.  Pitches (ldx and the like) are elements from row to row, no fewer than a row has; rows of two different
+ * pitches in one stretch of memory count as overlapping, and rows that reach over 2^39 elements are refused.  400 with a text in oa_last_error() where an argument cannot be served; nothing has been enqueued then.
  * `status` (device int32, or NULL): set to 400 where a device array asks for what there is not; never cleared. ---- */
 /* frequencies of rotary positions: base^(-2i / rot_dims), i < rot_dims / 2, in 64 bits.  scaling 0: as they are; 1: / factor; 2 (llama3): / factor below `first`
  * turns in `original` positions, as they are above `second` turns, blended in between; 3 (YaRN): blended along a ramp over i between where `first` (fast) and
