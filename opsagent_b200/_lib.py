@@ -45,6 +45,7 @@ SYMBOLS = [
     "oa_kernel_launches", "oa_version", "oa_host_apply_chat_template", "oa_host_decode_plan", "oa_host_decode_attention_plan", "oa_host_streamk_plan", "oa_host_bpe_encode", "oa_host_bpe_decode", "oa_host_model_info",
     "oa_k_gemm_streamk", "oa_k_hybrid_gemm", "oa_k_gemm_ext", "oa_host_gemm_kernel", "oa_host_gemm_pair_width", "oa_host_gemm_pair_swapped", "oa_host_prefill_attention_kernel", "oa_debug_kernel_times", "oa_engine_serve", "oa_host_grammar_step", "oa_host_grammar_step_ex", "oa_host_grammar_token_mask", "oa_http_start", "oa_http_port", "oa_http_stats", "oa_http_stop", "oa_http_last_error", "oa_host_json_roundtrip", "oa_chat_cancel", "oa_chat_submit_ex", "oa_chat_wait_ex", "oa_trace_step",
     "oa_host_rotary_freqs", "oa_k_rotary", "oa_k_rotary_cache", "oa_host_cache_grow", "oa_host_cache_free", "oa_host_cache_fork", "oa_host_cache_compact", "oa_k_cache_copy", "oa_k_prefix_attention",
+    "oa_k_cache8_write", "oa_k_cache8_read", "oa_k_cache8_copy", "oa_k_tree_attention",
 ]
 
 _lib = None
@@ -100,6 +101,10 @@ def load() -> C.CDLL:
     L.oa_host_cache_compact.argtypes = [table, moves, i32, C.POINTER(i32)]; L.oa_host_cache_compact.restype = C.c_int
     L.oa_k_cache_copy.argtypes = [vp, i32, i32, i32, i32, i32, moves, i32, vp]; L.oa_k_cache_copy.restype = C.c_int
     L.oa_k_prefix_attention.argtypes = [vp, i64, vp, i64, vp, i32, vp, i32, vp, vp, i32, vp, i32, vp, i32, i32, i32, i32, f32, vp, vp]; L.oa_k_prefix_attention.restype = C.c_int
+    L.oa_k_cache8_write.argtypes = [vp, vp, i64, vp, i32, vp, i32, i32, i32, i32, vp, vp]; L.oa_k_cache8_write.restype = C.c_int
+    L.oa_k_cache8_read.argtypes = [vp, i32, vp, i32, i32, i32, i32, vp, vp, i64, vp, vp]; L.oa_k_cache8_read.restype = C.c_int
+    L.oa_k_cache8_copy.argtypes = [vp, i32, i32, i32, i32, moves, i32, vp]; L.oa_k_cache8_copy.restype = C.c_int
+    L.oa_k_tree_attention.argtypes = [vp, i64, vp, i64, vp, i32, i32, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, vp, vp]; L.oa_k_tree_attention.restype = C.c_int
     L.oa_host_apply_chat_template.argtypes = [C.c_char_p, C.POINTER(OaMsg), i32, vp, i32, C.POINTER(i32)]; L.oa_host_apply_chat_template.restype = C.c_int
     L.oa_host_bpe_encode.argtypes = [C.c_char_p, C.c_char_p, i32, vp, i32, C.POINTER(i32)]; L.oa_host_bpe_encode.restype = C.c_int
     L.oa_host_bpe_decode.argtypes = [C.c_char_p, vp, i32, vp, i32, C.POINTER(i32)]; L.oa_host_bpe_decode.restype = C.c_int

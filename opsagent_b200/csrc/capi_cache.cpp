@@ -1,5 +1,5 @@
 // capi_cache.cpp — C entry points of the operators on a caller's paged cache: rotary positions, page bookkeeping and copies, decode attention over shared
-// prefixes.  Every argument that the host can judge is judged before anything is enqueued; what lies on the device the kernels check against the bounds they are given.
+// prefixes, caches of 8 bits, attention of several new tokens of a sequence.  Every argument that the host can judge is judged before anything is enqueued; what lies on the device the kernels check against the bounds they are given.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -58,6 +58,39 @@ bool apart_or_same(const void* x, int64_t ldx, const void* out, int64_t ldo, int
 bool outside_cache(const void* cache, int64_t num_pages, int64_t n_kv, int64_t head_dim, const void* x, int64_t ldx, int64_t cols, int64_t T) {
     const uintptr_t c = (uintptr_t)cache, p = (uintptr_t)x;
     return p + ((T - 1) * ldx + cols) * 2 <= c || c + 2 * num_pages * n_kv * CACHE_PAGE * head_dim * 2 <= p;
+}
+// a list of moves that one launch can carry out in any order (may throw)
+const char* moves_wrong(int32_t num_pages, const oa_page_move* moves, int32_t n_moves) {
+    if (n_moves < 0 || (n_moves > 0 && !moves)) return "cache copy: no moves";
+    std::vector<unsigned char> role((size_t)num_pages, 0);              // 1: a source, 2: a target
+    for (int i = 0; i < n_moves; ++i) {
+        const oa_page_move& m = moves[i];
+        if (m.src < 0 || m.src >= num_pages || m.dst < 0 || m.dst >= num_pages || m.tokens < 0 || m.tokens > CACHE_PAGE) return "cache copy: a move is outside the cache or its pages";
+        if (role[m.dst]) return "cache copy: a page is the target of two moves, or a target and a source";
+        role[m.dst] = 2;
+        if (role[m.src] == 2) return "cache copy: a page is the target of two moves, or a target and a source";
+        role[m.src] = 1;
+    }
+    return nullptr;
+}
+// what the entries on a cache of 8 bits share
+const char* cache8_wrong(int32_t num_pages, int32_t n_kv, int32_t head_dim) {
+    if (head_dim < 16 || head_dim % 16 || head_dim > 256) return "8-bit cache: head_dim is a multiple of 16, up to 256";
+    if (n_kv < 1 || n_kv > 4096 || num_pages < 1) return "8-bit cache: a page or more, of 1 to 4096 heads";
+    return nullptr;
+}
+const char* rows8_wrong(const void* k, const void* v, int64_t ldkv, const void* cache, int32_t num_pages, const int32_t* slots, int32_t T, int32_t n_kv, int32_t head_dim, int32_t format, const int32_t* status) {
+    if (const char* wrong = cache8_wrong(num_pages, n_kv, head_dim)) return wrong;
+    if (format != CACHE_E4M3 && format != CACHE_INT8) return "8-bit cache: format is 1 (e4m3) or 2 (int8)";
+    const int64_t cols = (int64_t)n_kv * head_dim;
+    if (T < 0 || ldkv < cols) return "8-bit cache: bad number of rows, or a row is longer than its pitch";
+    if (T == 0) return nullptr;
+    if (!k || !v || !cache || !slots) return "8-bit cache: null pointer";
+    if (((uintptr_t)k | (uintptr_t)v) % 2 || (uintptr_t)cache % 16 || ((uintptr_t)slots | (uintptr_t)status) % 4) return "8-bit cache: a pointer is not aligned (the cache to 16 bytes)";
+    if (beyond_memory(T, ldkv)) return "8-bit cache: rows further apart than memory reaches";
+    const uintptr_t c = (uintptr_t)cache, bytes = 2ull * num_pages * n_kv * CACHE_PAGE * (head_dim + 4);
+    for (const uintptr_t p : {(uintptr_t)k, (uintptr_t)v}) if (p < c + bytes && c < p + ((T - 1) * ldkv + cols) * 2) return "8-bit cache: rows overlap the cache";
+    return nullptr;
 }
 void rotary_turns(RotaryArgs& a, const double* freqs, int32_t rot_dims, float amplitude, bool transpose) {
     a.pairs = rot_dims / 2; a.amplitude = amplitude;
@@ -149,17 +182,8 @@ int oa_k_cache_copy(void* kv_cache, int32_t planes, int32_t num_pages, int32_t n
     if (planes < 1 || num_pages < 1 || n_kv < 1 || head_dim < 1 || (elem_bytes != 2 && elem_bytes != 4)) return bad("cache copy: bad cache");
     const int64_t row = (int64_t)head_dim * elem_bytes;
     if (row % 16 || row > 4096 || n_kv > 4096) return bad("cache copy: a row is a multiple of 16 bytes, up to 4096, with up to 4096 heads");
-    if (n_moves < 0 || (n_moves > 0 && !moves)) return bad("cache copy: no moves");
     try {
-        std::vector<unsigned char> role((size_t)num_pages, 0);          // 1: a source, 2: a target
-        for (int i = 0; i < n_moves; ++i) {
-            const oa_page_move& m = moves[i];
-            if (m.src < 0 || m.src >= num_pages || m.dst < 0 || m.dst >= num_pages || m.tokens < 0 || m.tokens > CACHE_PAGE) return bad("cache copy: a move is outside the cache or its pages");
-            if (role[m.dst]) return bad("cache copy: a page is the target of two moves, or a target and a source");
-            role[m.dst] = 2;
-            if (role[m.src] == 2) return bad("cache copy: a page is the target of two moves, or a target and a source");
-            role[m.src] = 1;
-        }
+        if (const char* wrong = moves_wrong(num_pages, moves, n_moves)) return bad(wrong);
         if (n_moves == 0) return OA_OK;
         if (!kv_cache || (uintptr_t)kv_cache % 16) return bad("cache copy: the cache starts on a 16-byte boundary");
         OA_ON_DEVICE_OF(kv_cache);
@@ -210,6 +234,83 @@ int oa_k_prefix_attention(const void* q, int64_t ldq, void* out, int64_t ldo, co
     a.pre_o = (float*)(base + plan.pre_o); a.pre_ml = (float*)(base + plan.pre_ml); a.own_o = (float*)(base + plan.own_o); a.own_ml = (float*)(base + plan.own_ml);
     a.more_o = (float*)(base + plan.more_o); a.more_ml = (float*)(base + plan.more_ml); a.own_parts = (int2*)(base + plan.own_parts); a.pre_ctas = plan.pre_ctas; a.own_ctas = plan.own_ctas; a.key_tile = plan.key_tile; a.sms = sms;
     return device_rc(launch_prefix_attention(&tm_q, &tm_page, head_dim, plan.long_prefix, a, (cudaStream_t)stream));
+}
+
+int oa_k_cache8_write(const void* k, const void* v, int64_t ldkv, void* kv_cache, int32_t num_pages, const int32_t* slots, int32_t T, int32_t n_kv, int32_t head_dim, int32_t format,
+                      int32_t* status, void* stream) {
+    if (const char* wrong = rows8_wrong(k, v, ldkv, kv_cache, num_pages, slots, T, n_kv, head_dim, format, status)) return bad(wrong);
+    if (T == 0) return OA_OK;
+    OA_ON_DEVICE_OF(k, v, kv_cache, slots, status);
+    Rows8Args a{};
+    a.k = k; a.v = v; a.ldkv = ldkv; a.cache = kv_cache; a.slots = slots; a.T = T; a.n_kv = n_kv; a.head_dim = head_dim; a.num_pages = num_pages; a.status = status;
+    return device_rc(launch_cache8_write(a, format == CACHE_E4M3, (cudaStream_t)stream));
+}
+
+int oa_k_cache8_read(const void* kv_cache, int32_t num_pages, const int32_t* slots, int32_t T, int32_t n_kv, int32_t head_dim, int32_t format, void* k_out, void* v_out, int64_t ldkv,
+                     int32_t* status, void* stream) {
+    if (const char* wrong = rows8_wrong(k_out, v_out, ldkv, kv_cache, num_pages, slots, T, n_kv, head_dim, format, status)) return bad(wrong);
+    if (T == 0) return OA_OK;
+    const int64_t cols = (int64_t)n_kv * head_dim;
+    if (!apart(k_out, ldkv, cols, v_out, ldkv, cols, T, 2)) return bad("8-bit cache: rows of keys and of values overlap");
+    OA_ON_DEVICE_OF(kv_cache, slots, k_out, v_out, status);
+    Rows8Args a{};
+    a.k_out = k_out; a.v_out = v_out; a.ldkv = ldkv; a.cache = const_cast<void*>(kv_cache); a.slots = slots; a.T = T; a.n_kv = n_kv; a.head_dim = head_dim; a.num_pages = num_pages; a.status = status;
+    return device_rc(launch_cache8_read(a, format == CACHE_E4M3, (cudaStream_t)stream));
+}
+
+int oa_k_cache8_copy(void* kv_cache, int32_t planes, int32_t num_pages, int32_t n_kv, int32_t head_dim, const oa_page_move* moves, int32_t n_moves, void* stream) {
+    if (const char* wrong = cache8_wrong(num_pages, n_kv, head_dim)) return bad(wrong);
+    if (planes < 1) return bad("8-bit cache: no planes");
+    try {
+        if (const char* wrong = moves_wrong(num_pages, moves, n_moves)) return bad(wrong);
+        if (n_moves == 0) return OA_OK;
+        if (!kv_cache || (uintptr_t)kv_cache % 16) return bad("8-bit cache: the cache starts on a 16-byte boundary");
+        OA_ON_DEVICE_OF(kv_cache);
+        return device_rc(launch_cache8_copy(kv_cache, planes, num_pages, n_kv, head_dim, reinterpret_cast<const PageMove*>(moves), n_moves, (cudaStream_t)stream));
+    } catch (const std::exception&) { return OA_ERR_INTERNAL; }
+}
+
+int oa_k_tree_attention(const void* q, int64_t ldq, void* out, int64_t ldo, const void* kv_cache, int32_t format, int32_t num_pages, const int32_t* block_tables, int32_t max_pages_per_seq,
+                        const int32_t* ctx_lens, const int32_t* row_starts, const uint64_t* seen, int32_t n_seqs, int32_t n_rows, int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t window,
+                        int32_t sinks, float scale, int32_t* status, void* stream) {
+    if (head_dim != 64 && head_dim != 128) return bad("tree attention: heads of 64 or 128");
+    if (format < CACHE_BF16 || format > CACHE_INT8) return bad("tree attention: format is 0 (bf16), 1 (e4m3) or 2 (int8)");
+    if (n_kv < 1 || n_kv > 1024 || n_heads < 1 || n_heads % n_kv || n_heads / n_kv > TREE_MAX_GROUP) return bad("tree attention: up to 16 query heads of a key/value head");
+    if (n_seqs < 0 || n_seqs > (1 << 20) || n_rows < 0 || n_rows > (1 << 24) || max_pages_per_seq < 1 || max_pages_per_seq > (1 << 24)) return bad("tree attention: bad number of sequences, rows or pages");
+    if (window != 0 && window < TREE_MAX_TOKENS) return bad("tree attention: a window is 0 (none) or at least 64");
+    if (sinks < 0 || (sinks > 0 && window == 0)) return bad("tree attention: first tokens that stay visible need a window");
+    const int64_t row_bytes = format == CACHE_BF16 ? 2 * head_dim : head_dim + 4, tm_rows = 2ll * num_pages * n_kv * CACHE_PAGE * row_bytes / (format == CACHE_BF16 ? 2 * head_dim : 128);
+    if (num_pages < 1 || tm_rows > INT32_MAX) return bad("tree attention: the cache's rows are counted in 31 bits");
+    const float scale_log2e = (scale > 0 ? scale : 1.0f / std::sqrt((float)head_dim)) * 1.4426950408889634f;
+    if (!std::isfinite(scale_log2e) || !(scale >= 0)) return bad("tree attention: the scale is positive, and finite times log2(e), or 0 for 1 / sqrt(head_dim)");
+    const int64_t width = (int64_t)n_heads * head_dim;
+    if (ldq < width || ldo < width || ldq % 8 || ldo % 8) return bad("tree attention: pitches hold a row and are multiples of 16 bytes");
+    if (n_seqs == 0 || n_rows == 0) return OA_OK;
+    if (!q || !out || !kv_cache || !block_tables || !ctx_lens || !row_starts) return bad("tree attention: null pointer");
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)kv_cache) % 16 || ((uintptr_t)block_tables | (uintptr_t)ctx_lens | (uintptr_t)row_starts | (uintptr_t)status) % 4 || (uintptr_t)seen % 8)
+        return bad("tree attention: a pointer is not aligned");
+    if (beyond_memory(n_rows, ldq) || beyond_memory(n_rows, ldo)) return bad("tree attention: rows further apart than memory reaches");
+    if (!apart_or_same(q, ldq, out, ldo, n_rows, width, 2)) return bad("tree attention: out overlaps q without being q");
+    const uintptr_t c = (uintptr_t)kv_cache, o = (uintptr_t)out;
+    if (o < c + 2ull * num_pages * n_kv * CACHE_PAGE * row_bytes && c < o + ((n_rows - 1) * ldo + width) * 2) return bad("tree attention: out overlaps the cache");
+    OA_ON_DEVICE_OF(kv_cache, q, out, block_tables, ctx_lens, row_starts, seen, status);
+    CUtensorMap tm_page;
+    if ((format == CACHE_BF16 ? make_tmap_bf16_2d(&tm_page, kv_cache, (uint64_t)tm_rows, head_dim, head_dim, CACHE_PAGE, 64)
+                              : make_tmap_bytes_2d(&tm_page, kv_cache, (uint64_t)tm_rows, CACHE_PAGE * head_dim / 128)) != 0) return call_failed(OA_ERR_INTERNAL, "tree attention: no tensor map of the cache");
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return device_rc(e);
+    const TreeAttnPlan plan = tree_attn_plan(n_seqs, n_rows, n_heads, n_kv, head_dim, format, max_pages_per_seq, sms);
+    DevBuf scratch(plan.bytes, (cudaStream_t)stream);
+    if (!scratch.p) return call_failed(OA_ERR_INTERNAL, "tree attention: no scratch memory");
+    char* base = (char*)scratch.p;
+    TreeAttnArgs a{};
+    a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo; a.cache = kv_cache; a.tables = block_tables; a.ctx_lens = ctx_lens; a.row_starts = row_starts; a.seen = seen;
+    a.max_pages = max_pages_per_seq; a.n_seqs = n_seqs; a.n_rows = n_rows; a.n_heads = n_heads; a.n_kv = n_kv; a.num_pages = num_pages; a.window = window; a.sinks = sinks;
+    a.scale_log2e = scale_log2e; a.status = status;
+    a.part_o = (float*)(base + plan.part_o); a.part_ml = (float*)(base + plan.part_ml); a.joins = (TreeJoin*)(base + plan.joins); a.ctas = plan.ctas; a.rows = plan.rows;
+    return device_rc(launch_tree_attention(&tm_page, head_dim, format, a, (cudaStream_t)stream));
 }
 
 }  // extern "C"

@@ -13,6 +13,8 @@ namespace oa {
 // 128-byte swizzle.  Returns 0 on success (driver entry point resolved through the runtime, no -lcuda).
 int make_tmap_bf16_2d(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch_elems,
                       uint32_t box_rows, uint32_t box_cols);
+// bytes as rows of 128, one after the other; box = box_rows (<= 256) of them, 128-byte swizzle
+int make_tmap_bytes_2d(CUtensorMap* out, const void* base, uint64_t rows, uint32_t box_rows);
 // rows of heads: bf16 [tokens][heads][head_dim], `pitch_elems` from token to token; box = {64 channels, box_heads, box_tokens}, which lies in shared memory as
 // box_tokens * box_heads rows of 128 bytes under the 128-byte swizzle
 int make_tmap_bf16_heads(CUtensorMap* out, const void* base, uint64_t tokens, uint64_t heads, uint64_t head_dim, uint64_t pitch_elems, uint32_t box_tokens, uint32_t box_heads);

@@ -40,6 +40,20 @@ int make_tmap_bf16_2d(CUtensorMap* out, const void* base, uint64_t rows, uint64_
     return r == CUDA_SUCCESS ? 0 : (int)r;
 }
 
+int make_tmap_bytes_2d(CUtensorMap* out, const void* base, uint64_t rows, uint32_t box_rows) {
+    EncodeTiledFn enc = resolve_encode();
+    if (!enc) return -1;
+    if (box_rows > 256 || (reinterpret_cast<uintptr_t>(base) & 15)) return -2;
+    cuuint64_t gdim[2] = {128, rows};
+    cuuint64_t gstride[1] = {128};
+    cuuint32_t box[2] = {128, box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), gdim, gstride, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : (int)r;
+}
+
 int make_tmap_bf16_heads(CUtensorMap* out, const void* base, uint64_t tokens, uint64_t heads, uint64_t head_dim, uint64_t pitch_elems, uint32_t box_tokens, uint32_t box_heads) {
     EncodeTiledFn enc = resolve_encode();
     if (!enc) return -1;
