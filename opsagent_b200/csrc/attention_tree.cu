@@ -88,6 +88,65 @@ OA_DEVINL uint64_t tree_seen(const TreeAttnArgs& a, const TreeSeq& s, int t) {
 }
 OA_DEVINL int tree_low(const TreeAttnArgs& a, const TreeSeq& s, uint64_t seen, int t) { return a.window > 0 ? s.ctx + __popcll(seen & ((1ull << t) - 1)) - a.window + 1 : 0; }
 
+// A place in the list of (sequence, key/value head, row tile) items.  An item's units are OVER for itself and one for each PAGES of its sequence's pages
+template <int PAGES, int OVER>
+struct TreeAt {
+    int seq, kvh, tile, tile_tokens; int64_t unit0; TreeSeq s;                   // unit0: the item's first unit
+    OA_DEVINL int steps() const { return (s.pages + PAGES - 1) / PAGES; }
+    OA_DEVINL int64_t units() const { return OVER + steps(); }
+    OA_DEVINL int64_t all_units(const TreeAttnArgs& a) const { return (int64_t)s.tiles(tile_tokens) * a.n_kv * units(); }      // of the sequence
+    OA_DEVINL void next(const TreeAttnArgs& a) {
+        unit0 += units();
+        if (++tile < s.tiles(tile_tokens)) return;
+        tile = 0;
+        if (++kvh < a.n_kv) return;
+        kvh = 0;
+        do { if (++seq >= a.n_seqs) { s.n = s.pages = 0; return; } s.read(a, seq); } while (s.n == 0);
+    }
+    OA_DEVINL int rows(int grp) const { return min(tile_tokens, s.n - tile * tile_tokens) * grp; }
+    OA_DEVINL int row0() const { return s.row0 + tile * tile_tokens; }
+};
+struct TreeShare { int64_t busy, total, begin, end; };                           // a CTA's units
+// The plan, by a whole CTA: what its share is and the item that it begins in
+template <int THREADS, int PAGES, int OVER>
+OA_DEVINL TreeShare tree_share(const TreeAttnArgs& a, int tile_tokens, int64_t* sums, TreeAt<PAGES, OVER>& start) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = (a.n_seqs + THREADS - 1) / THREADS, s0 = min(a.n_seqs, (int)threadIdx.x * per), s1 = min(a.n_seqs, s0 + per);
+    TreeAt<PAGES, OVER> at;
+    at.tile_tokens = tile_tokens;
+    int64_t units = 0; bool wrong = false;
+    for (at.seq = s0; at.seq < s1; ++at.seq) { at.s.read(a, at.seq); wrong = wrong || at.s.wrong; units += at.all_units(a); }
+    if (wrong && a.status) *a.status = 400;
+    int64_t before = units;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int64_t x = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += x; }
+    if (lane == 31) sums[warp] = before;
+    __syncthreads();
+    before -= units;
+    TreeShare share; share.total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) { if (w < warp) before += sums[w]; share.total += sums[w]; }
+    share.busy = busy_ctas(gridDim.x, share.total);
+    share.begin = first_unit(blockIdx.x, share.busy, share.total); share.end = first_unit(blockIdx.x + 1, share.busy, share.total);
+    if (share.begin < share.end && share.begin >= before && share.begin < before + units) {          // one thread
+        at.seq = s0; at.unit0 = before;
+        for (at.s.read(a, s0); share.begin >= at.unit0 + at.all_units(a);) { at.unit0 += at.all_units(a); ++at.seq; at.s.read(a, at.seq); }
+        const int item = (int)quotient(share.begin - at.unit0, at.units()), tiles = at.s.tiles(tile_tokens);
+        at.unit0 += (int64_t)item * at.units();
+        at.kvh = item / tiles; at.tile = item - at.kvh * tiles;
+        start = at;
+    }
+    if (threadIdx.x == 0) a.joins[blockIdx.x].parts = 0;
+    __syncthreads();
+    return share;
+}
+// whether a row sees anything at all
+OA_DEVINL bool tree_sees(const TreeAttnArgs& a, const TreeSeq& s, uint64_t seen, int low) {
+    const uint64_t there = s.end - s.ctx < 64 ? (1ull << (s.end - s.ctx)) - 1 : ~0ull;
+    return (seen & there) != 0 || (s.ctx > 0 && (a.window == 0 || a.sinks > 0 || low < s.ctx));
+}
+// what a part leaves in scratch: [slot][D / 4][rows][4], and m and l of each row.  Slot 2 c: of the item that CTA c begins, 2 c + 1: of one that an earlier one began.  l of -1 in the former: the row sees nothing
+OA_DEVINL void tree_record(const TreeAttnArgs& a, int later, int row0, int rows, int kvh) { TreeJoin j; j.parts = later; j.row0 = row0; j.rows = rows; j.kvh = kvh; a.joins[blockIdx.x] = j; }
+
 // =============================================================================================
 // up to 16 rows of an item: the warp path
 // =============================================================================================
@@ -103,7 +162,6 @@ struct FewCfg {
     static constexpr int CTAS = FMT != CACHE_BF16 && NB == 1 ? 2 : 1;            // of an SM
 };
 struct TreeMeta { uint64_t seen; int low; float factor; };
-struct FewAt { int seq, kvh, tile; int64_t unit0; TreeSeq s; };                  // an item and its first unit
 
 template <int D>
 OA_DEVINL uint32_t few_off(int r, int d) { return (uint32_t)((d >> 6) * (CACHE_PAGE * 128) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4)); }      // bf16: halves of 64 channels
@@ -127,8 +185,9 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
     float* vref_s = ml_s + 4 * ROWS * 2;                                                     // [4 quarters]: what values' scales are taken over
     uint64_t* full_bar = reinterpret_cast<uint64_t*>(vref_s + 4);
     uint64_t *empty_bar = full_bar + STAGES, *q_full = empty_bar + STAGES, *q_empty = q_full + 2, *states_full = q_empty + 2, *states_empty = states_full + 1;
+    using At = TreeAt<1, 1>;
     __shared__ int64_t sums[TREE_THREADS / 32];
-    __shared__ FewAt start;
+    __shared__ At start;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int grp = a.n_heads / a.n_kv, tile_tokens = ROWS / grp;
@@ -140,44 +199,11 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
         fence_barrier_init();
     }
     griddep_wait();
-    // ---- the plan ----
-    const int per = (a.n_seqs + TREE_THREADS - 1) / TREE_THREADS, s0 = min(a.n_seqs, (int)threadIdx.x * per), s1 = min(a.n_seqs, s0 + per);
-    FewAt at;
-    auto units_of = [&](const TreeSeq& s) { return (int64_t)s.tiles(tile_tokens) * a.n_kv * (1 + s.pages); };
-    int64_t units = 0; bool wrong = false;
-    for (at.seq = s0; at.seq < s1; ++at.seq) { at.s.read(a, at.seq); wrong = wrong || at.s.wrong; units += units_of(at.s); }
-    if (wrong && a.status) *a.status = 400;
-    int64_t before = units;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int64_t x = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += x; }
-    if (lane == 31) sums[warp] = before;
-    __syncthreads();
-    before -= units;
-    int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < TREE_THREADS / 32; ++w) { if (w < warp) before += sums[w]; total += sums[w]; }
-    const int64_t busy = busy_ctas(gridDim.x, total), u_begin = first_unit(blockIdx.x, busy, total), u_end = first_unit(blockIdx.x + 1, busy, total);
-    if (u_begin < u_end && u_begin >= before && u_begin < before + units) {                  // one thread
-        at.seq = s0; at.unit0 = before;
-        for (at.s.read(a, s0); u_begin >= at.unit0 + units_of(at.s);) { at.unit0 += units_of(at.s); ++at.seq; at.s.read(a, at.seq); }
-        const int item = (int)quotient(u_begin - at.unit0, 1 + at.s.pages), tiles = at.s.tiles(tile_tokens);
-        at.unit0 += (int64_t)item * (1 + at.s.pages);
-        at.kvh = item / tiles; at.tile = item - at.kvh * tiles;
-        start = at;
-    }
-    if (threadIdx.x == 0) a.joins[blockIdx.x].parts = 0;
-    __syncthreads();
+    const TreeShare share = tree_share<TREE_THREADS>(a, tile_tokens, sums, start);
+    const int64_t u_begin = share.begin, u_end = share.end;
     if (u_begin >= u_end) { griddep_launch(); return; }
-    at = start;
-    auto next = [&] {
-        at.unit0 += 1 + at.s.pages;
-        if (++at.tile < at.s.tiles(tile_tokens)) return;
-        at.tile = 0;
-        if (++at.kvh < a.n_kv) return;
-        at.kvh = 0;
-        do { if (++at.seq >= a.n_seqs) { at.s.n = at.s.pages = 0; return; } at.s.read(a, at.seq); } while (at.s.n == 0);
-    };
-    auto tile_rows = [&] { return min(tile_tokens, at.s.n - at.tile * tile_tokens) * grp; };
+    At at = start;
+    auto next = [&] { at.next(a); };
 
     if (warp == 8) {
         int st = 0; uint32_t ph = 0;
@@ -221,7 +247,7 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
             mbar_wait(&q_empty[k & 1], ((k >> 1) & 1) ^ 1);
             uint8_t* q_dst = q_s + (k & 1) * Cfg::Q_BYTES;
             TreeMeta* meta = meta_s + (k & 1) * ROWS;
-            const int live = tile_rows(), t0 = at.tile * tile_tokens;
+            const int live = at.rows(grp), t0 = at.tile * tile_tokens;
             constexpr int W = D / 64;                                                        // words of two channels a lane
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -278,18 +304,13 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
             const int64_t end = at.unit0 + 1 + at.s.pages;
             const bool first = at.unit0 >= u_begin, last = end <= u_end;
             u = min(end, u_end);
-            const int live = tile_rows(), row0 = at.s.row0 + at.tile * tile_tokens;
+            const int live = at.rows(grp), row0 = at.row0();
             mbar_wait(&q_full[k & 1], (k >> 1) & 1);
-            uint32_t blind = 0;                                                              // rows that see nothing
-            {
-                const TreeMeta m = meta_s[(k & 1) * ROWS + (lane < ROWS ? lane : 0)];
-                const uint64_t there = at.s.end - at.s.ctx < 64 ? (1ull << (at.s.end - at.s.ctx)) - 1 : ~0ull;
-                const bool sees = (m.seen & there) != 0 || (at.s.ctx > 0 && (a.window == 0 || a.sinks > 0 || m.low < at.s.ctx));
-                blind = __ballot_sync(0xffffffffu, lane < live && !sees);
-            }
+            const TreeMeta own = meta_s[(k & 1) * ROWS + (lane < ROWS ? lane : 0)];
+            const uint32_t blind = __ballot_sync(0xffffffffu, lane < live && !tree_sees(a, at.s, own.seen, own.low));      // rows that see nothing
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_empty[k & 1]);
-            if (lane == 0 && first && !last) { TreeJoin j; j.parts = cta_of(end - 1, busy, total) - (int)blockIdx.x; j.row0 = row0; j.rows = live; j.kvh = at.kvh; j.blind = blind; a.joins[blockIdx.x] = j; }
+            if (lane == 0 && first && !last) tree_record(a, cta_of(end - 1, share.busy, share.total) - (int)blockIdx.x, row0, live, at.kvh);
             float* po = a.part_o + ((int64_t)blockIdx.x * 2 + !first) * (ROWS * D);
             float2* ml = reinterpret_cast<float2*>(a.part_ml) + ((int64_t)blockIdx.x * 2 + !first) * ROWS;
             mbar_wait(states_full, k & 1);
@@ -314,14 +335,14 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
                         inv = blind >> row & 1 ? 0.f : 1.0f / l;
                         const int token = row / grp;
                         out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(row0 + token) * a.ldo + (int64_t)(at.kvh * grp + row - token * grp) * D;
-                    } else if (g == 0) ml[row] = make_float2(m, l);
+                    } else if (g == 0) ml[row] = make_float2(m, first && (blind >> row & 1) ? -1.0f : l);
 #pragma unroll 4
                     for (int r = 0; r < KS * 2; ++r) {                                       // channel block r / 2 and the one or the other of a lane's two channels there
                         const int i = r >> 1, up = r & 1, reg = (i / KH) * (Cfg::REGS / 2) + (b * KH + i % KH) * 4 + 2 * up + h, d = i * 16 + (BITS8 ? 2 * g + up : 8 * up + g);
                         float o = 0.f;
 #pragma unroll
                         for (int w = 0; w < 4; ++w) o += f[w] * states[(w * Cfg::REGS + reg) * 32 + lane];
-                        if (out) out[d] = f32_to_bf16_bits(o * inv); else po[row * D + d] = o;
+                        if (out) out[d] = f32_to_bf16_bits(o * inv); else po[(d >> 2) * (ROWS * 4) + row * 4 + (d & 3)] = o;
                     }
                 }
             __syncwarp();
@@ -523,57 +544,628 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
 }
 
 // =============================================================================================
+// more rows: tcgen05
+// =============================================================================================
+// 128 rows of an item (as many tokens' heads of a group as fit) x 128 keys a tile: S = Q K^T in three TMEM buffers, two tiles ahead, P over S's own columns as the second product's operand, O in
+// TMEM.  Two softmax warpgroups take the tiles in turn, one row a thread; the reference maximum rises (and O is rescaled) only where a score passes it by 2^8.  Over 8 bits four warps turn tiles (and
+// an item's queries) into fp16 under the swizzle that the products read, and one brings the scales of a tile's values under one power of two.
+template <int D, int FMT>
+struct ManyCfg {
+    static constexpr bool BITS8 = FMT != CACHE_BF16;
+    static constexpr int KEYS = 128, HALVES = D / 64, HALF = 128 * 128;          // 128 rows x 64 channels of 2 bytes under the 128-byte swizzle: of Q, of a tile
+    static constexpr int TILE_BYTES = HALVES * HALF, SLOTS = BITS8 ? (D == 128 ? 3 : 4) : D == 128 ? 5 : 8;
+    static constexpr int RAW_BYTES = KEYS * D, RAW = BITS8 ? (D == 128 ? 5 : 8) : 0;         // a tile of 8 bits, and how many wait
+    static constexpr int SC = 8, SC_FLOATS = 2 * KEYS + 4;                       // tiles whose scales wait: keys', values', their power of two, what O is multiplied by for it
+    static constexpr int THREADS = 128 + 256 + (BITS8 ? 128 : 0);                // producer, issuer, scales; eight softmax warps; four that convert
+    static constexpr int BARS = 12 + 2 * SLOTS + 2 * RAW + (BITS8 ? 3 * SC : 0);
+    static constexpr int SMEM_BYTES = TILE_BYTES + SLOTS * TILE_BYTES + RAW * RAW_BYTES + (BITS8 ? SC * SC_FLOATS * 4 + 2 * 128 * 4 : 0) + 3 * 128 * 4 + BARS * 8 + 16;
+    static constexpr uint32_t O_COL = 384;                                       // TMEM: S and P of the tiles in turn at 0, 128 and 256
+};
+struct TrueTag { static constexpr bool value = true; };
+struct FalseTag { static constexpr bool value = false; };
+constexpr int TREE_OVER = 2;                                                     // tiles that an item's beginning and end cost
+
+// what any row of an item sees: bits of new tokens, and the first cached place of the widest window.  By a whole warp
+struct TreeAny {
+    uint64_t seen; int low;
+    template <typename At>
+    OA_DEVINL void read(const TreeAttnArgs& a, const At& at, int lane) {
+        const int t0 = at.tile * at.tile_tokens, count = min(at.tile_tokens, at.s.n - t0);
+        uint64_t any = 0; int lo = 0x7fffffff;
+#pragma unroll
+        for (int i = 0; i < 64; i += 32)
+            if (lane + i < count) { const uint64_t x = tree_seen(a, at.s, t0 + lane + i); any |= x; lo = min(lo, tree_low(a, at.s, x, t0 + lane + i)); }
+        seen = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(any >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)any);
+        low = __reduce_min_sync(0xffffffffu, lo);
+    }
+    OA_DEVINL bool sees(const TreeAttnArgs& a, const TreeSeq& s, int key) const {
+        const int n = key - s.ctx;
+        return n < 0 ? key < a.sinks || key >= low : key < s.end && n < 64 && (seen >> (n & 63) & 1);
+    }
+};
+OA_DEVINL uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
+// which of the 64 places from `key` on a row sees
+OA_DEVINL uint64_t tree_word(const TreeAttnArgs& a, const TreeSeq& s, uint64_t seen, int low, int key) {
+    const uint64_t old = low_bits(s.ctx - key) & (low_bits(a.sinks - key) | ~low_bits(low - key));
+    const int d = s.ctx - key;
+    const uint64_t fresh = d >= 64 || d <= -64 ? 0ull : d >= 0 ? seen << d : seen >> -d;
+    return (old | fresh) & low_bits(s.end - key);
+}
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ TreeAttnArgs a) {
+    using Cfg = ManyCfg<D, FMT>;
+    using At = TreeAt<2, TREE_OVER>;
+    constexpr bool BITS8 = Cfg::BITS8;
+    constexpr int KEYS = Cfg::KEYS, HALVES = Cfg::HALVES, HALF = Cfg::HALF, TILE = Cfg::TILE_BYTES, SLOTS = Cfg::SLOTS, RAW = BITS8 ? Cfg::RAW : 1, SC = Cfg::SC, SOFTMAX = 256;
+    constexpr int64_t BLOCK_BYTES = CACHE_PAGE * (D + 4);
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* q_s = smem;
+    uint8_t* kv_s = q_s + TILE;
+    uint8_t* raw_s = kv_s + SLOTS * TILE;
+    float* sc_s = reinterpret_cast<float*>(raw_s + Cfg::RAW * Cfg::RAW_BYTES);
+    float* factor_s = sc_s + (BITS8 ? SC * Cfg::SC_FLOATS : 0);                  // [2 pieces][rows]
+    float* m_s = factor_s + (BITS8 ? 256 : 0);                                   // a row's reference maximum, and its two sums of a piece
+    float* l_s = m_s + 128;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(l_s + 256);
+    uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_full = bars + 5, *o_full = bars + 8, *full = bars + 12, *empty = full + SLOTS;
+    uint64_t *raw_full = empty + SLOTS, *raw_empty = raw_full + Cfg::RAW, *sc_in = raw_empty + Cfg::RAW, *sc_full = sc_in + SC, *sc_empty = sc_full + SC;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::BARS);
+    __shared__ int64_t sums[Cfg::THREADS / 32];
+    __shared__ At start;
+    __shared__ float sc_last;                                                    // 8 bits: what the values' scales of a piece's last tile are over
+
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int grp = a.n_heads / a.n_kv, tile_tokens = 128 / grp;
+    if (threadIdx.x == 0) {
+        if (!BITS8) { tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_kv); }
+        mbar_init(q_full, BITS8 ? 4 : 1); mbar_init(q_empty, 1);
+        for (int i = 0; i < 3; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
+        for (int i = 0; i < 4; ++i) mbar_init(&o_full[i], 1);
+        for (int i = 0; i < SLOTS; ++i) { mbar_init(&full[i], BITS8 ? 4 : 1); mbar_init(&empty[i], 1); }
+        if (BITS8) {
+            for (int i = 0; i < RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4); }
+            for (int i = 0; i < SC; ++i) { mbar_init(&sc_in[i], 1); mbar_init(&sc_full[i], 1); mbar_init(&sc_empty[i], 4); }
+        }
+        fence_barrier_init();
+    }
+    // Tensor memory is taken behind the wait: a kernel before this one that has not taken its own yet would otherwise wait for this one, and this one for it
+    griddep_wait();
+    if (warp == 1) tmem_alloc<512>(tmem_slot);
+    const TreeShare share = tree_share<Cfg::THREADS>(a, tile_tokens, sums, start);
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    const int64_t u_begin = share.begin, u_end = share.end;
+    At at;
+    if (u_begin < u_end) at = start;
+    // a CTA's piece of an item: key tiles c0 .. c1 - 1, none where its units are the item's own alone
+    int c0 = 0, c1 = 0;
+    auto take = [&](int64_t& u) {
+        c0 = (int)max(u - at.unit0 - TREE_OVER, (int64_t)0); c1 = (int)max((int64_t)c0, min((int64_t)at.steps(), u_end - at.unit0 - TREE_OVER));
+        u = min(at.unit0 + at.units(), u_end);
+    };
+    auto special = [&](int t) { return 2 * t + 1 >= at.s.pages || at.s.special(a, at.s.page(2 * t)) || at.s.special(a, at.s.page(2 * t + 1)); };
+
+    // Keys and values share one ring in the order of their products: K_0, K_1, K_2, V_0, K_3, V_1, ..: entry number of V_j is min(tiles, j + 3) + j
+    if constexpr (BITS8) {                                                       // 128 a thread at launch, 512 for four: 88 + 2 x 160 + 96
+        if (warp < 4) reg_dec<88>(); else if (warp < 12) reg_inc<160>(); else reg_dec<96>();
+    }
+    if (warp == 0) {
+        constexpr int RING = BITS8 ? RAW : SLOTS;
+        uint64_t *in = BITS8 ? raw_full : full, *out = BITS8 ? raw_empty : empty;
+        uint32_t n = 0, seg = 0, g = 0;                                          // entries, pieces and tiles loaded
+        for (int64_t u = u_begin; u < u_end; at.next(a)) {
+            take(u);
+            if (c1 == c0) continue;
+            if constexpr (!BITS8) {
+                mbar_wait(q_empty, (seg & 1) ^ 1);
+                if (elect_one()) {                                               // tokens behind the last row are zeros, other sequences' are not looked at
+                    mbar_expect_tx(q_full, HALVES * tile_tokens * grp * 128);
+#pragma unroll
+                    for (int h = 0; h < HALVES; ++h) tma_load_3d(q_s + h * HALF, &tm_q, q_full, h * 64, at.kvh * grp, at.row0(), kEvictNormal);
+                }
+                __syncwarp();
+            }
+            ++seg;
+            const int32_t* table = a.tables + (int64_t)at.seq * a.max_pages;
+            int page[3][2] = {}, have = 0;                                       // pages of this tile and of the two before
+            for (int kt = c0; kt < c1 + 2; ++kt) {
+                if (kt < c1 && (kt == c0 || (kt & 15) == 0)) { const int w = (2 * kt & ~31) + lane; have = w < min(2 * c1, at.s.pages) ? __ldcg(table + at.s.page(w)) : 0; }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    page[2][i] = page[1][i]; page[1][i] = page[0][i];
+                    page[0][i] = __shfl_sync(0xffffffffu, have, (2 * kt + i) & 31);
+                    if (kt >= c1 || 2 * kt + i >= at.s.pages) page[0][i] = 0;
+                    if (page[0][i] < 0 || page[0][i] >= a.num_pages) { if (lane == 0 && a.status) *a.status = 400; page[0][i] = 0; }
+                }
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    const int t = kt - 2 * v;                                    // K of this tile, V of the one two before
+                    if (t < c0 || t >= c1) continue;
+                    const int there = min(2, at.s.pages - 2 * t);                // a missing second page is not loaded: its scores are masked, its values set to zero
+                    const uint32_t slot = n % RING;
+                    if (BITS8 && v == 0) {
+                        const uint32_t buf = g % SC;
+                        mbar_wait(&sc_empty[buf], ((g / SC) & 1) ^ 1);
+                        if (elect_one()) {
+                            mbar_expect_tx(&sc_in[buf], there * 2 * CACHE_PAGE * 4);
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                for (int w = 0; w < 2; ++w)
+                                    if (i < there) bulk_load(sc_s + buf * Cfg::SC_FLOATS + w * KEYS + i * CACHE_PAGE, reinterpret_cast<const uint8_t*>(a.cache) +
+                                                             ((int64_t)(w * (int64_t)a.num_pages + page[0][i]) * a.n_kv + at.kvh) * BLOCK_BYTES + CACHE_PAGE * D, CACHE_PAGE * 4, &sc_in[buf]);
+                        }
+                        __syncwarp();
+                        ++g;
+                    }
+                    mbar_wait(&out[slot], ((n / RING) & 1) ^ 1);
+                    if (elect_one()) {
+                        mbar_expect_tx(&in[slot], there * (BITS8 ? CACHE_PAGE * D : HALVES * 8192));
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            if (i >= there) break;
+                            const int64_t block = ((int64_t)v * a.num_pages + (v ? page[2][i] : page[0][i])) * a.n_kv + at.kvh;
+                            if (BITS8) bulk_load(raw_s + slot * Cfg::RAW_BYTES + i * CACHE_PAGE * D, reinterpret_cast<const uint8_t*>(a.cache) + block * BLOCK_BYTES, CACHE_PAGE * D, &in[slot]);
+                            else
+#pragma unroll
+                                for (int h = 0; h < HALVES; ++h) tma_load_2d(kv_s + slot * TILE + h * HALF + i * 8192, &tm_kv, &in[slot], h * 64, (int)(block * CACHE_PAGE), kEvictNormal);
+                        }
+                    }
+                    __syncwarp();
+                    ++n;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // the whole warp walks the loop, an elected lane issues: descriptors stay in uniform registers
+        constexpr uint32_t f16 = BITS8 ? (1u << 7) | (1u << 10) : 0u;            // both operands fp16 instead of bf16
+        constexpr uint32_t idesc_s = umma_idesc_bf16(128, KEYS) ^ f16, idesc_o = umma_idesc_bf16_bmn(128, D) ^ f16;
+        const uint64_t q_desc = umma_desc_sw128(smem_u32(q_s)), k_desc = umma_desc_sw128(smem_u32(kv_s));
+        const uint64_t v_desc = umma_desc_sw128_mn(smem_u32(kv_s), (uint32_t)HALF, 1024u);
+        uint32_t n = 0, r = 0, seg = 0;                                          // tiles of the pieces before, entries of the ring, pieces
+        auto await = [&] {                                                       // the ring's next tile
+            const uint32_t slot = r % SLOTS;
+            mbar_wait(&full[slot], (r / SLOTS) & 1);
+            ++r;
+            tcgen05_fence_after();
+            return slot;
+        };
+        // products of one thread are carried out in the order of their issue: S of a tile goes over scores whose P a product ahead of it reads
+        for (int64_t u = u_begin; u < u_end; at.next(a)) {
+            take(u);
+            const int tiles = c1 - c0;
+            if (tiles == 0) continue;
+            mbar_wait(q_full, seg & 1);
+            ++seg;
+            tcgen05_fence_after();
+            for (int j = -2; j < tiles; ++j) {
+                if (j + 2 < tiles) {                                             // scores two tiles ahead, under the softmaxes of the tiles before
+                    const uint32_t slot = await(), to = (n + j + 2) % 3;
+                    if (elect_one()) {
+                        const uint64_t b = k_desc + (uint64_t)(slot * (TILE >> 4));
+#pragma unroll
+                        for (int ks = 0; ks < D / 16; ++ks) {
+                            const int half = ks >> 2, in = (ks & 3) * 32;
+                            umma_bf16(tmem_base + to * 128, q_desc + (uint64_t)((half * HALF + in) >> 4), b + (uint64_t)((half * HALF + in) >> 4), idesc_s, ks > 0 ? 1u : 0u);
+                        }
+                        umma_commit(&s_full[to]);
+                        umma_commit(&empty[slot]);
+                        if (j + 3 == tiles) umma_commit(q_empty);
+                    }
+                    __syncwarp();
+                }
+                if (j >= 0) {
+                    const uint32_t m = n + j, from = m % 3;
+                    mbar_wait(&p_full[from], (m / 3) & 1);
+                    const uint32_t slot = await();
+                    if (elect_one()) {
+                        const uint64_t b = v_desc + (uint64_t)(slot * (TILE >> 4));
+#pragma unroll
+                        for (int ks = 0; ks < KEYS / 16; ++ks)
+                            umma_bf16_ta(tmem_base + Cfg::O_COL, tmem_base + from * 128 + ks * 8, b + (uint64_t)(ks * (2048 >> 4)), idesc_o, (j > 0 || ks > 0) ? 1u : 0u);
+                        umma_commit(&o_full[m & 3]);
+                        umma_commit(&empty[slot]);
+                    }
+                    __syncwarp();
+                }
+            }
+            n += tiles;
+        }
+    } else if (warp >= 4 && warp < 12) {
+        // Two warpgroups take the tiles in turn, a row a thread: one's exponentials run under the other's loads and maxima.  A row's reference maximum goes from one to the other
+        // with each tile, as soon as the tile's own maximum is known; sums stay with either, O is one for both
+        const int quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t wg = (warp - 4) >> 2, lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16), o_addr = lane_addr + Cfg::O_COL;
+        auto meet = [] { asm volatile("bar.sync 2, %0;" ::"n"(SOFTMAX) : "memory"); };
+        auto take_turn = [](uint32_t n) {                                        // tile n - 1 has left its reference
+            if (n & 1) asm volatile("bar.sync 3, %0;" ::"n"(SOFTMAX) : "memory"); else asm volatile("bar.sync 4, %0;" ::"n"(SOFTMAX) : "memory");
+        };
+        auto pass_turn = [](uint32_t n) {                                        // to tile n
+            if (n & 1) asm volatile("bar.arrive 3, %0;" ::"n"(SOFTMAX) : "memory"); else asm volatile("bar.arrive 4, %0;" ::"n"(SOFTMAX) : "memory");
+        };
+        constexpr float kRaise = 8.0f;                                           // log2 units a score may pass the reference by
+        constexpr int COLS = D / 2;
+        uint32_t n0 = 0, seg = 0;                                                // tiles of the pieces before, pieces
+        for (int64_t u = u_begin; u < u_end; at.next(a)) {
+            take(u);
+            const int64_t end = at.unit0 + at.units();
+            const bool first = at.unit0 >= u_begin, last = end <= u_end;
+            const int live_rows = at.rows(grp), row0 = at.row0(), tiles = c1 - c0;
+            const bool live = row < live_rows;
+            const uint32_t n1 = n0 + tiles;
+            uint64_t seen = 0; int low = 0x7fffffff;
+            if (live) { const int t = at.tile * tile_tokens + row / grp; seen = tree_seen(a, at.s, t); low = tree_low(a, at.s, seen, t); }
+            const bool blind = live && !tree_sees(a, at.s, seen, low);
+            TreeAny any;
+            if (!BITS8) any.read(a, at, lane);
+            if (warp == 4 && lane == 0 && first && !last) tree_record(a, cta_of(end - 1, share.busy, share.total) - (int)blockIdx.x, row0, live_rows, at.kvh);
+            float* po = a.part_o + ((int64_t)blockIdx.x * 2 + !first) * (128 * D) + row * 4;         // [D / 4][128 rows][4]: a warp's rows lie next to each other
+            float2* ml = reinterpret_cast<float2*>(a.part_ml) + ((int64_t)blockIdx.x * 2 + !first) * 128 + row;
+            if (tiles == 0) {                                                    // units of the item's own alone
+                if (live)
+                    for (int c = wg * COLS; c < (int)(wg + 1) * COLS; c += 4) *reinterpret_cast<float4*>(po + c * 128) = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (live && wg == 0) *ml = make_float2(-INFINITY, first && blind ? -1.f : 0.f);
+                continue;
+            }
+            float fac = a.scale_log2e, vref = 1.0f;
+            if (BITS8) { mbar_wait(q_full, seg & 1); fac = factor_s[(seg & 1) * 128 + row] * a.scale_log2e; }
+            ++seg;
+            float m_mine = -INFINITY, l_run = 0.f;                               // the sum so far and the reference that it is under
+            auto tile = [&](uint32_t n, auto tag) {
+                constexpr bool SPECIAL = decltype(tag)::value;
+                const int kt = c0 + (int)(n - n0);
+                const uint32_t from = n % 3, s_addr = lane_addr + from * 128, buf = n % SC;
+                const float* sc = sc_s + buf * Cfg::SC_FLOATS;
+                uint64_t word[2] = {~0ull, ~0ull};
+                if (SPECIAL) {
+                    word[0] = tree_word(a, at.s, seen, low, at.s.page(2 * kt) * CACHE_PAGE);
+                    word[1] = 2 * kt + 1 < at.s.pages ? tree_word(a, at.s, seen, low, at.s.page(2 * kt + 1) * CACHE_PAGE) : 0ull;
+                }
+                float grown = 1.0f;
+                if (BITS8) { mbar_wait(&sc_full[buf], (n / SC) & 1); vref = sc[2 * KEYS]; grown = sc[2 * KEYS + 1]; }
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};     // four chains
+                mbar_wait(&s_full[from], (n / 3) & 1);
+                tcgen05_fence_after();
+                uint32_t v[2][32];
+                auto scores = [&](int k) {                                       // of keys k .. k + 63, their scales in them, -inf where the row does not see
+                    tmem_ld_32x32b_x32(s_addr + k, v[0]);
+                    tmem_ld_32x32b_x32(s_addr + k + 32, v[1]);
+                    tmem_ld_wait();
+                    const uint64_t w = k ? word[1] : word[0];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            float4 ks = make_float4(1.f, 1.f, 1.f, 1.f);
+                            if (BITS8) ks = *reinterpret_cast<const float4*>(sc + k + c * 32 + i);
+                            const float f[4] = {ks.x, ks.y, ks.z, ks.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                if (BITS8) v[c][i + e] = __float_as_uint(__uint_as_float(v[c][i + e]) * f[e]);
+                                if (SPECIAL && !((uint32_t)(w >> (c * 32)) >> (i + e) & 1)) v[c][i + e] = 0xff800000u;
+                            }
+                        }
+                };
+#pragma unroll 1
+                for (int k = KEYS - 64; k >= 0; k -= 64) {                       // the lower keys last: they stay in registers
+                    scores(k);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[c][i]));
+                }
+                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * fac;
+                if (n > n0) take_turn(n);
+                // A barrier's phases are seen one by one: PV of the tile three before is the last one that this tile can be sure of without a wait
+                if (n > 2) mbar_wait(&o_full[(n - 3) & 3], ((n - 3) >> 2) & 1);
+                const float m_last = n > n0 ? m_s[row] : -INFINITY;
+                const bool raise = mx > m_last + kRaise;
+                const float m_ref = raise ? mx : m_last;
+                m_s[row] = m_ref;
+                if (n + 1 < n1) pass_turn(n + 1);
+                if (n > n0 && (grown != 1.0f || __any_sync(0xffffffffu, raise))) {
+                    mbar_wait(&o_full[(n - 1) & 3], ((n - 1) >> 2) & 1);         // O has the products of all tiles before; this tile's are not issued before p_full
+                    tcgen05_fence_after();
+                    const float alpha = (raise ? exp2f(m_last - m_ref) : 1.0f) * grown;
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 16) {
+                        uint32_t o[16];
+                        tmem_ld_32x32b_x16(o_addr + c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        tmem_st_32x32b_x16(o_addr + c, o);
+                    }
+                }
+                if (SPECIAL && !BITS8) {
+                    // values that none of the rows sees may be anything, and 0 x inf is not 0: a thread looks after the key of its row's number
+                    const uint32_t entry = 2 * n0 + min(tiles, kt - c0 + 3) + (kt - c0), slot = entry % SLOTS;
+                    mbar_wait(&full[slot], (entry / SLOTS) & 1);
+                    const int c = 2 * kt + (row >> 6);
+                    if (c >= at.s.pages || !any.sees(a, at.s, at.s.page(c) * CACHE_PAGE + (row & 63))) {
+#pragma unroll
+                        for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(kv_s + slot * TILE + (c >> 3) * HALF + row * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    fence_proxy_async();
+                }
+                if (m_mine != m_ref) { l_run *= ex2_approx(m_mine - m_ref); m_mine = m_ref; }
+                const float neg_ref = -finite_or_zero(m_ref);
+                uint64_t sum = 0;
+#pragma unroll 1
+                for (int k = 0; k < KEYS; k += 64) {
+                    if (k > 0) scores(k);                                        // read again: P of the keys before lies over their own scores
+                    const uint64_t wk = k ? word[1] : word[0];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            float4 vs = make_float4(1.f, 1.f, 1.f, 1.f);
+                            if (BITS8) vs = *reinterpret_cast<const float4*>(sc + KEYS + k + c * 32 + 2 * i);
+                            const float f[4] = {vs.x, vs.y, vs.z, vs.w};
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                float x = ex2_approx(fmaf(__uint_as_float(v[c][2 * (i + e)]), fac, neg_ref)), y = ex2_approx(fmaf(__uint_as_float(v[c][2 * (i + e) + 1]), fac, neg_ref));
+                                sum = add_f32x2(sum, pack_f32x2(x, y));
+                                if (BITS8) {
+                                    x *= f[2 * e]; y *= f[2 * e + 1];
+                                    if (SPECIAL) {                               // 0 of a key that the row does not see, whatever its scale
+                                        const uint32_t bits = (uint32_t)(wk >> (c * 32)) >> (2 * (i + e));
+                                        if (!(bits & 1)) x = 0.f;
+                                        if (!(bits & 2)) y = 0.f;
+                                    }
+                                    w[i + e] = pack_f16x2(x, y);
+                                } else w[i + e] = pack_bf16x2(x, y);
+                            }
+                        }
+                        tmem_st_32x32b_x16(s_addr + k / 2 + c * 16, w);
+                    }
+                }
+                tmem_st_wait();
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(&p_full[from]); if (BITS8) mbar_arrive(&sc_empty[buf]); }
+                float lo, hi; unpack_f32x2(sum, lo, hi);
+                l_run += lo + hi;
+            };
+            for (uint32_t n = n0 + ((n0 ^ wg) & 1); n < n1; n += 2) {
+                if (special(c0 + (int)(n - n0))) tile(n, TrueTag{}); else tile(n, FalseTag{});
+            }
+            n0 = n1;
+            meet();                                                              // the last tile's reference is there
+            const float m_ref = m_s[row];
+            if (m_mine != m_ref) l_run *= ex2_approx(m_mine - m_ref);
+            l_s[wg * 128 + row] = l_run;
+            if (BITS8 && ((n1 - 1) & 1) == wg && row == 0) sc_last = vref;
+            meet();
+            const float l = l_s[row] + l_s[128 + row], undo = BITS8 ? sc_last * (1.0f / 128.0f) : 1.0f;
+            mbar_wait(&o_full[(n1 - 1) & 3], ((n1 - 1) >> 2) & 1);
+            tcgen05_fence_after();
+            const bool whole = first && last;
+            const float mult = undo * (whole ? (blind ? 0.f : 1.0f / l) : 1.0f);
+            const int token = row / grp;
+            uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(row0 + token) * a.ldo + (int64_t)(at.kvh * grp + row - token * grp) * D;
+#pragma unroll 1
+            for (int c = wg * COLS; c < (int)(wg + 1) * COLS; c += 32) {
+                uint32_t o[32];
+                tmem_ld_32x32b_x32(o_addr + c, o);
+                tmem_ld_wait();
+                if (!live) continue;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * mult);
+                if (whole) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(out + c + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                } else
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<float4*>(po + (c + i) * 128) = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+            }
+            tcgen05_fence_before();
+            if (live && !whole && wg == 0) *ml = make_float2(m_ref, first && blind ? -1.f : l);
+            meet();                                                              // O and the sums may be written again
+        }
+    } else if (warp == 2) {
+        // scales of a tile: keys' as they are, values' over a power of two that none so far passes and times 2^7 (a weight is 2^8 at most); 0 of what none of the rows sees
+        if constexpr (BITS8) {
+            uint32_t n = 0;
+            for (int64_t u = u_begin; u < u_end; at.next(a)) {
+                take(u);
+                if (c1 == c0) continue;
+                TreeAny any;
+                any.read(a, at, lane);
+                float vref = 0.f;
+                for (int kt = c0; kt < c1; ++kt, ++n) {
+                    const uint32_t buf = n % SC;
+                    float* sc = sc_s + buf * Cfg::SC_FLOATS;
+                    const bool sp = special(kt);
+                    mbar_wait(&sc_in[buf], (n / SC) & 1);
+                    float4 k4 = *reinterpret_cast<const float4*>(sc + 4 * lane), v4 = *reinterpret_cast<const float4*>(sc + KEYS + 4 * lane);
+                    float k[4] = {k4.x, k4.y, k4.z, k4.w}, v[4] = {v4.x, v4.y, v4.z, v4.w};
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int c = 2 * kt + (lane >> 4);
+                        if (sp && (c >= at.s.pages || !any.sees(a, at.s, at.s.page(c) * CACHE_PAGE + (4 * lane & 63) + i))) k[i] = v[i] = 0.f;
+                        if (fabsf(v[i]) < INFINITY) top = max(top, __float_as_uint(fabsf(v[i])));
+                    }
+                    top = __reduce_max_sync(0xffffffffu, top);
+                    const float need = __uint_as_float(min((top & 0x7f800000u) + 0x00800000u, 0x7e800000u));             // up to 2^126
+                    float grown = 1.0f;
+                    if (need > vref) { grown = vref > 0.f ? vref * (1.0f / need) : 1.0f; vref = need; }
+                    const float inv = 1.0f / vref;                               // powers of two: exact
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = v[i] * inv * 128.f;
+                    *reinterpret_cast<float4*>(sc + 4 * lane) = make_float4(k[0], k[1], k[2], k[3]);
+                    *reinterpret_cast<float4*>(sc + KEYS + 4 * lane) = make_float4(v[0], v[1], v[2], v[3]);
+                    if (lane == 0) { sc[2 * KEYS] = vref; sc[2 * KEYS + 1] = grown; }
+                    fence_proxy_async();                                         // the next scales to come here are another proxy's writes
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sc_full[buf]);
+                }
+            }
+        }
+    } else if (warp >= 12) {
+        // queries, then tiles in the ring's order, 16 channels of a key a step
+        if constexpr (BITS8) {
+            const int w = warp - 12, tid = w * 32 + lane;
+            uint32_t n = 0, seg = 0;
+            for (int64_t u = u_begin; u < u_end; at.next(a)) {
+                take(u);
+                const int tiles = c1 - c0;
+                if (tiles == 0) continue;
+                TreeAny any;
+                any.read(a, at, lane);
+                mbar_wait(q_empty, (seg & 1) ^ 1);
+                const int live = at.rows(grp);
+                constexpr int W = D / 64;                                        // words of two channels a lane
+                for (int r0 = w * 32; r0 < min(live, w * 32 + 32); r0 += 8) {
+                    uint32_t x[8][W];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = r0 + i, token = r / grp;
+                        const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(at.row0() + token) * a.ldq + (int64_t)(at.kvh * grp + r - token * grp) * D + lane * 2 * W;
+                        if (r < live) {
+                            if (W == 2) { const uint2 y = __ldcg(reinterpret_cast<const uint2*>(src)); x[i][0] = y.x; x[i][W - 1] = y.y; } else x[i][0] = __ldcg(reinterpret_cast<const uint32_t*>(src));
+                        } else
+#pragma unroll
+                            for (int j = 0; j < W; ++j) x[i][j] = 0u;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = r0 + i;
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int j = 0; j < W; ++j) top = max(top, max(x[i][j] << 16 & 0x7fffffffu, x[i][j] & 0x7fff0000u));
+                        top = __reduce_max_sync(0xffffffffu, top);
+                        const int e = top >= 0x7f800000u ? 14 : max((int)(top >> 23) - 127, -100);       // not finite: as it is
+                        const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+                        const int ch = lane * 2 * W;
+#pragma unroll
+                        for (int j = 0; j < W; ++j)
+                            *reinterpret_cast<uint32_t*>(q_s + (ch >> 6) * HALF + r * 128 + ((((ch & 63) >> 3) ^ (r & 7)) << 4) + (ch & 7) * 2 + j * 4) = pack_f16x2(bf16lo(x[i][j]) * up, bf16hi(x[i][j]) * up);
+                        if (lane == 0) factor_s[(seg & 1) * 128 + r] = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+                    }
+                }
+                ++seg;
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full);
+                for (int kt = 0; kt < tiles + 2; ++kt)
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) {
+                        const int t = kt - 2 * v;
+                        if (t < 0 || t >= tiles) continue;
+                        const uint32_t from = n % RAW, to = n % SLOTS;
+                        const bool sp = v && special(c0 + t);
+                        mbar_wait(&raw_full[from], (n / RAW) & 1);
+                        mbar_wait(&empty[to], ((n / SLOTS) & 1) ^ 1);
+                        const uint8_t* src = raw_s + from * Cfg::RAW_BYTES;
+                        uint8_t* dst = kv_s + to * TILE;
+                        constexpr int STEPS = Cfg::RAW_BYTES / 16 / 128;
+#pragma unroll
+                        for (int i = 0; i < STEPS; ++i) {
+                            const int c = i * 128 + tid, key = c / (D / 16), ch = c % (D / 16);          // 16 channels from 16 ch on
+                            uint4 x = *reinterpret_cast<const uint4*>(src + c * 16);
+                            uint32_t y[8];
+                            to_f16<FMT, false>(x.x, y[0], y[1]); to_f16<FMT, false>(x.y, y[2], y[3]); to_f16<FMT, false>(x.z, y[4], y[5]); to_f16<FMT, false>(x.w, y[6], y[7]);
+                            if (sp) {                                            // values that none of the rows sees may be anything, and 0 x inf is not 0
+                                const int pg = 2 * (c0 + t) + (key >> 6);
+                                if (pg >= at.s.pages || !any.sees(a, at.s, at.s.page(pg) * CACHE_PAGE + (key & 63)))
+#pragma unroll
+                                    for (int j = 0; j < 8; ++j) y[j] = 0u;
+                            }
+                            const int odd = ch >> 2 & 1;                         // which of the two pieces goes first: eight lanes' stores fall on eight pieces of a line
+                            const uint4 lo = make_uint4(y[0], y[1], y[2], y[3]), hi = make_uint4(y[4], y[5], y[6], y[7]);
+                            uint8_t* line = dst + (ch >> 2) * HALF + key * 128;
+                            const int p = 2 * (ch & 3);
+                            *reinterpret_cast<uint4*>(line + (((p + odd) ^ (key & 7)) << 4)) = odd ? hi : lo;
+                            *reinterpret_cast<uint4*>(line + (((p + 1 - odd) ^ (key & 7)) << 4)) = odd ? lo : hi;
+                        }
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) { mbar_arrive(&raw_empty[from]); mbar_arrive(&full[to]); }
+                        ++n;
+                    }
+            }
+        }
+    }
+    __syncthreads();
+    griddep_launch();
+    if (warp == 1) { tcgen05_fence_after(); tmem_dealloc<512>(tmem_base); }
+}
+
+// =============================================================================================
 // the join
 // =============================================================================================
-// Of the item that a CTA began and others ended: eight rows a CTA, a thread four channels of a row
+// Of the item that a CTA began and others ended: a thread eight channels of a row
+constexpr int TREE_JOIN_THREADS = 128;
 template <int D>
-__global__ void __launch_bounds__(2 * D) tree_join_kernel(const __grid_constant__ TreeAttnArgs a) {
-    const int cta = blockIdx.x, row = blockIdx.y * 8 + threadIdx.x / (D / 4), c = threadIdx.x % (D / 4) * 4, grp = a.n_heads / a.n_kv;
+__global__ void __launch_bounds__(TREE_JOIN_THREADS) tree_join_kernel(const __grid_constant__ TreeAttnArgs a) {
+    const int cta = blockIdx.x, x = blockIdx.y * TREE_JOIN_THREADS + threadIdx.x, row = x % a.rows, c = x / a.rows * 8, grp = a.n_heads / a.n_kv;
     griddep_launch();
     griddep_wait();
     const int parts = __ldcg(&a.joins[cta].parts);
-    if (parts == 0 || row >= __ldcg(&a.joins[cta].rows)) return;
+    if (parts == 0 || c >= D || row >= __ldcg(&a.joins[cta].rows)) return;
     const int row0 = __ldcg(&a.joins[cta].row0), kvh = __ldcg(&a.joins[cta].kvh);
-    const bool blind = __ldcg(&a.joins[cta].blind) >> row & 1;
     auto slot = [&](int i) { return i == 0 ? (int64_t)cta * 2 : (int64_t)(cta + i) * 2 + 1; };
-    float M = -INFINITY, l = 0.f; float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int MP = 8;
+    float M = -INFINITY, l = 0.f; float acc[8] = {};
+    bool blind = false;
+    constexpr int MP = 4;
     for (int i0 = 0; i0 <= parts; i0 += MP) {
-        float2 ml[MP]; float4 o[MP];
+        float2 ml[MP]; float4 o[MP][2];
 #pragma unroll
         for (int p = 0; p < MP; ++p) {
-            ml[p] = make_float2(-INFINITY, 0.f); o[p] = make_float4(0.f, 0.f, 0.f, 0.f);
+            ml[p] = make_float2(-INFINITY, 0.f); o[p][0] = o[p][1] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (i0 + p > parts) continue;
-            ml[p] = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + slot(i0 + p) * a.rows + row);
-            o[p] = __ldcg(reinterpret_cast<const float4*>(a.part_o + (slot(i0 + p) * a.rows + row) * D + c));
+            const int64_t at = slot(i0 + p) * a.rows;
+            ml[p] = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + at + row);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) o[p][h] = __ldcg(reinterpret_cast<const float4*>(a.part_o + at * D + (int64_t)(c / 4 + h) * (a.rows * 4) + row * 4));
         }
+        if (i0 == 0) blind = ml[0].y < 0.f;
         float m = M;
 #pragma unroll
         for (int p = 0; p < MP; ++p) m = fmaxf(m, ml[p].x);
         const float ref = finite_or_zero(m), f0 = ex2_approx(M - ref);
-        M = m; l *= f0; acc.x *= f0; acc.y *= f0; acc.z *= f0; acc.w *= f0;
+        M = m; l *= f0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] *= f0;
 #pragma unroll
         for (int p = 0; p < MP; ++p) {
             const float f = ex2_approx(ml[p].x - ref);
-            l += f * ml[p].y; acc.x += f * o[p].x; acc.y += f * o[p].y; acc.z += f * o[p].z; acc.w += f * o[p].w;
+            l += f * ml[p].y;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) { acc[4 * h] += f * o[p][h].x; acc[4 * h + 1] += f * o[p][h].y; acc[4 * h + 2] += f * o[p][h].z; acc[4 * h + 3] += f * o[p][h].w; }
         }
     }
     const float inv = blind ? 0.f : 1.0f / l;
     const int token = row / grp;
     uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(row0 + token) * a.ldo + (int64_t)(kvh * grp + row - token * grp) * D + c;
-    *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    *reinterpret_cast<uint4*>(out) = make_uint4(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv), pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv));
+}
+template <int D>
+static cudaError_t launch_tree_join(const TreeAttnArgs& a, cudaStream_t s) {
+    return launch_k(tree_join_kernel<D>, dim3(a.ctas, (a.rows * (D / 8) + TREE_JOIN_THREADS - 1) / TREE_JOIN_THREADS), dim3(TREE_JOIN_THREADS), 0, s, a);
 }
 
 // =============================================================================================
 // host
 // =============================================================================================
+constexpr int TREE_FEW_ROWS = 16;               // of a sequence on average
 TreeAttnPlan tree_attn_plan(int n_seqs, int n_rows, int n_heads, int n_kv, int head_dim, int format, int max_pages, int sms) {
     TreeAttnPlan p{};
     const int grp = n_heads / n_kv;
     const int64_t mean = ((int64_t)n_rows + n_seqs - 1) / n_seqs * grp;
-    p.rows = mean <= 8 && grp <= 8 ? 8 : 16;
+    p.rows = mean > TREE_FEW_ROWS ? 128 : mean <= 8 && grp <= 8 ? 8 : 16;
     const int tile_tokens = p.rows / grp;
-    const int64_t items = ((int64_t)n_rows / tile_tokens + n_seqs) * n_kv, units = items * (1 + (int64_t)max_pages);          // no more than that, however rows fall on sequences
+    const int64_t items = ((int64_t)n_rows / tile_tokens + n_seqs) * n_kv, units = items * (TREE_OVER + (int64_t)max_pages);          // no more than that, however rows fall on sequences
     const int64_t most = (int64_t)sms * (format != CACHE_BF16 && p.rows == 8 ? 2 : 1);
     p.ctas = (int)(units < most ? units : most);
     auto take = [&](size_t bytes) { const size_t at = p.bytes; p.bytes += (bytes + 255) & ~size_t(255); return at; };
@@ -586,20 +1178,30 @@ static cudaError_t launch_few(const CUtensorMap* tm_page, const TreeAttnArgs& a,
     using Cfg = FewCfg<D, FMT, NB, STAGES>;
     auto kern = tree_few_kernel<D, FMT, NB, STAGES>;
     static bool attr_done[16] = {};
-    cudaError_t e = ensure_dynamic_smem(kern, Cfg::SMEM_BYTES, attr_done);
-    if (e == cudaSuccess) e = launch_k(kern, dim3(a.ctas), dim3(TREE_THREADS), Cfg::SMEM_BYTES, s, *tm_page, a);
-    if (e == cudaSuccess) e = launch_k(tree_join_kernel<D>, dim3(a.ctas, NB), dim3(2 * D), 0, s, a);
-    return e;
+    const cudaError_t e = ensure_dynamic_smem(kern, Cfg::SMEM_BYTES, attr_done);
+    return e == cudaSuccess ? launch_k(kern, dim3(a.ctas), dim3(TREE_THREADS), Cfg::SMEM_BYTES, s, *tm_page, a) : e;
 }
 template <int D, int FMT>
-static cudaError_t launch_of(const CUtensorMap* tm_page, const TreeAttnArgs& a, cudaStream_t s) {
-    constexpr int MORE = D == 64 ? 2 : 1;
-    return a.rows == 8 ? launch_few<D, FMT, 1, 5 * MORE>(tm_page, a, s) : launch_few<D, FMT, 2, (FMT == CACHE_BF16 ? 5 : 9) * MORE>(tm_page, a, s);
+static cudaError_t launch_many(const CUtensorMap* tm_q, const CUtensorMap* tm_page, const TreeAttnArgs& a, cudaStream_t s) {
+    using Cfg = ManyCfg<D, FMT>;
+    auto kern = tree_many_kernel<D, FMT>;
+    static bool attr_done[16] = {};
+    const cudaError_t e = ensure_dynamic_smem(kern, Cfg::SMEM_BYTES, attr_done);
+    return e == cudaSuccess ? launch_k(kern, dim3(a.ctas), dim3(Cfg::THREADS), Cfg::SMEM_BYTES, s, *tm_q, *tm_page, a) : e;
 }
-cudaError_t launch_tree_attention(const CUtensorMap* tm_page, int head_dim, int format, const TreeAttnArgs& a, cudaStream_t s) {
-    if (head_dim == 64) return format == CACHE_BF16 ? launch_of<64, CACHE_BF16>(tm_page, a, s) : format == CACHE_E4M3 ? launch_of<64, CACHE_E4M3>(tm_page, a, s) : launch_of<64, CACHE_INT8>(tm_page, a, s);
-    if (head_dim == 128) return format == CACHE_BF16 ? launch_of<128, CACHE_BF16>(tm_page, a, s) : format == CACHE_E4M3 ? launch_of<128, CACHE_E4M3>(tm_page, a, s) : launch_of<128, CACHE_INT8>(tm_page, a, s);
-    return cudaErrorInvalidValue;
+template <int D, int FMT>
+static cudaError_t launch_parts(const CUtensorMap* tm_q, const CUtensorMap* tm_page, const TreeAttnArgs& a, cudaStream_t s) {
+    constexpr int MORE = D == 64 ? 2 : 1;
+    const cudaError_t e = a.rows == 128 ? launch_many<D, FMT>(tm_q, tm_page, a, s)
+                        : a.rows == 8 ? launch_few<D, FMT, 1, 5 * MORE>(tm_page, a, s) : launch_few<D, FMT, 2, (FMT == CACHE_BF16 ? 5 : 9) * MORE>(tm_page, a, s);
+    return e == cudaSuccess ? launch_tree_join<D>(a, s) : e;
+}
+template <int D>
+static cudaError_t launch_of(const CUtensorMap* tm_q, const CUtensorMap* tm_page, int format, const TreeAttnArgs& a, cudaStream_t s) {
+    return format == CACHE_BF16 ? launch_parts<D, CACHE_BF16>(tm_q, tm_page, a, s) : format == CACHE_E4M3 ? launch_parts<D, CACHE_E4M3>(tm_q, tm_page, a, s) : launch_parts<D, CACHE_INT8>(tm_q, tm_page, a, s);
+}
+cudaError_t launch_tree_attention(const CUtensorMap* tm_q, const CUtensorMap* tm_page, int head_dim, int format, const TreeAttnArgs& a, cudaStream_t s) {
+    return head_dim == 64 ? launch_of<64>(tm_q, tm_page, format, a, s) : head_dim == 128 ? launch_of<128>(tm_q, tm_page, format, a, s) : cudaErrorInvalidValue;
 }
 
 }  // namespace oa

@@ -64,7 +64,7 @@ cudaError_t launch_cache8_copy(void* cache, int planes, int num_pages, int n_kv,
 // ---- attention of several new tokens of a sequence -----------------------------------------------------------
 constexpr int TREE_MAX_TOKENS = 64;               // new tokens of a sequence: the bits of a row of `seen`
 constexpr int TREE_MAX_GROUP = 16;                // query heads of a key/value head
-struct TreeJoin { int32_t parts, row0, rows, kvh; uint32_t blind; };      // an item that several CTAs share: later parts, its first row, its rows, its head, rows that see nothing
+struct TreeJoin { int32_t parts, row0, rows, kvh; };      // an item that several CTAs share: later parts, its first row, its rows, its head
 struct TreeAttnArgs {
     const void* q; int64_t ldq; void* out; int64_t ldo;
     const void* cache; const int32_t* tables; const int32_t* ctx_lens; const int32_t* row_starts; const uint64_t* seen;      // seen null: a chain
@@ -77,7 +77,8 @@ struct TreeAttnArgs {
 };
 struct TreeAttnPlan { int ctas, rows; size_t part_o, part_ml, joins, bytes; };
 TreeAttnPlan tree_attn_plan(int n_seqs, int n_rows, int n_heads, int n_kv, int head_dim, int format, int max_pages, int sms);
-// tm_page: box of 64 rows over the layer's cache [2 * num_pages * n_kv * 64, head_dim] of bf16, or of a block's values over the same of 8 bits, rows of 128 bytes
-cudaError_t launch_tree_attention(const CUtensorMap* tm_page, int head_dim, int format, const TreeAttnArgs& a, cudaStream_t s);
+// tm_page: box of 64 rows over the layer's cache [2 * num_pages * n_kv * 64, head_dim] of bf16, or of a block's values over the same of 8 bits, rows of 128 bytes; tm_q, looked at for tiles of 128 rows
+// over bf16: box of 128 / group tokens by a group's heads over q
+cudaError_t launch_tree_attention(const CUtensorMap* tm_q, const CUtensorMap* tm_page, int head_dim, int format, const TreeAttnArgs& a, cudaStream_t s);
 
 }  // namespace oa

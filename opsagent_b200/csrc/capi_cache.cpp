@@ -294,14 +294,18 @@ int oa_k_tree_attention(const void* q, int64_t ldq, void* out, int64_t ldo, cons
     const uintptr_t c = (uintptr_t)kv_cache, o = (uintptr_t)out;
     if (o < c + 2ull * num_pages * n_kv * CACHE_PAGE * row_bytes && c < o + ((n_rows - 1) * ldo + width) * 2) return bad("tree attention: out overlaps the cache");
     OA_ON_DEVICE_OF(kv_cache, q, out, block_tables, ctx_lens, row_starts, seen, status);
-    CUtensorMap tm_page;
-    if ((format == CACHE_BF16 ? make_tmap_bf16_2d(&tm_page, kv_cache, (uint64_t)tm_rows, head_dim, head_dim, CACHE_PAGE, 64)
-                              : make_tmap_bytes_2d(&tm_page, kv_cache, (uint64_t)tm_rows, CACHE_PAGE * head_dim / 128)) != 0) return call_failed(OA_ERR_INTERNAL, "tree attention: no tensor map of the cache");
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return device_rc(e);
     const TreeAttnPlan plan = tree_attn_plan(n_seqs, n_rows, n_heads, n_kv, head_dim, format, max_pages_per_seq, sms);
+    if (n_rows == 1) ldq = ldo = width;                      // a single row has no pitch, and a tensor map takes none of 2^40 bytes
+    CUtensorMap tm_page, tm_q{};
+    const int group = n_heads / n_kv;
+    if ((format == CACHE_BF16 ? make_tmap_bf16_2d(&tm_page, kv_cache, (uint64_t)tm_rows, head_dim, head_dim, CACHE_PAGE, 64)
+                              : make_tmap_bytes_2d(&tm_page, kv_cache, (uint64_t)tm_rows, CACHE_PAGE * head_dim / 128)) != 0) return call_failed(OA_ERR_INTERNAL, "tree attention: no tensor map of the cache");
+    if (format == CACHE_BF16 && plan.rows == 128 &&
+        make_tmap_bf16_heads(&tm_q, q, (uint64_t)n_rows, (uint64_t)n_heads, (uint64_t)head_dim, (uint64_t)ldq, 128 / group, group) != 0) return call_failed(OA_ERR_INTERNAL, "tree attention: no tensor map of the queries");
     DevBuf scratch(plan.bytes, (cudaStream_t)stream);
     if (!scratch.p) return call_failed(OA_ERR_INTERNAL, "tree attention: no scratch memory");
     char* base = (char*)scratch.p;
@@ -310,7 +314,7 @@ int oa_k_tree_attention(const void* q, int64_t ldq, void* out, int64_t ldo, cons
     a.max_pages = max_pages_per_seq; a.n_seqs = n_seqs; a.n_rows = n_rows; a.n_heads = n_heads; a.n_kv = n_kv; a.num_pages = num_pages; a.window = window; a.sinks = sinks;
     a.scale_log2e = scale_log2e; a.status = status;
     a.part_o = (float*)(base + plan.part_o); a.part_ml = (float*)(base + plan.part_ml); a.joins = (TreeJoin*)(base + plan.joins); a.ctas = plan.ctas; a.rows = plan.rows;
-    return device_rc(launch_tree_attention(&tm_page, head_dim, format, a, (cudaStream_t)stream));
+    return device_rc(launch_tree_attention(&tm_q, &tm_page, head_dim, format, a, (cudaStream_t)stream));
 }
 
 }  // extern "C"
