@@ -37,6 +37,8 @@ OA_DEVINL void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+OA_DEVINL uint32_t mul_f16x2(uint32_t a, uint32_t b) { uint32_t r; asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+OA_DEVINL uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) { uint32_t r; asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c)); return r; }
 template <int FMT>
 OA_DEVINL void mma_of(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     if (FMT == CACHE_BF16) mma_bf16_16816(d, a0, a1, a2, a3, b0, b1); else mma_f16_16816(d, a0, a1, a2, a3, b0, b1);
@@ -555,8 +557,8 @@ struct ManyCfg {
     static constexpr int KEYS = 128, HALVES = D / 64, HALF = 128 * 128;          // 128 rows x 64 channels of 2 bytes under the 128-byte swizzle: of Q, of a tile
     static constexpr int TILE_BYTES = HALVES * HALF, SLOTS = BITS8 ? (D == 128 ? 3 : 4) : D == 128 ? 5 : 8;
     static constexpr int RAW_BYTES = KEYS * D, RAW = BITS8 ? (D == 128 ? 5 : 8) : 0;         // a tile of 8 bits, and how many wait
-    static constexpr int SC = 8, SC_FLOATS = 2 * KEYS + 4;                       // tiles whose scales wait: keys', values', their power of two, what O is multiplied by for it
-    static constexpr int THREADS = 128 + 256 + (BITS8 ? 128 : 0);                // producer, issuer, scales; eight softmax warps; four that convert
+    static constexpr int SC = 8, SC_FLOATS = 2 * KEYS + 4;                       // tiles whose scales wait: keys', values', what scores are multiplied by, what O is for larger scales of values and at its end
+    static constexpr int CONV = BITS8 ? 8 : 0, THREADS = 128 + 256 + 32 * CONV;     // producer, issuer, scales; eight softmax warps; warps that convert
     static constexpr int BARS = 12 + 2 * SLOTS + 2 * RAW + (BITS8 ? 3 * SC : 0);
     static constexpr int SMEM_BYTES = TILE_BYTES + SLOTS * TILE_BYTES + RAW * RAW_BYTES + (BITS8 ? SC * SC_FLOATS * 4 + 2 * 128 * 4 : 0) + 3 * 128 * 4 + BARS * 8 + 16;
     static constexpr uint32_t O_COL = 384;                                       // TMEM: S and P of the tiles in turn at 0, 128 and 256
@@ -592,6 +594,14 @@ OA_DEVINL uint64_t tree_word(const TreeAttnArgs& a, const TreeSeq& s, uint64_t s
     return (old | fresh) & low_bits(s.end - key);
 }
 
+// how many tiles of two of a sequence's pages begin below a place of its window
+OA_DEVINL int tiles_below(const TreeSeq& s, int place) {
+    if (place <= 0) return 0;
+    const int page = pages_of(place) - 1;                                        // the last page that begins below it
+    const int c = page < s.low_pages ? page : max(page - s.skip, s.low_pages - 1);
+    return (c + 2) / 2;
+}
+
 template <int D, int FMT>
 __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ TreeAttnArgs a) {
     using Cfg = ManyCfg<D, FMT>;
@@ -599,6 +609,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
     constexpr bool BITS8 = Cfg::BITS8;
     constexpr int KEYS = Cfg::KEYS, HALVES = Cfg::HALVES, HALF = Cfg::HALF, TILE = Cfg::TILE_BYTES, SLOTS = Cfg::SLOTS, RAW = BITS8 ? Cfg::RAW : 1, SC = Cfg::SC, SOFTMAX = 256;
     constexpr int64_t BLOCK_BYTES = CACHE_PAGE * (D + 4);
+    constexpr float kKeyUp = FMT == CACHE_INT8 ? 1.0f / 512.f : 64.f;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* q_s = smem;
     uint8_t* kv_s = q_s + TILE;
@@ -613,19 +624,20 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::BARS);
     __shared__ int64_t sums[Cfg::THREADS / 32];
     __shared__ At start;
+    __shared__ At soft;                                                          // the softmax warps' place, which would cost them registers
     __shared__ float sc_last;                                                    // 8 bits: what the values' scales of a piece's last tile are over
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int grp = a.n_heads / a.n_kv, tile_tokens = 128 / grp;
     if (threadIdx.x == 0) {
         if (!BITS8) { tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_kv); }
-        mbar_init(q_full, BITS8 ? 4 : 1); mbar_init(q_empty, 1);
+        mbar_init(q_full, BITS8 ? Cfg::CONV : 1); mbar_init(q_empty, 1);
         for (int i = 0; i < 3; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
         for (int i = 0; i < 4; ++i) mbar_init(&o_full[i], 1);
-        for (int i = 0; i < SLOTS; ++i) { mbar_init(&full[i], BITS8 ? 4 : 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < SLOTS; ++i) { mbar_init(&full[i], BITS8 ? Cfg::CONV : 1); mbar_init(&empty[i], 1); }
         if (BITS8) {
-            for (int i = 0; i < RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4); }
-            for (int i = 0; i < SC; ++i) { mbar_init(&sc_in[i], 1); mbar_init(&sc_full[i], 1); mbar_init(&sc_empty[i], 4); }
+            for (int i = 0; i < RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], Cfg::CONV); }
+            for (int i = 0; i < SC; ++i) { mbar_init(&sc_in[i], 1); mbar_init(&sc_full[i], 1); mbar_init(&sc_empty[i], 4 + Cfg::CONV); }
         }
         fence_barrier_init();
     }
@@ -633,6 +645,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
     griddep_wait();
     if (warp == 1) tmem_alloc<512>(tmem_slot);
     const TreeShare share = tree_share<Cfg::THREADS>(a, tile_tokens, sums, start);
+    if (threadIdx.x == 0) soft = start;
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
@@ -649,132 +662,192 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
     auto special = [&](int t) { return 2 * t + 1 >= at.s.pages || at.s.special(a, at.s.page(2 * t)) || at.s.special(a, at.s.page(2 * t + 1)); };
 
     // Keys and values share one ring in the order of their products: K_0, K_1, K_2, V_0, K_3, V_1, ..: entry number of V_j is min(tiles, j + 3) + j
-    if constexpr (BITS8) {                                                       // 128 a thread at launch, 512 for four: 88 + 2 x 160 + 96
-        if (warp < 4) reg_dec<88>(); else if (warp < 12) reg_inc<160>(); else reg_dec<96>();
-    }
-    if (warp == 0) {
-        constexpr int RING = BITS8 ? RAW : SLOTS;
-        uint64_t *in = BITS8 ? raw_full : full, *out = BITS8 ? raw_empty : empty;
-        uint32_t n = 0, seg = 0, g = 0;                                          // entries, pieces and tiles loaded
-        for (int64_t u = u_begin; u < u_end; at.next(a)) {
-            take(u);
-            if (c1 == c0) continue;
-            if constexpr (!BITS8) {
-                mbar_wait(q_empty, (seg & 1) ^ 1);
-                if (elect_one()) {                                               // tokens behind the last row are zeros, other sequences' are not looked at
-                    mbar_expect_tx(q_full, HALVES * tile_tokens * grp * 128);
+    // 8 bits: 96 registers a thread at launch, 480 for five warpgroups: 64 + 2 x 136 + 2 x 72.  A warpgroup's split is the same instruction for all of it, in the branch that lives by it
+    if (warp < 4) {
+        if constexpr (BITS8) reg_dec<64>();
+        if (warp == 0) {
+            constexpr int RING = BITS8 ? RAW : SLOTS;
+            uint64_t *in = BITS8 ? raw_full : full, *out = BITS8 ? raw_empty : empty;
+            uint32_t n = 0, seg = 0, g = 0;                                          // entries, pieces and tiles loaded
+            for (int64_t u = u_begin; u < u_end; at.next(a)) {
+                take(u);
+                if (c1 == c0) continue;
+                if constexpr (!BITS8) {
+                    mbar_wait(q_empty, (seg & 1) ^ 1);
+                    if (elect_one()) {                                               // tokens behind the last row are zeros, other sequences' are not looked at
+                        mbar_expect_tx(q_full, HALVES * tile_tokens * grp * 128);
 #pragma unroll
-                    for (int h = 0; h < HALVES; ++h) tma_load_3d(q_s + h * HALF, &tm_q, q_full, h * 64, at.kvh * grp, at.row0(), kEvictNormal);
+                        for (int h = 0; h < HALVES; ++h) tma_load_3d(q_s + h * HALF, &tm_q, q_full, h * 64, at.kvh * grp, at.row0(), kEvictNormal);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
-            }
-            ++seg;
-            const int32_t* table = a.tables + (int64_t)at.seq * a.max_pages;
-            int page[3][2] = {}, have = 0;                                       // pages of this tile and of the two before
-            for (int kt = c0; kt < c1 + 2; ++kt) {
-                if (kt < c1 && (kt == c0 || (kt & 15) == 0)) { const int w = (2 * kt & ~31) + lane; have = w < min(2 * c1, at.s.pages) ? __ldcg(table + at.s.page(w)) : 0; }
+                ++seg;
+                const int32_t* table = a.tables + (int64_t)at.seq * a.max_pages;
+                int page[3][2] = {}, have = 0;                                       // pages of this tile and of the two before
+                for (int kt = c0; kt < c1 + 2; ++kt) {
+                    if (kt < c1 && (kt == c0 || (kt & 15) == 0)) { const int w = (2 * kt & ~31) + lane; have = w < min(2 * c1, at.s.pages) ? __ldcg(table + at.s.page(w)) : 0; }
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    page[2][i] = page[1][i]; page[1][i] = page[0][i];
-                    page[0][i] = __shfl_sync(0xffffffffu, have, (2 * kt + i) & 31);
-                    if (kt >= c1 || 2 * kt + i >= at.s.pages) page[0][i] = 0;
-                    if (page[0][i] < 0 || page[0][i] >= a.num_pages) { if (lane == 0 && a.status) *a.status = 400; page[0][i] = 0; }
-                }
+                    for (int i = 0; i < 2; ++i) {
+                        page[2][i] = page[1][i]; page[1][i] = page[0][i];
+                        page[0][i] = __shfl_sync(0xffffffffu, have, (2 * kt + i) & 31);
+                        if (kt >= c1 || 2 * kt + i >= at.s.pages) page[0][i] = 0;
+                        if (page[0][i] < 0 || page[0][i] >= a.num_pages) { if (lane == 0 && a.status) *a.status = 400; page[0][i] = 0; }
+                    }
 #pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    const int t = kt - 2 * v;                                    // K of this tile, V of the one two before
-                    if (t < c0 || t >= c1) continue;
-                    const int there = min(2, at.s.pages - 2 * t);                // a missing second page is not loaded: its scores are masked, its values set to zero
-                    const uint32_t slot = n % RING;
-                    if (BITS8 && v == 0) {
-                        const uint32_t buf = g % SC;
-                        mbar_wait(&sc_empty[buf], ((g / SC) & 1) ^ 1);
+                    for (int v = 0; v < 2; ++v) {
+                        const int t = kt - 2 * v;                                    // K of this tile, V of the one two before
+                        if (t < c0 || t >= c1) continue;
+                        const int there = min(2, at.s.pages - 2 * t);                // a missing second page is not loaded: its scores are masked, its values set to zero
+                        const uint32_t slot = n % RING;
+                        if (BITS8 && v == 0) {
+                            const uint32_t buf = g % SC;
+                            mbar_wait(&sc_empty[buf], ((g / SC) & 1) ^ 1);
+                            if (elect_one()) {
+                                mbar_expect_tx(&sc_in[buf], there * 2 * CACHE_PAGE * 4);
+#pragma unroll
+                                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                    for (int w = 0; w < 2; ++w)
+                                        if (i < there) bulk_load(sc_s + buf * Cfg::SC_FLOATS + w * KEYS + i * CACHE_PAGE, reinterpret_cast<const uint8_t*>(a.cache) +
+                                                                 ((int64_t)(w * (int64_t)a.num_pages + page[0][i]) * a.n_kv + at.kvh) * BLOCK_BYTES + CACHE_PAGE * D, CACHE_PAGE * 4, &sc_in[buf]);
+                            }
+                            __syncwarp();
+                            ++g;
+                        }
+                        mbar_wait(&out[slot], ((n / RING) & 1) ^ 1);
                         if (elect_one()) {
-                            mbar_expect_tx(&sc_in[buf], there * 2 * CACHE_PAGE * 4);
+                            mbar_expect_tx(&in[slot], there * (BITS8 ? CACHE_PAGE * D : HALVES * 8192));
 #pragma unroll
-                            for (int i = 0; i < 2; ++i)
+                            for (int i = 0; i < 2; ++i) {
+                                if (i >= there) break;
+                                const int64_t block = ((int64_t)v * a.num_pages + (v ? page[2][i] : page[0][i])) * a.n_kv + at.kvh;
+                                if (BITS8) bulk_load(raw_s + slot * Cfg::RAW_BYTES + i * CACHE_PAGE * D, reinterpret_cast<const uint8_t*>(a.cache) + block * BLOCK_BYTES, CACHE_PAGE * D, &in[slot]);
+                                else
 #pragma unroll
-                                for (int w = 0; w < 2; ++w)
-                                    if (i < there) bulk_load(sc_s + buf * Cfg::SC_FLOATS + w * KEYS + i * CACHE_PAGE, reinterpret_cast<const uint8_t*>(a.cache) +
-                                                             ((int64_t)(w * (int64_t)a.num_pages + page[0][i]) * a.n_kv + at.kvh) * BLOCK_BYTES + CACHE_PAGE * D, CACHE_PAGE * 4, &sc_in[buf]);
+                                    for (int h = 0; h < HALVES; ++h) tma_load_2d(kv_s + slot * TILE + h * HALF + i * 8192, &tm_kv, &in[slot], h * 64, (int)(block * CACHE_PAGE), kEvictNormal);
+                            }
                         }
                         __syncwarp();
-                        ++g;
+                        ++n;
                     }
-                    mbar_wait(&out[slot], ((n / RING) & 1) ^ 1);
-                    if (elect_one()) {
-                        mbar_expect_tx(&in[slot], there * (BITS8 ? CACHE_PAGE * D : HALVES * 8192));
+                }
+            }
+        } else if (warp == 1) {
+            // the whole warp walks the loop, an elected lane issues: descriptors stay in uniform registers
+            constexpr uint32_t f16 = BITS8 ? (1u << 7) | (1u << 10) : 0u;            // both operands fp16 instead of bf16
+            constexpr uint32_t idesc_s = umma_idesc_bf16(128, KEYS) ^ f16, idesc_o = umma_idesc_bf16_bmn(128, D) ^ f16;
+            const uint64_t q_desc = umma_desc_sw128(smem_u32(q_s)), k_desc = umma_desc_sw128(smem_u32(kv_s));
+            const uint64_t v_desc = umma_desc_sw128_mn(smem_u32(kv_s), (uint32_t)HALF, 1024u);
+            uint32_t n = 0, r = 0, seg = 0;                                          // tiles of the pieces before, entries of the ring, pieces
+            auto await = [&] {                                                       // the ring's next tile
+                const uint32_t slot = r % SLOTS;
+                mbar_wait(&full[slot], (r / SLOTS) & 1);
+                ++r;
+                tcgen05_fence_after();
+                return slot;
+            };
+            // products of one thread are carried out in the order of their issue: S of a tile goes over scores whose P a product ahead of it reads
+            for (int64_t u = u_begin; u < u_end; at.next(a)) {
+                take(u);
+                const int tiles = c1 - c0;
+                if (tiles == 0) continue;
+                mbar_wait(q_full, seg & 1);
+                ++seg;
+                tcgen05_fence_after();
+                for (int j = -2; j < tiles; ++j) {
+                    if (j + 2 < tiles) {                                             // scores two tiles ahead, under the softmaxes of the tiles before
+                        const uint32_t slot = await(), to = (n + j + 2) % 3;
+                        if (elect_one()) {
+                            const uint64_t b = k_desc + (uint64_t)(slot * (TILE >> 4));
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            if (i >= there) break;
-                            const int64_t block = ((int64_t)v * a.num_pages + (v ? page[2][i] : page[0][i])) * a.n_kv + at.kvh;
-                            if (BITS8) bulk_load(raw_s + slot * Cfg::RAW_BYTES + i * CACHE_PAGE * D, reinterpret_cast<const uint8_t*>(a.cache) + block * BLOCK_BYTES, CACHE_PAGE * D, &in[slot]);
-                            else
-#pragma unroll
-                                for (int h = 0; h < HALVES; ++h) tma_load_2d(kv_s + slot * TILE + h * HALF + i * 8192, &tm_kv, &in[slot], h * 64, (int)(block * CACHE_PAGE), kEvictNormal);
+                            for (int ks = 0; ks < D / 16; ++ks) {
+                                const int half = ks >> 2, in = (ks & 3) * 32;
+                                umma_bf16(tmem_base + to * 128, q_desc + (uint64_t)((half * HALF + in) >> 4), b + (uint64_t)((half * HALF + in) >> 4), idesc_s, ks > 0 ? 1u : 0u);
+                            }
+                            umma_commit(&s_full[to]);
+                            umma_commit(&empty[slot]);
+                            if (j + 3 == tiles) umma_commit(q_empty);
                         }
+                        __syncwarp();
                     }
-                    __syncwarp();
-                    ++n;
+                    if (j >= 0) {
+                        const uint32_t m = n + j, from = m % 3;
+                        mbar_wait(&p_full[from], (m / 3) & 1);
+                        const uint32_t slot = await();
+                        if (elect_one()) {
+                            const uint64_t b = v_desc + (uint64_t)(slot * (TILE >> 4));
+#pragma unroll
+                            for (int ks = 0; ks < KEYS / 16; ++ks)
+                                umma_bf16_ta(tmem_base + Cfg::O_COL, tmem_base + from * 128 + ks * 8, b + (uint64_t)(ks * (2048 >> 4)), idesc_o, (j > 0 || ks > 0) ? 1u : 0u);
+                            umma_commit(&o_full[m & 3]);
+                            umma_commit(&empty[slot]);
+                        }
+                        __syncwarp();
+                    }
+                }
+                n += tiles;
+            }
+        } else if (warp == 2) {
+            // A tile's scales in fp16, twice: keys' over a power of two that none of the tile passes and times 2^6 (int8: 2^-9), values' over one that none of the piece so far passes and times 2^7, which bring the
+            // largest product to 28672 (0.25) and 57344; 0 of what none of the rows sees.  int8 keys u - 128 times s are the fused product u 2^-24 (a subnormal's bits) times s 2^24 less 128 s
+            if constexpr (BITS8) {
+                uint32_t n = 0;
+                for (int64_t u = u_begin; u < u_end; at.next(a)) {
+                    take(u);
+                    if (c1 == c0) continue;
+                    TreeAny any;
+                    any.read(a, at, lane);
+                    float vref = 0.f;
+                    for (int kt = c0; kt < c1; ++kt, ++n) {
+                        const uint32_t buf = n % SC;
+                        float* sc = sc_s + buf * Cfg::SC_FLOATS;
+                        const bool sp = special(kt);
+                        mbar_wait(&sc_in[buf], (n / SC) & 1);
+                        float4 in[2] = {*reinterpret_cast<const float4*>(sc + 4 * lane), *reinterpret_cast<const float4*>(sc + KEYS + 4 * lane)};
+                        uint32_t mask = 0xf;
+                        if (sp) {
+                            const int c = 2 * kt + (lane >> 4);
+                            mask = 0;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) if (c < at.s.pages && any.sees(a, at.s, at.s.page(c) * CACHE_PAGE + (4 * lane & 63) + i)) mask |= 1u << i;
+                        }
+                        float grown = 1.0f, ref[2] = {0.f, vref};
+#pragma unroll
+                        for (int v = 0; v < 2; ++v) {
+                            float x[4] = {in[v].x, in[v].y, in[v].z, in[v].w};
+                            uint32_t top = 0;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if (!(mask >> i & 1)) x[i] = 0.f;
+                                if (fabsf(x[i]) < INFINITY) top = max(top, __float_as_uint(fabsf(x[i])));
+                            }
+                            top = __reduce_max_sync(0xffffffffu, top);
+                            const float need = __uint_as_float(min((top & 0x7f800000u) + 0x00800000u, 0x7e800000u));             // up to 2^126
+                            if (need > ref[v]) { if (ref[v] > 0.f) grown = ref[v] * (1.0f / need); ref[v] = need; }
+                            const float inv = 1.0f / ref[v], up = v ? 128.f : kKeyUp;        // powers of two: exact
+                            uint32_t w[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float y = x[i] * inv * up;
+                                w[i] = pack_f16x2(y, y);
+                                if (!v && FMT == CACHE_INT8) {                       // s 2^24 and -128 s, of the same s
+                                    const float r = __half2float(__float2half_rn(y * 16777216.f));
+                                    w[i] = pack_f16x2(r, r * (-128.f / 16777216.f));
+                                }
+                            }
+                            *reinterpret_cast<uint4*>(sc + v * KEYS + 4 * lane) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                        vref = ref[1];
+                        if (lane == 0) { sc[2 * KEYS] = ref[0] * (1.0f / kKeyUp); sc[2 * KEYS + 1] = grown; sc[2 * KEYS + 2] = vref * (1.0f / 128.f); }
+                        fence_proxy_async();                                         // the next scales to come here are another proxy's writes
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sc_full[buf]);
+                    }
                 }
             }
         }
-    } else if (warp == 1) {
-        // the whole warp walks the loop, an elected lane issues: descriptors stay in uniform registers
-        constexpr uint32_t f16 = BITS8 ? (1u << 7) | (1u << 10) : 0u;            // both operands fp16 instead of bf16
-        constexpr uint32_t idesc_s = umma_idesc_bf16(128, KEYS) ^ f16, idesc_o = umma_idesc_bf16_bmn(128, D) ^ f16;
-        const uint64_t q_desc = umma_desc_sw128(smem_u32(q_s)), k_desc = umma_desc_sw128(smem_u32(kv_s));
-        const uint64_t v_desc = umma_desc_sw128_mn(smem_u32(kv_s), (uint32_t)HALF, 1024u);
-        uint32_t n = 0, r = 0, seg = 0;                                          // tiles of the pieces before, entries of the ring, pieces
-        auto await = [&] {                                                       // the ring's next tile
-            const uint32_t slot = r % SLOTS;
-            mbar_wait(&full[slot], (r / SLOTS) & 1);
-            ++r;
-            tcgen05_fence_after();
-            return slot;
-        };
-        // products of one thread are carried out in the order of their issue: S of a tile goes over scores whose P a product ahead of it reads
-        for (int64_t u = u_begin; u < u_end; at.next(a)) {
-            take(u);
-            const int tiles = c1 - c0;
-            if (tiles == 0) continue;
-            mbar_wait(q_full, seg & 1);
-            ++seg;
-            tcgen05_fence_after();
-            for (int j = -2; j < tiles; ++j) {
-                if (j + 2 < tiles) {                                             // scores two tiles ahead, under the softmaxes of the tiles before
-                    const uint32_t slot = await(), to = (n + j + 2) % 3;
-                    if (elect_one()) {
-                        const uint64_t b = k_desc + (uint64_t)(slot * (TILE >> 4));
-#pragma unroll
-                        for (int ks = 0; ks < D / 16; ++ks) {
-                            const int half = ks >> 2, in = (ks & 3) * 32;
-                            umma_bf16(tmem_base + to * 128, q_desc + (uint64_t)((half * HALF + in) >> 4), b + (uint64_t)((half * HALF + in) >> 4), idesc_s, ks > 0 ? 1u : 0u);
-                        }
-                        umma_commit(&s_full[to]);
-                        umma_commit(&empty[slot]);
-                        if (j + 3 == tiles) umma_commit(q_empty);
-                    }
-                    __syncwarp();
-                }
-                if (j >= 0) {
-                    const uint32_t m = n + j, from = m % 3;
-                    mbar_wait(&p_full[from], (m / 3) & 1);
-                    const uint32_t slot = await();
-                    if (elect_one()) {
-                        const uint64_t b = v_desc + (uint64_t)(slot * (TILE >> 4));
-#pragma unroll
-                        for (int ks = 0; ks < KEYS / 16; ++ks)
-                            umma_bf16_ta(tmem_base + Cfg::O_COL, tmem_base + from * 128 + ks * 8, b + (uint64_t)(ks * (2048 >> 4)), idesc_o, (j > 0 || ks > 0) ? 1u : 0u);
-                        umma_commit(&o_full[m & 3]);
-                        umma_commit(&empty[slot]);
-                    }
-                    __syncwarp();
-                }
-            }
-            n += tiles;
-        }
-    } else if (warp >= 4 && warp < 12) {
+    } else if (warp < 12) {
+        if constexpr (BITS8) reg_inc<136>();
         // Two warpgroups take the tiles in turn, a row a thread: one's exponentials run under the other's loads and maxima.  A row's reference maximum goes from one to the other
         // with each tile, as soon as the tile's own maximum is known; sums stay with either, O is one for both
         const int quarter = warp & 3, row = quarter * 32 + lane;
@@ -787,67 +860,72 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
             if (n & 1) asm volatile("bar.arrive 3, %0;" ::"n"(SOFTMAX) : "memory"); else asm volatile("bar.arrive 4, %0;" ::"n"(SOFTMAX) : "memory");
         };
         constexpr float kRaise = 8.0f;                                           // log2 units a score may pass the reference by
+        constexpr float kLift = BITS8 ? 7.0f : 0.0f;                             // of the weights, which fp16 holds up to 2^16 and with 8 bits down to 2^-17
         constexpr int COLS = D / 2;
         uint32_t n0 = 0, seg = 0;                                                // tiles of the pieces before, pieces
-        for (int64_t u = u_begin; u < u_end; at.next(a)) {
-            take(u);
-            const int64_t end = at.unit0 + at.units();
-            const bool first = at.unit0 >= u_begin, last = end <= u_end;
-            const int live_rows = at.rows(grp), row0 = at.row0(), tiles = c1 - c0;
-            const bool live = row < live_rows;
+        auto advance = [&] { if (threadIdx.x == 128) soft.next(a); meet(); };
+        for (bool more = u_begin < u_end; more; advance()) {
+            int c0, tiles; bool first, last;
+            {
+                const int64_t unit0 = soft.unit0, end = unit0 + soft.units();
+                first = unit0 >= u_begin; last = end <= u_end; more = end < u_end;
+                c0 = (int)max(u_begin - unit0 - TREE_OVER, (int64_t)0);
+                tiles = (int)max((int64_t)0, min((int64_t)soft.steps(), u_end - unit0 - TREE_OVER) - c0);
+                if (threadIdx.x == 128 && first && !last) tree_record(a, cta_of(end - 1, share.busy, share.total) - (int)blockIdx.x, soft.row0(), soft.rows(grp), soft.kvh);
+            }
+            const TreeSeq& s = soft.s;
+            const bool live = row < soft.rows(grp);
             const uint32_t n1 = n0 + tiles;
             uint64_t seen = 0; int low = 0x7fffffff;
-            if (live) { const int t = at.tile * tile_tokens + row / grp; seen = tree_seen(a, at.s, t); low = tree_low(a, at.s, seen, t); }
-            const bool blind = live && !tree_sees(a, at.s, seen, low);
+            if (live) { const int t = soft.tile * tile_tokens + row / grp; seen = tree_seen(a, s, t); low = tree_low(a, s, seen, t); }
+            const bool blind = live && !tree_sees(a, s, seen, low);
             TreeAny any;
-            if (!BITS8) any.read(a, at, lane);
-            if (warp == 4 && lane == 0 && first && !last) tree_record(a, cta_of(end - 1, share.busy, share.total) - (int)blockIdx.x, row0, live_rows, at.kvh);
+            if (!BITS8) any.read(a, soft, lane);
             float* po = a.part_o + ((int64_t)blockIdx.x * 2 + !first) * (128 * D) + row * 4;         // [D / 4][128 rows][4]: a warp's rows lie next to each other
             float2* ml = reinterpret_cast<float2*>(a.part_ml) + ((int64_t)blockIdx.x * 2 + !first) * 128 + row;
             if (tiles == 0) {                                                    // units of the item's own alone
                 if (live)
                     for (int c = wg * COLS; c < (int)(wg + 1) * COLS; c += 4) *reinterpret_cast<float4*>(po + c * 128) = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (live && wg == 0) *ml = make_float2(-INFINITY, first && blind ? -1.f : 0.f);
+                meet();                                                          // everyone has read the place
                 continue;
             }
-            float fac = a.scale_log2e, vref = 1.0f;
-            if (BITS8) { mbar_wait(q_full, seg & 1); fac = factor_s[(seg & 1) * 128 + row] * a.scale_log2e; }
+            // tiles of which some row may not see all: those before s0 and from s1 on
+            const int s1 = s.ctx / CACHE_PAGE < s.skip ? 0 : min((s.ctx / CACHE_PAGE - s.skip) / 2, s.pages / 2), s0 = a.window > 0 ? tiles_below(s, s.ctx + s.n - a.window) : 0;
+            float row_fac = a.scale_log2e, undo = 1.0f;
+            if (BITS8) { mbar_wait(q_full, seg & 1); row_fac = factor_s[(seg & 1) * 128 + row] * a.scale_log2e; }
             ++seg;
             float m_mine = -INFINITY, l_run = 0.f;                               // the sum so far and the reference that it is under
             auto tile = [&](uint32_t n, auto tag) {
                 constexpr bool SPECIAL = decltype(tag)::value;
                 const int kt = c0 + (int)(n - n0);
                 const uint32_t from = n % 3, s_addr = lane_addr + from * 128, buf = n % SC;
-                const float* sc = sc_s + buf * Cfg::SC_FLOATS;
                 uint64_t word[2] = {~0ull, ~0ull};
                 if (SPECIAL) {
-                    word[0] = tree_word(a, at.s, seen, low, at.s.page(2 * kt) * CACHE_PAGE);
-                    word[1] = 2 * kt + 1 < at.s.pages ? tree_word(a, at.s, seen, low, at.s.page(2 * kt + 1) * CACHE_PAGE) : 0ull;
+                    word[0] = tree_word(a, s, seen, low, s.page(2 * kt) * CACHE_PAGE);
+                    word[1] = 2 * kt + 1 < s.pages ? tree_word(a, s, seen, low, s.page(2 * kt + 1) * CACHE_PAGE) : 0ull;
                 }
-                float grown = 1.0f;
-                if (BITS8) { mbar_wait(&sc_full[buf], (n / SC) & 1); vref = sc[2 * KEYS]; grown = sc[2 * KEYS + 1]; }
+                float grown = 1.0f, fac = row_fac;
+                if (BITS8) {
+                    const float* sc = sc_s + buf * Cfg::SC_FLOATS + 2 * KEYS;
+                    mbar_wait(&sc_full[buf], (n / SC) & 1);
+                    fac *= sc[0]; grown = sc[1]; undo = sc[2];
+                }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};     // four chains
                 mbar_wait(&s_full[from], (n / 3) & 1);
                 tcgen05_fence_after();
                 uint32_t v[2][32];
-                auto scores = [&](int k) {                                       // of keys k .. k + 63, their scales in them, -inf where the row does not see
+                auto scores = [&](int k) {                                       // of keys k .. k + 63, -inf where the row does not see
                     tmem_ld_32x32b_x32(s_addr + k, v[0]);
                     tmem_ld_32x32b_x32(s_addr + k + 32, v[1]);
                     tmem_ld_wait();
-                    const uint64_t w = k ? word[1] : word[0];
+                    if (SPECIAL) {
+                        const uint64_t w = k ? word[1] : word[0];
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
+                        for (int c = 0; c < 2; ++c)
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            float4 ks = make_float4(1.f, 1.f, 1.f, 1.f);
-                            if (BITS8) ks = *reinterpret_cast<const float4*>(sc + k + c * 32 + i);
-                            const float f[4] = {ks.x, ks.y, ks.z, ks.w};
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                if (BITS8) v[c][i + e] = __float_as_uint(__uint_as_float(v[c][i + e]) * f[e]);
-                                if (SPECIAL && !((uint32_t)(w >> (c * 32)) >> (i + e) & 1)) v[c][i + e] = 0xff800000u;
-                            }
-                        }
+                            for (int i = 0; i < 32; ++i) if (!((uint32_t)(w >> (c * 32)) >> i & 1)) v[c][i] = 0xff800000u;
+                    }
                 };
 #pragma unroll 1
                 for (int k = KEYS - 64; k >= 0; k -= 64) {                       // the lower keys last: they stay in registers
@@ -862,7 +940,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                 // A barrier's phases are seen one by one: PV of the tile three before is the last one that this tile can be sure of without a wait
                 if (n > 2) mbar_wait(&o_full[(n - 3) & 3], ((n - 3) >> 2) & 1);
                 const float m_last = n > n0 ? m_s[row] : -INFINITY;
-                const bool raise = mx > m_last + kRaise;
+                const bool raise = live && mx > m_last + kRaise;
                 const float m_ref = raise ? mx : m_last;
                 m_s[row] = m_ref;
                 if (n + 1 < n1) pass_turn(n + 1);
@@ -885,41 +963,26 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                     const uint32_t entry = 2 * n0 + min(tiles, kt - c0 + 3) + (kt - c0), slot = entry % SLOTS;
                     mbar_wait(&full[slot], (entry / SLOTS) & 1);
                     const int c = 2 * kt + (row >> 6);
-                    if (c >= at.s.pages || !any.sees(a, at.s, at.s.page(c) * CACHE_PAGE + (row & 63))) {
+                    if (c >= s.pages || !any.sees(a, s, s.page(c) * CACHE_PAGE + (row & 63))) {
 #pragma unroll
                         for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(kv_s + slot * TILE + (c >> 3) * HALF + row * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
                     }
                     fence_proxy_async();
                 }
                 if (m_mine != m_ref) { l_run *= ex2_approx(m_mine - m_ref); m_mine = m_ref; }
-                const float neg_ref = -finite_or_zero(m_ref);
+                const float neg_ref = kLift - finite_or_zero(m_ref);
                 uint64_t sum = 0;
 #pragma unroll 1
                 for (int k = 0; k < KEYS; k += 64) {
                     if (k > 0) scores(k);                                        // read again: P of the keys before lies over their own scores
-                    const uint64_t wk = k ? word[1] : word[0];
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         uint32_t w[16];
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            float4 vs = make_float4(1.f, 1.f, 1.f, 1.f);
-                            if (BITS8) vs = *reinterpret_cast<const float4*>(sc + KEYS + k + c * 32 + 2 * i);
-                            const float f[4] = {vs.x, vs.y, vs.z, vs.w};
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                float x = ex2_approx(fmaf(__uint_as_float(v[c][2 * (i + e)]), fac, neg_ref)), y = ex2_approx(fmaf(__uint_as_float(v[c][2 * (i + e) + 1]), fac, neg_ref));
-                                sum = add_f32x2(sum, pack_f32x2(x, y));
-                                if (BITS8) {
-                                    x *= f[2 * e]; y *= f[2 * e + 1];
-                                    if (SPECIAL) {                               // 0 of a key that the row does not see, whatever its scale
-                                        const uint32_t bits = (uint32_t)(wk >> (c * 32)) >> (2 * (i + e));
-                                        if (!(bits & 1)) x = 0.f;
-                                        if (!(bits & 2)) y = 0.f;
-                                    }
-                                    w[i + e] = pack_f16x2(x, y);
-                                } else w[i + e] = pack_bf16x2(x, y);
-                            }
+                        for (int i = 0; i < 16; ++i) {
+                            const float x = ex2_approx(fmaf(__uint_as_float(v[c][2 * i]), fac, neg_ref)), y = ex2_approx(fmaf(__uint_as_float(v[c][2 * i + 1]), fac, neg_ref));
+                            sum = add_f32x2(sum, pack_f32x2(x, y));
+                            w[i] = BITS8 ? pack_f16x2(x, y) : pack_bf16x2(x, y);
                         }
                         tmem_st_32x32b_x16(s_addr + k / 2 + c * 16, w);
                     }
@@ -932,22 +995,24 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                 l_run += lo + hi;
             };
             for (uint32_t n = n0 + ((n0 ^ wg) & 1); n < n1; n += 2) {
-                if (special(c0 + (int)(n - n0))) tile(n, TrueTag{}); else tile(n, FalseTag{});
+                const int kt = c0 + (int)(n - n0);
+                if (kt < s0 || kt >= s1) tile(n, TrueTag{}); else tile(n, FalseTag{});
             }
             n0 = n1;
             meet();                                                              // the last tile's reference is there
             const float m_ref = m_s[row];
             if (m_mine != m_ref) l_run *= ex2_approx(m_mine - m_ref);
             l_s[wg * 128 + row] = l_run;
-            if (BITS8 && ((n1 - 1) & 1) == wg && row == 0) sc_last = vref;
+            if (BITS8 && ((n1 - 1) & 1) == wg && row == 0) sc_last = undo;
             meet();
-            const float l = l_s[row] + l_s[128 + row], undo = BITS8 ? sc_last * (1.0f / 128.0f) : 1.0f;
+            const float l = l_s[row] + l_s[128 + row];
+            if (BITS8) undo = sc_last;
             mbar_wait(&o_full[(n1 - 1) & 3], ((n1 - 1) >> 2) & 1);
             tcgen05_fence_after();
             const bool whole = first && last;
             const float mult = undo * (whole ? (blind ? 0.f : 1.0f / l) : 1.0f);
             const int token = row / grp;
-            uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(row0 + token) * a.ldo + (int64_t)(at.kvh * grp + row - token * grp) * D;
+            uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(soft.row0() + token) * a.ldo + (int64_t)(soft.kvh * grp + row - token * grp) * D;
 #pragma unroll 1
             for (int c = wg * COLS; c < (int)(wg + 1) * COLS; c += 32) {
                 uint32_t o[32];
@@ -968,55 +1033,20 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                         *reinterpret_cast<float4*>(po + (c + i) * 128) = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
             }
             tcgen05_fence_before();
-            if (live && !whole && wg == 0) *ml = make_float2(m_ref, first && blind ? -1.f : l);
+            if (live && !whole && wg == 0) *ml = make_float2(m_ref - kLift, first && blind ? -1.f : l);
             meet();                                                              // O and the sums may be written again
         }
-    } else if (warp == 2) {
-        // scales of a tile: keys' as they are, values' over a power of two that none so far passes and times 2^7 (a weight is 2^8 at most); 0 of what none of the rows sees
-        if constexpr (BITS8) {
-            uint32_t n = 0;
-            for (int64_t u = u_begin; u < u_end; at.next(a)) {
-                take(u);
-                if (c1 == c0) continue;
-                TreeAny any;
-                any.read(a, at, lane);
-                float vref = 0.f;
-                for (int kt = c0; kt < c1; ++kt, ++n) {
-                    const uint32_t buf = n % SC;
-                    float* sc = sc_s + buf * Cfg::SC_FLOATS;
-                    const bool sp = special(kt);
-                    mbar_wait(&sc_in[buf], (n / SC) & 1);
-                    float4 k4 = *reinterpret_cast<const float4*>(sc + 4 * lane), v4 = *reinterpret_cast<const float4*>(sc + KEYS + 4 * lane);
-                    float k[4] = {k4.x, k4.y, k4.z, k4.w}, v[4] = {v4.x, v4.y, v4.z, v4.w};
-                    uint32_t top = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int c = 2 * kt + (lane >> 4);
-                        if (sp && (c >= at.s.pages || !any.sees(a, at.s, at.s.page(c) * CACHE_PAGE + (4 * lane & 63) + i))) k[i] = v[i] = 0.f;
-                        if (fabsf(v[i]) < INFINITY) top = max(top, __float_as_uint(fabsf(v[i])));
-                    }
-                    top = __reduce_max_sync(0xffffffffu, top);
-                    const float need = __uint_as_float(min((top & 0x7f800000u) + 0x00800000u, 0x7e800000u));             // up to 2^126
-                    float grown = 1.0f;
-                    if (need > vref) { grown = vref > 0.f ? vref * (1.0f / need) : 1.0f; vref = need; }
-                    const float inv = 1.0f / vref;                               // powers of two: exact
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = v[i] * inv * 128.f;
-                    *reinterpret_cast<float4*>(sc + 4 * lane) = make_float4(k[0], k[1], k[2], k[3]);
-                    *reinterpret_cast<float4*>(sc + KEYS + 4 * lane) = make_float4(v[0], v[1], v[2], v[3]);
-                    if (lane == 0) { sc[2 * KEYS] = vref; sc[2 * KEYS + 1] = grown; }
-                    fence_proxy_async();                                         // the next scales to come here are another proxy's writes
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sc_full[buf]);
-                }
-            }
-        }
-    } else if (warp >= 12) {
+    } else {
+        if constexpr (BITS8) reg_dec<72>();
         // queries, then tiles in the ring's order, 16 channels of a key a step
         if constexpr (BITS8) {
             const int w = warp - 12, tid = w * 32 + lane;
-            uint32_t n = 0, seg = 0;
-            for (int64_t u = u_begin; u < u_end; at.next(a)) {
+            // 16 channels of a key a step.  Heads of 128: eight lanes take the lower half of one key and the upper of its neighbour, then the other way round, so that neither loads nor stores meet on a bank
+            constexpr int STEPS = Cfg::RAW_BYTES / 16 / (32 * Cfg::CONV), ROWS = 128 / Cfg::CONV, AHEAD = STEPS < 4 ? STEPS : 4;
+            const int ch = tid % (D / 16);
+            auto key_of = [&](int i) { return D == 128 ? 2 * ((tid >> 3) + 4 * Cfg::CONV * (i >> 1)) + ((ch >> 2) ^ (i & 1)) : (tid >> 2) + 8 * Cfg::CONV * i; };
+            uint32_t n = 0, seg = 0, g = 0;                                      // entries, pieces, tiles of the pieces before
+            for (int64_t u = u_begin; u < u_end; at.next(a), g += c1 - c0) {
                 take(u);
                 const int tiles = c1 - c0;
                 if (tiles == 0) continue;
@@ -1025,7 +1055,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                 mbar_wait(q_empty, (seg & 1) ^ 1);
                 const int live = at.rows(grp);
                 constexpr int W = D / 64;                                        // words of two channels a lane
-                for (int r0 = w * 32; r0 < min(live, w * 32 + 32); r0 += 8) {
+                for (int r0 = w * ROWS; r0 < min(live, w * ROWS + ROWS); r0 += 8) {
                     uint32_t x[8][W];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -1057,42 +1087,61 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_full);
-                for (int kt = 0; kt < tiles + 2; ++kt)
+#pragma unroll 1
+                for (int e = 0; e < 2 * tiles + 4; ++e) {                        // K of a tile, V of the one two before
+                    const int t = (e >> 1) - 2 * (e & 1);
+                    if (t < 0 || t >= tiles) continue;
+                    const uint32_t from = n % RAW, to = n % SLOTS;
+                    const uint32_t* sc = reinterpret_cast<const uint32_t*>(sc_s + (g + t) % SC * Cfg::SC_FLOATS + (e & 1) * KEYS);
+                    mbar_wait(&sc_full[(g + t) % SC], ((g + t) / SC) & 1);
+                    mbar_wait(&raw_full[from], (n / RAW) & 1);
+                    mbar_wait(&empty[to], ((n / SLOTS) & 1) ^ 1);
+                    const uint8_t* src = raw_s + from * Cfg::RAW_BYTES + ch * 16;
+                    uint8_t* dst = kv_s + to * TILE + (ch >> 2) * HALF;
+                    auto convert = [&](auto tag) {
+                    constexpr bool KEY = decltype(tag)::value;
 #pragma unroll
-                    for (int v = 0; v < 2; ++v) {
-                        const int t = kt - 2 * v;
-                        if (t < 0 || t >= tiles) continue;
-                        const uint32_t from = n % RAW, to = n % SLOTS;
-                        const bool sp = v && special(c0 + t);
-                        mbar_wait(&raw_full[from], (n / RAW) & 1);
-                        mbar_wait(&empty[to], ((n / SLOTS) & 1) ^ 1);
-                        const uint8_t* src = raw_s + from * Cfg::RAW_BYTES;
-                        uint8_t* dst = kv_s + to * TILE;
-                        constexpr int STEPS = Cfg::RAW_BYTES / 16 / 128;
+                    for (int h = 0; h < STEPS; h += AHEAD) {                     // loads ahead of their stores
+                        uint4 x[AHEAD]; uint32_t f[AHEAD];
 #pragma unroll
-                        for (int i = 0; i < STEPS; ++i) {
-                            const int c = i * 128 + tid, key = c / (D / 16), ch = c % (D / 16);          // 16 channels from 16 ch on
-                            uint4 x = *reinterpret_cast<const uint4*>(src + c * 16);
+                        for (int i = 0; i < AHEAD; ++i) { x[i] = *reinterpret_cast<const uint4*>(src + key_of(h + i) * D); f[i] = sc[key_of(h + i)]; }
+#pragma unroll
+                        for (int i = 0; i < AHEAD; ++i) {
                             uint32_t y[8];
-                            to_f16<FMT, false>(x.x, y[0], y[1]); to_f16<FMT, false>(x.y, y[2], y[3]); to_f16<FMT, false>(x.z, y[4], y[5]); to_f16<FMT, false>(x.w, y[6], y[7]);
-                            if (sp) {                                            // values that none of the rows sees may be anything, and 0 x inf is not 0
-                                const int pg = 2 * (c0 + t) + (key >> 6);
-                                if (pg >= at.s.pages || !any.sees(a, at.s, at.s.page(pg) * CACHE_PAGE + (key & 63)))
+                            const uint32_t w4[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                            if (FMT == CACHE_INT8 && KEY) {
+                                const uint32_t mul = __byte_perm(f[i], 0, 0x1010), add = __byte_perm(f[i], 0, 0x3232);
 #pragma unroll
-                                    for (int j = 0; j < 8; ++j) y[j] = 0u;
-                            }
-                            const int odd = ch >> 2 & 1;                         // which of the two pieces goes first: eight lanes' stores fall on eight pieces of a line
-                            const uint4 lo = make_uint4(y[0], y[1], y[2], y[3]), hi = make_uint4(y[4], y[5], y[6], y[7]);
-                            uint8_t* line = dst + (ch >> 2) * HALF + key * 128;
-                            const int p = 2 * (ch & 3);
-                            *reinterpret_cast<uint4*>(line + (((p + odd) ^ (key & 7)) << 4)) = odd ? hi : lo;
-                            *reinterpret_cast<uint4*>(line + (((p + 1 - odd) ^ (key & 7)) << 4)) = odd ? lo : hi;
+                                for (int k = 0; k < 4; ++k) {
+                                    const uint32_t u = w4[k] ^ 0x80808080u;
+                                    y[2 * k] = fma_f16x2(__byte_perm(u, 0, 0x4140), mul, add); y[2 * k + 1] = fma_f16x2(__byte_perm(u, 0, 0x4342), mul, add);
+                                }
+                            } else
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    to_f16<FMT, false>(w4[k], y[2 * k], y[2 * k + 1]);
+                                    y[2 * k] = mul_f16x2(y[2 * k], f[i]); y[2 * k + 1] = mul_f16x2(y[2 * k + 1], f[i]);
+                                }
+                            const int key = key_of(h + i);
+                            *reinterpret_cast<uint4*>(dst + key * 128 + (((2 * (ch & 3)) ^ (key & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+                            *reinterpret_cast<uint4*>(dst + key * 128 + (((2 * (ch & 3) + 1) ^ (key & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
                         }
-                        fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) { mbar_arrive(&raw_empty[from]); mbar_arrive(&full[to]); }
-                        ++n;
                     }
+                    };
+                    if (e & 1) convert(FalseTag{}); else convert(TrueTag{});
+                    if ((e & 1) && special(c0 + t))                              // values that none of the rows sees may be anything, and 0 x inf is not 0
+#pragma unroll 1
+                        for (int i = 0; i < STEPS; ++i) {
+                            const int key = key_of(i), pg = 2 * (c0 + t) + (key >> 6);
+                            if (pg < at.s.pages && any.sees(a, at.s, at.s.page(pg) * CACHE_PAGE + (key & 63))) continue;
+                            *reinterpret_cast<uint4*>(dst + key * 128 + (((2 * (ch & 3)) ^ (key & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+                            *reinterpret_cast<uint4*>(dst + key * 128 + (((2 * (ch & 3) + 1) ^ (key & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) { mbar_arrive(&raw_empty[from]); mbar_arrive(&full[to]); if (e & 1) mbar_arrive(&sc_empty[(g + t) % SC]); }
+                    ++n;
+                }
             }
         }
     }

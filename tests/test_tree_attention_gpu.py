@@ -3,7 +3,9 @@ bf16, e4m3 and int8, windows with first tokens that stay visible, rows that see 
 
 Tolerances come from arithmetic.  `U` is 2^-24.  A weight is rounded to bf16 (2^-8) or, over 8 bits, to fp16 (2^-11, and 2^-25 of a unit that is 2^-15 of a power of two above the largest scale)
 for the second product; scores are sums of D products in fp32 and three more factors ((D + 8) U of the sum of |q k|, scaled), which moves a weight by twice that at most (its own, and l's), 2^x by
-2^-21; joining parts rounds a dozen times in fp32; the output rounds once (2^-8)."""
+2^-21; joining parts rounds a dozen times in fp32; the output rounds once (2^-8).
+Over 8 bits, for sequences of more than 16 rows, scales are rounded to fp16 and so are keys and values times them: twice 2^-11 of a value, and of each product of a score; the products' own floor
+is 2^-24 beside a largest scaled key of 2^-3 or more, half a tile's largest: 2^-20 of a score's sum under the largest key."""
 import ctypes as C
 import math
 
@@ -128,7 +130,8 @@ class Batch:
                 p = torch.softmax(torch.einsum("khd,pkd->khp", x, k[see]) * scale, -1)
                 want, size = torch.einsum("khp,pkd->khd", p, v[see]), torch.einsum("khp,pkd->khd", p, v[see].abs())
                 score = torch.einsum("khd,pkd->khp", x.abs(), k[see].abs()).amax(-1, keepdim=True) * scale
-                weight = 2.0 ** -8 if self.fmt == BF16 else 2.0 ** -11
+                many = self.fmt != BF16 and -(-(self.before + self.rows + 2) // len(self.ctx)) * (self.heads // self.n_kv) > 8      # on the safe side of the kernels' border
+                weight = 2.0 ** -8 if self.fmt == BF16 else 2.0 ** -11 + (2.0 ** -10 * (1 + 2 * score) + 2.0 ** -19 * score if many else 0.0)
                 far = 0.0 if self.fmt == BF16 else len(see) * 2.0 ** -39 * v[see].abs().max()
                 tol = size * (weight + 2 * (self.dim + 8) * U * score + 2.0 ** -20 + 16 * U) + far + want.abs() * 2.0 ** -8 * (1 + 2.0 ** -7) + 2.0 ** -133
                 err = (got - want).abs()
