@@ -131,7 +131,8 @@ OA_DEVINL TreeShare tree_share(const TreeAttnArgs& a, int tile_tokens, int64_t* 
     share.begin = first_unit(blockIdx.x, share.busy, share.total); share.end = first_unit(blockIdx.x + 1, share.busy, share.total);
     if (share.begin < share.end && share.begin >= before && share.begin < before + units) {          // one thread
         at.seq = s0; at.unit0 = before;
-        for (at.s.read(a, s0); share.begin >= at.unit0 + at.all_units(a);) { at.unit0 += at.all_units(a); ++at.seq; at.s.read(a, at.seq); }
+        if (s1 - s0 > 1) at.s.read(a, s0);                                               // else it is there already
+        while (share.begin >= at.unit0 + at.all_units(a)) { at.unit0 += at.all_units(a); ++at.seq; at.s.read(a, at.seq); }
         const int item = (int)quotient(share.begin - at.unit0, at.units()), tiles = at.s.tiles(tile_tokens);
         at.unit0 += (int64_t)item * at.units();
         at.kvh = item / tiles; at.tile = item - at.kvh * tiles;
@@ -551,6 +552,27 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
 // 128 rows of an item (as many tokens' heads of a group as fit) x 128 keys a tile: S = Q K^T in three TMEM buffers, two tiles ahead, P over S's own columns as the second product's operand, O in
 // TMEM.  Two softmax warpgroups take the tiles in turn, one row a thread; the reference maximum rises (and O is rescaled) only where a score passes it by 2^8.  Over 8 bits four warps turn tiles (and
 // an item's queries) into fp16 under the swizzle that the products read, and one brings the scales of a tile's values under one power of two.
+struct TrueTag { static constexpr bool value = true; };
+struct FalseTag { static constexpr bool value = false; };
+constexpr int TREE_OVER = 2;                                                     // tiles that an item's beginning and end cost
+
+// what any row of an item sees: bits of new tokens, and the first cached place of the widest window
+struct TreeAny {
+    uint64_t seen; int low;
+    OA_DEVINL bool sees(const TreeAttnArgs& a, const TreeSeq& s, int key) const {
+        const int n = key - s.ctx;
+        return n < 0 ? key < a.sinks || key >= low : key < s.end && n < 64 && (seen >> (n & 63) & 1);
+    }
+};
+// A CTA's piece of an item: key tiles c0 .. c1 - 1 (none where its units are the item's own alone), of which those before s0 and from s1 on have places that some row may not see; what each row sees.  Made
+// by a warp of its own, a piece ahead of the others: each of its looks into the arrays is a latency of L2
+struct TreePiece {
+    uint64_t seen[128]; int low[128];
+    TreeSeq s; TreeAny any;
+    int c0, c1, s0, s1, seq, kvh, row0, rows;
+    bool first, last, more;                                                      // the CTA has the item's begin, its end; another piece follows
+};
+
 template <int D, int FMT>
 struct ManyCfg {
     static constexpr bool BITS8 = FMT != CACHE_BF16;
@@ -558,32 +580,10 @@ struct ManyCfg {
     static constexpr int TILE_BYTES = HALVES * HALF, SLOTS = BITS8 ? (D == 128 ? 3 : 4) : D == 128 ? 5 : 8;
     static constexpr int RAW_BYTES = KEYS * D, RAW = BITS8 ? (D == 128 ? 5 : 8) : 0;         // a tile of 8 bits, and how many wait
     static constexpr int SC = 8, SC_FLOATS = 2 * KEYS + 4;                       // tiles whose scales wait: keys', values', what scores are multiplied by, what O is for larger scales of values and at its end
-    static constexpr int CONV = BITS8 ? 8 : 0, THREADS = 128 + 256 + 32 * CONV;     // producer, issuer, scales; eight softmax warps; warps that convert
-    static constexpr int BARS = 12 + 2 * SLOTS + 2 * RAW + (BITS8 ? 3 * SC : 0);
-    static constexpr int SMEM_BYTES = TILE_BYTES + SLOTS * TILE_BYTES + RAW * RAW_BYTES + (BITS8 ? SC * SC_FLOATS * 4 + 2 * 128 * 4 : 0) + 3 * 128 * 4 + BARS * 8 + 16;
+    static constexpr int CONV = BITS8 ? 8 : 0, THREADS = 128 + 256 + 32 * CONV;     // producer, issuer, scales, pieces; eight softmax warps; warps that convert
+    static constexpr int BARS = 16 + 2 * SLOTS + 2 * RAW + (BITS8 ? 3 * SC : 0);
+    static constexpr int SMEM_BYTES = TILE_BYTES + SLOTS * TILE_BYTES + RAW * RAW_BYTES + (BITS8 ? SC * SC_FLOATS * 4 + 2 * 128 * 4 : 0) + 3 * 128 * 4 + BARS * 8 + 16 + 2 * sizeof(TreePiece);
     static constexpr uint32_t O_COL = 384;                                       // TMEM: S and P of the tiles in turn at 0, 128 and 256
-};
-struct TrueTag { static constexpr bool value = true; };
-struct FalseTag { static constexpr bool value = false; };
-constexpr int TREE_OVER = 2;                                                     // tiles that an item's beginning and end cost
-
-// what any row of an item sees: bits of new tokens, and the first cached place of the widest window.  By a whole warp
-struct TreeAny {
-    uint64_t seen; int low;
-    template <typename At>
-    OA_DEVINL void read(const TreeAttnArgs& a, const At& at, int lane) {
-        const int t0 = at.tile * at.tile_tokens, count = min(at.tile_tokens, at.s.n - t0);
-        uint64_t any = 0; int lo = 0x7fffffff;
-#pragma unroll
-        for (int i = 0; i < 64; i += 32)
-            if (lane + i < count) { const uint64_t x = tree_seen(a, at.s, t0 + lane + i); any |= x; lo = min(lo, tree_low(a, at.s, x, t0 + lane + i)); }
-        seen = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(any >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)any);
-        low = __reduce_min_sync(0xffffffffu, lo);
-    }
-    OA_DEVINL bool sees(const TreeAttnArgs& a, const TreeSeq& s, int key) const {
-        const int n = key - s.ctx;
-        return n < 0 ? key < a.sinks || key >= low : key < s.end && n < 64 && (seen >> (n & 63) & 1);
-    }
 };
 OA_DEVINL uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 // which of the 64 places from `key` on a row sees
@@ -620,11 +620,11 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
     float* l_s = m_s + 128;
     uint64_t* bars = reinterpret_cast<uint64_t*>(l_s + 256);
     uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_full = bars + 5, *o_full = bars + 8, *full = bars + 12, *empty = full + SLOTS;
-    uint64_t *raw_full = empty + SLOTS, *raw_empty = raw_full + Cfg::RAW, *sc_in = raw_empty + Cfg::RAW, *sc_full = sc_in + SC, *sc_empty = sc_full + SC;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::BARS);
+    uint64_t *piece_full = empty + SLOTS, *piece_empty = piece_full + 2, *raw_full = piece_empty + 2, *raw_empty = raw_full + Cfg::RAW, *sc_in = raw_empty + Cfg::RAW, *sc_full = sc_in + SC, *sc_empty = sc_full + SC;
+    TreePiece* piece_s = reinterpret_cast<TreePiece*>(bars + Cfg::BARS);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(piece_s + 2);
     __shared__ int64_t sums[Cfg::THREADS / 32];
     __shared__ At start;
-    __shared__ At soft;                                                          // the softmax warps' place, which would cost them registers
     __shared__ float sc_last;                                                    // 8 bits: what the values' scales of a piece's last tile are over
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -634,6 +634,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
         mbar_init(q_full, BITS8 ? Cfg::CONV : 1); mbar_init(q_empty, 1);
         for (int i = 0; i < 3; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
         for (int i = 0; i < 4; ++i) mbar_init(&o_full[i], 1);
+        for (int i = 0; i < 2; ++i) { mbar_init(&piece_full[i], 1); mbar_init(&piece_empty[i], BITS8 ? 11 + Cfg::CONV : 10); }
         for (int i = 0; i < SLOTS; ++i) { mbar_init(&full[i], BITS8 ? Cfg::CONV : 1); mbar_init(&empty[i], 1); }
         if (BITS8) {
             for (int i = 0; i < RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], Cfg::CONV); }
@@ -645,21 +646,24 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
     griddep_wait();
     if (warp == 1) tmem_alloc<512>(tmem_slot);
     const TreeShare share = tree_share<Cfg::THREADS>(a, tile_tokens, sums, start);
-    if (threadIdx.x == 0) soft = start;
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     const int64_t u_begin = share.begin, u_end = share.end;
-    At at;
-    if (u_begin < u_end) at = start;
-    // a CTA's piece of an item: key tiles c0 .. c1 - 1, none where its units are the item's own alone
-    int c0 = 0, c1 = 0;
-    auto take = [&](int64_t& u) {
-        c0 = (int)max(u - at.unit0 - TREE_OVER, (int64_t)0); c1 = (int)max((int64_t)c0, min((int64_t)at.steps(), u_end - at.unit0 - TREE_OVER));
-        u = min(at.unit0 + at.units(), u_end);
+    // what a warp does with each piece; p lies in shared memory until it is done
+    auto pieces = [&](auto&& work) {
+        if (u_begin >= u_end) return;
+        for (uint32_t k = 0;; ++k) {
+            mbar_wait(&piece_full[k & 1], (k >> 1) & 1);
+            const TreePiece& p = piece_s[k & 1];
+            const bool more = p.more;
+            work(p);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&piece_empty[k & 1]);
+            if (!more) return;
+        }
     };
-    auto special = [&](int t) { return 2 * t + 1 >= at.s.pages || at.s.special(a, at.s.page(2 * t)) || at.s.special(a, at.s.page(2 * t + 1)); };
 
     // Keys and values share one ring in the order of their products: K_0, K_1, K_2, V_0, K_3, V_1, ..: entry number of V_j is min(tiles, j + 3) + j
     // 8 bits: 96 registers a thread at launch, 480 for five warpgroups: 64 + 2 x 136 + 2 x 72.  A warpgroup's split is the same instruction for all of it, in the branch that lives by it
@@ -669,58 +673,68 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
             constexpr int RING = BITS8 ? RAW : SLOTS;
             uint64_t *in = BITS8 ? raw_full : full, *out = BITS8 ? raw_empty : empty;
             uint32_t n = 0, seg = 0, g = 0;                                          // entries, pieces and tiles loaded
-            for (int64_t u = u_begin; u < u_end; at.next(a)) {
-                take(u);
-                if (c1 == c0) continue;
+            pieces([&](const TreePiece& p) {
+                const int c0 = p.c0, c1 = p.c1;
+                if (c1 == c0) return;
                 if constexpr (!BITS8) {
                     mbar_wait(q_empty, (seg & 1) ^ 1);
                     if (elect_one()) {                                               // tokens behind the last row are zeros, other sequences' are not looked at
                         mbar_expect_tx(q_full, HALVES * tile_tokens * grp * 128);
 #pragma unroll
-                        for (int h = 0; h < HALVES; ++h) tma_load_3d(q_s + h * HALF, &tm_q, q_full, h * 64, at.kvh * grp, at.row0(), kEvictNormal);
+                        for (int h = 0; h < HALVES; ++h) tma_load_3d(q_s + h * HALF, &tm_q, q_full, h * 64, p.kvh * grp, p.row0, kEvictNormal);
                     }
                     __syncwarp();
                 }
                 ++seg;
-                const int32_t* table = a.tables + (int64_t)at.seq * a.max_pages;
-                int page[3][2] = {}, have = 0;                                       // pages of this tile and of the two before
+                const int32_t* table = a.tables + (int64_t)p.seq * a.max_pages;
+                int page[3][2] = {}, have = 0, later = 0, scales = c0;               // pages of this tile and of the two before
                 for (int kt = c0; kt < c1 + 2; ++kt) {
-                    if (kt < c1 && (kt == c0 || (kt & 15) == 0)) { const int w = (2 * kt & ~31) + lane; have = w < min(2 * c1, at.s.pages) ? __ldcg(table + at.s.page(w)) : 0; }
+                    if (kt < c1 && (kt == c0 || (kt & 15) == 0)) {                   // 32 page numbers, and the next 32 on their way
+                        const int w = (2 * kt & ~31) + lane, stop = min(2 * c1, p.s.pages);
+                        have = kt > c0 ? later : w < stop ? __ldcg(table + p.s.page(w)) : 0;
+                        later = w + 32 < stop ? __ldcg(table + p.s.page(w + 32)) : 0;
+                    }
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         page[2][i] = page[1][i]; page[1][i] = page[0][i];
                         page[0][i] = __shfl_sync(0xffffffffu, have, (2 * kt + i) & 31);
-                        if (kt >= c1 || 2 * kt + i >= at.s.pages) page[0][i] = 0;
+                        if (kt >= c1 || 2 * kt + i >= p.s.pages) page[0][i] = 0;
                         if (page[0][i] < 0 || page[0][i] >= a.num_pages) { if (lane == 0 && a.status) *a.status = 400; page[0][i] = 0; }
+                    }
+                    if constexpr (BITS8) {
+                        for (; scales < min(kt + 4, c1); ++scales, ++g) {            // scales go through a warp of their own first: they come early
+                            const uint32_t buf = g % SC;
+                            const int some = min(2, p.s.pages - 2 * scales);
+                            mbar_wait(&sc_empty[buf], ((g / SC) & 1) ^ 1);
+                            if (elect_one()) mbar_expect_tx(&sc_in[buf], some * 2 * CACHE_PAGE * 4);
+                            __syncwarp();
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                if (i >= some) break;
+                                int pg = __shfl_sync(0xffffffffu, (scales >> 4) == (kt >> 4) ? have : later, (2 * scales + i) & 31);
+                                if (pg < 0 || pg >= a.num_pages) pg = 0;
+                                if (elect_one()) {
+                                    for (int w = 0; w < 2; ++w)
+                                        bulk_load(sc_s + buf * Cfg::SC_FLOATS + w * KEYS + i * CACHE_PAGE, reinterpret_cast<const uint8_t*>(a.cache) +
+                                                  ((int64_t)(w * (int64_t)a.num_pages + pg) * a.n_kv + p.kvh) * BLOCK_BYTES + CACHE_PAGE * D, CACHE_PAGE * 4, &sc_in[buf]);
+                                }
+                                __syncwarp();
+                            }
+                        }
                     }
 #pragma unroll
                     for (int v = 0; v < 2; ++v) {
                         const int t = kt - 2 * v;                                    // K of this tile, V of the one two before
                         if (t < c0 || t >= c1) continue;
-                        const int there = min(2, at.s.pages - 2 * t);                // a missing second page is not loaded: its scores are masked, its values set to zero
+                        const int there = min(2, p.s.pages - 2 * t);                // a missing second page is not loaded: its scores are masked, its values set to zero
                         const uint32_t slot = n % RING;
-                        if (BITS8 && v == 0) {
-                            const uint32_t buf = g % SC;
-                            mbar_wait(&sc_empty[buf], ((g / SC) & 1) ^ 1);
-                            if (elect_one()) {
-                                mbar_expect_tx(&sc_in[buf], there * 2 * CACHE_PAGE * 4);
-#pragma unroll
-                                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                                    for (int w = 0; w < 2; ++w)
-                                        if (i < there) bulk_load(sc_s + buf * Cfg::SC_FLOATS + w * KEYS + i * CACHE_PAGE, reinterpret_cast<const uint8_t*>(a.cache) +
-                                                                 ((int64_t)(w * (int64_t)a.num_pages + page[0][i]) * a.n_kv + at.kvh) * BLOCK_BYTES + CACHE_PAGE * D, CACHE_PAGE * 4, &sc_in[buf]);
-                            }
-                            __syncwarp();
-                            ++g;
-                        }
                         mbar_wait(&out[slot], ((n / RING) & 1) ^ 1);
                         if (elect_one()) {
                             mbar_expect_tx(&in[slot], there * (BITS8 ? CACHE_PAGE * D : HALVES * 8192));
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
                                 if (i >= there) break;
-                                const int64_t block = ((int64_t)v * a.num_pages + (v ? page[2][i] : page[0][i])) * a.n_kv + at.kvh;
+                                const int64_t block = ((int64_t)v * a.num_pages + (v ? page[2][i] : page[0][i])) * a.n_kv + p.kvh;
                                 if (BITS8) bulk_load(raw_s + slot * Cfg::RAW_BYTES + i * CACHE_PAGE * D, reinterpret_cast<const uint8_t*>(a.cache) + block * BLOCK_BYTES, CACHE_PAGE * D, &in[slot]);
                                 else
 #pragma unroll
@@ -731,7 +745,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                         ++n;
                     }
                 }
-            }
+            });
         } else if (warp == 1) {
             // the whole warp walks the loop, an elected lane issues: descriptors stay in uniform registers
             constexpr uint32_t f16 = BITS8 ? (1u << 7) | (1u << 10) : 0u;            // both operands fp16 instead of bf16
@@ -747,10 +761,9 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                 return slot;
             };
             // products of one thread are carried out in the order of their issue: S of a tile goes over scores whose P a product ahead of it reads
-            for (int64_t u = u_begin; u < u_end; at.next(a)) {
-                take(u);
-                const int tiles = c1 - c0;
-                if (tiles == 0) continue;
+            pieces([&](const TreePiece& p) {
+                const int tiles = p.c1 - p.c0;
+                if (tiles == 0) return;
                 mbar_wait(q_full, seg & 1);
                 ++seg;
                 tcgen05_fence_after();
@@ -786,22 +799,19 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                     }
                 }
                 n += tiles;
-            }
+            });
         } else if (warp == 2) {
             // A tile's scales in fp16, twice: keys' over a power of two that none of the tile passes and times 2^6 (int8: 2^-9), values' over one that none of the piece so far passes and times 2^7, which bring the
             // largest product to 28672 (0.25) and 57344; 0 of what none of the rows sees.  int8 keys u - 128 times s are the fused product u 2^-24 (a subnormal's bits) times s 2^24 less 128 s
             if constexpr (BITS8) {
                 uint32_t n = 0;
-                for (int64_t u = u_begin; u < u_end; at.next(a)) {
-                    take(u);
-                    if (c1 == c0) continue;
-                    TreeAny any;
-                    any.read(a, at, lane);
+                pieces([&](const TreePiece& p) {
+                    const int c0 = p.c0, c1 = p.c1;
                     float vref = 0.f;
                     for (int kt = c0; kt < c1; ++kt, ++n) {
                         const uint32_t buf = n % SC;
                         float* sc = sc_s + buf * Cfg::SC_FLOATS;
-                        const bool sp = special(kt);
+                        const bool sp = kt < p.s0 || kt >= p.s1;
                         mbar_wait(&sc_in[buf], (n / SC) & 1);
                         float4 in[2] = {*reinterpret_cast<const float4*>(sc + 4 * lane), *reinterpret_cast<const float4*>(sc + KEYS + 4 * lane)};
                         uint32_t mask = 0xf;
@@ -809,7 +819,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                             const int c = 2 * kt + (lane >> 4);
                             mask = 0;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) if (c < at.s.pages && any.sees(a, at.s, at.s.page(c) * CACHE_PAGE + (4 * lane & 63) + i)) mask |= 1u << i;
+                            for (int i = 0; i < 4; ++i) if (c < p.s.pages && p.any.sees(a, p.s, p.s.page(c) * CACHE_PAGE + (4 * lane & 63) + i)) mask |= 1u << i;
                         }
                         float grown = 1.0f, ref[2] = {0.f, vref};
 #pragma unroll
@@ -843,7 +853,40 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sc_full[buf]);
                     }
+                });
+            }
+        } else {
+            At at;
+            at = start;
+            uint32_t k = 0;
+            for (int64_t u = u_begin; u < u_end; at.next(a), ++k) {
+                const int64_t end = at.unit0 + at.units();
+                const int c0 = (int)max(u - at.unit0 - TREE_OVER, (int64_t)0), c1 = (int)max((int64_t)c0, min((int64_t)at.steps(), u_end - at.unit0 - TREE_OVER));
+                u = min(end, u_end);
+                mbar_wait(&piece_empty[k & 1], ((k >> 1) & 1) ^ 1);
+                TreePiece& p = piece_s[k & 1];
+                const int rows = at.rows(grp);
+                uint64_t any = 0; int lowest = 0x7fffffff;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = i * 32 + lane;
+                    uint64_t seen = 0; int low = 0x7fffffff;
+                    if (r < rows) { const int t = at.tile * tile_tokens + r / grp; seen = tree_seen(a, at.s, t); low = tree_low(a, at.s, seen, t); }
+                    p.seen[r] = seen; p.low[r] = low;
+                    any |= seen; lowest = min(lowest, low);
                 }
+                any = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(any >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)any);
+                lowest = __reduce_min_sync(0xffffffffu, lowest);
+                if (lane == 0) {
+                    const TreeSeq& s = at.s;
+                    p.s = s; p.any.seen = any; p.any.low = lowest;
+                    p.c0 = c0; p.c1 = c1; p.seq = at.seq; p.kvh = at.kvh; p.row0 = at.row0(); p.rows = rows;
+                    p.s0 = a.window > 0 ? tiles_below(s, s.ctx + s.n - a.window) : 0; p.s1 = min((s.ctx / CACHE_PAGE - s.skip) / 2, s.pages / 2);
+                    p.first = at.unit0 >= u_begin; p.last = end <= u_end; p.more = end < u_end;
+                    if (p.first && !p.last) tree_record(a, cta_of(end - 1, share.busy, share.total) - (int)blockIdx.x, p.row0, rows, p.kvh);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&piece_full[k & 1]);
             }
         }
     } else if (warp < 12) {
@@ -863,35 +906,21 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
         constexpr float kLift = BITS8 ? 7.0f : 0.0f;                             // of the weights, which fp16 holds up to 2^16 and with 8 bits down to 2^-17
         constexpr int COLS = D / 2;
         uint32_t n0 = 0, seg = 0;                                                // tiles of the pieces before, pieces
-        auto advance = [&] { if (threadIdx.x == 128) soft.next(a); meet(); };
-        for (bool more = u_begin < u_end; more; advance()) {
-            int c0, tiles; bool first, last;
-            {
-                const int64_t unit0 = soft.unit0, end = unit0 + soft.units();
-                first = unit0 >= u_begin; last = end <= u_end; more = end < u_end;
-                c0 = (int)max(u_begin - unit0 - TREE_OVER, (int64_t)0);
-                tiles = (int)max((int64_t)0, min((int64_t)soft.steps(), u_end - unit0 - TREE_OVER) - c0);
-                if (threadIdx.x == 128 && first && !last) tree_record(a, cta_of(end - 1, share.busy, share.total) - (int)blockIdx.x, soft.row0(), soft.rows(grp), soft.kvh);
-            }
-            const TreeSeq& s = soft.s;
-            const bool live = row < soft.rows(grp);
+        pieces([&](const TreePiece& p) {
+            const TreeSeq& s = p.s;
+            const int c0 = p.c0, tiles = p.c1 - p.c0;
+            const bool live = row < p.rows, first = p.first;
             const uint32_t n1 = n0 + tiles;
-            uint64_t seen = 0; int low = 0x7fffffff;
-            if (live) { const int t = soft.tile * tile_tokens + row / grp; seen = tree_seen(a, s, t); low = tree_low(a, s, seen, t); }
+            const uint64_t seen = p.seen[row]; const int low = p.low[row];
             const bool blind = live && !tree_sees(a, s, seen, low);
-            TreeAny any;
-            if (!BITS8) any.read(a, soft, lane);
             float* po = a.part_o + ((int64_t)blockIdx.x * 2 + !first) * (128 * D) + row * 4;         // [D / 4][128 rows][4]: a warp's rows lie next to each other
             float2* ml = reinterpret_cast<float2*>(a.part_ml) + ((int64_t)blockIdx.x * 2 + !first) * 128 + row;
             if (tiles == 0) {                                                    // units of the item's own alone
                 if (live)
                     for (int c = wg * COLS; c < (int)(wg + 1) * COLS; c += 4) *reinterpret_cast<float4*>(po + c * 128) = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (live && wg == 0) *ml = make_float2(-INFINITY, first && blind ? -1.f : 0.f);
-                meet();                                                          // everyone has read the place
-                continue;
+                return;
             }
-            // tiles of which some row may not see all: those before s0 and from s1 on
-            const int s1 = s.ctx / CACHE_PAGE < s.skip ? 0 : min((s.ctx / CACHE_PAGE - s.skip) / 2, s.pages / 2), s0 = a.window > 0 ? tiles_below(s, s.ctx + s.n - a.window) : 0;
             float row_fac = a.scale_log2e, undo = 1.0f;
             if (BITS8) { mbar_wait(q_full, seg & 1); row_fac = factor_s[(seg & 1) * 128 + row] * a.scale_log2e; }
             ++seg;
@@ -963,7 +992,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                     const uint32_t entry = 2 * n0 + min(tiles, kt - c0 + 3) + (kt - c0), slot = entry % SLOTS;
                     mbar_wait(&full[slot], (entry / SLOTS) & 1);
                     const int c = 2 * kt + (row >> 6);
-                    if (c >= s.pages || !any.sees(a, s, s.page(c) * CACHE_PAGE + (row & 63))) {
+                    if (c >= s.pages || !p.any.sees(a, s, s.page(c) * CACHE_PAGE + (row & 63))) {
 #pragma unroll
                         for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(kv_s + slot * TILE + (c >> 3) * HALF + row * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
                     }
@@ -996,7 +1025,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
             };
             for (uint32_t n = n0 + ((n0 ^ wg) & 1); n < n1; n += 2) {
                 const int kt = c0 + (int)(n - n0);
-                if (kt < s0 || kt >= s1) tile(n, TrueTag{}); else tile(n, FalseTag{});
+                if (kt < p.s0 || kt >= p.s1) tile(n, TrueTag{}); else tile(n, FalseTag{});
             }
             n0 = n1;
             meet();                                                              // the last tile's reference is there
@@ -1009,10 +1038,10 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
             if (BITS8) undo = sc_last;
             mbar_wait(&o_full[(n1 - 1) & 3], ((n1 - 1) >> 2) & 1);
             tcgen05_fence_after();
-            const bool whole = first && last;
+            const bool whole = first && p.last;
             const float mult = undo * (whole ? (blind ? 0.f : 1.0f / l) : 1.0f);
             const int token = row / grp;
-            uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(soft.row0() + token) * a.ldo + (int64_t)(soft.kvh * grp + row - token * grp) * D;
+            uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(p.row0 + token) * a.ldo + (int64_t)(p.kvh * grp + row - token * grp) * D;
 #pragma unroll 1
             for (int c = wg * COLS; c < (int)(wg + 1) * COLS; c += 32) {
                 uint32_t o[32];
@@ -1035,7 +1064,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
             tcgen05_fence_before();
             if (live && !whole && wg == 0) *ml = make_float2(m_ref - kLift, first && blind ? -1.f : l);
             meet();                                                              // O and the sums may be written again
-        }
+        });
     } else {
         if constexpr (BITS8) reg_dec<72>();
         // queries, then tiles in the ring's order, 16 channels of a key a step
@@ -1046,42 +1075,35 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
             const int ch = tid % (D / 16);
             auto key_of = [&](int i) { return D == 128 ? 2 * ((tid >> 3) + 4 * Cfg::CONV * (i >> 1)) + ((ch >> 2) ^ (i & 1)) : (tid >> 2) + 8 * Cfg::CONV * i; };
             uint32_t n = 0, seg = 0, g = 0;                                      // entries, pieces, tiles of the pieces before
-            for (int64_t u = u_begin; u < u_end; at.next(a), g += c1 - c0) {
-                take(u);
-                const int tiles = c1 - c0;
-                if (tiles == 0) continue;
-                TreeAny any;
-                any.read(a, at, lane);
-                mbar_wait(q_empty, (seg & 1) ^ 1);
-                const int live = at.rows(grp);
+            pieces([&](const TreePiece& p) {
+                const int c0 = p.c0, tiles = p.c1 - c0, live = p.rows;
+                if (tiles == 0) return;
                 constexpr int W = D / 64;                                        // words of two channels a lane
-                for (int r0 = w * ROWS; r0 < min(live, w * ROWS + ROWS); r0 += 8) {
-                    uint32_t x[8][W];
+                uint32_t x[ROWS][W];                                             // rows of the warp, ahead of the wait
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = r0 + i, token = r / grp;
-                        const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(at.row0() + token) * a.ldq + (int64_t)(at.kvh * grp + r - token * grp) * D + lane * 2 * W;
-                        if (r < live) {
-                            if (W == 2) { const uint2 y = __ldcg(reinterpret_cast<const uint2*>(src)); x[i][0] = y.x; x[i][W - 1] = y.y; } else x[i][0] = __ldcg(reinterpret_cast<const uint32_t*>(src));
-                        } else
+                for (int i = 0; i < ROWS; ++i) {
+                    const int r = w * ROWS + i, token = r / grp;
+                    const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(p.row0 + token) * a.ldq + (int64_t)(p.kvh * grp + r - token * grp) * D + lane * 2 * W;
 #pragma unroll
-                            for (int j = 0; j < W; ++j) x[i][j] = 0u;
-                    }
+                    for (int j = 0; j < W; ++j) x[i][j] = 0u;
+                    if (r < live) { if (W == 2) { const uint2 y = __ldcg(reinterpret_cast<const uint2*>(src)); x[i][0] = y.x; x[i][W - 1] = y.y; } else x[i][0] = __ldcg(reinterpret_cast<const uint32_t*>(src)); }
+                }
+                mbar_wait(q_empty, (seg & 1) ^ 1);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = r0 + i;
-                        uint32_t top = 0;
+                for (int i = 0; i < ROWS; ++i) {
+                    const int r = w * ROWS + i;
+                    if (r >= live) break;
+                    uint32_t top = 0;
 #pragma unroll
-                        for (int j = 0; j < W; ++j) top = max(top, max(x[i][j] << 16 & 0x7fffffffu, x[i][j] & 0x7fff0000u));
-                        top = __reduce_max_sync(0xffffffffu, top);
-                        const int e = top >= 0x7f800000u ? 14 : max((int)(top >> 23) - 127, -100);       // not finite: as it is
-                        const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
-                        const int ch = lane * 2 * W;
+                    for (int j = 0; j < W; ++j) top = max(top, max(x[i][j] << 16 & 0x7fffffffu, x[i][j] & 0x7fff0000u));
+                    top = __reduce_max_sync(0xffffffffu, top);
+                    const int e = top >= 0x7f800000u ? 14 : max((int)(top >> 23) - 127, -100);           // not finite: as it is
+                    const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+                    const int c = lane * 2 * W;
 #pragma unroll
-                        for (int j = 0; j < W; ++j)
-                            *reinterpret_cast<uint32_t*>(q_s + (ch >> 6) * HALF + r * 128 + ((((ch & 63) >> 3) ^ (r & 7)) << 4) + (ch & 7) * 2 + j * 4) = pack_f16x2(bf16lo(x[i][j]) * up, bf16hi(x[i][j]) * up);
-                        if (lane == 0) factor_s[(seg & 1) * 128 + r] = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
-                    }
+                    for (int j = 0; j < W; ++j)
+                        *reinterpret_cast<uint32_t*>(q_s + (c >> 6) * HALF + r * 128 + ((((c & 63) >> 3) ^ (r & 7)) << 4) + (c & 7) * 2 + j * 4) = pack_f16x2(bf16lo(x[i][j]) * up, bf16hi(x[i][j]) * up);
+                    if (lane == 0) factor_s[(seg & 1) * 128 + r] = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
                 }
                 ++seg;
                 fence_proxy_async();
@@ -1093,7 +1115,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                     if (t < 0 || t >= tiles) continue;
                     const uint32_t from = n % RAW, to = n % SLOTS;
                     const uint32_t* sc = reinterpret_cast<const uint32_t*>(sc_s + (g + t) % SC * Cfg::SC_FLOATS + (e & 1) * KEYS);
-                    mbar_wait(&sc_full[(g + t) % SC], ((g + t) / SC) & 1);
+                    if (!(e & 1)) mbar_wait(&sc_full[(g + t) % SC], ((g + t) / SC) & 1);
                     mbar_wait(&raw_full[from], (n / RAW) & 1);
                     mbar_wait(&empty[to], ((n / SLOTS) & 1) ^ 1);
                     const uint8_t* src = raw_s + from * Cfg::RAW_BYTES + ch * 16;
@@ -1129,11 +1151,11 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                     }
                     };
                     if (e & 1) convert(FalseTag{}); else convert(TrueTag{});
-                    if ((e & 1) && special(c0 + t))                              // values that none of the rows sees may be anything, and 0 x inf is not 0
+                    if ((e & 1) && (c0 + t < p.s0 || c0 + t >= p.s1))                              // values that none of the rows sees may be anything, and 0 x inf is not 0
 #pragma unroll 1
                         for (int i = 0; i < STEPS; ++i) {
                             const int key = key_of(i), pg = 2 * (c0 + t) + (key >> 6);
-                            if (pg < at.s.pages && any.sees(a, at.s, at.s.page(pg) * CACHE_PAGE + (key & 63))) continue;
+                            if (pg < p.s.pages && p.any.sees(a, p.s, p.s.page(pg) * CACHE_PAGE + (key & 63))) continue;
                             *reinterpret_cast<uint4*>(dst + key * 128 + (((2 * (ch & 3)) ^ (key & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
                             *reinterpret_cast<uint4*>(dst + key * 128 + (((2 * (ch & 3) + 1) ^ (key & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
                         }
@@ -1142,7 +1164,8 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                     if (lane == 0) { mbar_arrive(&raw_empty[from]); mbar_arrive(&full[to]); if (e & 1) mbar_arrive(&sc_empty[(g + t) % SC]); }
                     ++n;
                 }
-            }
+                g += tiles;
+            });
         }
     }
     __syncthreads();
