@@ -567,7 +567,7 @@ struct TreeAny {
 // A CTA's piece of an item: key tiles c0 .. c1 - 1 (none where its units are the item's own alone), of which those before s0 and from s1 on have places that some row may not see; what each row sees.  Made
 // by a warp of its own, a piece ahead of the others: each of its looks into the arrays is a latency of L2
 struct TreePiece {
-    uint64_t seen[128]; int low[128];
+    uint64_t seen[128]; int low[128]; float factor[128];                         // factor: of a row's scores
     TreeSeq s; TreeAny any;
     int c0, c1, s0, s1, seq, kvh, row0, rows;
     bool first, last, more;                                                      // the CTA has the item's begin, its end; another piece follows
@@ -581,8 +581,8 @@ struct ManyCfg {
     static constexpr int RAW_BYTES = KEYS * D, RAW = BITS8 ? (D == 128 ? 5 : 8) : 0;         // a tile of 8 bits, and how many wait
     static constexpr int SC = 8, SC_FLOATS = 2 * KEYS + 4;                       // tiles whose scales wait: keys', values', what scores are multiplied by, what O is for larger scales of values and at its end
     static constexpr int CONV = BITS8 ? 8 : 0, THREADS = 128 + 256 + 32 * CONV;     // producer, issuer, scales, pieces; eight softmax warps; warps that convert
-    static constexpr int BARS = 16 + 2 * SLOTS + 2 * RAW + (BITS8 ? 3 * SC : 0);
-    static constexpr int SMEM_BYTES = TILE_BYTES + SLOTS * TILE_BYTES + RAW * RAW_BYTES + (BITS8 ? SC * SC_FLOATS * 4 + 2 * 128 * 4 : 0) + 3 * 128 * 4 + BARS * 8 + 16 + 2 * sizeof(TreePiece);
+    static constexpr int BARS = 18 + 2 * SLOTS + 2 * RAW + (BITS8 ? 3 * SC : 0);
+    static constexpr int SMEM_BYTES = TILE_BYTES + SLOTS * TILE_BYTES + RAW * RAW_BYTES + (BITS8 ? SC * SC_FLOATS * 4 : 0) + 3 * 128 * 4 + BARS * 8 + 16 + 2 * sizeof(TreePiece);
     static constexpr uint32_t O_COL = 384;                                       // TMEM: S and P of the tiles in turn at 0, 128 and 256
 };
 OA_DEVINL uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
@@ -602,6 +602,40 @@ OA_DEVINL int tiles_below(const TreeSeq& s, int place) {
     return (c + 2) / 2;
 }
 
+// Queries in fp16, a row of a head under a power of two that brings its largest magnitude to [2^14, 2^15): a warp eight rows.  What the next kernel reads besides was written by kernels that have ended
+template <int D>
+__global__ void __launch_bounds__(128) tree_queries_kernel(const __grid_constant__ TreeAttnArgs a) {
+    constexpr int W = D / 64, ROWS = 8;                                          // words of two channels a lane
+    const int lane = threadIdx.x & 31;
+    const int64_t total = (int64_t)a.n_rows * a.n_heads, r0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 5)) * ROWS;
+    griddep_wait();
+    griddep_launch();
+    uint32_t x[ROWS][W];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int64_t token = quotient(r0 + i, a.n_heads);
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + token * a.ldq + (r0 + i - token * a.n_heads) * D + lane * 2 * W;
+#pragma unroll
+        for (int j = 0; j < W; ++j) x[i][j] = 0u;
+        if (r0 + i < total) { if (W == 2) { const uint2 y = __ldcg(reinterpret_cast<const uint2*>(src)); x[i][0] = y.x; x[i][W - 1] = y.y; } else x[i][0] = __ldcg(reinterpret_cast<const uint32_t*>(src)); }
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < W; ++j) top = max(top, max(x[i][j] << 16 & 0x7fffffffu, x[i][j] & 0x7fff0000u));
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (r0 + i >= total) return;
+        const int e = top >= 0x7f800000u ? 14 : max((int)(top >> 23) - 127, -100);           // not finite: as it is
+        const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+        uint32_t* dst = a.q16 + (r0 + i) * (D / 2) + lane * W;
+#pragma unroll
+        for (int j = 0; j < W; ++j) x[i][j] = pack_f16x2(bf16lo(x[i][j]) * up, bf16hi(x[i][j]) * up);
+        if (W == 2) *reinterpret_cast<uint2*>(dst) = make_uint2(x[i][0], x[i][W - 1]); else dst[0] = x[i][0];
+        if (lane == 0) a.q_factor[r0 + i] = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+    }
+}
+
 template <int D, int FMT>
 __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ TreeAttnArgs a) {
     using Cfg = ManyCfg<D, FMT>;
@@ -615,12 +649,11 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
     uint8_t* kv_s = q_s + TILE;
     uint8_t* raw_s = kv_s + SLOTS * TILE;
     float* sc_s = reinterpret_cast<float*>(raw_s + Cfg::RAW * Cfg::RAW_BYTES);
-    float* factor_s = sc_s + (BITS8 ? SC * Cfg::SC_FLOATS : 0);                  // [2 pieces][rows]
-    float* m_s = factor_s + (BITS8 ? 256 : 0);                                   // a row's reference maximum, and its two sums of a piece
+    float* m_s = sc_s + (BITS8 ? SC * Cfg::SC_FLOATS : 0);                                   // a row's reference maximum, and its two sums of a piece
     float* l_s = m_s + 128;
     uint64_t* bars = reinterpret_cast<uint64_t*>(l_s + 256);
     uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_full = bars + 5, *o_full = bars + 8, *full = bars + 12, *empty = full + SLOTS;
-    uint64_t *piece_full = empty + SLOTS, *piece_empty = piece_full + 2, *raw_full = piece_empty + 2, *raw_empty = raw_full + Cfg::RAW, *sc_in = raw_empty + Cfg::RAW, *sc_full = sc_in + SC, *sc_empty = sc_full + SC;
+    uint64_t *piece_full = empty + SLOTS, *rows_full = piece_full + 2, *piece_empty = rows_full + 2, *raw_full = piece_empty + 2, *raw_empty = raw_full + Cfg::RAW, *sc_in = raw_empty + Cfg::RAW, *sc_full = sc_in + SC, *sc_empty = sc_full + SC;
     TreePiece* piece_s = reinterpret_cast<TreePiece*>(bars + Cfg::BARS);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(piece_s + 2);
     __shared__ int64_t sums[Cfg::THREADS / 32];
@@ -630,11 +663,12 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int grp = a.n_heads / a.n_kv, tile_tokens = 128 / grp;
     if (threadIdx.x == 0) {
-        if (!BITS8) { tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_kv); }
-        mbar_init(q_full, BITS8 ? Cfg::CONV : 1); mbar_init(q_empty, 1);
+        tma_prefetch_desc(&tm_q);
+        if (!BITS8) tma_prefetch_desc(&tm_kv);
+        mbar_init(q_full, 1); mbar_init(q_empty, 1);
         for (int i = 0; i < 3; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
         for (int i = 0; i < 4; ++i) mbar_init(&o_full[i], 1);
-        for (int i = 0; i < 2; ++i) { mbar_init(&piece_full[i], 1); mbar_init(&piece_empty[i], BITS8 ? 11 + Cfg::CONV : 10); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&piece_full[i], 1); mbar_init(&rows_full[i], 1); mbar_init(&piece_empty[i], BITS8 ? 11 + Cfg::CONV : 10); }
         for (int i = 0; i < SLOTS; ++i) { mbar_init(&full[i], BITS8 ? Cfg::CONV : 1); mbar_init(&empty[i], 1); }
         if (BITS8) {
             for (int i = 0; i < RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], Cfg::CONV); }
@@ -642,8 +676,9 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
         }
         fence_barrier_init();
     }
-    // Tensor memory is taken behind the wait: a kernel before this one that has not taken its own yet would otherwise wait for this one, and this one for it
-    griddep_wait();
+    // Tensor memory is taken behind the wait: a kernel before this one that has not taken its own yet would otherwise wait for this one, and this one for it.  8 bits: the kernel before this one is the
+    // queries', which takes none and has let this one start behind its own wait; only what it writes is waited for, later
+    if (!BITS8) griddep_wait();
     if (warp == 1) tmem_alloc<512>(tmem_slot);
     const TreeShare share = tree_share<Cfg::THREADS>(a, tile_tokens, sums, start);
     tcgen05_fence_before();
@@ -651,12 +686,13 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
     tcgen05_fence_after();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     const int64_t u_begin = share.begin, u_end = share.end;
-    // what a warp does with each piece; p lies in shared memory until it is done
-    auto pieces = [&](auto&& work) {
+    // what a warp does with each piece; p lies in shared memory until it is done.  What rows see comes a latency later
+    auto pieces = [&](bool rows, auto&& work) {
         if (u_begin >= u_end) return;
         for (uint32_t k = 0;; ++k) {
             mbar_wait(&piece_full[k & 1], (k >> 1) & 1);
             const TreePiece& p = piece_s[k & 1];
+            if (rows) mbar_wait(&rows_full[k & 1], (k >> 1) & 1);
             const bool more = p.more;
             work(p);
             __syncwarp();
@@ -673,19 +709,23 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
             constexpr int RING = BITS8 ? RAW : SLOTS;
             uint64_t *in = BITS8 ? raw_full : full, *out = BITS8 ? raw_empty : empty;
             uint32_t n = 0, seg = 0, g = 0;                                          // entries, pieces and tiles loaded
-            pieces([&](const TreePiece& p) {
+            pieces(false, [&](const TreePiece& p) {
                 const int c0 = p.c0, c1 = p.c1;
                 if (c1 == c0) return;
-                if constexpr (!BITS8) {
+                bool q_due = true;
+                auto load_q = [&] {
                     mbar_wait(q_empty, (seg & 1) ^ 1);
+                    if (BITS8 && seg == 0) { griddep_wait(); fence_proxy_async_all(); }          // written by threads of the kernel before
                     if (elect_one()) {                                               // tokens behind the last row are zeros, other sequences' are not looked at
                         mbar_expect_tx(q_full, HALVES * tile_tokens * grp * 128);
 #pragma unroll
                         for (int h = 0; h < HALVES; ++h) tma_load_3d(q_s + h * HALF, &tm_q, q_full, h * 64, p.kvh * grp, p.row0, kEvictNormal);
                     }
                     __syncwarp();
-                }
-                ++seg;
+                    ++seg;
+                    q_due = false;
+                };
+                if (!BITS8) load_q();
                 const int32_t* table = a.tables + (int64_t)p.seq * a.max_pages;
                 int page[3][2] = {}, have = 0, later = 0, scales = c0;               // pages of this tile and of the two before
                 for (int kt = c0; kt < c1 + 2; ++kt) {
@@ -743,6 +783,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                         }
                         __syncwarp();
                         ++n;
+                        if (BITS8 && q_due) load_q();                                // behind the first tile of keys, which takes longer to be one
                     }
                 }
             });
@@ -761,7 +802,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                 return slot;
             };
             // products of one thread are carried out in the order of their issue: S of a tile goes over scores whose P a product ahead of it reads
-            pieces([&](const TreePiece& p) {
+            pieces(false, [&](const TreePiece& p) {
                 const int tiles = p.c1 - p.c0;
                 if (tiles == 0) return;
                 mbar_wait(q_full, seg & 1);
@@ -805,7 +846,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
             // largest product to 28672 (0.25) and 57344; 0 of what none of the rows sees.  int8 keys u - 128 times s are the fused product u 2^-24 (a subnormal's bits) times s 2^24 less 128 s
             if constexpr (BITS8) {
                 uint32_t n = 0;
-                pieces([&](const TreePiece& p) {
+                pieces(true, [&](const TreePiece& p) {
                     const int c0 = p.c0, c1 = p.c1;
                     float vref = 0.f;
                     for (int kt = c0; kt < c1; ++kt, ++n) {
@@ -866,20 +907,9 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                 mbar_wait(&piece_empty[k & 1], ((k >> 1) & 1) ^ 1);
                 TreePiece& p = piece_s[k & 1];
                 const int rows = at.rows(grp);
-                uint64_t any = 0; int lowest = 0x7fffffff;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = i * 32 + lane;
-                    uint64_t seen = 0; int low = 0x7fffffff;
-                    if (r < rows) { const int t = at.tile * tile_tokens + r / grp; seen = tree_seen(a, at.s, t); low = tree_low(a, at.s, seen, t); }
-                    p.seen[r] = seen; p.low[r] = low;
-                    any |= seen; lowest = min(lowest, low);
-                }
-                any = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(any >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)any);
-                lowest = __reduce_min_sync(0xffffffffu, lowest);
                 if (lane == 0) {
                     const TreeSeq& s = at.s;
-                    p.s = s; p.any.seen = any; p.any.low = lowest;
+                    p.s = s;
                     p.c0 = c0; p.c1 = c1; p.seq = at.seq; p.kvh = at.kvh; p.row0 = at.row0(); p.rows = rows;
                     p.s0 = a.window > 0 ? tiles_below(s, s.ctx + s.n - a.window) : 0; p.s1 = min((s.ctx / CACHE_PAGE - s.skip) / 2, s.pages / 2);
                     p.first = at.unit0 >= u_begin; p.last = end <= u_end; p.more = end < u_end;
@@ -887,6 +917,25 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&piece_full[k & 1]);
+                if (BITS8 && k == 0) griddep_wait();                             // the queries in fp16 are there
+                uint64_t any = 0; int lowest = 0x7fffffff;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = i * 32 + lane, token = r / grp;
+                    uint64_t seen = 0; int low = 0x7fffffff; float factor = a.scale_log2e;
+                    if (r < rows) {
+                        const int t = at.tile * tile_tokens + token;
+                        seen = tree_seen(a, at.s, t); low = tree_low(a, at.s, seen, t);
+                        if (BITS8) factor *= __ldcg(a.q_factor + (int64_t)(at.row0() + token) * a.n_heads + at.kvh * grp + r - token * grp);
+                    }
+                    p.seen[r] = seen; p.low[r] = low; p.factor[r] = factor;
+                    any |= seen; lowest = min(lowest, low);
+                }
+                any = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(any >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)any);
+                lowest = __reduce_min_sync(0xffffffffu, lowest);
+                if (lane == 0) { p.any.seen = any; p.any.low = lowest; }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&rows_full[k & 1]);
             }
         }
     } else if (warp < 12) {
@@ -905,8 +954,8 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
         constexpr float kRaise = 8.0f;                                           // log2 units a score may pass the reference by
         constexpr float kLift = BITS8 ? 7.0f : 0.0f;                             // of the weights, which fp16 holds up to 2^16 and with 8 bits down to 2^-17
         constexpr int COLS = D / 2;
-        uint32_t n0 = 0, seg = 0;                                                // tiles of the pieces before, pieces
-        pieces([&](const TreePiece& p) {
+        uint32_t n0 = 0;                                                         // tiles of the pieces before
+        pieces(true, [&](const TreePiece& p) {
             const TreeSeq& s = p.s;
             const int c0 = p.c0, tiles = p.c1 - p.c0;
             const bool live = row < p.rows, first = p.first;
@@ -921,9 +970,8 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                 if (live && wg == 0) *ml = make_float2(-INFINITY, first && blind ? -1.f : 0.f);
                 return;
             }
-            float row_fac = a.scale_log2e, undo = 1.0f;
-            if (BITS8) { mbar_wait(q_full, seg & 1); row_fac = factor_s[(seg & 1) * 128 + row] * a.scale_log2e; }
-            ++seg;
+            const float row_fac = p.factor[row];
+            float undo = 1.0f;
             float m_mine = -INFINITY, l_run = 0.f;                               // the sum so far and the reference that it is under
             auto tile = [&](uint32_t n, auto tag) {
                 constexpr bool SPECIAL = decltype(tag)::value;
@@ -934,15 +982,14 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                     word[0] = tree_word(a, s, seen, low, s.page(2 * kt) * CACHE_PAGE);
                     word[1] = 2 * kt + 1 < s.pages ? tree_word(a, s, seen, low, s.page(2 * kt + 1) * CACHE_PAGE) : 0ull;
                 }
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};     // four chains
+                mbar_wait(&s_full[from], (n / 3) & 1);                           // the tile's scales, which its keys were turned with, are there too
+                tcgen05_fence_after();
                 float grown = 1.0f, fac = row_fac;
                 if (BITS8) {
                     const float* sc = sc_s + buf * Cfg::SC_FLOATS + 2 * KEYS;
-                    mbar_wait(&sc_full[buf], (n / SC) & 1);
                     fac *= sc[0]; grown = sc[1]; undo = sc[2];
                 }
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};     // four chains
-                mbar_wait(&s_full[from], (n / 3) & 1);
-                tcgen05_fence_after();
                 uint32_t v[2][32];
                 auto scores = [&](int k) {                                       // of keys k .. k + 63, -inf where the row does not see
                     tmem_ld_32x32b_x32(s_addr + k, v[0]);
@@ -1067,48 +1114,17 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
         });
     } else {
         if constexpr (BITS8) reg_dec<72>();
-        // queries, then tiles in the ring's order, 16 channels of a key a step
+        // tiles in the ring's order, 16 channels of a key a step
         if constexpr (BITS8) {
             const int w = warp - 12, tid = w * 32 + lane;
             // 16 channels of a key a step.  Heads of 128: eight lanes take the lower half of one key and the upper of its neighbour, then the other way round, so that neither loads nor stores meet on a bank
-            constexpr int STEPS = Cfg::RAW_BYTES / 16 / (32 * Cfg::CONV), ROWS = 128 / Cfg::CONV, AHEAD = STEPS < 4 ? STEPS : 4;
+            constexpr int STEPS = Cfg::RAW_BYTES / 16 / (32 * Cfg::CONV), AHEAD = STEPS < 4 ? STEPS : 4;
             const int ch = tid % (D / 16);
             auto key_of = [&](int i) { return D == 128 ? 2 * ((tid >> 3) + 4 * Cfg::CONV * (i >> 1)) + ((ch >> 2) ^ (i & 1)) : (tid >> 2) + 8 * Cfg::CONV * i; };
-            uint32_t n = 0, seg = 0, g = 0;                                      // entries, pieces, tiles of the pieces before
-            pieces([&](const TreePiece& p) {
-                const int c0 = p.c0, tiles = p.c1 - c0, live = p.rows;
+            uint32_t n = 0, g = 0;                                               // entries, tiles of the pieces before
+            pieces(true, [&](const TreePiece& p) {
+                const int c0 = p.c0, tiles = p.c1 - p.c0;
                 if (tiles == 0) return;
-                constexpr int W = D / 64;                                        // words of two channels a lane
-                uint32_t x[ROWS][W];                                             // rows of the warp, ahead of the wait
-#pragma unroll
-                for (int i = 0; i < ROWS; ++i) {
-                    const int r = w * ROWS + i, token = r / grp;
-                    const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(p.row0 + token) * a.ldq + (int64_t)(p.kvh * grp + r - token * grp) * D + lane * 2 * W;
-#pragma unroll
-                    for (int j = 0; j < W; ++j) x[i][j] = 0u;
-                    if (r < live) { if (W == 2) { const uint2 y = __ldcg(reinterpret_cast<const uint2*>(src)); x[i][0] = y.x; x[i][W - 1] = y.y; } else x[i][0] = __ldcg(reinterpret_cast<const uint32_t*>(src)); }
-                }
-                mbar_wait(q_empty, (seg & 1) ^ 1);
-#pragma unroll
-                for (int i = 0; i < ROWS; ++i) {
-                    const int r = w * ROWS + i;
-                    if (r >= live) break;
-                    uint32_t top = 0;
-#pragma unroll
-                    for (int j = 0; j < W; ++j) top = max(top, max(x[i][j] << 16 & 0x7fffffffu, x[i][j] & 0x7fff0000u));
-                    top = __reduce_max_sync(0xffffffffu, top);
-                    const int e = top >= 0x7f800000u ? 14 : max((int)(top >> 23) - 127, -100);           // not finite: as it is
-                    const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
-                    const int c = lane * 2 * W;
-#pragma unroll
-                    for (int j = 0; j < W; ++j)
-                        *reinterpret_cast<uint32_t*>(q_s + (c >> 6) * HALF + r * 128 + ((((c & 63) >> 3) ^ (r & 7)) << 4) + (c & 7) * 2 + j * 4) = pack_f16x2(bf16lo(x[i][j]) * up, bf16hi(x[i][j]) * up);
-                    if (lane == 0) factor_s[(seg & 1) * 128 + r] = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
-                }
-                ++seg;
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(q_full);
 #pragma unroll 1
                 for (int e = 0; e < 2 * tiles + 4; ++e) {                        // K of a tile, V of the one two before
                     const int t = (e >> 1) - 2 * (e & 1);
@@ -1168,6 +1184,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
             });
         }
     }
+    if (BITS8) griddep_wait();                   // also a CTA without units: what follows this kernel follows the queries' too
     __syncthreads();
     griddep_launch();
     if (warp == 1) { tcgen05_fence_after(); tmem_dealloc<512>(tmem_base); }
@@ -1242,6 +1259,7 @@ TreeAttnPlan tree_attn_plan(int n_seqs, int n_rows, int n_heads, int n_kv, int h
     p.ctas = (int)(units < most ? units : most);
     auto take = [&](size_t bytes) { const size_t at = p.bytes; p.bytes += (bytes + 255) & ~size_t(255); return at; };
     p.part_o = take((size_t)p.ctas * 2 * p.rows * head_dim * 4); p.part_ml = take((size_t)p.ctas * 2 * p.rows * 8); p.joins = take((size_t)p.ctas * sizeof(TreeJoin));
+    if (p.rows == 128 && format != CACHE_BF16) { p.q16 = take((size_t)n_rows * n_heads * head_dim * 2); p.q_factor = take((size_t)n_rows * n_heads * 4); }
     return p;
 }
 
@@ -1258,7 +1276,8 @@ static cudaError_t launch_many(const CUtensorMap* tm_q, const CUtensorMap* tm_pa
     using Cfg = ManyCfg<D, FMT>;
     auto kern = tree_many_kernel<D, FMT>;
     static bool attr_done[16] = {};
-    const cudaError_t e = ensure_dynamic_smem(kern, Cfg::SMEM_BYTES, attr_done);
+    cudaError_t e = ensure_dynamic_smem(kern, Cfg::SMEM_BYTES, attr_done);
+    if (e == cudaSuccess && FMT != CACHE_BF16) e = launch_k(tree_queries_kernel<D>, dim3((unsigned)(((int64_t)a.n_rows * a.n_heads + 31) / 32)), dim3(128), 0, s, a);
     return e == cudaSuccess ? launch_k(kern, dim3(a.ctas), dim3(Cfg::THREADS), Cfg::SMEM_BYTES, s, *tm_q, *tm_page, a) : e;
 }
 template <int D, int FMT>

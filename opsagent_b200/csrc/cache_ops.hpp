@@ -73,12 +73,13 @@ struct TreeAttnArgs {
     int32_t* status;
     // scratch (tree_attn_plan): each CTA's part of an item that it begins and others end, its part of one that another began, and who they belong to
     float *part_o, *part_ml; TreeJoin* joins;
+    uint32_t* q16; float* q_factor;                // tiles of 128 rows over 8 bits: queries in fp16 [n_rows][n_heads][head_dim] and their scores' factors [n_rows][n_heads]
     int32_t ctas, rows;                            // rows: of a tile
 };
-struct TreeAttnPlan { int ctas, rows; size_t part_o, part_ml, joins, bytes; };
+struct TreeAttnPlan { int ctas, rows; size_t part_o, part_ml, joins, q16, q_factor, bytes; };
 TreeAttnPlan tree_attn_plan(int n_seqs, int n_rows, int n_heads, int n_kv, int head_dim, int format, int max_pages, int sms);
-// tm_page: box of 64 rows over the layer's cache [2 * num_pages * n_kv * 64, head_dim] of bf16, or of a block's values over the same of 8 bits, rows of 128 bytes; tm_q, looked at for tiles of 128 rows
-// over bf16: box of 128 / group tokens by a group's heads over q
+// tm_page: box of 64 rows over the layer's cache [2 * num_pages * n_kv * 64, head_dim] of bf16, or of a block's values over the same of 8 bits, rows of 128 bytes; tm_q, looked at for tiles of 128 rows:
+// box of 128 / group tokens by a group's heads over q, or over q16 where the cache has 8 bits
 cudaError_t launch_tree_attention(const CUtensorMap* tm_q, const CUtensorMap* tm_page, int head_dim, int format, const TreeAttnArgs& a, cudaStream_t s);
 
 }  // namespace oa

@@ -304,16 +304,17 @@ int oa_k_tree_attention(const void* q, int64_t ldq, void* out, int64_t ldo, cons
     const int group = n_heads / n_kv;
     if ((format == CACHE_BF16 ? make_tmap_bf16_2d(&tm_page, kv_cache, (uint64_t)tm_rows, head_dim, head_dim, CACHE_PAGE, 64)
                               : make_tmap_bytes_2d(&tm_page, kv_cache, (uint64_t)tm_rows, CACHE_PAGE * head_dim / 128)) != 0) return call_failed(OA_ERR_INTERNAL, "tree attention: no tensor map of the cache");
-    if (format == CACHE_BF16 && plan.rows == 128 &&
-        make_tmap_bf16_heads(&tm_q, q, (uint64_t)n_rows, (uint64_t)n_heads, (uint64_t)head_dim, (uint64_t)ldq, 128 / group, group) != 0) return call_failed(OA_ERR_INTERNAL, "tree attention: no tensor map of the queries");
     DevBuf scratch(plan.bytes, (cudaStream_t)stream);
     if (!scratch.p) return call_failed(OA_ERR_INTERNAL, "tree attention: no scratch memory");
     char* base = (char*)scratch.p;
+    const bool bits8 = format != CACHE_BF16;
+    if (plan.rows == 128 && make_tmap_bf16_heads(&tm_q, bits8 ? base + plan.q16 : q, (uint64_t)n_rows, (uint64_t)n_heads, (uint64_t)head_dim, (uint64_t)(bits8 ? width : ldq), 128 / group, group) != 0)
+        return call_failed(OA_ERR_INTERNAL, "tree attention: no tensor map of the queries");
     TreeAttnArgs a{};
     a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo; a.cache = kv_cache; a.tables = block_tables; a.ctx_lens = ctx_lens; a.row_starts = row_starts; a.seen = seen;
     a.max_pages = max_pages_per_seq; a.n_seqs = n_seqs; a.n_rows = n_rows; a.n_heads = n_heads; a.n_kv = n_kv; a.num_pages = num_pages; a.window = window; a.sinks = sinks;
     a.scale_log2e = scale_log2e; a.status = status;
-    a.part_o = (float*)(base + plan.part_o); a.part_ml = (float*)(base + plan.part_ml); a.joins = (TreeJoin*)(base + plan.joins); a.ctas = plan.ctas; a.rows = plan.rows;
+    a.part_o = (float*)(base + plan.part_o); a.part_ml = (float*)(base + plan.part_ml); a.joins = (TreeJoin*)(base + plan.joins); a.q16 = (uint32_t*)(base + plan.q16); a.q_factor = (float*)(base + plan.q_factor); a.ctas = plan.ctas; a.rows = plan.rows;
     return device_rc(launch_tree_attention(&tm_q, &tm_page, head_dim, format, a, (cudaStream_t)stream));
 }
 
