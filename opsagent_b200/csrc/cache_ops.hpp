@@ -56,6 +56,7 @@ struct Rows8Args {
     // T rows of n_kv heads of keys and of values (bf16, pitch ldkv in elements) and a layer's two planes; token t is place slots[t] % 64 of page slots[t] / 64.  A negative slot: the
     // token is passed over; one beyond the cache: the same, *status = 400
     const void *k, *v; void *k_out, *v_out; int64_t ldkv; void* cache; const int32_t* slots; int32_t T, n_kv, head_dim, num_pages; int32_t* status;
+    int32_t step_tokens, step_rows;                // of a thread's next row (the launchers')
 };
 cudaError_t launch_cache8_write(const Rows8Args& a, bool e4m3, cudaStream_t s);          // k, v -> cache
 cudaError_t launch_cache8_read(const Rows8Args& a, bool e4m3, cudaStream_t s);           // cache -> k_out, v_out

@@ -134,11 +134,12 @@ def test_write_and_read(L, tokens, n_kv, dim, pad, off, fmt):
 def test_every_value_is_written_to_the_nearest(L, fmt):
     """All magnitudes of bf16 between 2^-14 and 1 under a largest one of 1, and the ties among them."""
     bits = torch.arange(0x3880, 0x3f81, dtype=torch.int32).to(torch.int16).view(torch.bfloat16).cuda()
-    n = -(-len(bits) // 127)
+    n = -(-len(bits) // 126)
     x = torch.ones((n, 128), dtype=torch.bfloat16, device="cuda")
     for i in range(n):
-        part = bits[i * 127: (i + 1) * 127]
+        part = bits[i * 126: (i + 1) * 126]
         x[i, 1: 1 + len(part)] = part * (-1) ** i
+    x[:, 127] = torch.where(torch.arange(n, device="cuda") % 2 == 0, -0.0, 0.0)      # zeros keep their sign
     cache, s = torch.zeros((2, -(-n // PAGE), 1, PAGE * 132), dtype=torch.uint8, device="cuda"), dev(np.arange(n))
     assert L.oa_k_cache8_write(ptr(x), ptr(x), 128, ptr(cache), cache.shape[1], ptr(s), n, 1, 128, fmt, None, now()) == 0
     torch.cuda.synchronize()
