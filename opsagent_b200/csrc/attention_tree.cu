@@ -83,6 +83,12 @@ struct TreeSeq {
     // whether some row may not see all of a page's places
     OA_DEVINL bool special(const TreeAttnArgs& a, int page) const { return (page + 1) * CACHE_PAGE > ctx || (a.window > 0 && page * CACHE_PAGE < ctx + n - a.window); }
 };
+// how many of a sequence's pages begin below a place of its window
+OA_DEVINL int pages_below(const TreeSeq& s, int place) {
+    if (place <= 0) return 0;
+    const int page = pages_of(place) - 1;                                        // the last one that does
+    return 1 + (page < s.low_pages ? page : max(page - s.skip, s.low_pages - 1));
+}
 // which new tokens token t of a sequence of n sees, and the first cached place of its window
 OA_DEVINL uint64_t tree_seen(const TreeAttnArgs& a, const TreeSeq& s, int t) {
     const uint64_t there = s.n < 64 ? (1ull << s.n) - 1 : ~0ull;
@@ -153,18 +159,22 @@ OA_DEVINL void tree_record(const TreeAttnArgs& a, int later, int row0, int rows,
 // =============================================================================================
 // up to 16 rows of an item: the warp path
 // =============================================================================================
+// What eight warps do with pages: bf16, which memory bounds, take every page together, 16 tokens and half of the channels a warp; 8 bits, which issue slots bound, take pages in turn, four warps a page, 16
+// tokens and all channels a warp: scores, weights and keys' fp16 once instead of twice
 template <int D, int FMT, int NB, int STAGES>
 struct FewCfg {
-    static constexpr int ESZ = FMT == CACHE_BF16 ? 2 : 1;
+    static constexpr int ESZ = FMT == CACHE_BF16 ? 2 : 1, GROUPS = FMT == CACHE_BF16 ? 1 : 2, PARTS = 2 / GROUPS;       // groups of warps that take pages in turn; parts of the channels
+    static_assert(GROUPS == 1 || STAGES % 2 == 0, "a page of the ring belongs to one group");
     static constexpr int KV_BYTES = CACHE_PAGE * D * ESZ, STAGE_BYTES = 2 * KV_BYTES, SCALE_BYTES = FMT == CACHE_BF16 ? 0 : 2 * CACHE_PAGE * 4;
-    static constexpr int ROWS = 8 * NB, REGS = D / 4 * NB;                       // output values of a lane and its twin's in the other half
+    static constexpr int ROWS = 8 * NB, REGS = D / 4 * NB, STATES = 4 * GROUPS;  // output values of a lane in all parts; states of an item that meet
     static constexpr int Q_PITCH = D * 2 + (FMT == CACHE_BF16 ? 16 : 64), Q_BYTES = ROWS * Q_PITCH;      // no bank conflicts
-    static constexpr int META_BYTES = ROWS * 16;                                 // seen, first place, factor
-    static constexpr int STATE_BYTES = 4 * REGS * 32 * 4 + 4 * ROWS * 2 * 4 + 16;
-    static constexpr int SMEM_BYTES = STAGES * (STAGE_BYTES + SCALE_BYTES) + 2 * (Q_BYTES + META_BYTES) + STATE_BYTES + (2 * STAGES + 6) * 8;
+    static constexpr int STATE_BYTES = STATES * (REGS * 32 * 4 + ROWS * 2 * 4 + 4);
+    static constexpr int SMEM_BYTES = STAGES * (STAGE_BYTES + SCALE_BYTES) + 2 * (Q_BYTES + ROWS * 16 + 80) + STATE_BYTES + (2 * STAGES + 6) * 8;
     static constexpr int CTAS = FMT != CACHE_BF16 && NB == 1 ? 2 : 1;            // of an SM
 };
 struct TreeMeta { uint64_t seen; int low; float factor; };
+struct FewItem { TreeSeq s; int c0, c1, low, high, row0, rows, kvh, later; bool first, last, more; };      // a CTA's pages of an item, special ones below `low` and from `high` on; CTAs that have later parts
+static_assert(sizeof(FewItem) <= 80, "an item's place in shared memory");
 
 template <int D>
 OA_DEVINL uint32_t few_off(int r, int d) { return (uint32_t)((d >> 6) * (CACHE_PAGE * 128) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4)); }      // bf16: halves of 64 channels
@@ -177,16 +187,17 @@ OA_DEVINL uint32_t few_off8(int r, int chunk) {                                 
 template <int D, int FMT, int NB, int STAGES>
 __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS) tree_few_kernel(const __grid_constant__ CUtensorMap tm_page, const __grid_constant__ TreeAttnArgs a) {
     using Cfg = FewCfg<D, FMT, NB, STAGES>;
-    constexpr int KS = D / 16, KH = KS / 2, ROWS = Cfg::ROWS;
+    constexpr int KS = D / 16, KH = KS / Cfg::PARTS, ROWS = Cfg::ROWS, STATES = Cfg::STATES;
     constexpr bool BITS8 = FMT != CACHE_BF16;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* scales_s = smem + STAGES * Cfg::STAGE_BYTES;                                    // [stage][keys', values'][64]
     uint8_t* q_s = scales_s + STAGES * Cfg::SCALE_BYTES;                                     // [2 items][rows]
     TreeMeta* meta_s = reinterpret_cast<TreeMeta*>(q_s + 2 * Cfg::Q_BYTES);                  // [2 items][rows]
-    float* states = reinterpret_cast<float*>(meta_s + 2 * ROWS);                             // [4 quarters][values][32 lanes]
-    float* ml_s = states + 4 * Cfg::REGS * 32;                                               // [4 quarters][rows][2]
-    float* vref_s = ml_s + 4 * ROWS * 2;                                                     // [4 quarters]: what values' scales are taken over
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(vref_s + 4);
+    uint8_t* item_s = reinterpret_cast<uint8_t*>(meta_s + 2 * ROWS);                         // [2 items]
+    float* states = reinterpret_cast<float*>(item_s + 2 * 80);                               // [states][values][32 lanes]
+    float* ml_s = states + Cfg::STATES * Cfg::REGS * 32;                                     // [states][rows][2]
+    float* vref_s = ml_s + Cfg::STATES * ROWS * 2;                                           // [states]: what values' scales are taken over
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(vref_s + Cfg::STATES);
     uint64_t *empty_bar = full_bar + STAGES, *q_full = empty_bar + STAGES, *q_empty = q_full + 2, *states_full = q_empty + 2, *states_empty = states_full + 1;
     using At = TreeAt<1, 1>;
     __shared__ int64_t sums[TREE_THREADS / 32];
@@ -196,7 +207,7 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
     const int grp = a.n_heads / a.n_kv, tile_tokens = ROWS / grp;
     if (threadIdx.x == 0) {
         tma_prefetch_desc(&tm_page);
-        for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], TREE_CONSUMERS / 32); }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], TREE_CONSUMERS / 32 / Cfg::GROUPS); }
         for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], TREE_CONSUMERS / 32 + 1); }
         mbar_init(states_full, TREE_CONSUMERS / 32); mbar_init(states_empty, 1);
         fence_barrier_init();
@@ -246,8 +257,16 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
         // queries of an item, and what its rows see.  8 bits: fp16 under a power of two, pieces of eight channels where the consumers' lanes find them side by side
         uint32_t k = 0;
         for (int64_t u = u_begin; u < u_end; next(), ++k) {
-            u = min(at.unit0 + 1 + at.s.pages, u_end);
+            const int64_t end = at.unit0 + 1 + at.s.pages;
+            FewItem item;
+            item.s = at.s; item.c0 = (int)max(u - at.unit0 - 1, (int64_t)0); item.c1 = (int)min((int64_t)at.s.pages, u_end - at.unit0 - 1);
+            item.low = a.window > 0 ? pages_below(at.s, at.s.ctx + at.s.n - a.window) : 0; item.high = at.s.ctx / CACHE_PAGE - at.s.skip;
+            item.row0 = at.row0(); item.rows = at.rows(grp); item.kvh = at.kvh;
+            item.first = at.unit0 >= u_begin; item.last = end <= u_end; item.more = end < u_end;
+            item.later = item.first && !item.last ? cta_of(end - 1, share.busy, share.total) - (int)blockIdx.x : 0;
+            u = min(end, u_end);
             mbar_wait(&q_empty[k & 1], ((k >> 1) & 1) ^ 1);
+            if (lane == 0) *reinterpret_cast<FewItem*>(item_s + (k & 1) * 80) = item;
             uint8_t* q_dst = q_s + (k & 1) * Cfg::Q_BYTES;
             TreeMeta* meta = meta_s + (k & 1) * ROWS;
             const int live = at.rows(grp), t0 = at.tile * tile_tokens;
@@ -302,70 +321,66 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
     if (warp == 9) {
         // An item's states under one maximum: its rows of the output where the CTA has all of it, a part elsewhere
         const int g = lane >> 2, t = lane & 3;
-        uint32_t k = 0;
-        for (int64_t u = u_begin; u < u_end; next(), ++k) {
-            const int64_t end = at.unit0 + 1 + at.s.pages;
-            const bool first = at.unit0 >= u_begin, last = end <= u_end;
-            u = min(end, u_end);
-            const int live = at.rows(grp), row0 = at.row0();
+        for (uint32_t k = 0;; ++k) {
             mbar_wait(&q_full[k & 1], (k >> 1) & 1);
+            const FewItem& item = *reinterpret_cast<const FewItem*>(item_s + (k & 1) * 80);
+            const bool first = item.first, whole = item.first && item.last, more = item.more;
+            const int live = item.rows, row0 = item.row0, kvh = item.kvh;
             const TreeMeta own = meta_s[(k & 1) * ROWS + (lane < ROWS ? lane : 0)];
-            const uint32_t blind = __ballot_sync(0xffffffffu, lane < live && !tree_sees(a, at.s, own.seen, own.low));      // rows that see nothing
+            const uint32_t blind = __ballot_sync(0xffffffffu, lane < live && !tree_sees(a, item.s, own.seen, own.low));       // rows that see nothing
+            if (lane == 0 && first && !whole) tree_record(a, item.later, row0, live, kvh);
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_empty[k & 1]);
-            if (lane == 0 && first && !last) tree_record(a, cta_of(end - 1, share.busy, share.total) - (int)blockIdx.x, row0, live, at.kvh);
             float* po = a.part_o + ((int64_t)blockIdx.x * 2 + !first) * (ROWS * D);
             float2* ml = reinterpret_cast<float2*>(a.part_ml) + ((int64_t)blockIdx.x * 2 + !first) * ROWS;
             mbar_wait(states_full, k & 1);
-            float vref[4];
-#pragma unroll
-            for (int w = 0; w < 4; ++w) vref[w] = BITS8 ? vref_s[w] : 1.0f;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
-#pragma unroll
+#pragma unroll 1
                 for (int h = 0; h < 2; ++h) {
                     const int row = b * 8 + 2 * t + h;
-                    float2 s4[4]; float m = -INFINITY, l = 0.f, f[4];
+                    float2 s4[STATES]; float m = -INFINITY, l = 0.f, f[STATES];
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) { s4[w] = *reinterpret_cast<const float2*>(ml_s + (w * ROWS + row) * 2); m = fmaxf(m, s4[w].x); }
+                    for (int w = 0; w < STATES; ++w) { s4[w] = *reinterpret_cast<const float2*>(ml_s + (w * ROWS + row) * 2); m = fmaxf(m, s4[w].x); }
                     const float ref = finite_or_zero(m);
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) { f[w] = ex2_approx(s4[w].x - ref); l += f[w] * s4[w].y; f[w] *= vref[w]; }
+                    for (int w = 0; w < STATES; ++w) { f[w] = ex2_approx(s4[w].x - ref); l += f[w] * s4[w].y; if (BITS8) f[w] *= vref_s[w]; }
                     if (row >= live) continue;
-                    float inv = 1.0f;
-                    uint16_t* out = nullptr;
-                    if (first && last) {
-                        inv = blind >> row & 1 ? 0.f : 1.0f / l;
-                        const int token = row / grp;
-                        out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(row0 + token) * a.ldo + (int64_t)(at.kvh * grp + row - token * grp) * D;
-                    } else if (g == 0) ml[row] = make_float2(m, first && (blind >> row & 1) ? -1.0f : l);
+                    const int token = row / grp;
+                    uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(row0 + token) * a.ldo + (int64_t)(kvh * grp + row - token * grp) * D;
+                    const float inv = whole ? (blind >> row & 1 ? 0.f : 1.0f / l) : 1.0f;
+                    if (!whole && g == 0) ml[row] = make_float2(m, first && (blind >> row & 1) ? -1.0f : l);
 #pragma unroll 4
                     for (int r = 0; r < KS * 2; ++r) {                                       // channel block r / 2 and the one or the other of a lane's two channels there
-                        const int i = r >> 1, up = r & 1, reg = (i / KH) * (Cfg::REGS / 2) + (b * KH + i % KH) * 4 + 2 * up + h, d = i * 16 + (BITS8 ? 2 * g + up : 8 * up + g);
+                        const int i = r >> 1, up = r & 1, reg = (i / KH) * (Cfg::REGS / Cfg::PARTS) + (b * KH + i % KH) * 4 + 2 * up + h, d = i * 16 + (BITS8 ? 2 * g + up : 8 * up + g);
                         float o = 0.f;
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) o += f[w] * states[(w * Cfg::REGS + reg) * 32 + lane];
-                        if (out) out[d] = f32_to_bf16_bits(o * inv); else po[(d >> 2) * (ROWS * 4) + row * 4 + (d & 3)] = o;
+                        for (int w = 0; w < STATES; ++w) o += f[w] * states[(w * Cfg::REGS + reg) * 32 + lane];
+                        if (whole) out[d] = f32_to_bf16_bits(o * inv); else po[(d >> 2) * (ROWS * 4) + row * 4 + (d & 3)] = o;
                     }
                 }
             __syncwarp();
             if (lane == 0) mbar_arrive(states_empty);
+            if (!more) break;
         }
         griddep_launch();
         return;
     }
 
-    // Warps w and w + 4 take the same 16 tokens of every page and half of the channels each.  Tokens are the 16 rows of the first product and channels those of the second, the item's rows the 8
-    // columns of both: S^T = K Q^T, O^T = V^T P^T
-    const int g = lane >> 2, t = lane & 3, quarter = warp & 3, half = warp >> 2;
-    int st = 0, n_items = 0; uint32_t ph = 0;
-    for (int64_t u = u_begin; u < u_end; next(), ++n_items) {
-        const int c0 = (int)max(u - at.unit0 - 1, (int64_t)0), c1 = (int)min((int64_t)at.s.pages, u_end - at.unit0 - 1);
-        u = at.unit0 + 1 + c1;
-        float oacc[NB][KH][4], m_run[NB][2], l_run[NB][2], factor[NB][2];                    // O^T: two channels of a lane in each block of 16, rows 2 t and 2 t + 1; maxima, sums and score factors of these rows
-        float vref = 0.f;                                                                    // 8 bits: a power of two that no value's scale so far passes
+    // Tokens are the 16 rows of the first product and channels those of the second, the item's rows the 8 columns of both: S^T = K Q^T, O^T = V^T P^T.  A row's reference maximum rises (and its sums are
+    // rescaled) only where a score passes it by 2^8
+    const int g = lane >> 2, t = lane & 3, quarter = warp & 3, half = Cfg::PARTS == 2 ? warp >> 2 : 0, group = Cfg::GROUPS == 2 ? warp >> 2 : 0;
+    constexpr float kRaise = 8.0f;
+    constexpr float kValueUp = 128.f;                                                        // a weight is 2^8 at most: fp16 holds it times a value's scale
+    uint32_t pages = 0, n_items = 0;                                                         // of the items before
+    for (bool more = true; more; ++n_items) {
         mbar_wait(&q_full[n_items & 1], (n_items >> 1) & 1);
+        const FewItem& item = *reinterpret_cast<const FewItem*>(item_s + (n_items & 1) * 80);
         const TreeMeta* meta = meta_s + (n_items & 1) * ROWS;
+        const int c0 = item.c0, c1 = max(item.c0, item.c1), special_below = item.low, special_from = item.high;
+        more = item.more;
+        float oacc[NB][KH][4], m_run[NB][2], l_run[NB][2], factor[NB][2];                    // O^T: two channels of a lane in each block of 16, rows 2 t and 2 t + 1; references, sums and score factors of these rows
+        float vref = 0.f;                                                                    // 8 bits: a power of two that no value's scale so far passes
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -374,11 +389,12 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
             for (int h = 0; h < 2; ++h) { m_run[b][h] = -INFINITY; l_run[b][h] = 0.f; factor[b][h] = meta[b * 8 + 2 * t + h].factor; }
         }
         const uint8_t* q_item = q_s + (n_items & 1) * Cfg::Q_BYTES;
-        for (int c = c0; c < c1; ++c) {
-            const int page = at.s.page(c), key0 = page * CACHE_PAGE + quarter * 16;
-            const bool special = at.s.special(a, page);
-            mbar_wait(&full_bar[st], ph);
-            if (key0 < at.s.end) {
+        for (int c = c0 + (Cfg::GROUPS == 2 ? (int)((pages ^ group) & 1) : 0); c < c1; c += Cfg::GROUPS) {
+            const uint32_t n = pages + (c - c0), st = n % STAGES;
+            const bool special = c < special_below || c >= special_from;
+            mbar_wait(&full_bar[st], (n / STAGES) & 1);
+            const int key0 = special ? item.s.page(c) * CACHE_PAGE + quarter * 16 : 0;
+            if (!special || key0 < item.s.end) {
                 const uint8_t* stage = smem + st * Cfg::STAGE_BYTES;
                 const uint32_t kbase = smem_u32(stage), vbase = kbase + Cfg::KV_BYTES;
                 float sacc[NB][2][4];                                                        // even and odd steps apart: two chains of products
@@ -439,9 +455,9 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
                             const TreeMeta m = meta[b * 8 + 2 * t + h];
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                const int key = key0 + g + 8 * e, n = key - at.s.ctx;
-                                const bool sees = n < 0 ? key < a.sinks || key >= m.low : key < at.s.end && n < 64 && (m.seen >> (n & 63) & 1);
-                                if (sees && b * 8 + 2 * t + h < ROWS) vis |= 1u << (b * 4 + e * 2 + h);
+                                const int key = key0 + g + 8 * e, u = key - item.s.ctx;
+                                const bool sees = u < 0 ? key < a.sinks || key >= m.low : key < item.s.end && u < 64 && (m.seen >> (u & 63) & 1);
+                                if (sees) vis |= 1u << (b * 4 + e * 2 + h);
                             }
                         }
                     constexpr uint32_t LO = NB == 2 ? 0x33u : 0x3u;
@@ -451,80 +467,103 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
                 if constexpr (BITS8) {
                     // a bit of a token is in its four lanes together: whoever is not seen by anyone counts for nothing
                     const bool see_lo = any_lo >> (g * 4) & 0xfu, see_hi = any_hi >> (g * 4) & 0xfu;
-                    uint32_t top = max(see_lo && vscale[0] < INFINITY ? __float_as_uint(fabsf(vscale[0])) : 0u, see_hi && vscale[1] < INFINITY ? __float_as_uint(fabsf(vscale[1])) : 0u);
-                    top = __reduce_max_sync(0xffffffffu, top);
-                    const float need = __uint_as_float(min((top & 0x7f800000u) + 0x00800000u, 0x7e800000u));         // up to 2^126
-                    if (need > vref) { grown = vref * (1.0f / need); vref = need; }
-                    const float inv = 1.0f / vref;                                           // powers of two: exact
-                    vfac[0] = vscale[0] * inv * 32768.f; vfac[1] = vscale[1] * inv * 32768.f;
+                    const float top = fmaxf(see_lo && vscale[0] < INFINITY ? fabsf(vscale[0]) : 0.f, see_hi && vscale[1] < INFINITY ? fabsf(vscale[1]) : 0.f);
+                    if (__any_sync(0xffffffffu, top >= vref)) {
+                        const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+                        const float need = __uint_as_float(min(max((most & 0x7f800000u) + 0x00800000u, 0x0d800000u), 0x7e800000u));     // 2^-100 to 2^126
+                        if (need > vref) { grown = vref * (1.0f / need); vref = need; }
+                    }
+                    const float inv = kValueUp / vref;                                       // powers of two: exact
+                    vfac[0] = vscale[0] * inv; vfac[1] = vscale[1] * inv;
                 }
-                uint32_t pb[NB][2]; float alpha[NB][2];
-                bool same = grown == 1.0f;
+                uint32_t pb[NB][2]; float sc[NB][2][2];
+                bool raise = false;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        sc[b][h][0] = vis >> (b * 4 + h) & 1 ? (sacc[b][0][h] + sacc[b][1][h]) * (BITS8 ? kscale[0] * factor[b][h] : factor[b][h]) : -INFINITY;
+                        sc[b][h][1] = vis >> (b * 4 + 2 + h) & 1 ? (sacc[b][0][2 + h] + sacc[b][1][2 + h]) * (BITS8 ? kscale[1] * factor[b][h] : factor[b][h]) : -INFINITY;
+                        raise = raise || fmaxf(sc[b][h][0], sc[b][h][1]) > m_run[b][h] + kRaise;
+                    }
+                if (__any_sync(0xffffffffu, raise) || grown != 1.0f) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        float alpha[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float mx = fmaxf(sc[b][h][0], sc[b][h][1]);
+#pragma unroll
+                            for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                            const float m_new = mx > m_run[b][h] + kRaise ? mx : m_run[b][h];
+                            alpha[h] = m_new == m_run[b][h] ? 1.0f : ex2_approx(m_run[b][h] - finite_or_zero(m_new));
+                            m_run[b][h] = m_new;
+                            l_run[b][h] *= alpha[h]; alpha[h] *= grown;
+                        }
+#pragma unroll
+                        for (int i = 0; i < KH; ++i) { oacc[b][i][0] *= alpha[0]; oacc[b][i][1] *= alpha[1]; oacc[b][i][2] *= alpha[0]; oacc[b][i][3] *= alpha[1]; }
+                    }
+                }
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     float pr[4];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const bool s0 = vis >> (b * 4 + h) & 1, s1 = vis >> (b * 4 + 2 + h) & 1;
-                        const float lo = s0 ? (sacc[b][0][h] + sacc[b][1][h]) * (BITS8 ? kscale[0] * factor[b][h] : factor[b][h]) : -INFINITY;
-                        const float hi = s1 ? (sacc[b][0][2 + h] + sacc[b][1][2 + h]) * (BITS8 ? kscale[1] * factor[b][h] : factor[b][h]) : -INFINITY;
-                        float mx = fmaxf(lo, hi);
-#pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                        const float m_new = fmaxf(m_run[b][h], mx), ref = finite_or_zero(m_new);
-                        alpha[b][h] = ex2_approx(m_run[b][h] - ref);
-                        const float p0 = ex2_approx(lo - ref), p1 = ex2_approx(hi - ref);
-                        l_run[b][h] = l_run[b][h] * alpha[b][h] + (p0 + p1);
-                        alpha[b][h] *= grown;
-                        pr[h] = s0 && BITS8 ? p0 * vfac[0] : p0; pr[2 + h] = s1 && BITS8 ? p1 * vfac[1] : p1;       // 0 of a token that the row does not see, whatever its scale
-                        same = same && m_new == m_run[b][h];
-                        m_run[b][h] = m_new;
+                        const float ref = finite_or_zero(m_run[b][h]);
+                        const float p0 = ex2_approx(sc[b][h][0] - ref), p1 = ex2_approx(sc[b][h][1] - ref);
+                        l_run[b][h] += p0 + p1;
+                        // 0 of a token that the row does not see, whatever its scale
+                        pr[h] = !BITS8 ? p0 : vis >> (b * 4 + h) & 1 ? p0 * vfac[0] : 0.f; pr[2 + h] = !BITS8 ? p1 : vis >> (b * 4 + 2 + h) & 1 ? p1 * vfac[1] : 0.f;
                     }
                     if (BITS8) { pb[b][0] = transpose_8x8(pack_f16x2(pr[0], pr[1])); pb[b][1] = transpose_8x8(pack_f16x2(pr[2], pr[3])); }
                     else { pb[b][0] = transpose_8x8(pack_bf16x2(pr[0], pr[1])); pb[b][1] = transpose_8x8(pack_bf16x2(pr[2], pr[3])); }
                 }
-                if (!__all_sync(0xffffffffu, same)) {
-#pragma unroll
-                    for (int b = 0; b < NB; ++b)
-#pragma unroll
-                        for (int i = 0; i < KH; ++i) { oacc[b][i][0] *= alpha[b][0]; oacc[b][i][1] *= alpha[b][1]; oacc[b][i][2] *= alpha[b][0]; oacc[b][i][3] *= alpha[b][1]; }
+                // values of tokens 2 t, 2 t + 1 and these + 8; what nobody sees may be anything, and 0 x inf is not 0
+                uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+                if (special) {
+                    keep0 = (any_lo >> (8 * t) & 0xfu ? 0xffffu : 0u) | (any_lo >> (8 * t + 4) & 0xfu ? 0xffff0000u : 0u);
+                    keep1 = (any_hi >> (8 * t) & 0xfu ? 0xffffu : 0u) | (any_hi >> (8 * t + 4) & 0xfu ? 0xffff0000u : 0u);
                 }
-                // values of tokens 2 t, 2 t + 1 and these + 8
-                uint32_t vf[KH][4];
                 if constexpr (BITS8) {
                     const int r = quarter * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
 #pragma unroll
                     for (int i = 0; i < KH; i += 2) {
-                        uint32_t w[4];
-                        ldmatrix_x4_trans(vbase + few_off8<D>(r, half * KH + i + (lane >> 4)), w[0], w[1], w[2], w[3]);
+                        uint32_t w[4], vf[2][4];
+                        ldmatrix_x4_trans(vbase + few_off8<D>(r, i + (lane >> 4)), w[0], w[1], w[2], w[3]);
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) { to_f16<FMT, true>(w[2 * e], vf[i + e][0], vf[i + e][1]); to_f16<FMT, true>(w[2 * e + 1], vf[i + e][2], vf[i + e][3]); }
+                        for (int e = 0; e < 2; ++e) { to_f16<FMT, true>(w[2 * e], vf[e][0], vf[e][1]); to_f16<FMT, true>(w[2 * e + 1], vf[e][2], vf[e][3]); }
+                        if (special)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) { vf[e][0] &= keep0; vf[e][1] &= keep0; vf[e][2] &= keep1; vf[e][3] &= keep1; }
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) mma_of<FMT>(oacc[b][i + e], vf[e][0], vf[e][1], vf[e][2], vf[e][3], pb[b][0], pb[b][1]);
                     }
                 } else {
                     const int r = quarter * 16 + ((lane >> 4) << 3) + (lane & 7), dsel = ((lane >> 3) & 1) << 3;
+                    uint32_t vf[KH][4];
 #pragma unroll
                     for (int i = 0; i < KH; ++i) ldmatrix_x4_trans(vbase + few_off<D>(r, (half * KH + i) * 16 + dsel), vf[i][0], vf[i][1], vf[i][2], vf[i][3]);
+                    if (special)
+#pragma unroll
+                        for (int i = 0; i < KH; ++i) { vf[i][0] &= keep0; vf[i][1] &= keep0; vf[i][2] &= keep1; vf[i][3] &= keep1; }
+#pragma unroll
+                    for (int i = 0; i < KH; ++i)
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) mma_of<FMT>(oacc[b][i], vf[i][0], vf[i][1], vf[i][2], vf[i][3], pb[b][0], pb[b][1]);
                 }
-                if (special) {                                                               // values that nobody sees may be anything, and 0 x inf is not 0
-                    const uint32_t keep0 = (any_lo >> (8 * t) & 0xfu ? 0xffffu : 0u) | (any_lo >> (8 * t + 4) & 0xfu ? 0xffff0000u : 0u);
-                    const uint32_t keep1 = (any_hi >> (8 * t) & 0xfu ? 0xffffu : 0u) | (any_hi >> (8 * t + 4) & 0xfu ? 0xffff0000u : 0u);
-#pragma unroll
-                    for (int i = 0; i < KH; ++i) { vf[i][0] &= keep0; vf[i][1] &= keep0; vf[i][2] &= keep1; vf[i][3] &= keep1; }
-                }
-#pragma unroll
-                for (int i = 0; i < KH; ++i)
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) mma_of<FMT>(oacc[b][i], vf[i][0], vf[i][1], vf[i][2], vf[i][3], pb[b][0], pb[b][1]);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty_bar[st]);
-            if (++st == STAGES) { st = 0; ph ^= 1; }
         }
+        pages += c1 - c0;
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_empty[n_items & 1]);
-        // the four quarters' states, for the warp that brings them together while this one goes on
+        // the states of the quarters (of either group's), for the warp that brings them together while this one goes on
         mbar_wait(states_empty, (n_items & 1) ^ 1);
-        float* mine = states + (quarter * Cfg::REGS + half * (Cfg::REGS / 2)) * 32 + lane;   // value [half][b][i][e]
+        const int state = group * 4 + quarter;
+        float* mine = states + (state * Cfg::REGS + half * (Cfg::REGS / Cfg::PARTS)) * 32 + lane;                // value [part][b][i][e]
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -532,14 +571,14 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
                 float l = l_run[b][h];
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-                if (half == 0 && g == 0) *reinterpret_cast<float2*>(ml_s + (quarter * ROWS + b * 8 + 2 * t + h) * 2) = make_float2(m_run[b][h], l);
+                if (half == 0 && g == 0) *reinterpret_cast<float2*>(ml_s + (state * ROWS + b * 8 + 2 * t + h) * 2) = make_float2(m_run[b][h], l);
             }
 #pragma unroll
             for (int i = 0; i < KH; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mine[((b * KH + i) * 4 + e) * 32] = oacc[b][i][e];
         }
-        if (BITS8 && half == 0 && lane == 0) vref_s[quarter] = vref * (1.0f / 32768.f);
+        if (BITS8 && lane == 0) vref_s[state] = vref * (1.0f / kValueUp);
         __syncwarp();
         if (lane == 0) mbar_arrive(states_full);
     }
@@ -592,14 +631,6 @@ OA_DEVINL uint64_t tree_word(const TreeAttnArgs& a, const TreeSeq& s, uint64_t s
     const int d = s.ctx - key;
     const uint64_t fresh = d >= 64 || d <= -64 ? 0ull : d >= 0 ? seen << d : seen >> -d;
     return (old | fresh) & low_bits(s.end - key);
-}
-
-// how many tiles of two of a sequence's pages begin below a place of its window
-OA_DEVINL int tiles_below(const TreeSeq& s, int place) {
-    if (place <= 0) return 0;
-    const int page = pages_of(place) - 1;                                        // the last page that begins below it
-    const int c = page < s.low_pages ? page : max(page - s.skip, s.low_pages - 1);
-    return (c + 2) / 2;
 }
 
 // Queries in fp16, a row of a head under a power of two that brings its largest magnitude to [2^14, 2^15): a warp eight rows.  What the next kernel reads besides was written by kernels that have ended
@@ -911,7 +942,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                     const TreeSeq& s = at.s;
                     p.s = s;
                     p.c0 = c0; p.c1 = c1; p.seq = at.seq; p.kvh = at.kvh; p.row0 = at.row0(); p.rows = rows;
-                    p.s0 = a.window > 0 ? tiles_below(s, s.ctx + s.n - a.window) : 0; p.s1 = min((s.ctx / CACHE_PAGE - s.skip) / 2, s.pages / 2);
+                    p.s0 = a.window > 0 ? (pages_below(s, s.ctx + s.n - a.window) + 1) / 2 : 0; p.s1 = min((s.ctx / CACHE_PAGE - s.skip) / 2, s.pages / 2);
                     p.first = at.unit0 >= u_begin; p.last = end <= u_end; p.more = end < u_end;
                     if (p.first && !p.last) tree_record(a, cta_of(end - 1, share.busy, share.total) - (int)blockIdx.x, p.row0, rows, p.kvh);
                 }
@@ -1284,7 +1315,7 @@ template <int D, int FMT>
 static cudaError_t launch_parts(const CUtensorMap* tm_q, const CUtensorMap* tm_page, const TreeAttnArgs& a, cudaStream_t s) {
     constexpr int MORE = D == 64 ? 2 : 1;
     const cudaError_t e = a.rows == 128 ? launch_many<D, FMT>(tm_q, tm_page, a, s)
-                        : a.rows == 8 ? launch_few<D, FMT, 1, 5 * MORE>(tm_page, a, s) : launch_few<D, FMT, 2, (FMT == CACHE_BF16 ? 5 : 9) * MORE>(tm_page, a, s);
+                        : a.rows == 8 ? launch_few<D, FMT, 1, (FMT == CACHE_BF16 ? 5 : 4) * MORE>(tm_page, a, s) : launch_few<D, FMT, 2, (FMT == CACHE_BF16 ? 5 : 8) * MORE>(tm_page, a, s);
     return e == cudaSuccess ? launch_tree_join<D>(a, s) : e;
 }
 template <int D>
