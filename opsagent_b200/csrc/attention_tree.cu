@@ -1004,6 +1004,32 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
             const float row_fac = p.factor[row];
             float undo = 1.0f;
             float m_mine = -INFINITY, l_run = 0.f;                               // the sum so far and the reference that it is under
+            auto clear_unseen = [&](uint32_t n) {
+                const int kt = c0 + (int)(n - n0);
+                    // values that none of the rows sees may be anything, and 0 x inf is not 0: a thread looks after the key of its row's number
+                    const uint32_t entry = 2 * n0 + min(tiles, kt - c0 + 3) + (kt - c0), slot = entry % SLOTS;
+                    mbar_wait(&full[slot], (entry / SLOTS) & 1);
+                    const int c = 2 * kt + (row >> 6);
+                    if (c >= s.pages || !p.any.sees(a, s, s.page(c) * CACHE_PAGE + (row & 63))) {
+#pragma unroll
+                        for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(kv_s + slot * TILE + (c >> 3) * HALF + row * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    fence_proxy_async();
+            };
+            // a warp without rows keeps the others' pace and clears the keys that it looks after
+            auto pace = [&](uint32_t n, bool special) {
+                const uint32_t from = n % 3;
+                mbar_wait(&s_full[from], (n / 3) & 1);
+                if (n > n0) take_turn(n);
+                if (n > 2) mbar_wait(&o_full[(n - 3) & 3], ((n - 3) >> 2) & 1);
+                if (n + 1 < n1) pass_turn(n + 1);
+                if (special && !BITS8) clear_unseen(n);
+                if (BITS8) undo = sc_s[n % SC * Cfg::SC_FLOATS + 2 * KEYS + 2];
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(&p_full[from]); if (BITS8) mbar_arrive(&sc_empty[n % SC]); }
+            };
+            const bool idle = quarter * 32 >= p.rows;
             auto tile = [&](uint32_t n, auto tag) {
                 constexpr bool SPECIAL = decltype(tag)::value;
                 const int kt = c0 + (int)(n - n0);
@@ -1065,17 +1091,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                         tmem_st_32x32b_x16(o_addr + c, o);
                     }
                 }
-                if (SPECIAL && !BITS8) {
-                    // values that none of the rows sees may be anything, and 0 x inf is not 0: a thread looks after the key of its row's number
-                    const uint32_t entry = 2 * n0 + min(tiles, kt - c0 + 3) + (kt - c0), slot = entry % SLOTS;
-                    mbar_wait(&full[slot], (entry / SLOTS) & 1);
-                    const int c = 2 * kt + (row >> 6);
-                    if (c >= s.pages || !p.any.sees(a, s, s.page(c) * CACHE_PAGE + (row & 63))) {
-#pragma unroll
-                        for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(kv_s + slot * TILE + (c >> 3) * HALF + row * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    }
-                    fence_proxy_async();
-                }
+                if (SPECIAL && !BITS8) clear_unseen(n);
                 if (m_mine != m_ref) { l_run *= ex2_approx(m_mine - m_ref); m_mine = m_ref; }
                 const float neg_ref = kLift - finite_or_zero(m_ref);
                 uint64_t sum = 0;
@@ -1103,7 +1119,8 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
             };
             for (uint32_t n = n0 + ((n0 ^ wg) & 1); n < n1; n += 2) {
                 const int kt = c0 + (int)(n - n0);
-                if (kt < p.s0 || kt >= p.s1) tile(n, TrueTag{}); else tile(n, FalseTag{});
+                const bool special = kt < p.s0 || kt >= p.s1;
+                if (idle) pace(n, special); else if (special) tile(n, TrueTag{}); else tile(n, FalseTag{});
             }
             n0 = n1;
             meet();                                                              // the last tile's reference is there
