@@ -231,19 +231,19 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
                 int page = __shfl_sync(0xffffffffu, have, c & 31);
                 if (page < 0 || page >= a.num_pages) { if (lane == 0 && a.status) *a.status = 400; page = 0; }
                 mbar_wait(&empty_bar[st], ph ^ 1);
-                if (lane == 0) {
-                    uint8_t* dst = smem + st * Cfg::STAGE_BYTES;
-                    mbar_expect_tx(&full_bar[st], Cfg::STAGE_BYTES + Cfg::SCALE_BYTES);
-#pragma unroll
-                    for (int v = 0; v < 2; ++v) {
-                        const int64_t block = (int64_t)(v * a.num_pages + page) * a.n_kv + at.kvh;
-                        if (BITS8) {
-                            constexpr int BLOCK_BYTES = CACHE_PAGE * (D + 4);
-                            tma_load_2d(dst + v * Cfg::KV_BYTES, &tm_page, &full_bar[st], 0, (int)(block * (BLOCK_BYTES / 128)), kEvictFirst);
-                            bulk_load(scales_s + st * Cfg::SCALE_BYTES + v * CACHE_PAGE * 4, reinterpret_cast<const uint8_t*>(a.cache) + block * BLOCK_BYTES + CACHE_PAGE * D, CACHE_PAGE * 4, &full_bar[st]);
-                        } else
-#pragma unroll
-                            for (int h = 0; h < D / 64; ++h) tma_load_2d(dst + v * Cfg::KV_BYTES + h * (CACHE_PAGE * 128), &tm_page, &full_bar[st], h * 64, (int)(block * CACHE_PAGE), kEvictFirst);
+                if (lane == 0) mbar_expect_tx(&full_bar[st], Cfg::STAGE_BYTES + Cfg::SCALE_BYTES);
+                __syncwarp();
+                // a lane a copy: one that issues them all takes longer for it than a page's warps do
+                constexpr int COPIES = BITS8 ? 2 : D / 64;                                   // of keys, of values
+                if (lane < 2 * COPIES) {
+                    const int v = lane / COPIES, part = lane % COPIES;
+                    uint8_t* dst = smem + st * Cfg::STAGE_BYTES + v * Cfg::KV_BYTES;
+                    const int64_t block = (int64_t)(v * a.num_pages + page) * a.n_kv + at.kvh;
+                    if (!BITS8) tma_load_2d(dst + part * (CACHE_PAGE * 128), &tm_page, &full_bar[st], part * 64, (int)(block * CACHE_PAGE), kEvictFirst);
+                    else {
+                        constexpr int BLOCK_BYTES = CACHE_PAGE * (D + 4);
+                        if (part == 0) tma_load_2d(dst, &tm_page, &full_bar[st], 0, (int)(block * (BLOCK_BYTES / 128)), kEvictFirst);
+                        else bulk_load(scales_s + st * Cfg::SCALE_BYTES + v * CACHE_PAGE * 4, reinterpret_cast<const uint8_t*>(a.cache) + block * BLOCK_BYTES + CACHE_PAGE * D, CACHE_PAGE * 4, &full_bar[st]);
                     }
                 }
                 __syncwarp();
@@ -620,7 +620,7 @@ struct ManyCfg {
     static constexpr int RAW_BYTES = KEYS * D, RAW = BITS8 ? (D == 128 ? 5 : 8) : 0;         // a tile of 8 bits, and how many wait
     static constexpr int SC = 8, SC_FLOATS = 2 * KEYS + 4;                       // tiles whose scales wait: keys', values', what scores are multiplied by, what O is for larger scales of values and at its end
     static constexpr int CONV = BITS8 ? 8 : 0, THREADS = 128 + 256 + 32 * CONV;     // producer, issuer, scales, pieces; eight softmax warps; warps that convert
-    static constexpr int BARS = 18 + 2 * SLOTS + 2 * RAW + (BITS8 ? 3 * SC : 0);
+    static constexpr int BARS = 18 + 2 * SLOTS + 2 * RAW + (BITS8 ? 2 * SC : 0);
     static constexpr int SMEM_BYTES = TILE_BYTES + SLOTS * TILE_BYTES + RAW * RAW_BYTES + (BITS8 ? SC * SC_FLOATS * 4 : 0) + 3 * 128 * 4 + BARS * 8 + 16 + 2 * sizeof(TreePiece);
     static constexpr uint32_t O_COL = 384;                                       // TMEM: S and P of the tiles in turn at 0, 128 and 256
 };
@@ -684,7 +684,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
     float* l_s = m_s + 128;
     uint64_t* bars = reinterpret_cast<uint64_t*>(l_s + 256);
     uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_full = bars + 5, *o_full = bars + 8, *full = bars + 12, *empty = full + SLOTS;
-    uint64_t *piece_full = empty + SLOTS, *rows_full = piece_full + 2, *piece_empty = rows_full + 2, *raw_full = piece_empty + 2, *raw_empty = raw_full + Cfg::RAW, *sc_in = raw_empty + Cfg::RAW, *sc_full = sc_in + SC, *sc_empty = sc_full + SC;
+    uint64_t *piece_full = empty + SLOTS, *rows_full = piece_full + 2, *piece_empty = rows_full + 2, *raw_full = piece_empty + 2, *raw_empty = raw_full + Cfg::RAW, *sc_full = raw_empty + Cfg::RAW, *sc_empty = sc_full + SC;
     TreePiece* piece_s = reinterpret_cast<TreePiece*>(bars + Cfg::BARS);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(piece_s + 2);
     __shared__ int64_t sums[Cfg::THREADS / 32];
@@ -703,7 +703,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
         for (int i = 0; i < SLOTS; ++i) { mbar_init(&full[i], BITS8 ? Cfg::CONV : 1); mbar_init(&empty[i], 1); }
         if (BITS8) {
             for (int i = 0; i < RAW; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], Cfg::CONV); }
-            for (int i = 0; i < SC; ++i) { mbar_init(&sc_in[i], 1); mbar_init(&sc_full[i], 1); mbar_init(&sc_empty[i], 4 + Cfg::CONV); }
+            for (int i = 0; i < SC; ++i) { mbar_init(&sc_full[i], 1); mbar_init(&sc_empty[i], 4 + Cfg::CONV); }
         }
         fence_barrier_init();
     }
@@ -739,7 +739,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
         if (warp == 0) {
             constexpr int RING = BITS8 ? RAW : SLOTS;
             uint64_t *in = BITS8 ? raw_full : full, *out = BITS8 ? raw_empty : empty;
-            uint32_t n = 0, seg = 0, g = 0;                                          // entries, pieces and tiles loaded
+            uint32_t n = 0, seg = 0;                                                 // entries and pieces loaded
             pieces(false, [&](const TreePiece& p) {
                 const int c0 = p.c0, c1 = p.c1;
                 if (c1 == c0) return;
@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                 };
                 if (!BITS8) load_q();
                 const int32_t* table = a.tables + (int64_t)p.seq * a.max_pages;
-                int page[3][2] = {}, have = 0, later = 0, scales = c0;               // pages of this tile and of the two before
+                int page[3][2] = {}, have = 0, later = 0;                            // pages of this tile and of the two before
                 for (int kt = c0; kt < c1 + 2; ++kt) {
                     if (kt < c1 && (kt == c0 || (kt & 15) == 0)) {                   // 32 page numbers, and the next 32 on their way
                         const int w = (2 * kt & ~31) + lane, stop = min(2 * c1, p.s.pages);
@@ -772,27 +772,6 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                         if (kt >= c1 || 2 * kt + i >= p.s.pages) page[0][i] = 0;
                         if (page[0][i] < 0 || page[0][i] >= a.num_pages) { if (lane == 0 && a.status) *a.status = 400; page[0][i] = 0; }
                     }
-                    if constexpr (BITS8) {
-                        for (; scales < min(kt + 4, c1); ++scales, ++g) {            // scales go through a warp of their own first: they come early
-                            const uint32_t buf = g % SC;
-                            const int some = min(2, p.s.pages - 2 * scales);
-                            mbar_wait(&sc_empty[buf], ((g / SC) & 1) ^ 1);
-                            if (elect_one()) mbar_expect_tx(&sc_in[buf], some * 2 * CACHE_PAGE * 4);
-                            __syncwarp();
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                if (i >= some) break;
-                                int pg = __shfl_sync(0xffffffffu, (scales >> 4) == (kt >> 4) ? have : later, (2 * scales + i) & 31);
-                                if (pg < 0 || pg >= a.num_pages) pg = 0;
-                                if (elect_one()) {
-                                    for (int w = 0; w < 2; ++w)
-                                        bulk_load(sc_s + buf * Cfg::SC_FLOATS + w * KEYS + i * CACHE_PAGE, reinterpret_cast<const uint8_t*>(a.cache) +
-                                                  ((int64_t)(w * (int64_t)a.num_pages + pg) * a.n_kv + p.kvh) * BLOCK_BYTES + CACHE_PAGE * D, CACHE_PAGE * 4, &sc_in[buf]);
-                                }
-                                __syncwarp();
-                            }
-                        }
-                    }
 #pragma unroll
                     for (int v = 0; v < 2; ++v) {
                         const int t = kt - 2 * v;                                    // K of this tile, V of the one two before
@@ -800,17 +779,14 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                         const int there = min(2, p.s.pages - 2 * t);                // a missing second page is not loaded: its scores are masked, its values set to zero
                         const uint32_t slot = n % RING;
                         mbar_wait(&out[slot], ((n / RING) & 1) ^ 1);
-                        if (elect_one()) {
-                            mbar_expect_tx(&in[slot], there * (BITS8 ? CACHE_PAGE * D : HALVES * 8192));
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                if (i >= there) break;
-                                const int64_t block = ((int64_t)v * a.num_pages + (v ? page[2][i] : page[0][i])) * a.n_kv + p.kvh;
-                                if (BITS8) bulk_load(raw_s + slot * Cfg::RAW_BYTES + i * CACHE_PAGE * D, reinterpret_cast<const uint8_t*>(a.cache) + block * BLOCK_BYTES, CACHE_PAGE * D, &in[slot]);
-                                else
-#pragma unroll
-                                    for (int h = 0; h < HALVES; ++h) tma_load_2d(kv_s + slot * TILE + h * HALF + i * 8192, &tm_kv, &in[slot], h * 64, (int)(block * CACHE_PAGE), kEvictNormal);
-                            }
+                        if (lane == 0) mbar_expect_tx(&in[slot], there * (BITS8 ? CACHE_PAGE * D : HALVES * 8192));
+                        __syncwarp();
+                        constexpr int COPIES = BITS8 ? 1 : HALVES;                   // of a page, a lane each: one lane that issues them all takes longer for it than the tile does
+                        if (lane < there * COPIES) {
+                            const int i = lane / COPIES, h = lane % COPIES;
+                            const int64_t block = ((int64_t)v * a.num_pages + (v ? (i ? page[2][1] : page[2][0]) : (i ? page[0][1] : page[0][0]))) * a.n_kv + p.kvh;
+                            if (BITS8) bulk_load(raw_s + slot * Cfg::RAW_BYTES + i * CACHE_PAGE * D, reinterpret_cast<const uint8_t*>(a.cache) + block * BLOCK_BYTES, CACHE_PAGE * D, &in[slot]);
+                            else tma_load_2d(kv_s + slot * TILE + h * HALF + i * 8192, &tm_kv, &in[slot], h * 64, (int)(block * CACHE_PAGE), kEvictNormal);
                         }
                         __syncwarp();
                         ++n;
@@ -878,14 +854,32 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
             if constexpr (BITS8) {
                 uint32_t n = 0;
                 pieces(true, [&](const TreePiece& p) {
-                    const int c0 = p.c0, c1 = p.c1;
+                    const int c0 = p.c0, c1 = p.c1, stop = min(2 * c1, p.s.pages);
+                    const int32_t* table = a.tables + (int64_t)p.seq * a.max_pages;
+                    int have = 0, later = 0;
+                    auto entry = [&](int w) { return w < stop ? __ldcg(table + p.s.page(w)) : 0; };
+                    // four keys' and values' scales a lane, a tile ahead; a bad page number is told where its bytes are loaded
+                    auto load = [&](int kt, float4 (&x)[2]) {
+                        if (kt == c0 || (kt & 15) == 0) { have = kt == c0 ? entry((2 * kt & ~31) + lane) : later; later = entry((2 * kt & ~31) + 32 + lane); }
+                        const int w = 2 * kt + (lane >> 4);
+                        int page = __shfl_sync(0xffffffffu, have, w & 31);
+                        if (page < 0 || page >= a.num_pages) page = 0;
+#pragma unroll
+                        for (int v = 0; v < 2; ++v) {
+                            x[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (w < stop) x[v] = __ldcg(reinterpret_cast<const float4*>(reinterpret_cast<const uint8_t*>(a.cache) + (((int64_t)v * a.num_pages + page) * a.n_kv + p.kvh) * BLOCK_BYTES + CACHE_PAGE * D) + (lane & 15));
+                        }
+                    };
+                    float4 ahead[2];
+                    if (c0 < c1) load(c0, ahead);
                     float vref = 0.f;
                     for (int kt = c0; kt < c1; ++kt, ++n) {
                         const uint32_t buf = n % SC;
                         float* sc = sc_s + buf * Cfg::SC_FLOATS;
                         const bool sp = kt < p.s0 || kt >= p.s1;
-                        mbar_wait(&sc_in[buf], (n / SC) & 1);
-                        float4 in[2] = {*reinterpret_cast<const float4*>(sc + 4 * lane), *reinterpret_cast<const float4*>(sc + KEYS + 4 * lane)};
+                        const float4 in[2] = {ahead[0], ahead[1]};
+                        if (kt + 1 < c1) load(kt + 1, ahead);
+                        mbar_wait(&sc_empty[buf], ((n / SC) & 1) ^ 1);
                         uint32_t mask = 0xf;
                         if (sp) {
                             const int c = 2 * kt + (lane >> 4);
@@ -921,7 +915,6 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                         }
                         vref = ref[1];
                         if (lane == 0) { sc[2 * KEYS] = ref[0] * (1.0f / kKeyUp); sc[2 * KEYS + 1] = grown; sc[2 * KEYS + 2] = vref * (1.0f / 128.f); }
-                        fence_proxy_async();                                         // the next scales to come here are another proxy's writes
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sc_full[buf]);
                     }
