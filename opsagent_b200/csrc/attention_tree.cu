@@ -30,6 +30,14 @@ OA_DEVINL void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(smem_u32(smem_dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
+OA_DEVINL void mbar_wait3(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, uint64_t* c, uint32_t pc) {        // phases that do not pass before this thread's own arrivals
+    uint32_t spins = 0;
+    for (;;) {
+        const bool x = mbar_try_wait(a, pa), y = mbar_try_wait(b, pb), z = mbar_try_wait(c, pc);
+        if (x && y && z) return;
+        if (++spins > OA_MBAR_SPIN_LIMIT) { __trap(); }
+    }
+}
 OA_DEVINL uint32_t pack_f16x2(float a, float b) { uint32_t r; asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a)); return r; }
 OA_DEVINL void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -1172,9 +1180,8 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                     if (t < 0 || t >= tiles) continue;
                     const uint32_t from = n % RAW, to = n % SLOTS;
                     const uint32_t* sc = reinterpret_cast<const uint32_t*>(sc_s + (g + t) % SC * Cfg::SC_FLOATS + (e & 1) * KEYS);
-                    if (!(e & 1)) mbar_wait(&sc_full[(g + t) % SC], ((g + t) / SC) & 1);
-                    mbar_wait(&raw_full[from], (n / RAW) & 1);
-                    mbar_wait(&empty[to], ((n / SLOTS) & 1) ^ 1);
+                    // keys' scales came with theirs for values.  Asked together: an answer takes 140 cycles
+                    mbar_wait3(&raw_full[from], (n / RAW) & 1, &empty[to], ((n / SLOTS) & 1) ^ 1, &sc_full[(g + t) % SC], ((g + t) / SC) & 1);
                     const uint8_t* src = raw_s + from * Cfg::RAW_BYTES + ch * 16;
                     uint8_t* dst = kv_s + to * TILE + (ch >> 2) * HALF;
                     auto convert = [&](auto tag) {
