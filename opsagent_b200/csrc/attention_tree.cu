@@ -102,7 +102,7 @@ OA_DEVINL uint64_t tree_seen(const TreeAttnArgs& a, const TreeSeq& s, int t) {
     const uint64_t there = s.n < 64 ? (1ull << s.n) - 1 : ~0ull;
     return (a.seen ? __ldcg(reinterpret_cast<const unsigned long long*>(a.seen) + s.row0 + t) : (2ull << t) - 1) & there;
 }
-OA_DEVINL int tree_low(const TreeAttnArgs& a, const TreeSeq& s, uint64_t seen, int t) { return a.window > 0 ? s.ctx + __popcll(seen & ((1ull << t) - 1)) - a.window + 1 : 0; }
+OA_DEVINL int tree_low(const TreeAttnArgs& a, const TreeSeq& s, uint64_t seen, int t) { return a.window > 0 ? max(s.ctx + __popcll(seen & ((1ull << t) - 1)) - a.window + 1, 0) : 0; }
 
 // A place in the list of (sequence, key/value head, row tile) items.  An item's units are OVER for itself and one for each PAGES of its sequence's pages
 template <int PAGES, int OVER>
