@@ -225,13 +225,14 @@ OA_API int oa_k_cache8_read(const void* kv_cache, int32_t num_pages, const int32
 OA_API int oa_k_cache8_copy(void* kv_cache, int32_t planes, int32_t num_pages, int32_t n_kv, int32_t head_dim, const oa_page_move* moves, int32_t n_moves, void* stream);
 /* attention of up to 64 new tokens of each sequence (one, a chain, a tree of drafts) over a layer's two planes of bf16 (format 0) or 8 bits.  Rows row_starts[i] .. row_starts[i + 1] - 1 of q (bf16) are
  * sequence i's new tokens; it has ctx_lens[i] cached tokens, and its new ones' keys and values lie behind them already, at places ctx_lens[i] + u of the pages block_tables[i, :].  Row r, token t of
- * its sequence, sees new token u where bit u of seen[r] is set (its ancestors, which come before it, and itself; bits of tokens that there are not say nothing); seen NULL: a chain, tokens 0 .. t.
+ * its sequence, sees new token u where bit u of seen[r] (a word a row of q) is set (its ancestors, which come before it, and itself; bits of tokens that there are not say nothing); seen NULL: a chain, 0 .. t.
  * It sees all cached tokens, or with a window (64 or more; 0: none) those less than `window` places before it and the first `sinks` ones; its place is ctx_lens[i] and the number of its
  * ancestors behind the first new one: bits of seen[r] below t.  A row that sees nothing gets zeros; rows of q that no sequence has are left as they are in out.
  * All arrays are on the device (row_starts [n_seqs + 1] rises; n_rows: rows of q).  scale 0: 1 / sqrt(head_dim).  head_dim 64 or 128, up to 16 query heads of a key/value head, 2^20 sequences, 2^24 rows,
  * 2^10 key/value heads and 2^24 pages a table; the cache is counted in 31 bits, by rows of 64 channels of bf16 or pieces of 128 bytes.  out is q itself (same pitch) or apart from it; pitches and addresses are multiples of
  * 16 bytes.  What lies behind a sequence's end or is seen by none of its rows may be anything; values of a token that some rows see and others do not are finite, or NaN may come out for all of them.
- * Softmax weights are rounded to bf16 (fp16 over 8 bits) for their product with the values, sums are fp32.  A page number beyond the cache, row bounds that fall or leave the rows, more than 64 new tokens, or a
+ * Softmax weights are rounded to bf16 (fp16 over 8 bits) for their product with the values, sums are fp32; over 8 bits, where sequences have more than 16 rows (new tokens' heads of a group) on average, scales
+ * and keys and values times them are rounded to fp16 as well.  A page number beyond the cache, row bounds that fall or leave the rows, more than 64 new tokens, or a
  * length beyond the table set *status; rows that read such a page hold no meaningful value, the rest is cut to what there is (the first 64 new tokens are computed) */
 OA_API int oa_k_tree_attention(const void* q, int64_t ldq, void* out, int64_t ldo, const void* kv_cache, int32_t format, int32_t num_pages, const int32_t* block_tables, int32_t max_pages_per_seq,
                          const int32_t* ctx_lens, const int32_t* row_starts, const uint64_t* seen, int32_t n_seqs, int32_t n_rows, int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t window,
