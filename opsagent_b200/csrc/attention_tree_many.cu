@@ -640,7 +640,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                             }
                         }
                     };
-                    if (e & 1) convert(FalseTag{}); else convert(TrueTag{});
+                    if (FMT == CACHE_INT8 && !(e & 1)) convert(TrueTag{}); else convert(FalseTag{});
                     if ((e & 1) && (c0 + t < p.s0 || c0 + t >= p.s1))                              // values that none of the rows sees may be anything, and 0 x inf is not 0
 #pragma unroll 1
                         for (int i = 0; i < STEPS; ++i) {
