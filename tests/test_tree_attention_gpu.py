@@ -446,3 +446,91 @@ def test_one_token_agrees_with_the_other_entries(L, fmt):
     torch.cuda.synchronize()
     big = b.values[1].nan_to_num().abs().max().item()
     assert (out.double() - b.out[:3].double()).abs().max().item() <= big * (2.0 ** -7 + (2.0 ** -8 if fmt != BF16 else 0) + 2.0 ** -9 * (64 if fmt != BF16 else 1) ** 0.5)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("new", [1, 24])
+def test_queries_that_are_not_finite(L, fmt, new):
+    """A NaN in a head of a row makes that head of that row NaN and nothing else."""
+    b = Batch(8, 2, 128, fmt, [150, 70], [new, 2], seed=24)
+    run(L, b)
+    good = b.out.clone()
+    q = b.q.clone()
+    q[0, 3 * 128 + 5] = math.nan
+    run(L, b, q=q)
+    assert torch.isnan(b.out[0, 3 * 128: 4 * 128]).all()
+    b.out[0, 3 * 128: 4 * 128] = good[0, 3 * 128: 4 * 128]
+    assert torch.equal(b.out, good)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_one_row_has_no_pitch(L, fmt):
+    b = Batch(4, 1, 64, fmt, [100], [1], seed=25, chain=True)
+    run(L, b)
+    want = b.out.clone()
+    d = b.d
+    for pitch in (256, 1 << 38):
+        b.out.fill_(5.0)
+        assert L.oa_k_tree_attention(ptr(b.q), pitch, ptr(b.out), pitch, ptr(b.cache), fmt, b.pages, ptr(d["tables"]), b.tables.shape[1], ptr(d["ctx"]), ptr(d["starts"]), None, 1, 1, 4, 1, 64, 0, 0, 0.0, None,
+                                     now()) == 0, _lib.last_error()
+        torch.cuda.synchronize()
+        assert torch.equal(b.out, want)
+
+
+@pytest.mark.parametrize("fmt", [BF16, INT8])
+@pytest.mark.parametrize("heads", [1, 16])
+def test_very_many_sequences(L, fmt, heads):
+    """70000 sequences of no or one new token on pages that they share."""
+    n, dim = 70000, 64
+    b = Batch(heads, 1, dim, fmt, [60], [1], seed=26, chain=True)
+    rng = np.random.default_rng(2)
+    new = (rng.random(n) < 0.7).astype(np.int32)
+    starts, rows = np.concatenate([[0], np.cumsum(new)]), int(new.sum())
+    tables = dev(np.full((n, 1), b.tables[0, 0]))
+    ctx = dev(np.full(n, 60))
+    q = b.q[:1, : heads * dim].repeat(rows, 1).contiguous()
+    out = torch.full((rows + 1, heads * dim), 5.0, dtype=torch.bfloat16, device="cuda")
+    s = dev(starts)
+    assert L.oa_k_tree_attention(ptr(q), heads * dim, ptr(out), heads * dim, ptr(b.cache), fmt, b.pages, ptr(tables), 1, ptr(ctx), ptr(s), None, n, rows, heads, 1, dim, 0, 0, 0.0, ptr(b.status), now()) == 0
+    torch.cuda.synchronize()
+    assert b.status.item() == 0 and (out[rows] == 5.0).all()
+    b.check(out=torch.cat([out[:1], torch.full_like(b.out[1:], 5.0)]))
+    assert (out[:rows] == out[0]).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_calls_from_two_threads(L, fmt):
+    import threading
+    bs = [Batch(8, 2, 64, fmt, [300, 40, 700], new, seed=27) for new in ([1, 2, 1], [30, 5, 64])]
+    want = []
+    for b in bs:
+        run(L, b)
+        want.append(b.out.clone())
+        b.out.fill_(5.0)
+    torch.cuda.synchronize()
+    streams, codes = [torch.cuda.Stream(), torch.cuda.Stream()], []
+
+    def work(b, st):
+        for _ in range(50):
+            code = b.call(L, stream=C.c_void_p(st.cuda_stream))
+            codes.append((code, _lib.last_error() if code else ""))
+    threads = [threading.Thread(target=work, args=x) for x in zip(bs, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert codes == [(0, "")] * 100, codes[0]
+    for b, w in zip(bs, want):
+        assert torch.equal(b.out, w)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("window", [0, 70])
+def test_trees_that_cross_tiles(L, fmt, window):
+    """New tokens on either side of pages, tiles of keys and tiles of rows, each seeing every third one before it."""
+    seen = [sum(1 << u for u in range(t + 1) if (t - u) % 3 == 0) for t in range(64)]
+    ctx = [0, 1, 63, 64, 65, 100, 127, 128, 129, 191, 192, 255, 256, 320]
+    b = Batch(10, 2, 128, fmt, ctx, [64] * len(ctx), seen=[seen] * len(ctx), seed=28, window=window, sinks=3 if window else 0)
+    run(L, b)
+    b.check()
