@@ -59,6 +59,8 @@ bool outside_cache(const void* cache, int64_t num_pages, int64_t n_kv, int64_t h
     const uintptr_t c = (uintptr_t)cache, p = (uintptr_t)x;
     return p + ((T - 1) * ldx + cols) * 2 <= c || c + 2 * num_pages * n_kv * CACHE_PAGE * head_dim * 2 <= p;
 }
+// whether n bytes at x lie in m bytes at y or the other way round (none of a null pointer's)
+bool meet(const void* x, uintptr_t n, const void* y, uintptr_t m) { return x && y && (uintptr_t)x < (uintptr_t)y + m && (uintptr_t)y < (uintptr_t)x + n; }
 // a list of moves that one launch can carry out in any order (may throw)
 const char* moves_wrong(int32_t num_pages, const oa_page_move* moves, int32_t n_moves) {
     if (n_moves < 0 || (n_moves > 0 && !moves)) return "cache copy: no moves";
@@ -88,8 +90,12 @@ const char* rows8_wrong(const void* k, const void* v, int64_t ldkv, const void* 
     if (!k || !v || !cache || !slots) return "8-bit cache: null pointer";
     if (((uintptr_t)k | (uintptr_t)v) % 2 || (uintptr_t)cache % 16 || ((uintptr_t)slots | (uintptr_t)status) % 4) return "8-bit cache: a pointer is not aligned (the cache to 16 bytes)";
     if (beyond_memory(T, ldkv)) return "8-bit cache: rows further apart than memory reaches";
-    const uintptr_t c = (uintptr_t)cache, bytes = 2ull * num_pages * n_kv * CACHE_PAGE * (head_dim + 4);
-    for (const uintptr_t p : {(uintptr_t)k, (uintptr_t)v}) if (p < c + bytes && c < p + ((T - 1) * ldkv + cols) * 2) return "8-bit cache: rows overlap the cache";
+    const uintptr_t bytes = 2ull * num_pages * n_kv * CACHE_PAGE * (head_dim + 4), row_bytes = ((T - 1) * ldkv + cols) * 2;
+    for (const void* p : {k, v}) {
+        if (meet(p, row_bytes, cache, bytes)) return "8-bit cache: rows overlap the cache";
+        if (meet(p, row_bytes, slots, 4ull * T) || meet(p, row_bytes, status, 4)) return "8-bit cache: rows overlap slots or status";
+    }
+    if (meet(cache, bytes, slots, 4ull * T) || meet(cache, bytes, status, 4) || meet(slots, 4ull * T, status, 4)) return "8-bit cache: the cache, slots and status overlap";
     return nullptr;
 }
 void rotary_turns(RotaryArgs& a, const double* freqs, int32_t rot_dims, float amplitude, bool transpose) {
@@ -291,8 +297,15 @@ int oa_k_tree_attention(const void* q, int64_t ldq, void* out, int64_t ldo, cons
         return bad("tree attention: a pointer is not aligned");
     if (beyond_memory(n_rows, ldq) || beyond_memory(n_rows, ldo)) return bad("tree attention: rows further apart than memory reaches");
     if (!apart_or_same(q, ldq, out, ldo, n_rows, width, 2)) return bad("tree attention: out overlaps q without being q");
-    const uintptr_t c = (uintptr_t)kv_cache, o = (uintptr_t)out;
-    if (o < c + 2ull * num_pages * n_kv * CACHE_PAGE * row_bytes && c < o + ((n_rows - 1) * ldo + width) * 2) return bad("tree attention: out overlaps the cache");
+    const uintptr_t out_bytes = ((n_rows - 1) * ldo + width) * 2, q_bytes = ((n_rows - 1) * ldq + width) * 2, cache_bytes = 2ull * num_pages * n_kv * CACHE_PAGE * row_bytes;
+    const struct { const void* p; uintptr_t bytes; } arrays[] = {{block_tables, 4ull * n_seqs * max_pages_per_seq}, {ctx_lens, 4ull * n_seqs}, {row_starts, 4ull * n_seqs + 4}, {seen, 8ull * n_rows}};
+    if (meet(out, out_bytes, kv_cache, cache_bytes)) return bad("tree attention: out overlaps the cache");
+    if (meet(out, out_bytes, status, 4)) return bad("tree attention: out overlaps status");
+    for (const auto& x : arrays) {
+        if (meet(out, out_bytes, x.p, x.bytes)) return bad("tree attention: out overlaps an array that is read");
+        if (meet(status, 4, x.p, x.bytes)) return bad("tree attention: status overlaps an array that is read");
+    }
+    if (meet(status, 4, q, q_bytes) || meet(status, 4, kv_cache, cache_bytes)) return bad("tree attention: status overlaps an array that is read");
     OA_ON_DEVICE_OF(kv_cache, q, out, block_tables, ctx_lens, row_starts, seen, status);
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);

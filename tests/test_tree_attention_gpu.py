@@ -534,3 +534,20 @@ def test_trees_that_cross_tiles(L, fmt, window):
     b = Batch(10, 2, 128, fmt, ctx, [64] * len(ctx), seen=[seen] * len(ctx), seed=28, window=window, sinks=3 if window else 0)
     run(L, b)
     b.check()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("group", range(1, 17))
+def test_groups_of_any_size(L, fmt, group):
+    for new in ([1, 1, 0, 1], [min(64, 128 // group + 1), 17, 1, 64]):
+        b = Batch(2 * group, 2, 64, fmt, [70, 200, 5, 0], new, seed=29 + group)
+        run(L, b)
+        b.check()
+
+
+@pytest.mark.parametrize("fmt", [BF16, E4M3])
+@pytest.mark.parametrize("heads,n_kv,new", [(1024, 1024, 2), (1024, 1024, 20), (2048, 128, 3)])
+def test_very_many_heads(L, fmt, heads, n_kv, new):
+    b = Batch(heads, n_kv, 64, fmt, [130], [new], seed=30)
+    run(L, b)
+    b.check()
