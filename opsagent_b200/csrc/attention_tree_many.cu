@@ -7,10 +7,10 @@
 // (over a power of two that none of a tile's, or of a piece's so far, passes): a softmax thread that multiplied 128 scores and weights by scales from shared memory took twice as long for a tile.
 // Roundings to fp16, 2^-11 each: a scale, a key or value times it, a weight.  Queries are scaled by a power of two as for few rows, by a kernel before.
 //
-// Trees of 64 tokens behind 8 sequences of 2000 to 8000 over bf16, 32 / 8 heads of 128: 55 us in a graph, for bytes 24 at the copy rate and products 23: 0.95 us a tile (1700 cycles at the 1.7 to
-// 1.8 GHz that the power cap leaves: the exponentials and the tensor pipe take 1024 each), 5 to begin, 4 to 5 for each piece that begins inside a CTA's share (the last product, 64 KB of parts, the
-// first scores), 5 for the join.  Over 8 bits a tile takes 1.4 us, 800 cycles for either half's conversion by the eight warps, whose loads from shared memory wait beside the products' reads: 25
-// tokens of 64 / 8 heads behind 100001 tokens, int8, 128 to 133 us in a graph; unequal trees of 3 to 40 tokens, e4m3, 94.
+// Trees of 64 tokens behind 8 sequences of 2000 to 8000 over bf16, 32 / 8 heads of 128: 54 us in a graph, for bytes 24 at the copy rate and products 23: 0.95 us a tile (1700 cycles at the 1.7 to
+// 1.8 GHz that the power cap leaves: the exponentials and the tensor pipe take 1024 each), 5 to begin, 4.5 for each piece that begins inside a CTA's share (the last product, 64 KB of parts under the next
+// one's first weights, the first scores), 5 for the join.  Over 8 bits a tile takes 1.4 us, 800 cycles for either half's conversion by the eight warps, whose loads from shared memory wait beside the products' reads: 25
+// tokens of 64 / 8 heads behind 100001 tokens, int8, 128 to 133 us in a graph; unequal trees of 3 to 40 tokens, e4m3, 91 (92.5 where both warpgroups wrote a piece's end).
 #include "attention_tree.cuh"
 
 namespace oa {
@@ -54,8 +54,8 @@ struct ManyCfg {
     static constexpr int RAW_BYTES = KEYS * D, RAW = BITS8 ? (D == 128 ? 5 : 8) : 0;         // a tile of 8 bits, and how many wait
     static constexpr int SC = 8, SC_FLOATS = 2 * KEYS + 4;                       // tiles whose scales wait: keys', values', what scores are multiplied by, what O is for larger scales of values and at its end
     static constexpr int CONV = BITS8 ? 8 : 0, THREADS = 128 + 256 + 32 * CONV;     // producer, issuer, scales, pieces; eight softmax warps; warps that convert
-    static constexpr int BARS = 18 + 2 * SLOTS + 2 * RAW + (BITS8 ? 2 * SC : 0);
-    static constexpr int SMEM_BYTES = TILE_BYTES + SLOTS * TILE_BYTES + RAW * RAW_BYTES + (BITS8 ? SC * SC_FLOATS * 4 : 0) + 3 * 128 * 4 + BARS * 8 + 16 + 2 * sizeof(TreePiece);
+    static constexpr int BARS = 19 + 2 * SLOTS + 2 * RAW + (BITS8 ? 2 * SC : 0);
+    static constexpr int SMEM_BYTES = TILE_BYTES + SLOTS * TILE_BYTES + RAW * RAW_BYTES + (BITS8 ? SC * SC_FLOATS * 4 : 0) + 5 * 128 * 4 + BARS * 8 + 16 + 2 * sizeof(TreePiece);
     static constexpr uint32_t O_COL = 384;                                       // TMEM: S and P of the tiles in turn at 0, 128 and 256
 };
 OA_DEVINL uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
@@ -114,23 +114,22 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
     uint8_t* kv_s = q_s + TILE;
     uint8_t* raw_s = kv_s + SLOTS * TILE;
     float* sc_s = reinterpret_cast<float*>(raw_s + Cfg::RAW * Cfg::RAW_BYTES);
-    float* m_s = sc_s + (BITS8 ? SC * Cfg::SC_FLOATS : 0);                                   // a row's reference maximum, and its two sums of a piece
-    float* l_s = m_s + 128;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(l_s + 256);
-    uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_full = bars + 5, *o_full = bars + 8, *full = bars + 12, *empty = full + SLOTS;
+    float* m_s = sc_s + (BITS8 ? SC * Cfg::SC_FLOATS : 0);                                   // a row's reference maximum, and a warpgroup's reference and sum of a piece [piece & 1][row]
+    float2* ml_s = reinterpret_cast<float2*>(m_s + 128);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(ml_s + 256);
+    uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_full = bars + 5, *o_full = bars + 8, *o_read = bars + 12, *full = bars + 13, *empty = full + SLOTS;
     uint64_t *piece_full = empty + SLOTS, *rows_full = piece_full + 2, *piece_empty = rows_full + 2, *raw_full = piece_empty + 2, *raw_empty = raw_full + Cfg::RAW, *sc_full = raw_empty + Cfg::RAW, *sc_empty = sc_full + SC;
     TreePiece* piece_s = reinterpret_cast<TreePiece*>(bars + Cfg::BARS);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(piece_s + 2);
     __shared__ int64_t sums[Cfg::THREADS / 32];
     __shared__ At start;
-    __shared__ float sc_last;                                                    // 8 bits: what the values' scales of a piece's last tile are over
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int grp = a.n_heads / a.n_kv, tile_tokens = 128 / grp;
     if (threadIdx.x == 0) {
         tma_prefetch_desc(&tm_q);
         if (!BITS8) tma_prefetch_desc(&tm_kv);
-        mbar_init(q_full, 1); mbar_init(q_empty, 1);
+        mbar_init(q_full, 1); mbar_init(q_empty, 1); mbar_init(o_read, 4);
         for (int i = 0; i < 3; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
         for (int i = 0; i < 4; ++i) mbar_init(&o_full[i], 1);
         for (int i = 0; i < 2; ++i) { mbar_init(&piece_full[i], 1); mbar_init(&rows_full[i], 1); mbar_init(&piece_empty[i], BITS8 ? 11 + Cfg::CONV : 10); }
@@ -268,6 +267,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                     if (j >= 0) {
                         const uint32_t m = n + j, from = m % 3;
                         mbar_wait(&p_full[from], (m / 3) & 1);
+                        if (j == 0 && seg > 1) mbar_wait(o_read, seg & 1);           // O of the piece before has been read
                         const uint32_t slot = await();
                         if (elect_one()) {
                             const uint64_t b = v_desc + (uint64_t)(slot * (TILE >> 4));
@@ -402,7 +402,9 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
         // with each tile, as soon as the tile's own maximum is known; sums stay with either, O is one for both
         const int quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t wg = (warp - 4) >> 2, lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16), o_addr = lane_addr + Cfg::O_COL;
-        auto meet = [] { asm volatile("bar.sync 2, %0;" ::"n"(SOFTMAX) : "memory"); };
+        // Of a piece's end: the warpgroup that had its last tile waits for the other's sum and writes the piece, under the other's first tile of the next one.  Neither is two pieces behind the other
+        auto take_sum = [](uint32_t k) { if (k & 1) asm volatile("bar.sync 5, %0;" ::"n"(SOFTMAX) : "memory"); else asm volatile("bar.sync 2, %0;" ::"n"(SOFTMAX) : "memory"); };
+        auto pass_sum = [](uint32_t k) { if (k & 1) asm volatile("bar.arrive 5, %0;" ::"n"(SOFTMAX) : "memory"); else asm volatile("bar.arrive 2, %0;" ::"n"(SOFTMAX) : "memory"); };
         auto take_turn = [](uint32_t n) {                                        // tile n - 1 has left its reference
             if (n & 1) asm volatile("bar.sync 3, %0;" ::"n"(SOFTMAX) : "memory"); else asm volatile("bar.sync 4, %0;" ::"n"(SOFTMAX) : "memory");
         };
@@ -411,8 +413,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
         };
         constexpr float kRaise = 8.0f;                                           // log2 units a score may pass the reference by
         constexpr float kLift = BITS8 ? 7.0f : 0.0f;                             // of the weights, which fp16 holds up to 2^16 and with 8 bits down to 2^-17
-        constexpr int COLS = D / 2;
-        uint32_t n0 = 0;                                                         // tiles of the pieces before
+        uint32_t n0 = 0, seg = 0;                                                // tiles of the pieces before, pieces
         pieces(true, [&](const TreePiece& p) {
             const TreeSeq& s = p.s;
             const int c0 = p.c0, tiles = p.c1 - p.c0;
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
             float2* ml = reinterpret_cast<float2*>(a.part_ml) + ((int64_t)blockIdx.x * 2 + !first) * 128 + row;
             if (tiles == 0) {                                                    // units of the item's own alone
                 if (live)
-                    for (int c = wg * COLS; c < (int)(wg + 1) * COLS; c += 4) *reinterpret_cast<float4*>(po + c * 128) = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int c = wg * (D / 2); c < (int)(wg + 1) * (D / 2); c += 4) *reinterpret_cast<float4*>(po + c * 128) = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (live && wg == 0) *ml = make_float2(-INFINITY, first && blind ? -1.f : 0.f);
                 return;
             }
@@ -550,14 +551,15 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                 if (idle) pace(n, special); else if (special) tile(n, TrueTag{}); else tile(n, FalseTag{});
             }
             n0 = n1;
-            meet();                                                              // the last tile's reference is there
-            const float m_ref = m_s[row];
-            if (m_mine != m_ref) l_run *= ex2_approx(m_mine - m_ref);
-            l_s[wg * 128 + row] = l_run;
-            if (BITS8 && ((n1 - 1) & 1) == wg && row == 0) sc_last = undo;
-            meet();
-            const float l = l_s[row] + l_s[128 + row];
-            if (BITS8) undo = sc_last;
+            float2* pair = ml_s + (seg & 1) * 128 + row;
+            if (((n1 - 1) & 1) != wg) {
+                *pair = make_float2(m_mine, l_run);
+                pass_sum(seg++);
+                return;
+            }
+            take_sum(seg++);
+            const float2 other = *pair;
+            const float m_ref = m_mine, l = l_run + (other.x == m_ref ? other.y : other.y * ex2_approx(other.x - m_ref));       // the last tile's reference is the piece's
             mbar_wait(&o_full[(n1 - 1) & 3], ((n1 - 1) >> 2) & 1);
             tcgen05_fence_after();
             const bool whole = first && p.last;
@@ -565,7 +567,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
             const int token = row / grp;
             uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)(p.row0 + token) * a.ldo + (int64_t)(p.kvh * grp + row - token * grp) * D;
 #pragma unroll 1
-            for (int c = wg * COLS; c < (int)(wg + 1) * COLS; c += 32) {
+            for (int c = 0; c < D; c += 32) {
                 uint32_t o[32];
                 tmem_ld_32x32b_x32(o_addr + c, o);
                 tmem_ld_wait();
@@ -584,8 +586,9 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                         *reinterpret_cast<float4*>(po + (c + i) * 128) = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
             }
             tcgen05_fence_before();
-            if (live && !whole && wg == 0) *ml = make_float2(m_ref - kLift, first && blind ? -1.f : l);
-            meet();                                                              // O and the sums may be written again
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_read);
+            if (live && !whole) *ml = make_float2(m_ref - kLift, first && blind ? -1.f : l);
         });
     } else {
         if constexpr (BITS8) reg_dec<72>();
