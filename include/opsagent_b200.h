@@ -204,7 +204,7 @@ OA_API int oa_k_cache_copy(void* kv_cache, int32_t planes, int32_t num_pages, in
  * tokens behind it: rows prefix_rows[p] .. prefix_rows[p + 1] - 1 see the first prefix_lens[p] places of the pages prefix_tables[p, :], and row i the first own_lens[i]
  * places of own_tables[i, :] (its new token among them, if it is to be seen).  A row without a prefix (before, behind or between the runs, or of a prefix of length 0) sees its
  * own tokens alone, one that sees nothing gets zeros.  All tables and lengths are on the device.  scale 0: 1 / sqrt(head_dim).  head_dim 64 or 128, up to 16 query heads of a key/value head, up to 32
- * prefixes, 2^20 sequences, 2^10 key/value heads and 2^24 pages a table; 2 num_pages n_kv 64 rows of the cache are counted in 31 bits.  out is q itself (same pitch) or apart from it, and from all else; pitches and
+ * prefixes, 2^20 sequences, 2^10 key/value heads and 2^24 pages a table; 2 num_pages n_kv 64 rows of the cache are counted in 31 bits.  out is q itself (same pitch) or apart from it; pitches and
  * addresses are multiples of 16 bytes.  Softmax weights are rounded to bf16 for their product with the values, sums are fp32.  The host, which knows no length, divides the work by max_prefix_pages
  * and max_own_pages: tables much wider than their prefixes cost time (128 rows on 1536 tokens: 41 us with 24 or 64 entries a prefix, 45 with 128).  A page number beyond the cache, a length beyond its table or run
  * bounds that fall set *status; rows that read such a page hold no meaningful value, lengths and bounds are cut to what there is */
