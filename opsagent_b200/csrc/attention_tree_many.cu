@@ -473,7 +473,8 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                 float grown = 1.0f, fac = row_fac;
                 if (BITS8) {
                     const float* sc = sc_s + buf * Cfg::SC_FLOATS + 2 * KEYS;
-                    fac *= sc[0]; grown = sc[1]; undo = sc[2];
+                    // never 0, by which a masked score, -inf, would be NaN: scores of a tile whose visible keys are all zero, or whose row of queries is, are 0 times this, others so small move by less than 2^-80
+                    fac = fmaxf(fac * sc[0], 0x1p-126f); grown = sc[1]; undo = sc[2];
                 }
                 uint32_t v[2][32];
                 auto scores = [&](int k) {                                       // of keys k .. k + 63, -inf where the row does not see
