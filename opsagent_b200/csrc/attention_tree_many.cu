@@ -52,7 +52,7 @@ struct ManyCfg {
     static constexpr int KEYS = 128, HALVES = D / 64, HALF = 128 * 128;          // 128 rows x 64 channels of 2 bytes under the 128-byte swizzle: of Q, of a tile
     static constexpr int TILE_BYTES = HALVES * HALF, SLOTS = BITS8 ? (D == 128 ? 3 : 4) : D == 128 ? 5 : 8;
     static constexpr int RAW_BYTES = KEYS * D, RAW = BITS8 ? (D == 128 ? 5 : 8) : 0;         // a tile of 8 bits, and how many wait
-    static constexpr int SC = 8, SC_FLOATS = 2 * KEYS + 4;                       // tiles whose scales wait: keys', values', what scores are multiplied by, what O is for larger scales of values and at its end
+    static constexpr int SC = 8, SC_FLOATS = 2 * KEYS + 4;                       // tiles whose scales wait: keys', values', what keys' are over, what O is multiplied by for larger scales of values and at its end
     static constexpr int CONV = BITS8 ? 8 : 0, THREADS = 128 + 256 + 32 * CONV;     // producer, issuer, scales, pieces; eight softmax warps; warps that convert
     static constexpr int BARS = 19 + 2 * SLOTS + 2 * RAW + (BITS8 ? 2 * SC : 0);
     static constexpr int SMEM_BYTES = TILE_BYTES + SLOTS * TILE_BYTES + RAW * RAW_BYTES + (BITS8 ? SC * SC_FLOATS * 4 : 0) + 5 * 128 * 4 + BARS * 8 + 16 + 2 * sizeof(TreePiece);
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                             *reinterpret_cast<uint4*>(sc + v * KEYS + 4 * lane) = make_uint4(w[0], w[1], w[2], w[3]);
                         }
                         vref = ref[1];
-                        if (lane == 0) { sc[2 * KEYS] = ref[0] * (1.0f / kKeyUp); sc[2 * KEYS + 1] = grown; sc[2 * KEYS + 2] = vref * (1.0f / 128.f); }
+                        if (lane == 0) { sc[2 * KEYS] = ref[0]; sc[2 * KEYS + 1] = grown; sc[2 * KEYS + 2] = vref * (1.0f / 128.f); }
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sc_full[buf]);
                     }
@@ -473,8 +473,8 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                 float grown = 1.0f, fac = row_fac;
                 if (BITS8) {
                     const float* sc = sc_s + buf * Cfg::SC_FLOATS + 2 * KEYS;
-                    // never 0, by which a masked score, -inf, would be NaN: scores of a tile whose visible keys are all zero, or whose row of queries is, are 0 times this, others so small move by less than 2^-80
-                    fac = fmaxf(fac * sc[0], 0x1p-126f); grown = sc[1]; undo = sc[2];
+                    // The row's factor first: the keys' reference may be 2^126, and 512 of that is none.  Never 0, by which a masked score, -inf, would be NaN: scores of a tile whose visible keys are all zero, or whose row of queries is, are 0 times this, others so small move by less than 2^-80
+                    fac = fmaxf(fac * sc[0] * (1.0f / kKeyUp), 0x1p-126f); grown = sc[1]; undo = sc[2];
                 }
                 uint32_t v[2][32];
                 auto scores = [&](int k) {                                       // of keys k .. k + 63, -inf where the row does not see

@@ -57,3 +57,18 @@ def test_rows_that_see_nothing_beside_small_scores(L, fmt):
         q = (b.q.float() * size).bfloat16()
         run(L, b, q=q)
         b.check(q=q)
+
+
+@pytest.mark.parametrize("fmt", [E4M3, INT8])
+@pytest.mark.parametrize("new", [1, 30])
+def test_largest_keys_under_small_queries(L, fmt, new):
+    """Keys up to 2^127 and queries that bring their scores to ordinary sizes."""
+    def factors(shape):
+        f = torch.ones(shape, device="cuda")
+        f[0] = 2.0 ** 125
+        return f
+    b = Batch(8, 2, 128, fmt, [300, 20], [new, 1], seed=34, scales=factors)
+    q = (b.q.double() * 2.0 ** -125).bfloat16()
+    assert key_scales(b)[key_scales(b).isfinite()].max() > 2.0 ** 118
+    run(L, b, q=q)
+    b.check(q=q)
