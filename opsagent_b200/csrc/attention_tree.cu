@@ -85,11 +85,10 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
     const int64_t u_begin = share.begin, u_end = share.end;
     if (u_begin >= u_end) { griddep_launch(); return; }
     At at = start;
-    auto next = [&] { at.next(a); };
 
     if (warp == 8) {
         int st = 0; uint32_t ph = 0;
-        for (int64_t u = u_begin; u < u_end; next()) {
+        for (int64_t u = u_begin;; at.next(a)) {
             const int c0 = (int)max(u - at.unit0 - 1, (int64_t)0), c1 = (int)min((int64_t)at.s.pages, u_end - at.unit0 - 1);
             u = at.unit0 + 1 + c1;
             const int32_t* table = a.tables + (int64_t)at.seq * a.max_pages;
@@ -117,6 +116,7 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
                 __syncwarp();
                 if (++st == STAGES) { st = 0; ph ^= 1; }
             }
+            if (u >= u_end) break;
         }
         griddep_launch();
         return;
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
     if (warp == 10) {
         // queries of an item, and what its rows see.  8 bits: fp16 under a power of two, pieces of eight channels where the consumers' lanes find them side by side
         uint32_t k = 0;
-        for (int64_t u = u_begin; u < u_end; next(), ++k) {
+        for (int64_t u = u_begin;; at.next(a), ++k) {
             const int64_t end = at.unit0 + 1 + at.s.pages;
             FewItem item;
             item.s = at.s; item.c0 = (int)max(u - at.unit0 - 1, (int64_t)0); item.c1 = (int)min((int64_t)at.s.pages, u_end - at.unit0 - 1);
@@ -182,6 +182,7 @@ __global__ void __launch_bounds__(TREE_THREADS, FewCfg<D, FMT, NB, STAGES>::CTAS
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full[k & 1]);
+            if (u >= u_end) break;
         }
         griddep_launch();
         return;

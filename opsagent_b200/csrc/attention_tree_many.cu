@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
             At at;
             at = start;
             uint32_t k = 0;
-            for (int64_t u = u_begin; u < u_end; at.next(a), ++k) {
+            for (int64_t u = u_begin; u < u_end; ++k) {
                 const int64_t end = at.unit0 + at.units();
                 const int c0 = (int)max(u - at.unit0 - TREE_OVER, (int64_t)0), c1 = (int)max((int64_t)c0, min((int64_t)at.steps(), u_end - at.unit0 - TREE_OVER));
                 u = min(end, u_end);
@@ -394,6 +394,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                 if (lane == 0) { p.any.seen = any; p.any.low = lowest; }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&rows_full[k & 1]);
+                if (u < u_end) at.next(a);
             }
         }
     } else if (warp < 12) {
