@@ -5,12 +5,16 @@
 //
 // bf16: P is rounded to bf16.  8 bits: tiles are turned into fp16 under the swizzle that the products read, by eight warps of their own.  Keys and values are multiplied by their scales on the way
 // (over a power of two that none of a tile's, or of a piece's so far, passes): a softmax thread that multiplied 128 scores and weights by scales from shared memory took twice as long for a tile.
-// Roundings to fp16, 2^-11 each: a scale, a key or value times it, a weight.  Queries are scaled by a power of two as for few rows, by a kernel before.
+// Roundings to fp16, 2^-11 each: a key or value times its scale, a weight.  Scales come in two halves: rounded to one, an error that all channels of a key share, they left 2.4e-3 to 3.6e-3 of the output for
+// scores up to 20 and 80 (single rows 6e-3 and 2.3e-2) instead of 1.8e-3 and 2.1e-3 (3.8e-3 and 1.0e-2), at 89 and 100 us for unequal trees of 3 to 40 tokens over e4m3 and int8, 122 and 128 for 25 tokens behind
+// 100001, instead of 91, 96, 127 and 139; scores times fp32 scales in the softmax threads leave 1.7e-3 at any size and took 122, 127, 148 and 155.  Keys and values go through one code: a second copy of it cost
+// the unequal trees 10 us.
+// Queries are scaled by a power of two as for few rows, by a kernel before.
 //
 // Trees of 64 tokens behind 8 sequences of 2000 to 8000 over bf16, 32 / 8 heads of 128: 54 us in a graph, for bytes 24 at the copy rate and products 23: 0.95 us a tile (1700 cycles at the 1.7 to
 // 1.8 GHz that the power cap leaves: the exponentials and the tensor pipe take 1024 each), 5 to begin, 4.5 for each piece that begins inside a CTA's share (the last product, 64 KB of parts under the next
-// one's first weights, the first scores), 5 for the join.  Over 8 bits a tile takes 1.4 us, 800 cycles for either half's conversion by the eight warps, whose loads from shared memory wait beside the products' reads: 25
-// tokens of 64 / 8 heads behind 100001 tokens, int8, 128 to 133 us in a graph; unequal trees of 3 to 40 tokens, e4m3, 91 (92.5 where both warpgroups wrote a piece's end).
+// one's first weights, the first scores), 5 for the join.  Over 8 bits a tile takes 1.35 us (e4m3) to 1.5 (int8), 800 cycles and more for either half's conversion by the eight warps, whose loads from shared memory wait beside the products' reads: 25
+// tokens of 64 / 8 heads behind 100001 tokens, int8, 139 us in a graph; unequal trees of 3 to 40 tokens, e4m3, 91 (1.5 more where both warpgroups wrote a piece's end).
 #include "attention_tree.cuh"
 
 namespace oa {
@@ -108,7 +112,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
     constexpr bool BITS8 = Cfg::BITS8;
     constexpr int KEYS = Cfg::KEYS, HALVES = Cfg::HALVES, HALF = Cfg::HALF, TILE = Cfg::TILE_BYTES, SLOTS = Cfg::SLOTS, RAW = BITS8 ? Cfg::RAW : 1, SC = Cfg::SC, SOFTMAX = 256;
     constexpr int64_t BLOCK_BYTES = CACHE_PAGE * (D + 4);
-    constexpr float kKeyUp = FMT == CACHE_INT8 ? 1.0f / 512.f : 64.f;
+    constexpr float kUp = 128.f;                                                             // scales over their reference times this: the largest product is 57344 (e4m3), which fp16 holds
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* q_s = smem;
     uint8_t* kv_s = q_s + TILE;
@@ -283,8 +287,8 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                 n += tiles;
             });
         } else if (warp == 2) {
-            // A tile's scales in fp16, twice: keys' over a power of two that none of the tile passes and times 2^6 (int8: 2^-9), values' over one that none of the piece so far passes and times 2^7, which bring the
-            // largest product to 28672 (0.25) and 57344; 0 of what none of the rows sees.  int8 keys u - 128 times s are the fused product u 2^-24 (a subnormal's bits) times s 2^24 less 128 s
+            // A tile's scales, keys' over a power of two that none of the tile passes, values' over one that none of the piece so far passes, and either times 2^7; 0 of what none of the rows sees.  In two halves of
+            // fp16: one alone would be off by 2^-11 of itself, which all of a key's channels share, so that a score would be off by as much
             if constexpr (BITS8) {
                 uint32_t n = 0;
                 pieces(true, [&](const TreePiece& p) {
@@ -334,21 +338,17 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                             top = __reduce_max_sync(0xffffffffu, top);
                             const float need = __uint_as_float(min((top & 0x7f800000u) + 0x00800000u, 0x7e800000u));             // up to 2^126
                             if (need > ref[v]) { if (ref[v] > 0.f) grown = ref[v] * (1.0f / need); ref[v] = need; }
-                            const float inv = 1.0f / ref[v], up = v ? 128.f : kKeyUp;        // powers of two: exact
+                            const float inv = 1.0f / ref[v];                         // a power of two: exact
                             uint32_t w[4];
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                const float y = x[i] * inv * up;
-                                w[i] = pack_f16x2(y, y);
-                                if (!v && FMT == CACHE_INT8) {                       // s 2^24 and -128 s, of the same s
-                                    const float r = __half2float(__float2half_rn(y * 16777216.f));
-                                    w[i] = pack_f16x2(r, r * (-128.f / 16777216.f));
-                                }
+                                const float y = x[i] * inv * kUp, hi = __half2float(__float2half_rn(y));
+                                w[i] = pack_f16x2(hi, y == hi ? 0.f : y - hi);       // an infinite one has no second half
                             }
                             *reinterpret_cast<uint4*>(sc + v * KEYS + 4 * lane) = make_uint4(w[0], w[1], w[2], w[3]);
                         }
                         vref = ref[1];
-                        if (lane == 0) { sc[2 * KEYS] = ref[0]; sc[2 * KEYS + 1] = grown; sc[2 * KEYS + 2] = vref * (1.0f / 128.f); }
+                        if (lane == 0) { sc[2 * KEYS] = ref[0]; sc[2 * KEYS + 1] = grown; sc[2 * KEYS + 2] = vref * (1.0f / kUp); }
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sc_full[buf]);
                     }
@@ -474,8 +474,8 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                 float grown = 1.0f, fac = row_fac;
                 if (BITS8) {
                     const float* sc = sc_s + buf * Cfg::SC_FLOATS + 2 * KEYS;
-                    // The row's factor first: the keys' reference may be 2^126, and 512 of that is none.  Never 0, by which a masked score, -inf, would be NaN: scores of a tile whose visible keys are all zero, or whose row of queries is, are 0 times this, others so small move by less than 2^-80
-                    fac = fmaxf(fac * sc[0] * (1.0f / kKeyUp), 0x1p-126f); grown = sc[1]; undo = sc[2];
+                    // Never 0, by which a masked score, -inf, would be NaN: scores of a tile whose visible keys are all zero, or whose row of queries is, are 0 times this, others so small move by less than 2^-80
+                    fac = fmaxf(fac * sc[0] * (1.0f / kUp), 0x1p-126f); grown = sc[1]; undo = sc[2];
                 }
                 uint32_t v[2][32];
                 auto scores = [&](int k) {                                       // of keys k .. k + 63, -inf where the row does not see
@@ -615,8 +615,7 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
                     mbar_wait3(&raw_full[from], (n / RAW) & 1, &empty[to], ((n / SLOTS) & 1) ^ 1, &sc_full[(g + t) % SC], ((g + t) / SC) & 1);
                     const uint8_t* src = raw_s + from * Cfg::RAW_BYTES + ch * 16;
                     uint8_t* dst = kv_s + to * TILE + (ch >> 2) * HALF;
-                    auto convert = [&](auto tag) {
-                        constexpr bool KEY = decltype(tag)::value;
+                    auto convert = [&] {                             // as a function of its own: written in line the compiler's order took 92, 98, 128.5 and 140 us
 #pragma unroll
                         for (int h = 0; h < STEPS; h += AHEAD) {                     // loads ahead of their stores
                             uint4 x[AHEAD]; uint32_t f[AHEAD];
@@ -625,27 +624,19 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
 #pragma unroll
                             for (int i = 0; i < AHEAD; ++i) {
                                 uint32_t y[8];
-                                const uint32_t w4[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-                                if (FMT == CACHE_INT8 && KEY) {
-                                    const uint32_t mul = __byte_perm(f[i], 0, 0x1010), add = __byte_perm(f[i], 0, 0x3232);
+                                const uint32_t w4[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, hi = __byte_perm(f[i], 0, 0x1010), lo = __byte_perm(f[i], 0, 0x3232);
 #pragma unroll
-                                    for (int k = 0; k < 4; ++k) {
-                                        const uint32_t u = w4[k] ^ 0x80808080u;
-                                        y[2 * k] = fma_f16x2(__byte_perm(u, 0, 0x4140), mul, add); y[2 * k + 1] = fma_f16x2(__byte_perm(u, 0, 0x4342), mul, add);
-                                    }
-                                } else
-#pragma unroll
-                                    for (int k = 0; k < 4; ++k) {
-                                        to_f16<FMT, false>(w4[k], y[2 * k], y[2 * k + 1]);
-                                        y[2 * k] = mul_f16x2(y[2 * k], f[i]); y[2 * k + 1] = mul_f16x2(y[2 * k + 1], f[i]);
-                                    }
+                                for (int k = 0; k < 4; ++k) {
+                                    to_f16<FMT, false>(w4[k], y[2 * k], y[2 * k + 1]);
+                                    y[2 * k] = fma_f16x2(y[2 * k], hi, mul_f16x2(y[2 * k], lo)); y[2 * k + 1] = fma_f16x2(y[2 * k + 1], hi, mul_f16x2(y[2 * k + 1], lo));
+                                }
                                 const int key = key_of(h + i);
                                 *reinterpret_cast<uint4*>(dst + key * 128 + (((2 * (ch & 3)) ^ (key & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
                                 *reinterpret_cast<uint4*>(dst + key * 128 + (((2 * (ch & 3) + 1) ^ (key & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
                             }
                         }
                     };
-                    if (FMT == CACHE_INT8 && !(e & 1)) convert(TrueTag{}); else convert(FalseTag{});
+                    convert();
                     if ((e & 1) && (c0 + t < p.s0 || c0 + t >= p.s1))                              // values that none of the rows sees may be anything, and 0 x inf is not 0
 #pragma unroll 1
                         for (int i = 0; i < STEPS; ++i) {

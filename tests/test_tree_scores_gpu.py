@@ -72,3 +72,61 @@ def test_largest_keys_under_small_queries(L, fmt, new):
     assert key_scales(b)[key_scales(b).isfinite()].max() > 2.0 ** 118
     run(L, b, q=q)
     b.check(q=q)
+
+
+def expected_error(b, q, many):
+    """The norm of the error that roundings leave, and of the output, by the formula: a rounding is off by a step over sqrt(12) in the mean, independently of the others.  bf16 steps of the output; a weight's
+    steps, of bf16 or fp16, taken as 2 half-steps of the weight; over 8 bits and tiles of 128 rows fp16 steps of keys and values, where a key's move its score s_j and that moves the
+    output by p_j ds_j (v_j - o).  Few rows over 8 bits have values' scales in their weights."""
+    def step(x, bits):
+        return torch.exp2(torch.floor(torch.log2(x.abs().clamp_min(2.0 ** -200))) - bits)
+    width, scale, total, size, err = b.heads * b.dim, b.dim ** -0.5, 0.0, 0.0, 0.0
+    for i in range(len(b.ctx)):
+        pages = torch.tensor(b.tables[i, : b.need[i]].astype(np.int64), device="cuda")
+        k, v = (b.values[j, pages].transpose(1, 2).reshape(-1, b.n_kv, b.dim) for j in (0, 1))
+        for t in range(b.new[i]):
+            r = int(b.starts[i]) + t
+            see = torch.tensor(sorted(b.places(i, t)), device="cuda", dtype=torch.long)
+            x, ks, vs = q[r, :width].double().view(b.n_kv, -1, b.dim), k[see], v[see]
+            p = torch.softmax(torch.einsum("khd,pkd->khp", x, ks) * scale, -1)
+            o = torch.einsum("khp,pkd->khd", p, vs)
+            weight = (2.0 ** -7 if b.fmt == BF16 else 2.0 ** -10) / 12 ** 0.5
+            var = step(o, 7).square().sum() / 12 + weight ** 2 * torch.einsum("khp,pkd->", p.square(), vs.square())
+            if many:
+                var += torch.einsum("khp,pkd->", p.square(), step(vs, 10).square()) / 12
+                score = scale ** 2 / 12 * torch.einsum("khd,pkd->khp", x.square(), step(ks, 10).square())
+                away = torch.einsum("pkd,pkd->kp", vs, vs)[:, None] - 2 * torch.einsum("khd,pkd->khp", o, vs) + o.square().sum(-1, keepdim=True)
+                var += (p.square() * score * away).sum()
+            total += var.item()
+            size += o.square().sum().item()
+            err += (b.out[r, :width].double().view(b.n_kv, -1, b.dim) - o).square().sum().item()
+    return err ** 0.5 / size ** 0.5, total ** 0.5 / size ** 0.5
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("size", [1, 4, 8, 16])
+@pytest.mark.parametrize("new", [1, 3, 20])
+def test_errors_of_large_scores(L, fmt, dim, size, new):
+    """The error's norm is what independent roundings make it, for scores up to about 80: a quarter is left for a sum over some thousand rows of heads.  4 and 12 rows of a sequence, and 80."""
+    b = Batch(32, 8, dim, fmt, [700 + 13 * i for i in range(64 // new)] if new < 20 else [2500, 900, 40], [new] * (64 // new if new < 20 else 3), seed=35)
+    q = (b.q.float() * size).bfloat16()
+    run(L, b, q=q)
+    b.check(q=q)
+    err, want = expected_error(b, q, b.fmt != BF16 and new == 20)
+    assert err <= 1.25 * want, (err, want)
+
+
+@pytest.mark.parametrize("fmt", [E4M3, INT8])
+@pytest.mark.parametrize("new", [1, 30])
+def test_values_under_an_infinite_scale(L, fmt, new):
+    """A value under a scale of infinity is infinite, of its own sign, and 0 times infinity none."""
+    b = Batch(4, 1, 128, fmt, [200], [new], seed=36, chain=True)
+    run(L, b)
+    page = int(b.tables[0, 1])
+    b.cache[1, page, 0, PAGE * 128:].view(torch.float32)[9] = float("inf")
+    b.values[1, page, 0, 9] *= float("inf")
+    run(L, b)
+    want, got = b.values[1, page, 0, 9], b.out[:new, :512].view(new, 4, 128).double()
+    finite_zero = torch.isnan(want)
+    assert torch.isnan(got[..., finite_zero]).all() and (got[..., ~finite_zero] == want[~finite_zero]).all()
