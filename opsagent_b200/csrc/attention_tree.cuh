@@ -66,10 +66,8 @@ struct TreeSeq {
     }
     OA_DEVINL int page(int c) const { return c < low_pages ? c : c + skip; }
     OA_DEVINL int tiles(int tile_tokens) const { return (n + tile_tokens - 1) / tile_tokens; }
-    // whether some row may not see all of a page's places
-    OA_DEVINL bool special(const TreeAttnArgs& a, int page) const { return (page + 1) * CACHE_PAGE > ctx || (a.window > 0 && page * CACHE_PAGE < ctx + n - a.window); }
 };
-// how many of a sequence's pages begin below a place of its window
+// How many of a sequence's pages begin below a place of its window.  Some row may not see all of a page where it begins below ctx + n - window (the deepest row's window), or does not end by ctx
 OA_DEVINL int pages_below(const TreeSeq& s, int place) {
     if (place <= 0) return 0;
     const int page = pages_of(place) - 1;                                        // the last one that does

@@ -435,15 +435,15 @@ __global__ void __launch_bounds__(ManyCfg<D, FMT>::THREADS, 1) tree_many_kernel(
             float m_mine = -INFINITY, l_run = 0.f;                               // the sum so far and the reference that it is under
             auto clear_unseen = [&](uint32_t n) {
                 const int kt = c0 + (int)(n - n0);
-                    // values that none of the rows sees may be anything, and 0 x inf is not 0: a thread looks after the key of its row's number
-                    const uint32_t entry = 2 * n0 + min(tiles, kt - c0 + 3) + (kt - c0), slot = entry % SLOTS;
-                    mbar_wait(&full[slot], (entry / SLOTS) & 1);
-                    const int c = 2 * kt + (row >> 6);
-                    if (c >= s.pages || !p.any.sees(a, s, s.page(c) * CACHE_PAGE + (row & 63))) {
+                // values that none of the rows sees may be anything, and 0 x inf is not 0: a thread looks after the key of its row's number
+                const uint32_t entry = 2 * n0 + min(tiles, kt - c0 + 3) + (kt - c0), slot = entry % SLOTS;
+                mbar_wait(&full[slot], (entry / SLOTS) & 1);
+                const int c = 2 * kt + (row >> 6);
+                if (c >= s.pages || !p.any.sees(a, s, s.page(c) * CACHE_PAGE + (row & 63))) {
 #pragma unroll
-                        for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(kv_s + slot * TILE + (c >> 3) * HALF + row * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    }
-                    fence_proxy_async();
+                    for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(kv_s + slot * TILE + (c >> 3) * HALF + row * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_proxy_async();
             };
             // a warp without rows keeps the others' pace and clears the keys that it looks after
             auto pace = [&](uint32_t n, bool special) {
