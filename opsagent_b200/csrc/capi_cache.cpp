@@ -43,6 +43,8 @@ const char* rotary_wrong(int64_t T, int64_t heads, int32_t head_dim, int32_t rot
 }
 // T rows whose last one no device's memory holds beside the first: 2^39 elements, below which products of rows, pitches and element sizes stay in 64 bits and a tensor map takes the pitch
 bool beyond_memory(int64_t T, int64_t ld) { return T > 1 && ld >= ((int64_t)1 << 39) / (T - 1); }
+// a cache of 2^40 bytes or more: below, offsets of its blocks stay in 64 bits and CTAs of a launch in 31
+bool cache_beyond_memory(int64_t planes, int64_t num_pages, int64_t page_bytes) { return planes >= ((int64_t)1 << 40) / page_bytes / num_pages; }
 // rows of T x wa and T x wb elements share no memory: they are other memory, or other columns of the same rows
 bool apart(const void* x, int64_t ldx, int64_t wa, const void* y, int64_t ldy, int64_t wb, int64_t T, int64_t esz) {
     const uintptr_t a = (uintptr_t)x, b = (uintptr_t)y;
@@ -188,6 +190,7 @@ int oa_k_cache_copy(void* kv_cache, int32_t planes, int32_t num_pages, int32_t n
     if (planes < 1 || num_pages < 1 || n_kv < 1 || head_dim < 1 || (elem_bytes != 2 && elem_bytes != 4)) return bad("cache copy: bad cache");
     const int64_t row = (int64_t)head_dim * elem_bytes;
     if (row % 16 || row > 4096 || n_kv > 4096) return bad("cache copy: a row is a multiple of 16 bytes, up to 4096, with up to 4096 heads");
+    if (cache_beyond_memory(planes, num_pages, row * n_kv * CACHE_PAGE)) return bad("cache copy: a cache larger than memory reaches");
     try {
         if (const char* wrong = moves_wrong(num_pages, moves, n_moves)) return bad(wrong);
         if (n_moves == 0) return OA_OK;
@@ -267,6 +270,7 @@ int oa_k_cache8_read(const void* kv_cache, int32_t num_pages, const int32_t* slo
 int oa_k_cache8_copy(void* kv_cache, int32_t planes, int32_t num_pages, int32_t n_kv, int32_t head_dim, const oa_page_move* moves, int32_t n_moves, void* stream) {
     if (const char* wrong = cache8_wrong(num_pages, n_kv, head_dim)) return bad(wrong);
     if (planes < 1) return bad("8-bit cache: no planes");
+    if (cache_beyond_memory(planes, num_pages, (int64_t)n_kv * CACHE_PAGE * (head_dim + 4))) return bad("8-bit cache: a cache larger than memory reaches");
     try {
         if (const char* wrong = moves_wrong(num_pages, moves, n_moves)) return bad(wrong);
         if (n_moves == 0) return OA_OK;

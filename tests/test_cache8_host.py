@@ -94,3 +94,14 @@ def test_host_memory_is_not_run_on(L):
     assert L.oa_k_cache8_copy(p, 2, 2, 2, 64, moves, 1, None) in (400, 500)
     assert L.oa_k_tree_attention(p, 128, p + 4096, 128, p + 65536, 1, 2, p + 8192, 1, p + 8192, p + 8192, None, 1, 1, 2, 2, 64, 0, 0, 0.0, None, None) in (400, 500)
     assert L.oa_kernel_launches() == before
+
+
+def test_copies_in_caches_that_no_memory_holds(L):
+    """What a launch cannot count is refused as other arguments are, and not as a fault of the device."""
+    one = (_lib.OaPageMove * 1)(_lib.OaPageMove(0, 1, 64))
+    for planes, pages, kv, dim in [(2 ** 31 - 1, 8, 4096, 256), (2 ** 31 - 1, 2 ** 31 - 1, 1, 16), (2 ** 22, 64, 8, 128), (64, 2 ** 30, 4096, 64)]:
+        assert L.oa_k_cache8_copy(P, planes, pages, kv, dim, one, 1, None) == 400 and "memory" in _lib.last_error(), (planes, pages)
+        assert L.oa_k_cache_copy(P, planes, pages, kv, dim, 2, one, 1, None) == 400 and "memory" in _lib.last_error(), (planes, pages)
+    for planes, pages, kv, dim in [(2, 2, 1, 16), (128, 2 ** 15, 8, 128)]:
+        assert "memory reaches" not in (L.oa_k_cache8_copy(P, planes, pages, kv, dim, one, 1, None), _lib.last_error())[1]
+        assert "memory reaches" not in (L.oa_k_cache_copy(P, planes, pages, kv, dim, 2, one, 1, None), _lib.last_error())[1]
