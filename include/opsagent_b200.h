@@ -228,6 +228,9 @@ OA_API int oa_k_cache8_copy(void* kv_cache, int32_t planes, int32_t num_pages, i
  * its sequence, sees new token u where bit u of seen[r] (a word a row of q) is set (its ancestors, which come before it, and itself; bits of tokens that there are not say nothing); seen NULL: a chain, 0 .. t.
  * It sees all cached tokens, or with a window (64 or more; 0: none) those less than `window` places before it and the first `sinks` ones; its place is ctx_lens[i] and the number of its
  * ancestors behind the first new one: bits of seen[r] below t.  A row that sees nothing gets zeros; rows of q that no sequence has are left as they are in out.
+ * More than 64 new tokens of one sequence, a prompt's, are several sequences that name the same pages: the i-th has ctx_lens + 64 i cached tokens and rows 64 i and on, once all keys and values are written.
+ * The kernel, for up to 16 or for 128 rows a tile, is chosen by n_rows / n_seqs, the sequences' average (those without rows among them): one large tree among many single tokens is read once for every 16 of its
+ * rows, and is faster in a call of its own.
  * All arrays are on the device (row_starts [n_seqs + 1] rises; n_rows: rows of q).  scale 0: 1 / sqrt(head_dim).  head_dim 64 or 128, up to 16 query heads of a key/value head, 2^20 sequences, 2^24 rows,
  * 2^10 key/value heads and 2^24 pages a table; the cache is counted in 31 bits, by rows of 64 channels of bf16 or pieces of 128 bytes.  out is q itself (same pitch) or apart from it, and from all else; pitches and addresses are multiples of
  * 16 bytes.  What lies behind a sequence's end or is seen by none of its rows may be anything; values of a token that some rows see and others do not are finite, or NaN may come out for all of them.
