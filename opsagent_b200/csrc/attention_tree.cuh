@@ -87,14 +87,15 @@ struct TreeAt {
     OA_DEVINL int steps() const { return (s.pages + PAGES - 1) / PAGES; }
     OA_DEVINL int64_t units() const { return OVER + steps(); }
     OA_DEVINL int64_t all_units(const TreeAttnArgs& a) const { return (int64_t)s.tiles(tile_tokens) * a.n_kv * units(); }      // of the sequence
-    // of an item that is not the last one with units; by a whole warp
+    // by a whole warp
     OA_DEVINL void next(const TreeAttnArgs& a) {
         unit0 += units();
         if (++tile < s.tiles(tile_tokens)) return;
         tile = 0;
         if (++kvh < a.n_kv) return;
         kvh = 0;
-        s.read(a, ++seq);
+        if (++seq >= a.n_seqs) { s.n = s.pages = 0; return; }
+        s.read(a, seq);
         // sequences without rows, as a padded batch has behind its last one, 32 at a time: each is a latency of L2
         while (s.n == 0) {
             const int lane = threadIdx.x & 31;
