@@ -38,7 +38,7 @@ struct FewCfg {
     static constexpr int Q_PITCH = D * 2 + (FMT == CACHE_BF16 ? 16 : 64), Q_BYTES = ROWS * Q_PITCH;      // no bank conflicts
     static constexpr int STATE_BYTES = STATES * (REGS * 32 * 4 + ROWS * 2 * 4 + 4);
     static constexpr int SMEM_BYTES = STAGES * (STAGE_BYTES + SCALE_BYTES) + 2 * (Q_BYTES + ROWS * 16 + 80) + STATE_BYTES + (2 * STAGES + 6) * 8;
-    static constexpr int CTAS = FMT != CACHE_BF16 && NB == 1 ? 2 : 1;            // of an SM
+    static constexpr int CTAS = FMT != CACHE_BF16 && NB == 1 ? 2 : 1;            // of an SM: two leave 80 registers, of which up to 44 bytes spill, and take 81 us for the decoding step above; one with ten pages in its ring took 93
 };
 struct TreeMeta { uint64_t seen; int low; float factor; };
 struct FewItem { TreeSeq s; int c0, c1, low, high, row0, rows, kvh, later; bool first, last, more; };      // a CTA's pages of an item, special ones below `low` and from `high` on; CTAs that have later parts
