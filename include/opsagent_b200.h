@@ -235,8 +235,8 @@ OA_API int oa_k_cache8_copy(void* kv_cache, int32_t planes, int32_t num_pages, i
  * 2^10 key/value heads and 2^24 pages a table; the cache is counted in 31 bits, by rows of 64 channels of bf16 or pieces of 128 bytes.  out is q itself (same pitch) or apart from it, and from all else; pitches and addresses are multiples of
  * 16 bytes.  What lies behind a sequence's end or is seen by none of its rows may be anything; values of a token that some rows see and others do not are finite, or NaN may come out for all of them.
  * Softmax weights are rounded to bf16 (fp16 over 8 bits) for their product with the values, sums are fp32; over 8 bits, where sequences have more than 16 rows (new tokens' heads of a group) on average, keys
- * and values times their scales are rounded to fp16 as well (2^-11 of each product of a score at most, so that errors grow with scores: 1.8e-3 of the output for scores up to 20, 2.1e-3 up to 80, of single rows
- * 3.8e-3 and 1.0e-2, instead of 1.7e-3), and values lose bits where their scale is below 2^-20 of a larger one that any row of the sequence sees.
+ * and values times their scales are rounded to fp16 as well (2^-11 of each product of a score at most, so that errors grow with scores: 1.9e-3 of the output for scores up to 20, 2.2e-3 up to 80, of single rows
+ * 3.6e-3 and 1.0e-2, instead of 1.7e-3), and values lose bits where their scale is below 2^-20 of a larger one that any row of the sequence sees.
  * Weights in fp16, which up to 16 rows hold their values' scales, are lost below 2^-31 of the largest.  A page number beyond the cache, row bounds that fall or leave the rows, more than 64 new tokens, or a
  * length beyond the table set *status; rows that read such a page hold no meaningful value, the rest is cut to what there is (the first 64 new tokens are computed) */
 OA_API int oa_k_tree_attention(const void* q, int64_t ldq, void* out, int64_t ldo, const void* kv_cache, int32_t format, int32_t num_pages, const int32_t* block_tables, int32_t max_pages_per_seq,

@@ -6,7 +6,7 @@
 // bf16: P is rounded to bf16.  8 bits: tiles are turned into fp16 under the swizzle that the products read, by eight warps of their own.  Keys and values are multiplied by their scales on the way
 // (over a power of two that none of a tile's, or of a piece's so far, passes): a softmax thread that multiplied 128 scores and weights by scales from shared memory took twice as long for a tile.
 // Roundings to fp16, 2^-11 each: a key or value times its scale, a weight.  Scales come in two halves: rounded to one, an error that all channels of a key share, they left 2.4e-3 to 3.6e-3 of the output for
-// scores up to 20 and 80 (single rows 6e-3 and 2.3e-2) instead of 1.8e-3 and 2.1e-3 (3.8e-3 and 1.0e-2), at 89 and 100 us for unequal trees of 3 to 40 tokens over e4m3 and int8, 122 and 128 for 25 tokens behind
+// scores up to 20 and 80 (single rows 6.7e-3 and 2.3e-2) instead of 1.9e-3 and 2.2e-3 (3.6e-3 and 1.0e-2), at 89 and 100 us for unequal trees of 3 to 40 tokens over e4m3 and int8, 122 and 128 for 25 tokens behind
 // 100001, instead of 91, 96, 127 and 139; scores times fp32 scales in the softmax threads leave 1.7e-3 at any size and took 122, 127, 148 and 155.  Keys and values go through one code: a second copy of it cost
 // the unequal trees 10 us.
 // Queries are scaled by a power of two as for few rows, by a kernel before.
